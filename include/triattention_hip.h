@@ -358,6 +358,82 @@ int tri_compress_step_static(const tri_kv_layout* kv, const tri_batch* batch, co
                              const tri_select_params* sel, int32_t* keep, const uint32_t** status_out,
                              void* stream);
 
+/* Attention of new tokens over one layer of the paged cache, the step between two compressions (no counterpart in the
+ * reference, which leaves attention to its engine).  The new tokens of a sequence are the last n of its seq_lens tokens,
+ * their K and V rows are in the cache; each is a row of q.  A row sees every token before the new ones, itself and its
+ * ancestors among the new ones.  out = softmax(scale * k_scale * q . k) v * v_scale, lse the natural logarithm of the
+ * sum of exponentials.  A row that sees nothing (seq_lens 0), or nothing but scores of -inf, gets zeros and -inf.  Rows from row_starts[num_seqs] on
+ * are left as they were, and so are their lse.  Scores and sums are held in fp32, weights rounded to 16 bits for the product
+ * with V (bf16 for fp8 caches, else the cache's type).
+ * A table entry outside [0, num_blocks) counts as a block without tokens.  Lengths above max_seq_len count as it, rows beyond
+ * max_rows of a sequence are left out.  kv: bf16 or fp16 with queries of that type, fp8 (a scale per row where v_scale_layers is set,
+ * none otherwise) with queries of either. */
+typedef struct tri_attend_params {
+  int32_t layer;                /* of the layout */
+  int32_t num_q_heads;          /* a multiple of num_kv_heads */
+  int32_t num_rows;             /* rows of q, out and lse */
+  int32_t max_rows;             /* 1 to 64: most rows of a sequence */
+  int32_t q_dtype;              /* TRI_KV_BF16 or TRI_KV_FP16 */
+  int32_t num_blocks;           /* physical blocks of the cache */
+  const void* q;                /* element (row, head, d) at q + row*q_stride_row + head*q_stride_head + d; 16-byte aligned rows */
+  int64_t q_stride_row, q_stride_head;
+  void* out;                    /* q's type, likewise */
+  int64_t out_stride_row, out_stride_head;
+  float* lse;                   /* [num_rows][num_q_heads], or NULL */
+  const int32_t* row_starts;    /* [num_seqs + 1] ascending: rows of sequence b are row_starts[b] to row_starts[b+1] - 1;
+                                   NULL: one row per sequence */
+  const int32_t* parents;       /* [num_rows] of every row, counted from the sequence's first row: the row it follows; any value
+                                   outside [0, own index): it follows the last token before the new ones.  NULL: each follows the one before it */
+  float scale, k_scale, v_scale;
+  float* weights;               /* the layer's accumulated weights [num_blocks][block_size][num_kv_heads] (the place of a slot's
+                                   weight is that of an fp8 slot's scale), or NULL: every slot the rows see receives the sum of
+                                   their softmax weights over rows and query heads of its KV head */
+  int32_t weight_mode;          /* 0: added, for the new tokens' own slots written; 1: written for every token of a sequence */
+} tri_attend_params;
+uint64_t tri_attend_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p);
+int tri_attend_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p, void* workspace,
+                     uint64_t workspace_bytes, void* stream);
+
+/* Bounds of the keys of every block that holds one of the new_tokens last tokens of a sequence (0: of every block), all
+ * layers: bounds[l*stride_layer + ((block*num_kv_heads + head)*2 + {0: least, 1: largest})*head_dim + d], in the cache's type
+ * (fp8: bf16, of the scaled keys).  A NaN key makes its bounds NaN.  Blocks outside [0, num_blocks) are left out. */
+int tri_block_bounds(const tri_kv_layout* kv, const tri_batch* batch, int32_t num_blocks, int32_t new_tokens, void* bounds,
+                     int64_t bounds_stride_layer, void* stream);
+
+/* tri_attend_paged for one new token per sequence, over the top_blocks blocks of each KV head that score highest: sum over d
+ * of max(q*least, q*largest), the largest (or mean) over the query heads of the KV head.  The first sink_blocks and the last
+ * recent_blocks blocks of a sequence are always among them; ties go to the lowest block, a NaN score counts as
+ * the highest.  blocks receives int32 [num_seqs][num_kv_heads][top_blocks], logical blocks ascending, -1 behind the last.
+ * row_starts, parents and weights of the attention parameters must be NULL. */
+typedef struct tri_block_params {
+  const void* bounds;           /* the layer's part of tri_block_bounds' array */
+  int32_t top_blocks, sink_blocks, recent_blocks;
+  int32_t group_reduce;         /* tri_reduce */
+  int32_t* blocks;
+} tri_block_params;
+uint64_t tri_attend_blocks_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p,
+                                           const tri_block_params* bp);
+int tri_attend_blocks(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p, const tri_block_params* bp,
+                      void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Eviction by the weights tri_attend_paged adds up, in place of the calibrated scores: per sequence and KV head the budget
+ * tokens of the largest weight (mean over layers summed in 64 bits, or maximum; layer_reduce -1: a keep set per layer), the
+ * last window_size tokens and, with protect_prefill, those before prefill_lens always among the first choices; ties keep
+ * the lowest token.  keep: int32 [rows][max_budget] as tri_select's, -1 behind a sequence's budget; final_scores (may be
+ * NULL): [rows][max_seq_len], +inf where guarded, -inf behind the sequence.  tri_evict_step also moves K, V, their scales
+ * and the weights of the kept tokens into the first slots (tri_compact_paged); its block table must be valid. */
+typedef struct tri_evict_params {
+  int32_t num_blocks;
+  int32_t window_size, protect_prefill, layer_reduce, shared;      /* as in tri_select_params */
+  float* weights;               /* [num_layers][num_blocks][block_size][num_kv_heads] */
+  int64_t weights_stride_layer; /* floats */
+} tri_evict_params;
+uint64_t tri_evict_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p);
+int tri_select_by_weight(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, float* final_scores,
+                         int32_t* keep, void* workspace, uint64_t workspace_bytes, void* stream);
+int tri_evict_step(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, int32_t* keep, void* workspace,
+                   uint64_t workspace_bytes, void* stream);
+
 /* Calibration: per-query-head frequency statistics of one layer's captured query states;
  * replaces the RoPE inversion and the per-head means of scripts/calibrate.py:196-224
  * (helpers :38-98; same arithmetic as triattention/methods/pruning_utils.py:40-98).

@@ -37,6 +37,8 @@ EXPORTS = (
     "tri_dense_workspace_bytes", "tri_dense_compress",
     "tri_compact_paged", "tri_compact_full_staging_bytes",
     "tri_compact_paged_full", "tri_compress_step", "tri_compress_step_static", "tri_qstats_workspace_bytes", "tri_qstats",
+    "tri_attend_workspace_bytes", "tri_attend_paged", "tri_block_bounds", "tri_attend_blocks_workspace_bytes", "tri_attend_blocks",
+    "tri_evict_workspace_bytes", "tri_select_by_weight", "tri_evict_step",
 )
 
 
@@ -91,6 +93,26 @@ class DenseParams(C.Structure):
         + [(n, C.c_int64) for n in ("k_stride_head", "k_stride_token", "v_stride_head", "v_stride_token")]
         + [(n, C.c_void_p) for n in ("q_mean_complex", "q_abs_mean", "freq_scale_sq", "omega", "offsets", "out_k", "out_v",
                                      "out_keep")])
+
+
+class AttendParams(C.Structure):
+    _fields_ = (
+        [(n, C.c_int32) for n in ("layer", "num_q_heads", "num_rows", "max_rows", "q_dtype", "num_blocks")]
+        + [("q", C.c_void_p), ("q_stride_row", C.c_int64), ("q_stride_head", C.c_int64),
+           ("out", C.c_void_p), ("out_stride_row", C.c_int64), ("out_stride_head", C.c_int64)]
+        + [(n, C.c_void_p) for n in ("lse", "row_starts", "parents")]
+        + [(n, C.c_float) for n in ("scale", "k_scale", "v_scale")]
+        + [("weights", C.c_void_p), ("weight_mode", C.c_int32)])
+
+
+class BlockParams(C.Structure):
+    _fields_ = [("bounds", C.c_void_p), ("top_blocks", C.c_int32), ("sink_blocks", C.c_int32), ("recent_blocks", C.c_int32),
+                ("group_reduce", C.c_int32), ("blocks", C.c_void_p)]
+
+
+class EvictParams(C.Structure):
+    _fields_ = [("num_blocks", C.c_int32), ("window_size", C.c_int32), ("protect_prefill", C.c_int32), ("layer_reduce", C.c_int32),
+                ("shared", C.c_int32), ("weights", C.c_void_p), ("weights_stride_layer", C.c_int64)]
 
 
 class TriError(RuntimeError):
@@ -154,6 +176,19 @@ def load() -> C.CDLL:
     lib.tri_qstats_workspace_bytes.argtypes = [I32, I32, I32]
     lib.tri_qstats_workspace_bytes.restype = U64
     lib.tri_qstats.argtypes = [P, I64, I64, P, P, I32, I32, I32, I32, I32, C.c_float, P, P, P, P, U64, P]
+    AP, BP, EP = C.POINTER(AttendParams), C.POINTER(BlockParams), C.POINTER(EvictParams)
+    KV, BT = C.POINTER(KvLayout), C.POINTER(Batch)
+    lib.tri_attend_workspace_bytes.argtypes = [KV, BT, AP]
+    lib.tri_attend_workspace_bytes.restype = U64
+    lib.tri_attend_paged.argtypes = [KV, BT, AP, P, U64, P]
+    lib.tri_block_bounds.argtypes = [KV, BT, I32, I32, P, I64, P]
+    lib.tri_attend_blocks_workspace_bytes.argtypes = [KV, BT, AP, BP]
+    lib.tri_attend_blocks_workspace_bytes.restype = U64
+    lib.tri_attend_blocks.argtypes = [KV, BT, AP, BP, P, U64, P]
+    lib.tri_evict_workspace_bytes.argtypes = [KV, BT, EP]
+    lib.tri_evict_workspace_bytes.restype = U64
+    lib.tri_select_by_weight.argtypes = [KV, BT, EP, P, P, P, U64, P]
+    lib.tri_evict_step.argtypes = [KV, BT, EP, P, P, U64, P]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if fn.restype is C.c_int and name not in ("tri_abi_version",):

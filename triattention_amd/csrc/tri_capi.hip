@@ -880,6 +880,285 @@ int tri_compress_step_static(const tri_kv_layout* kv, const tri_batch* batch, co
   return launch_status(tri::launch_compact(c, s), "compact");
 }
 
+namespace {
+
+// How a call of attend_kernel is cut, and what it needs of the workspace.
+struct AttendPlan {
+  tri::AttendLaunch a{};
+  int64_t part_out, part_ml, lse2, scores, total;
+  // block selection
+  int64_t block_scores, counts;
+  int max_count;
+};
+
+constexpr int kMaxNewTokens = 64;          // a word of ancestors
+constexpr int kAttendWorkgroups = 768;     // three for every CU: what is aimed at where the tokens allow it
+constexpr int kAttendStep = 128;           // tokens the waves of a workgroup take at a time
+
+bool is_finite(float x) { return x - x == 0.f; }
+
+int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p, const tri_block_params* bp,
+                AttendPlan& d) {
+  int rc = check_layout(kv, true);
+  if (!rc) rc = check_batch(batch, false);
+  if (rc) return rc;
+  if (!p) return fail(TRI_ERR_INVALID_ARGUMENT, "attention params are NULL");
+  if (p->layer < 0 || p->layer >= kv->num_layers) return fail(TRI_ERR_INVALID_ARGUMENT, "layer %d of %d", p->layer, kv->num_layers);
+  if (p->num_q_heads <= 0 || p->num_q_heads % kv->num_kv_heads)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "num_q_heads %d is not a multiple of num_kv_heads %d", p->num_q_heads, kv->num_kv_heads);
+  if (p->q_dtype != TRI_KV_BF16 && p->q_dtype != TRI_KV_FP16)
+    return fail(TRI_ERR_UNSUPPORTED, "q_dtype %d (bf16 or fp16 queries)", p->q_dtype);
+  if (kv->kv_dtype != TRI_KV_FP8_E4M3 && p->q_dtype != kv->kv_dtype)
+    return fail(TRI_ERR_UNSUPPORTED, "queries of type %d over a cache of type %d", p->q_dtype, kv->kv_dtype);
+  if (p->num_blocks <= 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_blocks %d", p->num_blocks);
+  if (p->max_rows < 1 || p->max_rows > kMaxNewTokens)
+    return fail(TRI_ERR_UNSUPPORTED, "max_rows %d not in [1, %d]", p->max_rows, kMaxNewTokens);
+  if (p->num_rows < 0 || p->num_rows > INT_MAX / p->num_q_heads) return fail(TRI_ERR_INVALID_ARGUMENT, "num_rows %d", p->num_rows);
+  if (!p->row_starts && (p->num_rows != batch->num_seqs || p->max_rows != 1 || p->parents))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "without row_starts there is one row per sequence (%d rows of at most %d, %d sequences) and no parents",
+                p->num_rows, p->max_rows, batch->num_seqs);
+  if (p->q_stride_row % 8 || p->q_stride_head % 8 || p->out_stride_row % 8 || p->out_stride_head % 8)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "strides of q and out must be multiples of 8 elements (16 bytes)");
+  if (p->num_q_heads > 1 && p->out_stride_head < kv->head_dim)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "out_stride_head %lld < head_dim", (long long)p->out_stride_head);
+  if (!is_finite(p->scale) || !is_finite(p->k_scale) || !is_finite(p->v_scale) || !is_finite(p->scale * p->k_scale * 1.44269504f))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "scale, k_scale and v_scale must be finite");
+  if (p->weight_mode != 0 && p->weight_mode != 1) return fail(TRI_ERR_INVALID_ARGUMENT, "weight_mode %d", p->weight_mode);
+  if (bp) {
+    if (p->row_starts || p->parents || p->weights)
+      return fail(TRI_ERR_UNSUPPORTED, "attention over chosen blocks takes one row per sequence and adds up no weights");
+    if (bp->top_blocks <= 0 || bp->sink_blocks < 0 || bp->recent_blocks < 0 ||
+        (int64_t)bp->sink_blocks + bp->recent_blocks > bp->top_blocks)
+      return fail(TRI_ERR_INVALID_ARGUMENT, "%d sink and %d recent blocks of %d", bp->sink_blocks, bp->recent_blocks, bp->top_blocks);
+    if (bp->group_reduce != TRI_REDUCE_MEAN && bp->group_reduce != TRI_REDUCE_MAX)
+      return fail(TRI_ERR_INVALID_ARGUMENT, "group_reduce %d", bp->group_reduce);
+  }
+  tri::AttendLaunch& a = d.a;
+  a.B = batch->num_seqs; a.Hkv = kv->num_kv_heads; a.Hq = p->num_q_heads; a.G = a.Hq / a.Hkv; a.D = kv->head_dim;
+  a.block_size = kv->block_size; a.kv_dtype = kv->kv_dtype; a.q_dtype = p->q_dtype; a.layer = p->layer;
+  a.Tmax = batch->max_seq_len; a.num_blocks = p->num_blocks;
+  a.stride_block = kv->stride_block; a.stride_token = kv->stride_token; a.stride_head = kv->stride_head;
+  a.k_layers = kv->k_layers; a.v_layers = kv->v_layers;
+  if (kv->kv_dtype == TRI_KV_FP8_E4M3 && kv->v_scale_layers) {
+    a.k_scale_layers = kv->k_scale_layers;
+    a.v_scale_layers = kv->v_scale_layers;
+  }
+  a.block_table = batch->block_table; a.block_table_pitch = batch->block_table_pitch; a.seq_lens = batch->seq_lens;
+  a.q = p->q; a.q_stride_row = p->q_stride_row; a.q_stride_head = p->q_stride_head;
+  a.out = p->out; a.out_stride_row = p->out_stride_row; a.out_stride_head = p->out_stride_head; a.lse = p->lse;
+  a.row_starts = p->row_starts; a.parents = p->parents; a.num_rows = p->num_rows; a.max_rows = p->max_rows;
+  a.scale_log2 = p->scale * p->k_scale * 1.44269504088896340736f;
+  a.v_scale = p->v_scale;
+  // Blocks and tokens a sequence has at most, and tokens of the batch.
+  d.max_count = tri::ceil_div(a.Tmax, a.block_size);
+  const int64_t chosen = bp ? (int64_t)std::min(bp->top_blocks, d.max_count) * a.block_size : INT_MAX;
+  if (bp && chosen > INT_MAX / 2) return fail(TRI_ERR_UNSUPPORTED, "%d blocks of %d tokens", bp->top_blocks, a.block_size);
+  const int64_t longest = std::min<int64_t>(bp ? chosen : a.Tmax, bp ? (int64_t)d.max_count * a.block_size : a.Tmax);
+  int64_t total = 0;
+  for (int b = 0; b < a.B; ++b) total += std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest);
+  const int rows = a.max_rows * a.G;
+  a.row_tiles = rows <= 16 ? 1 : rows <= 32 || a.D == 256 ? 2 : 4;
+  a.row_blocks = tri::ceil_div(rows, 16 * a.row_tiles);
+  const int64_t per = tri::ceil_div64(total * a.Hkv * a.row_blocks, kAttendWorkgroups);
+  a.split_tokens = (int)std::min<int64_t>(tri::align_up(std::max<int64_t>(per, 1), kAttendStep), tri::align_up(longest, kAttendStep));
+  a.nsplit = (int)tri::ceil_div64(longest, a.split_tokens);
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) { const int64_t o = off; off = tri::align_up(off + bytes, 256); return o; };
+  const int64_t parts = a.nsplit > 1 ? (int64_t)a.B * a.Hkv * a.nsplit * rows : 0;
+  if ((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) > INT_MAX ||
+      (int64_t)a.B * a.Hkv * rows > INT_MAX)
+    return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d rows and %d KV heads in one call", a.B, a.max_rows, a.Hkv);
+  a.score_pitch = tri::align_up(a.Tmax, 32);
+  d.part_out = take(parts * a.D * 4);
+  d.part_ml = take(parts * 8);
+  d.lse2 = take(p->weights ? (int64_t)a.num_rows * a.Hq * 4 : 0);
+  d.scores = take(p->weights ? (int64_t)a.B * a.Hkv * rows * a.score_pitch * 4 : 0);
+  d.block_scores = take(bp ? (int64_t)a.B * a.Hkv * d.max_count * 4 : 0);
+  d.counts = take(bp ? (int64_t)a.B * 8 : 0);
+  d.total = std::max<int64_t>(off, 256);
+  return TRI_OK;
+}
+
+int check_attend_pointers(const tri_attend_params* p, const AttendPlan& d, void* ws, uint64_t ws_bytes) {
+  if (!p->q || !p->out) return fail(TRI_ERR_INVALID_ARGUMENT, "q / out is NULL");
+  if (!is_aligned(p->q, 16) || !is_aligned(p->out, 16)) return fail(TRI_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
+  tri::Workspace need{};
+  need.total = d.total;
+  return check_workspace(need, ws, ws_bytes);
+}
+
+int do_attend(AttendPlan& d, void* ws, hipStream_t s) {
+  tri::AttendLaunch& a = d.a;
+  if (a.nsplit > 1) {
+    a.part_out = at<float>(ws, d.part_out);
+    a.part_ml = at<float>(ws, d.part_ml);
+  }
+  int rc = launch_status(a.D == 64 ? tri::launch_attend_64(a, s) : a.D == 128 ? tri::launch_attend_128(a, s) : tri::launch_attend_256(a, s),
+                         "attend");
+  if (!rc && a.nsplit > 1) rc = launch_status(tri::launch_attend_join(a, s), "attend_join");
+  return rc;
+}
+
+int fill_evict(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, int32_t* keep, tri::EvictLaunch& a) {
+  int rc = check_layout(kv, false);
+  if (!rc) rc = check_batch(batch, true);
+  if (rc) return rc;
+  if (!p) return fail(TRI_ERR_INVALID_ARGUMENT, "evict params are NULL");
+  if (p->num_blocks <= 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_blocks %d", p->num_blocks);
+  if (p->window_size < 0) return fail(TRI_ERR_INVALID_ARGUMENT, "window_size %d", p->window_size);
+  if (p->layer_reduce != TRI_REDUCE_MEAN && p->layer_reduce != TRI_REDUCE_MAX && p->layer_reduce != -1)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "layer_reduce %d", p->layer_reduce);
+  if (p->protect_prefill && !batch->prefill_lens) return fail(TRI_ERR_INVALID_ARGUMENT, "protect_prefill without prefill_lens");
+  if (kv->num_layers > 1 && p->weights_stride_layer < (int64_t)p->num_blocks * kv->block_size * kv->num_kv_heads)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "weights_stride_layer %lld is less than a layer", (long long)p->weights_stride_layer);
+  const int64_t width = std::max(batch->max_seq_len, batch->max_budget);
+  if (tri::ceil_div64(width * kv->num_kv_heads, 256) * batch->num_seqs * kv->num_layers > INT_MAX)
+    return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d layers in one call", batch->num_seqs, batch->max_seq_len, kv->num_layers);
+  a.B = batch->num_seqs; a.L = kv->num_layers; a.Hkv = kv->num_kv_heads; a.block_size = kv->block_size;
+  a.Tmax = batch->max_seq_len; a.max_budget = batch->max_budget; a.num_blocks = p->num_blocks;
+  a.window_size = p->window_size; a.protect_prefill = p->protect_prefill; a.layer_reduce = p->layer_reduce; a.shared = p->shared ? 1 : 0;
+  a.block_table = batch->block_table; a.block_table_pitch = batch->block_table_pitch; a.seq_lens = batch->seq_lens;
+  a.prefill_lens = batch->prefill_lens; a.budgets = batch->budgets;
+  a.weights = p->weights; a.weights_stride_layer = p->weights_stride_layer; a.keep = keep;
+  return TRI_OK;
+}
+
+int64_t evict_rows(const tri::EvictLaunch& a) { return (int64_t)a.B * (a.layer_reduce < 0 ? a.L : 1) * (a.shared ? 1 : a.Hkv); }
+
+int do_select_by_weight(tri::EvictLaunch& a, const tri_evict_params* p, float* final_scores, void* ws, uint64_t ws_bytes, hipStream_t s) {
+  if (!p->weights || !a.keep) return fail(TRI_ERR_INVALID_ARGUMENT, "weights / keep is NULL");
+  tri::Workspace need{};
+  need.total = tri::align_up(evict_rows(a) * a.Tmax * 4, 256);
+  if (!final_scores) {
+    const int rc = check_workspace(need, ws, ws_bytes);
+    if (rc) return rc;
+  }
+  a.fin = final_scores ? final_scores : at<float>(ws, 0);
+  int rc = launch_status(tri::launch_weight_rows(a, s), "weight_rows");
+  if (rc) return rc;
+  const int rows = (int)evict_rows(a);
+  return launch_status(tri::launch_topk_rows(a.fin, a.Tmax, rows, a.seq_lens, a.budgets, rows / a.B, a.Tmax, a.keep, a.max_budget, s),
+                       "topk_rows");
+}
+
+}  // namespace
+
+uint64_t tri_attend_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p) {
+  AttendPlan d;
+  return plan_attend(kv, batch, p, nullptr, d) ? 0 : (uint64_t)d.total;
+}
+
+int tri_attend_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p, void* ws, uint64_t ws_bytes,
+                     void* stream) {
+  AttendPlan d;
+  int rc = plan_attend(kv, batch, p, nullptr, d);
+  if (!rc) rc = check_attend_pointers(p, d, ws, ws_bytes);
+  if (rc) return rc;
+  if (p->num_rows == 0) return TRI_OK;
+  hipStream_t s = (hipStream_t)stream;
+  if (p->weights) {
+    d.a.lse2 = at<float>(ws, d.lse2);
+    d.a.scores = at<float>(ws, d.scores);
+  }
+  rc = do_attend(d, ws, s);
+  if (rc || !p->weights) return rc;
+  return launch_status(tri::launch_attend_weights(d.a, p->weights, p->weight_mode, s), "attend_weights");
+}
+
+int tri_block_bounds(const tri_kv_layout* kv, const tri_batch* batch, int32_t num_blocks, int32_t new_tokens, void* bounds,
+                     int64_t bounds_stride_layer, void* stream) {
+  int rc = check_layout(kv, false);
+  if (!rc) rc = check_batch(batch, false);
+  if (rc) return rc;
+  if (num_blocks <= 0 || new_tokens < 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_blocks %d, new_tokens %d", num_blocks, new_tokens);
+  if (!bounds || !is_aligned(bounds, 16) || bounds_stride_layer % 8)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "bounds must be 16-byte aligned, layer by layer");
+  if (kv->num_layers > 1 && bounds_stride_layer < (int64_t)num_blocks * kv->num_kv_heads * 2 * kv->head_dim)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "bounds_stride_layer %lld is less than a layer", (long long)bounds_stride_layer);
+  const int64_t waves = tri::ceil_div(kv->num_kv_heads * (kv->head_dim / 8), 64);
+  if ((int64_t)batch->num_seqs * kv->num_layers * tri::ceil_div(batch->max_seq_len, kv->block_size) * waves > INT_MAX)
+    return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d layers in one call", batch->num_seqs, batch->max_seq_len, kv->num_layers);
+  tri::BoundsLaunch a{};
+  a.B = batch->num_seqs; a.L = kv->num_layers; a.Hkv = kv->num_kv_heads; a.D = kv->head_dim; a.block_size = kv->block_size;
+  a.kv_dtype = kv->kv_dtype; a.Tmax = batch->max_seq_len; a.num_blocks = num_blocks; a.new_tokens = new_tokens;
+  a.stride_block = kv->stride_block; a.stride_token = kv->stride_token; a.stride_head = kv->stride_head;
+  a.k_layers = kv->k_layers;
+  if (kv->kv_dtype == TRI_KV_FP8_E4M3 && kv->v_scale_layers) a.k_scale_layers = kv->k_scale_layers;
+  a.block_table = batch->block_table; a.block_table_pitch = batch->block_table_pitch; a.seq_lens = batch->seq_lens;
+  a.bounds = bounds; a.bounds_stride_layer = bounds_stride_layer;
+  return launch_status(tri::launch_block_bounds(a, (hipStream_t)stream), "block_bounds");
+}
+
+uint64_t tri_attend_blocks_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p,
+                                           const tri_block_params* bp) {
+  AttendPlan d;
+  if (!bp) {
+    fail(TRI_ERR_INVALID_ARGUMENT, "block params are NULL");
+    return 0;
+  }
+  return plan_attend(kv, batch, p, bp, d) ? 0 : (uint64_t)d.total;
+}
+
+int tri_attend_blocks(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p, const tri_block_params* bp,
+                      void* ws, uint64_t ws_bytes, void* stream) {
+  if (!bp) return fail(TRI_ERR_INVALID_ARGUMENT, "block params are NULL");
+  AttendPlan d;
+  int rc = plan_attend(kv, batch, p, bp, d);
+  if (!rc) rc = check_attend_pointers(p, d, ws, ws_bytes);
+  if (rc) return rc;
+  if (!bp->bounds || !bp->blocks || !is_aligned(bp->bounds, 16))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "bounds / blocks is NULL or bounds not 16-byte aligned");
+  if ((int64_t)d.a.B * d.a.Hkv > INT_MAX / std::max(bp->top_blocks, 1))
+    return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d blocks", d.a.B, bp->top_blocks);
+  hipStream_t s = (hipStream_t)stream;
+  tri::BlockScoreLaunch c{};
+  c.B = d.a.B; c.Hkv = d.a.Hkv; c.G = d.a.G; c.D = d.a.D; c.block_size = d.a.block_size;
+  c.bounds_dtype = kv->kv_dtype == TRI_KV_FP8_E4M3 ? TRI_KV_BF16 : kv->kv_dtype; c.q_dtype = p->q_dtype;
+  c.Tmax = d.a.Tmax; c.num_blocks = d.a.num_blocks; c.max_count = d.max_count;
+  c.top = bp->top_blocks; c.sinks = bp->sink_blocks; c.recent = bp->recent_blocks; c.group_max = bp->group_reduce == TRI_REDUCE_MAX;
+  c.block_table = d.a.block_table; c.block_table_pitch = d.a.block_table_pitch; c.seq_lens = d.a.seq_lens;
+  c.q = p->q; c.q_stride_row = p->q_stride_row; c.q_stride_head = p->q_stride_head; c.bounds = bp->bounds;
+  c.scores = at<float>(ws, d.block_scores); c.counts = at<int32_t>(ws, d.counts); c.blocks = bp->blocks;
+  rc = launch_status(tri::launch_block_scores(c, s), "block_scores");
+  if (rc) return rc;
+  rc = launch_status(tri::launch_topk_rows(c.scores, d.max_count, c.B * c.Hkv, c.counts, c.counts + c.B, c.Hkv, d.max_count, bp->blocks,
+                                           bp->top_blocks, s),
+                     "topk_rows");
+  if (rc) return rc;
+  d.a.list = bp->blocks; d.a.list_k = bp->top_blocks; d.a.list_pitch = bp->top_blocks;
+  return do_attend(d, ws, s);
+}
+
+uint64_t tri_evict_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p) {
+  tri::EvictLaunch a{};
+  if (fill_evict(kv, batch, p, nullptr, a)) return 0;
+  return (uint64_t)tri::align_up(evict_rows(a) * a.Tmax * 4, 256);
+}
+
+int tri_select_by_weight(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, float* final_scores,
+                         int32_t* keep, void* ws, uint64_t ws_bytes, void* stream) {
+  tri::EvictLaunch a{};
+  const int rc = fill_evict(kv, batch, p, keep, a);
+  if (rc) return rc;
+  return do_select_by_weight(a, p, final_scores, ws, ws_bytes, (hipStream_t)stream);
+}
+
+int tri_evict_step(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, int32_t* keep, void* ws,
+                   uint64_t ws_bytes, void* stream) {
+  tri::EvictLaunch a{};
+  int rc = fill_evict(kv, batch, p, keep, a);
+  if (rc) return rc;
+  tri::CompactLaunch c{};
+  rc = fill_compact(kv, batch, keep, p->layer_reduce < 0, p->shared, c);
+  if (rc) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  rc = do_select_by_weight(a, p, nullptr, ws, ws_bytes, s);
+  if (rc) return rc;
+  rc = launch_status(tri::launch_compact(c, s), "compact");
+  if (rc) return rc;
+  return launch_status(tri::launch_move_weights(a, s), "move_weights");
+}
+
 uint64_t tri_qstats_workspace_bytes(int32_t num_heads, int32_t num_tokens, int32_t head_dim) {
   if (num_heads <= 0 || num_tokens <= 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
   return (uint64_t)tri::qstats_workspace_bytes(num_heads, num_tokens, head_dim);

@@ -253,6 +253,89 @@ struct DenseLaunch {
 hipError_t launch_dense_prologue(const DenseLaunch& d, hipStream_t s);
 hipError_t launch_dense_gather(const DenseLaunch& d, hipStream_t s);
 
+// Attention over one layer of the paged cache (tri_attend_device.h, tri_attend.hip).
+struct AttendLaunch {
+  int B, Hkv, G, Hq, D, block_size, kv_dtype, q_dtype, layer, Tmax, num_blocks;
+  int64_t stride_block, stride_token, stride_head;         // elements
+  const void* const* k_layers;
+  const void* const* v_layers;
+  const float* const* k_scale_layers;                      // both NULL: rows without scales of their own
+  const float* const* v_scale_layers;
+  const int32_t* block_table;                              // NULL: dense, physical block = sequence
+  int block_table_pitch;
+  const int32_t* seq_lens;
+  const void* q;
+  int64_t q_stride_row, q_stride_head;                     // elements
+  void* out;
+  int64_t out_stride_row, out_stride_head;                 // elements
+  float* lse;                                              // [num_rows][Hq], or NULL
+  const int32_t* row_starts;                               // [B + 1], or NULL: row b
+  const int32_t* parents;                                  // [num_rows], or NULL: a chain
+  int num_rows, max_rows;
+  float scale_log2, v_scale;                               // softmax scale (the keys' scale in it) times log2 e
+  // blocks chosen per (sequence, KV head), ascending, in place of the whole cache
+  const int32_t* list;
+  int list_k, list_pitch;
+  // how the work is cut
+  int row_tiles, row_blocks, nsplit, split_tokens;
+  // workspace
+  float* part_out;                                         // [B][Hkv][nsplit][max_rows * G][D], not normalised (nsplit > 1)
+  float* part_ml;                                          // the same rows' maximum (base 2) and sum
+  float* lse2;                                             // [num_rows][Hq], base 2, or NULL
+  float* scores;                                           // [B][Hkv][max_rows * G][score_pitch] base 2, or NULL
+  int64_t score_pitch;
+};
+hipError_t launch_attend_64(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_128(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_256(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_join(const AttendLaunch& a, hipStream_t s);
+// weights: the layer's [num_blocks][block_size][Hkv]; set: written, not added to.
+hipError_t launch_attend_weights(const AttendLaunch& a, float* weights, int set, hipStream_t s);
+
+// Bounds of a block's keys and the scores that choose blocks by them (tri_blocks.hip).
+struct BoundsLaunch {
+  int B, L, Hkv, D, block_size, kv_dtype, Tmax, num_blocks, new_tokens;    // new_tokens 0: every block
+  int64_t stride_block, stride_token, stride_head;
+  const void* const* k_layers;
+  const float* const* k_scale_layers;                      // NULL: rows without scales of their own
+  const int32_t* block_table;
+  int block_table_pitch;
+  const int32_t* seq_lens;
+  void* bounds;                                            // [L][num_blocks][Hkv][2][D]
+  int64_t bounds_stride_layer;                             // elements
+};
+hipError_t launch_block_bounds(const BoundsLaunch& a, hipStream_t s);
+struct BlockScoreLaunch {
+  int B, Hkv, G, D, block_size, bounds_dtype, q_dtype, Tmax, num_blocks, max_count, top, sinks, recent, group_max;
+  const int32_t* block_table;
+  int block_table_pitch;
+  const int32_t* seq_lens;
+  const void* q;
+  int64_t q_stride_row, q_stride_head;
+  const void* bounds;                                      // one layer's
+  float* scores;                                           // [B * Hkv][max_count]
+  int32_t* counts;                                         // [2][B]: blocks of a sequence, and how many of them are taken
+  int32_t* blocks;                                         // [B * Hkv][top]: -1 behind what is taken
+};
+hipError_t launch_block_scores(const BlockScoreLaunch& a, hipStream_t s);
+
+// Eviction by accumulated weight (tri_evict.hip).
+struct EvictLaunch {
+  int B, L, Hkv, block_size, Tmax, max_budget, num_blocks;
+  int window_size, protect_prefill, layer_reduce, shared;
+  const int32_t* block_table;
+  int block_table_pitch;
+  const int32_t* seq_lens;
+  const int32_t* prefill_lens;
+  const int32_t* budgets;
+  float* weights;                                          // [L][num_blocks][block_size][Hkv]
+  int64_t weights_stride_layer;
+  float* fin;                                              // [rows][Tmax]
+  int32_t* keep;                                           // [rows][max_budget]
+};
+hipError_t launch_weight_rows(const EvictLaunch& a, hipStream_t s);
+hipError_t launch_move_weights(const EvictLaunch& a, hipStream_t s);
+
 // Calibration statistics of one layer's captured queries (tri_calib.hip).
 struct QStatsLaunch {
   const void* q_rot;      // [H][T][D] through (stride_head, stride_token), 16-bit elements

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from ._lib import (KV_BF16, KV_FP16, KV_FP8_E4M3, REDUCE_MAX, REDUCE_MEAN, REDUCE_NONE, ROPE_HALF,
-                   ROPE_INTERLEAVED, Batch, KvLayout, ScoreParams, SelectParams)
+                   ROPE_INTERLEAVED, AttendParams, Batch, BlockParams, EvictParams, KvLayout, ScoreParams, SelectParams)
 
 _DTYPES = {torch.bfloat16: KV_BF16, torch.float16: KV_FP16}
 _UNIT_SCALES: dict = {}
@@ -698,3 +698,234 @@ def compress_step_static(kv: PagedKV, batch: StepBatch, sc: ScoreConfig, sel: Se
     _lib.check(lib.tri_compress_step_static(C.byref(kv.struct), C.byref(batch.struct), C.byref(sp), C.byref(ss),
                                             _ptr(keep), C.byref(status), _stream()))
     return int(status.value or 0)
+
+
+class _on_device:
+    """Makes a cache's device the current one for the calls of a block (kernels go to the current stream of the
+    current device)."""
+
+    def __init__(self, device):
+        self.index = device.index
+        self.back = None
+
+    def __enter__(self):
+        now = torch.cuda.current_device()
+        if self.index is not None and self.index != now:
+            self.back = now
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+        return False
+
+
+def _on(kv: PagedKV, name: str, t: torch.Tensor, dtype=None) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.device != kv.device or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be a{'' if dtype is None else ' ' + str(dtype)} tensor on {kv.device}")
+    return t
+
+
+def _scratch(kv: PagedKV, nbytes: int, what: str):
+    """Scratch of one call from torch's allocator, of the current stream (under graph capture: of the graph's own pool, so
+    two graphs never share any)."""
+    if nbytes == 0:
+        raise ValueError(f"invalid {what}: " + _lib.load().tri_last_error().decode("utf-8", "replace"))
+    buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=kv.device)
+    at = buf.data_ptr()
+    return buf, at + (-at) % 256
+
+
+def _layer_weights(kv: PagedKV, weights: torch.Tensor) -> torch.Tensor:
+    shape = (kv.num_layers, kv.num_blocks, kv.block_size, kv.num_kv_heads)
+    if tuple(_on(kv, "weights", weights, torch.float32).shape) != shape or not weights[0].is_contiguous():
+        raise ValueError(f"weights must be fp32 {shape}, contiguous within a layer")
+    return weights
+
+
+def _check_attention_batch(kv: PagedKV, batch: StepBatch) -> None:
+    if batch.device != kv.device and torch.device(batch.device) != kv.device:
+        raise ValueError(f"the batch lies on {batch.device}, the cache on {kv.device}")
+    batch.check_capacity(kv.block_size)
+    if kv.ks_ptrs is not None and kv.vs_ptrs is None and not hasattr(kv, "_unit"):
+        raise ValueError("an fp8 cache has scales for K and V rows, or for neither")
+    if batch.block_table is None and (batch.max_seq_len > kv.block_size or batch.num_seqs > kv.num_blocks):
+        raise ValueError("without a block table a sequence is one block of the cache")
+
+
+def _attend_params(kv: PagedKV, batch: StepBatch, q, layer, row_starts, parents, max_rows, scale, k_scale, v_scale, out, want_lse):
+    """(parameters, out, lse) of an attention call after the checks that need the tensors."""
+    _check_attention_batch(kv, batch)
+    if kv.v_ptrs is None:
+        raise ValueError("attention needs the values of the cache")
+    _on(kv, "q", q)
+    if q.ndim != 3 or q.dtype not in (torch.bfloat16, torch.float16) or int(q.shape[2]) != kv.head_dim or q.stride(2) != 1:
+        raise ValueError(f"q must be a bf16 or fp16 [rows, heads, {kv.head_dim}] tensor with contiguous head_dim")
+    if not 0 <= layer < kv.num_layers:
+        raise IndexError(f"layer {layer} of {kv.num_layers}")
+    rows, heads = int(q.shape[0]), int(q.shape[1])
+    if row_starts is not None:
+        _on(kv, "row_starts", row_starts, torch.int32)
+        if tuple(row_starts.shape) != (batch.num_seqs + 1,) or not row_starts.is_contiguous():
+            raise ValueError(f"row_starts must be a contiguous tensor of {batch.num_seqs + 1} entries")
+        if parents is not None:
+            _on(kv, "parents", parents, torch.int32)
+            if tuple(parents.shape) != (rows,) or not parents.is_contiguous():
+                raise ValueError(f"parents must be a contiguous tensor of {rows} entries")
+    if out is None:
+        out = torch.empty((rows, heads, kv.head_dim), dtype=q.dtype, device=kv.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != kv.device or out.stride(2) != 1:
+        raise ValueError("out must have q's shape and type on the cache's device, with contiguous head_dim")
+    lse = torch.empty((rows, heads), dtype=torch.float32, device=kv.device) if want_lse else None
+    p = AttendParams(layer=layer, num_q_heads=heads, num_rows=rows, max_rows=max_rows, q_dtype=_DTYPES[q.dtype],
+                     num_blocks=kv.num_blocks, q=_ptr(q), q_stride_row=q.stride(0), q_stride_head=q.stride(1), out=_ptr(out),
+                     out_stride_row=out.stride(0), out_stride_head=out.stride(1), lse=_ptr(lse), row_starts=_ptr(row_starts),
+                     parents=_ptr(parents), scale=kv.head_dim ** -0.5 if scale is None else scale, k_scale=k_scale, v_scale=v_scale)
+    return p, out, lse
+
+
+def attend_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, *, layer: int = 0, row_starts: torch.Tensor | None = None,
+                 parents: torch.Tensor | None = None, max_rows: int = 1, scale: float | None = None, k_scale: float = 1.0,
+                 v_scale: float = 1.0, weights: torch.Tensor | None = None, weight_mode: str = "add",
+                 out: torch.Tensor | None = None, want_lse: bool = False):
+    """Attention of the newest tokens of every sequence over one layer of the cache (``tri_attend_paged``).
+
+    ``q`` [rows, Hq, D], after RoPE, of the cache's type (fp8 caches: bf16 or fp16).  The new tokens are the last ones of
+    ``batch.seq_lens``, their keys and values are in the cache already.  Without ``row_starts`` there is one per
+    sequence: a decoding step.  With it (int32 [sequences + 1] on the device, ascending) sequence b has the rows
+    ``row_starts[b]`` to ``row_starts[b + 1] - 1``, at most ``max_rows`` <= 64, and ``parents`` (int32 [rows]) says which earlier
+    row of its sequence each follows, counted from the sequence's first (anything else, such as -1: the
+    last token before them; None: each follows the one before): a tree of drafted tokens, or a short chunk of a
+    prompt.  A row sees every token before the new ones, its ancestors and itself.  Rows behind ``row_starts[-1]`` are
+    left as they were (in a new ``out``: whatever was in that memory).
+
+    ``weights`` (fp32 [layers, blocks, block_size, Hkv], beside the cache) receives the softmax weight of every cached token, summed over
+    rows and the query heads of its KV head: added ("add"; the slots of the new tokens themselves are written) or written
+    ("set").  ``select_by_weight`` and ``evict_step`` go by them.
+
+    Lengths are read on the device: a program that replays a captured call may rewrite ``batch.seq_lens`` in place, up to
+    the batch's ``max_seq_len``; a sequence of no tokens gives zeros.  Returns (out, lse or None)."""
+    lib = _lib.load()
+    if weight_mode not in ("add", "set"):
+        raise ValueError(f"weight_mode must be 'add' or 'set', got {weight_mode!r}")
+    p, out, lse = _attend_params(kv, batch, q, layer, row_starts, parents, max_rows, scale, k_scale, v_scale, out, want_lse)
+    if weights is not None:
+        p.weights = _ptr(_layer_weights(kv, weights)[layer])
+        p.weight_mode = int(weight_mode == "set")
+    with _on_device(kv.device):
+        nbytes = int(lib.tri_attend_workspace_bytes(C.byref(kv.struct), C.byref(batch.struct), C.byref(p)))
+        buf, at = _scratch(kv, nbytes, "attention call")
+        _lib.check(lib.tri_attend_paged(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), at, nbytes, _stream()))
+    return out, lse
+
+
+def block_bounds(kv: PagedKV) -> torch.Tensor:
+    """An array for ``update_block_bounds``: [layers, blocks, Hkv, 2, D] of the cache's type (fp8 caches: bf16)."""
+    dtype = torch.bfloat16 if _DTYPES[kv.dtype] == KV_FP8_E4M3 else kv.dtype
+    return torch.zeros(kv.num_layers, kv.num_blocks, kv.num_kv_heads, 2, kv.head_dim, dtype=dtype, device=kv.device)
+
+
+def _checked_bounds(kv: PagedKV, bounds: torch.Tensor) -> torch.Tensor:
+    dtype = torch.bfloat16 if _DTYPES[kv.dtype] == KV_FP8_E4M3 else kv.dtype
+    shape = (kv.num_layers, kv.num_blocks, kv.num_kv_heads, 2, kv.head_dim)
+    if tuple(_on(kv, "bounds", bounds, dtype).shape) != shape or not bounds[0].is_contiguous():
+        raise ValueError(f"bounds must be {dtype} {shape}, contiguous within a layer")
+    return bounds
+
+
+def update_block_bounds(kv: PagedKV, batch: StepBatch, bounds: torch.Tensor, *, new_tokens: int | None = None) -> torch.Tensor:
+    """Least and largest key per dimension of the blocks that hold the last ``new_tokens`` tokens of every sequence (None: of
+    all its blocks; after a prompt or a compaction), every layer, into ``bounds`` (``tri_block_bounds``)."""
+    lib = _lib.load()
+    _check_attention_batch(kv, batch)
+    _checked_bounds(kv, bounds)
+    if new_tokens is not None and new_tokens < 1:
+        raise ValueError(f"new_tokens must be positive or None, got {new_tokens}")
+    with _on_device(kv.device):
+        _lib.check(lib.tri_block_bounds(C.byref(kv.struct), C.byref(batch.struct), kv.num_blocks, new_tokens or 0, _ptr(bounds),
+                                        int(bounds.stride(0)), _stream()))
+    return bounds
+
+
+def attend_blocks(kv: PagedKV, batch: StepBatch, q: torch.Tensor, bounds: torch.Tensor, *, top_blocks: int, layer: int = 0,
+                  sink_blocks: int = 1, recent_blocks: int = 1, group_reduce: str = "max", scale: float | None = None,
+                  k_scale: float = 1.0, v_scale: float = 1.0, out: torch.Tensor | None = None, want_lse: bool = False):
+    """A decoding step that reads, per KV head, the ``top_blocks`` blocks whose keys may score highest with its queries
+    (``tri_attend_blocks``): the upper bounds of q . k that ``update_block_bounds`` allows, the largest (``group_reduce``
+    "mean": the mean) over the query heads of the KV head; the first ``sink_blocks`` and last ``recent_blocks`` blocks always.
+
+    ``q`` [sequences, Hq, D].  Returns (out, lse or None, blocks int32 [sequences, Hkv, top_blocks]: logical
+    blocks ascending, -1 behind the last)."""
+    lib = _lib.load()
+    if group_reduce not in ("max", "mean"):
+        raise ValueError(f"group_reduce must be 'max' or 'mean', got {group_reduce!r}")
+    _checked_bounds(kv, bounds)
+    p, out, lse = _attend_params(kv, batch, q, layer, None, None, 1, scale, k_scale, v_scale, out, want_lse)
+    blocks = torch.empty((batch.num_seqs, kv.num_kv_heads, max(top_blocks, 0)), dtype=torch.int32, device=kv.device)
+    bp = BlockParams(bounds=_ptr(bounds[layer]), top_blocks=top_blocks, sink_blocks=sink_blocks, recent_blocks=recent_blocks,
+                     group_reduce=REDUCE_MAX if group_reduce == "max" else REDUCE_MEAN, blocks=_ptr(blocks))
+    with _on_device(kv.device):
+        nbytes = int(lib.tri_attend_blocks_workspace_bytes(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), C.byref(bp)))
+        buf, at = _scratch(kv, nbytes, "attention call")
+        _lib.check(lib.tri_attend_blocks(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), C.byref(bp), at, nbytes, _stream()))
+    return out, lse, blocks
+
+
+@dataclass
+class EvictConfig:
+    """How ``select_by_weight`` / ``evict_step`` turn accumulated weights into keep sets."""
+    window_size: int = 128               # recent tokens that always stay
+    protect_prefill: bool = False        # those of the prompt (the batch's prefill_lens) as well
+    layer_reduce: str | None = "mean"    # "max"; None: one keep set per layer
+    shared: bool = False                 # one list for all KV heads (the largest of their weights)
+
+
+def _evict_params(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: EvictConfig, keep):
+    if batch.budgets is None:
+        raise ValueError("batch has no budgets")
+    _check_attention_batch(kv, batch)
+    _layer_weights(kv, weights)
+    if ev.layer_reduce not in ("mean", "max", None):
+        raise ValueError(f"layer_reduce must be 'mean', 'max' or None, got {ev.layer_reduce!r}")
+    if ev.protect_prefill and batch.prefill_lens is None:
+        raise ValueError("protect_prefill needs the batch's prefill_lens")
+    rows = batch.num_seqs * (kv.num_layers if ev.layer_reduce is None else 1) * (1 if ev.shared else kv.num_kv_heads)
+    if keep is None:
+        keep = torch.empty(rows, batch.max_budget, dtype=torch.int32, device=kv.device)
+    elif (keep.numel() != rows * batch.max_budget or keep.dtype != torch.int32 or not keep.is_contiguous()
+          or keep.device != kv.device):
+        raise ValueError(f"keep must be a contiguous int32 tensor with {rows} x {batch.max_budget} entries")
+    lr = REDUCE_NONE if ev.layer_reduce is None else (REDUCE_MAX if ev.layer_reduce == "max" else REDUCE_MEAN)
+    return EvictParams(num_blocks=kv.num_blocks, window_size=int(ev.window_size), protect_prefill=int(ev.protect_prefill),
+                       layer_reduce=lr, shared=int(ev.shared), weights=_ptr(weights),
+                       weights_stride_layer=int(weights.stride(0))), keep, rows
+
+
+def select_by_weight(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: EvictConfig, *, want_scores: bool = False,
+                     keep: torch.Tensor | None = None):
+    """keep int32 [rows, max_budget] (ascending, -1 behind a sequence's budget) of the tokens with the largest accumulated
+    weight, and optionally the scores they were chosen by [rows, max_seq_len] (``tri_select_by_weight``); rows as
+    ``select``'s.  Nothing is moved: ``compact`` takes the rows where every sequence has the same budget or more tokens."""
+    lib = _lib.load()
+    p, keep, rows = _evict_params(kv, batch, weights, ev, keep)
+    fin = torch.empty(rows, batch.max_seq_len, dtype=torch.float32, device=kv.device) if want_scores else None
+    with _on_device(kv.device):
+        nbytes = int(lib.tri_evict_workspace_bytes(C.byref(kv.struct), C.byref(batch.struct), C.byref(p)))
+        buf, at = _scratch(kv, nbytes, "eviction") if fin is None or nbytes == 0 else (None, None)
+        _lib.check(lib.tri_select_by_weight(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _ptr(fin), _ptr(keep), at,
+                                            nbytes if at else 0, _stream()))
+    return keep, fin
+
+
+def evict_step(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: EvictConfig, *, keep: torch.Tensor | None = None) -> torch.Tensor:
+    """``select_by_weight``, then K, V, their scales and the weights of the kept tokens moved into the first slots of every
+    sequence, every layer (``tri_evict_step``): ``compress_step`` by accumulated weight.  Returns the keep rows."""
+    lib = _lib.load()
+    if batch.block_table is None or kv.v_ptrs is None:
+        raise ValueError("evict_step needs block tables and the values of the cache")
+    p, keep, _ = _evict_params(kv, batch, weights, ev, keep)
+    with _on_device(kv.device):
+        nbytes = int(lib.tri_evict_workspace_bytes(C.byref(kv.struct), C.byref(batch.struct), C.byref(p)))
+        buf, at = _scratch(kv, nbytes, "eviction")
+        _lib.check(lib.tri_evict_step(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _ptr(keep), at, nbytes, _stream()))
+    return keep
