@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendLaunch a) {
   uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + i * a.out_stride_row + (int64_t)hq * a.out_stride_head + d;
   *reinterpret_cast<uint2*>(dst) = uint2{Half<QT>::pack(v[0] * inv, v[1] * inv), Half<QT>::pack(v[2] * inv, v[3] * inv)};
   if (d == 0) {
-    const float l2 = total == 0.f ? -INFINITY : top + log2f(total);
+    const float l2 = lse_of(top, total);
     if (a.lse) a.lse[i * a.Hq + hq] = l2 * 0.69314718055994530942f;
     if (a.lse2) a.lse2[i * a.Hq + hq] = l2;
   }
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void attend_weights_kernel(AttendLaunch a, flo
       const float* lse = a.lse2 + (int64_t)(rows.first + i) * a.Hq + h * a.G;
       for (int g = 0; g < a.G; ++g) {
         const float l = lse[g];
-        if (l != -INFINITY) sum += exp2f(s[(int64_t)(i * a.G + g) * a.score_pitch] - l);
+        if (l != -INFINITY) sum += pow2(s[(int64_t)(i * a.G + g) * a.score_pitch] - l);
       }
     }
     w[h] = fresh ? sum : w[h] + sum;
@@ -87,6 +87,13 @@ hipError_t launch_join_typed(const AttendLaunch& a, hipStream_t s) {
 }
 
 }  // namespace
+
+hipError_t launch_attend(const AttendLaunch& a, hipStream_t s) {
+  const bool bf16 = a.q_dtype == TRI_KV_BF16;
+  if (a.D == 64) return bf16 ? launch_attend_64_bf16(a, s) : launch_attend_64_fp16(a, s);
+  if (a.D == 128) return bf16 ? launch_attend_128_bf16(a, s) : launch_attend_128_fp16(a, s);
+  return bf16 ? launch_attend_256_bf16(a, s) : launch_attend_256_fp16(a, s);
+}
 
 hipError_t launch_attend_join(const AttendLaunch& a, hipStream_t s) {
   return a.q_dtype == TRI_KV_BF16 ? launch_join_typed<TRI_KV_BF16>(a, s) : launch_join_typed<TRI_KV_FP16>(a, s);

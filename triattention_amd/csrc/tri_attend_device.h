@@ -7,13 +7,17 @@
 // Rows: a sequence has n new tokens, the last n of its cache; KV head h serves the M = n * G rows (token i, query head
 // h * G + g), m = i * G + g.  Row m sees every token before the new ones, and of those token i and its ancestors.
 //
-// A wave takes 32 tokens at a time and RT tiles of 16 rows.  S^T = K Q^T on the matrix cores (16 tokens x 16 rows x 32
-// elements) leaves in a lane the scores of one row (lane & 15) for tokens (lane >> 4) * 4 + r of either half: exactly
-// the order in which the B operand of O^T = V^T P^T wants them, if the 32 tokens are numbered (lane >> 4) * 8 + j =
-// token (j & 4) * 4 + (lane >> 4) * 4 + (j & 3).  So the weights never leave their lane, a row's maximum is two
-// exchanges between lanes, and the rescaling of O is a multiplication inside a lane.  V^T comes out of LDS by the
-// transposing read (16 lanes, 4 tokens x 16 elements).  The four waves of a workgroup take tiles in turn and meet once
-// at the end; a sequence is cut into splits where there are few rows, joined by attend_join_kernel.
+// S^T = K Q^T on the matrix cores (16 tokens x 16 rows x 32 elements) leaves in a lane the scores of one row (lane & 15) for
+// tokens (lane >> 4) * 4 + r: exactly the order in which the B operand of O^T = V^T P^T wants them, if the 32 tokens of that
+// product are numbered (lane >> 4) * 8 + j = token (j & 4) * 4 + (lane >> 4) * 4 + (j & 3).  So the weights never leave
+// their lane, a row's maximum is two exchanges between lanes, and the rescaling of O is a multiplication inside a lane.
+// V^T comes out of LDS by the transposing read (16 lanes, 4 tokens x 16 elements).
+//
+// Up to 16 rows (attend_few_kernel) the four waves of a workgroup take tiles of 32 tokens in turn, keys straight from
+// memory into the operand's registers, and meet once at the end: such a call is bound by reading K and V, and what
+// counts is how many bytes are asked for at a time.  Beyond that (attend_rows_kernel) every wave has rows of its own and
+// the workgroup shares the tiles through LDS: a tile is read from memory once for up to 256 rows.  A sequence is cut into
+// splits where there are few rows, joined by attend_join_kernel.
 #pragma once
 
 #include "tri_common.h"
@@ -25,7 +29,7 @@ namespace {
 
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / kWave;
-constexpr int kAttendTile = 32;       // tokens a wave takes at a time
+constexpr int kAttendTile = 32;       // tokens of one product with V
 
 template <int T>
 struct Half;                          // the type of the products
@@ -60,15 +64,43 @@ struct Half<TRI_KV_FP16> {
 
 // Eight fp8 codes (two dwords) as eight 16-bit numbers; exact in either type.
 template <int T>
-__device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b) {
-  return uint4{Half<T>::widen_lo(a), Half<T>::widen_hi(a), Half<T>::widen_lo(b), Half<T>::widen_hi(b)};
+__device__ __forceinline__ u32x4 widen8(uint32_t a, uint32_t b) {
+  return u32x4{Half<T>::widen_lo(a), Half<T>::widen_hi(a), Half<T>::widen_lo(b), Half<T>::widen_hi(b)};
 }
 
-// Whether a packed pair of 16-bit numbers holds an infinity or a NaN (all exponent bits set).
+// The bits of the infinities and NaNs among the numbers of a word, to replace them by 0.  (16-bit types: all exponent bits set;
+// e4m3 has no infinity, its NaN is all bits but the sign.)
 template <int T>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
-  constexpr uint32_t e = T == TRI_KV_FP16 ? 0x7c00u : 0x7f80u;
-  return (w & e) == e || (w >> 16 & e) == e;
+__device__ __forceinline__ uint32_t odd_bits(uint32_t w) {
+  constexpr int bits = T == TRI_KV_FP8_E4M3 ? 8 : 16;
+  constexpr uint32_t e = T == TRI_KV_FP16 ? 0x7c00u : T == TRI_KV_BF16 ? 0x7f80u : 0x7fu;
+  uint32_t drop = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += bits)
+    if ((w >> i & e) == e) drop |= (bits == 8 ? 0xffu : 0xffffu) << i;
+  return drop;
+}
+template <int T>
+__device__ __forceinline__ bool clear_odd(u32x4& w) {
+  const u32x4 drop = {odd_bits<T>(w[0]), odd_bits<T>(w[1]), odd_bits<T>(w[2]), odd_bits<T>(w[3])};
+  w &= ~drop;
+  return (drop[0] | drop[1] | drop[2] | drop[3]) != 0;
+}
+
+// One matrix-core step on operands as they come out of memory and LDS.
+template <int T>
+__device__ __forceinline__ f32x4 mfma(const u32x4& x, const u32x4& y, f32x4 c) {
+  if constexpr (T == TRI_KV_FP16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
+}
+
+// The lane's number where the compiler must not compute what follows from it before a loop: rare branches would hold
+// registers all the time.
+__device__ __forceinline__ int here(int lane) {
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 
 typedef short i16x4 __attribute__((ext_vector_type(4)));
@@ -77,13 +109,16 @@ typedef __attribute__((address_space(3))) i16x4* LdsI16x4;
 // The transposing read: each 16 lanes read a piece of 4 rows (4 lanes of 8 bytes each, lane / 4 the row) x 16 columns
 // and lane c receives column c, rows 0 to 3.
 typedef __attribute__((address_space(3))) unsigned char* LdsBytes;
-__device__ __forceinline__ uint2 lds_read_transposed(LdsBytes at) {
+__device__ __forceinline__ u32x2 lds_read_transposed(LdsBytes at) {
   const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsI16x4)at);
-  return __builtin_bit_cast(uint2, v);
+  return __builtin_bit_cast(u32x2, v);
 }
 
+// 2^x, the instruction alone: results below 2^-126 become 0, which no sum of weights that holds a 1 sees.
+__device__ __forceinline__ float pow2(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // Two 2^(x) terms of one sum: -inf - -inf is a row without tokens on either side, and a factor of 0.
-__device__ __forceinline__ float rescale(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+__device__ __forceinline__ float rescale(float m, float top) { return m == -INFINITY ? 0.f : pow2(m - top); }
 
 __device__ __forceinline__ int64_t shfl64(int64_t v, int lane) {
   const int lo = __shfl((int)(uint32_t)v, lane), hi = __shfl((int)(v >> 32), lane);
@@ -127,21 +162,409 @@ __device__ __forceinline__ int tokens_of(const AttendLaunch& a, int b, int T) {
   return min(a.list_k, ceil_div(T, a.block_size)) * a.block_size;
 }
 
-template <int QT, bool FP8, int D, int RT>
-__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendLaunch a) {
+// Places of tokens: a lane holds one token of a tile -- list entry, then page, then byte offset, each asked for a tile ahead
+// of the next (a wait for a young load would be a wait for every older one).
+struct Place {
+  int64_t byte, row;     // offset of the row, index of its scale; 0 for a token that is not there
+  bool ok;
+};
+template <int ES>
+struct Walk {
+  const AttendLaunch& a;
+  const int32_t* table;
+  const int32_t* list;
+  int b, T, end, mine;
+  __device__ __forceinline__ Walk(const AttendLaunch& a_, int b_, int h, int T_, int end_, int mine_) : a(a_), b(b_), T(T_), end(end_), mine(mine_) {
+    table = a.block_table ? a.block_table + (int64_t)b * a.block_table_pitch : nullptr;
+    list = a.list ? a.list + ((int64_t)b * a.Hkv + h) * a.list_pitch : nullptr;
+  }
+  // (t >= 0; exact below 2^31: the factor is 2^div_shift / block_size rounded up, div_shift = 31 + log2 block_size rounded up)
+  __device__ __forceinline__ int div(int t) const { return (int)((uint64_t)(uint32_t)t * a.div_factor >> a.div_shift); }
+  __device__ __forceinline__ int mod(int t) const { return t - div(t) * a.block_size; }
+  __device__ __forceinline__ int entry(int tile) const {
+    const int t = tile + mine;
+    return list && t < end ? list[div(t)] : 0;
+  }
+  __device__ __forceinline__ int token(int tile, int entry) const {     // position in the sequence, or -1
+    const int t = tile + mine;
+    const int tok = list ? entry * a.block_size + mod(t) : t;
+    return t < end && entry >= 0 && tok < T ? tok : -1;
+  }
+  __device__ __forceinline__ int page(int tok) const {
+    if (tok < 0) return -1;
+    return table ? table[div(tok)] : b;
+  }
+  __device__ __forceinline__ Place place(int tok, int page) const {
+    Place p;
+    p.ok = tok >= 0 && page >= 0 && page < a.num_blocks;
+    const int in = p.ok ? mod(tok) : 0;
+    const int64_t pg = p.ok ? page : 0;
+    p.byte = (pg * a.stride_block + (int64_t)in * a.stride_token) * ES;
+    p.row = (pg * a.block_size + in) * a.Hkv;
+    return p;
+  }
+};
+
+// Address of row `row` of a tile (lane row holds its place).  UNI: blocks of a multiple of 16 tokens, so that 16 tokens
+// in a row lie behind one another and their base is the same for the wave (row0: the first of the 16 that this
+// load takes rows of; it must be a constant).
+template <bool UNI, int ES>
+__device__ __forceinline__ const char* row_at(const char* base, int64_t byte, int row0, int row, int64_t stride_token) {
+  if constexpr (UNI) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)byte, row0), hi = __builtin_amdgcn_readlane((int)(byte >> 32), row0);
+    return base + (int64_t)((uint64_t)hi << 32 | lo) + (uint32_t)((row - row0) * (int)stride_token * ES);
+  } else {
+    return base + shfl64(byte, row);
+  }
+}
+
+// Queries of row c16 of 16 rows from m0 on: elements as the keys are loaded (fp8: 16 in a piece, two steps of 8).
+template <bool FP8, int D>
+__device__ __forceinline__ void load_queries(const AttendLaunch& a, const RowRange& rows, int h, int m0, int M, int lane, u32x4 (&qf)[D / 32]) {
+  const int m = m0 + (lane & 15), q4 = lane >> 4;
+  const int i = m < M ? m / a.G : 0, g = m < M ? m % a.G : 0;
+  const char* qp = reinterpret_cast<const char*>(a.q) + ((int64_t)(rows.first + i) * a.q_stride_row + (int64_t)(h * a.G + g) * a.q_stride_head) * 2;
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+    const int el = FP8 ? (s / 2) * 64 + q4 * 16 + (s & 1) * 8 : s * 32 + q4 * 8;
+    qf[s] = m < M ? *reinterpret_cast<const u32x4*>(qp + el * 2) : u32x4{0, 0, 0, 0};
+  }
+}
+
+// Infinities and NaNs among the values of new tokens reach the rows that see the token and no others (0 * inf in the matrix
+// product would put them into all of them, so there they are 0): rare, at the end, read from memory again.  Tokens from
+// first_tok to end of which every step-th piece of 32, from the piece-th on, is the caller's.
+template <int PT, bool FP8, int NT, int RT, int ES>
+__device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Walk<ES>& walk, const char* vb, int begin, int end, int base,
+                                               const uint64_t (&seen)[RT], int lane, int piece, int step) {
+#pragma unroll 1
+  for (int tok = max(begin, base); tok < end; ++tok) {
+    if ((tok - begin) / kAttendTile % step != piece) continue;
+    const Place p = walk.place(tok, walk.page(tok));
+    if (!p.ok) continue;
+    const char* row = vb + p.byte;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = t * 16 + (lane >> 4) * 4 + e;
+        float v;
+        if constexpr (FP8) v = __builtin_amdgcn_cvt_f32_fp8((int)(uint8_t)row[d], 0);
+        else v = Half<PT>::value(*reinterpret_cast<const uint16_t*>(row + d * ES));
+        if (!(v - v == 0.f)) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            if (seen[rt] >> ((tok - base) & 63) & 1) o[rt][t][e] += v;
+        }
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float lse_of(float top, float total) { return total == 0.f ? -INFINITY : top + log2f(total); }
+
+// One row's four elements d to d + 3 of a workgroup's result: its part, or the output itself.
+template <int QT, int D>
+__device__ __forceinline__ void put_row(const AttendLaunch& a, const RowRange& rows, int b, int h, int split, int m, int d, const f32x4& v,
+                                        float top, float total) {
+  if (a.nsplit > 1) {
+    const int64_t at = (((int64_t)b * a.Hkv + h) * a.nsplit + split) * a.max_rows * a.G + m;
+    *reinterpret_cast<f32x4*>(a.part_out + at * D + d) = v;
+    if (d == 0) {
+      a.part_ml[at * 2] = top;
+      a.part_ml[at * 2 + 1] = total;
+    }
+    return;
+  }
+  const int64_t i = rows.first + m / a.G;
+  const int hq = h * a.G + m % a.G;
+  const float inv = total == 0.f ? 0.f : a.v_scale / total;       // (a row that saw nothing: zeros and -inf)
+  uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + i * a.out_stride_row + (int64_t)hq * a.out_stride_head + d;
+  *reinterpret_cast<uint2*>(dst) = uint2{Half<QT>::pack(v[0] * inv, v[1] * inv), Half<QT>::pack(v[2] * inv, v[3] * inv)};
+  if (d == 0) {
+    const float l2 = lse_of(top, total);
+    if (a.lse) a.lse[i * a.Hq + hq] = l2 * 0.69314718055994530942f;
+    if (a.lse2) a.lse2[i * a.Hq + hq] = l2;
+  }
+}
+
+// The softmax of 32 tokens of one row a lane: sc holds q . k of tokens (i * 16 + (lane >> 4) * 4 + r) and becomes the weights
+// 2^(x - top); returns them packed for the product with V, which vs scales (fp8 rows with scales of their own).
+// The weights are rounded to 16 bits there while the sum adds them unrounded: errors of half a step each and of either
+// sign, below the one rounding of the output.
+struct RowState {
+  float top, sum;
+};
+template <int PT, bool SCALED, int NT>
+__device__ __forceinline__ u32x4 softmax32(f32x4 (&sc)[2], RowState& st, f32x4 (&o)[NT], float scale, const f32x4 (&ks)[2], const f32x4 (&vs)[2],
+                                           bool masked, bool drafts, uint32_t okm, int first, uint64_t seen, int lane, float* scores) {
+  float best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) sc[i] *= SCALED ? ks[i] : f32x4{scale, scale, scale, scale};
+  if (masked) {
+    const int l = here(lane);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = i * 16 + (l >> 4) * 4 + r, d = first + j;
+        const bool sees = (okm >> j & 1) && (!drafts || d < 0 || (seen >> (d & 63) & 1));
+        sc[i][r] = sees ? sc[i][r] : -INFINITY;
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) best = fmaxf(best, sc[i][r]);
+  if (scores) {
+    *reinterpret_cast<f32x4*>(scores) = sc[0];
+    *reinterpret_cast<f32x4*>(scores + 16) = sc[1];
+  }
+  best = fmaxf(best, __shfl_xor(best, 16));
+  best = fmaxf(best, __shfl_xor(best, 32));
+  if (__ballot(best > st.top)) {
+    const float top = fmaxf(st.top, best);
+    const float alpha = rescale(st.top, top);
+    st.top = top;
+    st.sum *= alpha;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] *= alpha;
+  }
+  const float safe = st.top == -INFINITY ? 0.f : st.top;
+  float part = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      sc[i][r] = pow2(sc[i][r] - safe);
+      part += sc[i][r];
+    }
+  st.sum += part;
+  if (SCALED) {
+    sc[0] *= vs[0];
+    sc[1] *= vs[1];
+  }
+  return u32x4{Half<PT>::pack(sc[0][0], sc[0][1]), Half<PT>::pack(sc[0][2], sc[0][3]), Half<PT>::pack(sc[1][0], sc[1][1]),
+               Half<PT>::pack(sc[1][2], sc[1][3])};
+}
+
+// ---- up to 16 rows of a KV head
+template <int QT, bool FP8, int D, bool UNI>
+__global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 3) void attend_few_kernel(AttendLaunch a) {
   constexpr int PT = FP8 ? TRI_KV_BF16 : QT;              // fp8 rows with a scale of their own: the weight carries it, which fp16 has no room for
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int KC = D * ES / 64;                         // 16-byte pieces of a key in a lane
   constexpr int LPR = D * ES / 16;                        // lanes that load one value row
-  constexpr int NV = LPR / 2;                             // 16-byte pieces of a tile's values in a lane
+  constexpr int RPL = kWave / LPR;                        // rows of one load
+  constexpr int NV = kAttendTile / RPL;                   // 16-byte pieces of a tile's values in a lane
   constexpr int NT = D / 16;
   constexpr int kPitch = D * 2 + 32;                      // bytes of a value row in LDS: eight rows reach all banks
   constexpr int kWaveBytes = kAttendTile * kPitch;
+  constexpr int kStep = kAttendWaves * kAttendTile;
   __shared__ __align__(16) unsigned char s_v[kAttendWaves * kWaveBytes];
   __shared__ __align__(16) float s_scale[kAttendWaves][2][kAttendTile];
-  __shared__ float s_ml[kAttendWaves][RT * 16][2];
+  __shared__ float s_ml[kAttendWaves][16][2];
 
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c16 = lane & 15, q4 = lane >> 4;
+  int idx = blockIdx.x;
+  const int h = idx % a.Hkv; idx /= a.Hkv;
+  const int split = idx % a.nsplit;
+  const int b = idx / a.nsplit;
+
+  const int T = min(max(a.seq_lens[b], 0), a.Tmax);
+  const RowRange rows = rows_of(a, b);
+  const int n = rows.n, M = n * a.G;
+  if (M == 0) return;
+  const int Tv = tokens_of(a, b, T);
+  const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
+  if (begin >= Tv && split > 0) return;
+  const int base = T - n;                                 // first new token (negative: not all of them are in the cache)
+  const char* kb = reinterpret_cast<const char*>(a.k_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
+  const char* vb = reinterpret_cast<const char*>(a.v_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
+  const bool scaled = FP8 && a.k_scale_layers;
+  const float* ksc = scaled ? a.k_scale_layers[a.layer] + h : nullptr;
+  const float* vsc = scaled ? a.v_scale_layers[a.layer] + h : nullptr;
+
+  const Walk<ES> walk(a, b, h, T, end, lane & (kAttendTile - 1));
+  const int first_tile = begin + wave * kAttendTile;
+  u32x4 kr[2][KC], vr[NV];
+  float ks_mine = 0.f, vs_mine = 0.f;
+  auto load_keys = [&](const Place& p) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const char* src = row_at<UNI, ES>(kb, p.byte, i * 16, i * 16 + c16, a.stride_token) + q4 * 16;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) kr[i][c] = *reinterpret_cast<const u32x4*>(src + c * 64);
+    }
+    if (scaled) {
+      ks_mine = ksc[p.row];
+      vs_mine = vsc[p.row];
+    }
+  };
+  auto load_values = [&](const Place& p) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      vr[i] = *reinterpret_cast<const u32x4*>(row_at<UNI, ES>(vb, p.byte, i * RPL / 16 * 16, i * RPL + lane / LPR, a.stride_token) + (lane % LPR) * 16);
+  };
+
+  Place now{}, next{};
+  int next_tok = -1, next_page = -1, next2_entry = 0;
+  if (first_tile < end) {
+    const int tok = walk.token(first_tile, walk.entry(first_tile));
+    next_tok = walk.token(first_tile + kStep, walk.entry(first_tile + kStep));
+    const int page = walk.page(tok);
+    next_page = walk.page(next_tok);
+    next2_entry = walk.entry(first_tile + 2 * kStep);
+    now = walk.place(tok, page);
+    load_keys(now);
+    load_values(now);
+  }
+  u32x4 qf[D / 32];
+  load_queries<FP8, D>(a, rows, h, 0, M, lane, qf);
+  uint64_t seen[1] = {1};
+  if (n > 1) seen[0] = (uint64_t)shfl64((int64_t)ancestor_mask(a.parents, rows.first, n, lane), min(c16, M - 1) / a.G);
+  float* const scores = a.scores && c16 < M ? a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + c16) * a.score_pitch + q4 * 4 : nullptr;
+
+  f32x4 o[1][NT];
+  bool odd = false;
+  RowState st{-INFINITY, 0.f};
+#pragma unroll
+  for (int t = 0; t < NT; ++t) o[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  unsigned char* const my_v = s_v + wave * kWaveBytes;
+  const LdsBytes my_lds = (LdsBytes)my_v + (q4 * 4 + (c16 >> 2)) * kPitch + (c16 & 3) * 8;
+  for (int tile = first_tile; tile < end; tile += kStep) {
+    const bool more = tile + kStep < end;
+    const uint32_t okm = (uint32_t)__ballot(now.ok);
+    const bool drafts = n > 1 && tile + kAttendTile > base;
+
+    f32x4 sc[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) {
+        u32x4 kf;
+        if constexpr (FP8) {
+          kf = widen8<QT>(kr[i][s / 2][(s & 1) * 2], kr[i][s / 2][(s & 1) * 2 + 1]);
+        } else {
+          kf = kr[i][s];
+        }
+        sc[i] = mfma<QT>(kf, qf[s], sc[i]);
+      }
+    }
+    if (scaled && lane < kAttendTile) {
+      s_scale[wave][0][lane] = ks_mine * a.scale_log2;
+      s_scale[wave][1][lane] = vs_mine;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // the next tile's keys into the registers of this one's, this one's values into LDS
+    if (more) {
+      next = walk.place(next_tok, next_page);
+      next_tok = walk.token(tile + 2 * kStep, next2_entry);
+      next_page = walk.page(next_tok);
+      next2_entry = walk.entry(tile + 3 * kStep);
+      load_keys(next);
+    }
+    if (okm != 0xffffffffu || drafts) {
+      // What lies behind the end is 0 in the product (0 * what is there could be NaN), and so are a new token's infinities.
+      const int l = here(lane);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int row = i * RPL + l / LPR;
+        if (!(okm >> row & 1)) vr[i] = u32x4{0, 0, 0, 0};
+        if (drafts && tile + row >= base) odd |= clear_odd<FP8 ? TRI_KV_FP8_E4M3 : PT>(vr[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      u32x4* dst = reinterpret_cast<u32x4*>(my_v + (i * RPL + lane / LPR) * kPitch + (lane % LPR) * (FP8 ? 32 : 16));
+      if constexpr (FP8) {
+        dst[0] = widen8<PT>(vr[i][0], vr[i][1]);
+        dst[1] = widen8<PT>(vr[i][2], vr[i][3]);
+      } else {
+        dst[0] = vr[i];
+      }
+    }
+    if (more) load_values(next);
+    __builtin_amdgcn_sched_barrier(0);
+    const bool masked = okm != 0xffffffffu || drafts;
+    u32x4 pf;
+    f32x4 ks[2] = {}, vs[2] = {};
+    if (scaled) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][0][i * 16 + q4 * 4]);
+        vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][1][i * 16 + q4 * 4]);
+      }
+      pf = softmax32<PT, true, NT>(sc, st, o[0], 0.f, ks, vs, masked, drafts, okm, tile - base, seen[0], lane, scores ? scores + tile : nullptr);
+    } else {
+      pf = softmax32<PT, false, NT>(sc, st, o[0], a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen[0], lane, scores ? scores + tile : nullptr);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const u32x2 lo = lds_read_transposed(my_lds + t * 32), hi = lds_read_transposed(my_lds + t * 32 + 16 * kPitch);
+      o[0][t] = mfma<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[0][t]);
+    }
+    __builtin_amdgcn_wave_barrier();
+    now = next;
+  }
+  if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, walk, vb, begin, end, base, seen, lane, wave, kAttendWaves);
+
+  // the four waves meet
+  st.sum += __shfl_xor(st.sum, 16);
+  st.sum += __shfl_xor(st.sum, 32);
+  if (q4 == 0) {
+    s_ml[wave][c16][0] = st.top;
+    s_ml[wave][c16][1] = st.sum;
+  }
+  __syncthreads();
+  f32x4* const box = reinterpret_cast<f32x4*>(s_v);       // [wave][NT][64]
+  static_assert(NT * kWave * 16 <= kWaveBytes, "the exchange fits the value tiles");
+  float all = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kAttendWaves; ++w) all = fmaxf(all, s_ml[w][c16][0]);
+  const float mine = rescale(st.top, all);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) box[(wave * NT + t) * kWave + lane] = o[0][t] * mine;
+  __syncthreads();
+  for (int it = threadIdx.x; it < NT * kWave; it += kAttendThreads) {
+    const int t = it / kWave, l = it % kWave, m = l & 15;
+    if (m >= M) continue;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f, top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kAttendWaves; ++w) top = fmaxf(top, s_ml[w][m][0]);
+#pragma unroll
+    for (int w = 0; w < kAttendWaves; ++w) {
+      v += box[(w * NT + t) * kWave + l];
+      total += rescale(s_ml[w][m][0], top) * s_ml[w][m][1];
+    }
+    put_row<QT, D>(a, rows, b, h, split, m, t * 16 + (l >> 4) * 4, v, top, total);
+  }
+}
+
+// ---- more rows: RT tiles of 16 rows a wave, four waves, K and V of BT tokens in LDS for all of them
+template <int QT, bool FP8, int D, int RT, bool UNI>
+__global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunch a) {
+  constexpr int PT = FP8 ? TRI_KV_BF16 : QT;
+  constexpr int ES = FP8 ? 1 : 2;
+  constexpr int BT = D == 256 ? 32 : 64;                  // tokens of a tile
+  constexpr int LPR = D * ES / 16;                        // lanes that load one row
+  constexpr int RPL = kWave / LPR;                        // rows of a wave's load
+  constexpr int NL = BT / (RPL * kAttendWaves);           // loads of a lane for K, and for V
+  constexpr int NT = D / 16;
+  constexpr int kKeyPitch = D * 2 + 16;                   // 16 rows, 16 bytes of each, reach all banks
+  constexpr int kValPitch = D * 2 + 32;                   // 8 rows, 32 bytes of each
+  static_assert(RPL <= 16 && NL >= 1, "a wave's load stays within 16 rows");
+  __shared__ __align__(16) unsigned char s_k[2][BT * kKeyPitch];
+  __shared__ __align__(16) unsigned char s_v[2][BT * kValPitch];
+  __shared__ __align__(16) float s_scale[2][2][BT];
+  __shared__ int s_odd;
+
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c16 = lane & 15, q4 = lane >> 4;
   int idx = blockIdx.x;
   const int h = idx % a.Hkv; idx /= a.Hkv;
@@ -151,354 +574,204 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendLaunch a) 
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   const RowRange rows = rows_of(a, b);
-  const int n = rows.n, M = n * a.G, m0 = rb * RT * 16;
-  if (m0 >= M) return;
+  const int n = rows.n, M = n * a.G;
+  if (rb * RT * 16 * kAttendWaves >= M) return;
+  const int m0 = (rb * kAttendWaves + wave) * RT * 16;
   const int Tv = tokens_of(a, b, T);
   const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
   if (begin >= Tv && split > 0) return;
-  const int base = T - n;                                 // first new token (negative: not all of them are in the cache)
-  const int32_t* table = a.block_table ? a.block_table + (int64_t)b * a.block_table_pitch : nullptr;
-  const int32_t* list = a.list ? a.list + ((int64_t)b * a.Hkv + h) * a.list_pitch : nullptr;
+  const int base = T - n;
   const char* kb = reinterpret_cast<const char*>(a.k_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
   const char* vb = reinterpret_cast<const char*>(a.v_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
-  const float* ksc = a.k_scale_layers ? a.k_scale_layers[a.layer] + h : nullptr;
-  const float* vsc = a.v_scale_layers ? a.v_scale_layers[a.layer] + h : nullptr;
+  const bool scaled = FP8 && a.k_scale_layers;
+  const float* ksc = scaled ? a.k_scale_layers[a.layer] + h : nullptr;
+  const float* vsc = scaled ? a.v_scale_layers[a.layer] + h : nullptr;
 
-  // Queries: lane = row c16 of a tile, elements as the keys are loaded (fp8: 16 in a piece, two steps of 8).
-  uint4 qf[RT][D / 32];
+  const Walk<ES> walk(a, b, h, T, end, lane & (BT - 1));
+  u32x4 kr[NL], vr[NL];
+  float ks_mine = 0.f, vs_mine = 0.f;
+  Place p[2] = {};                       // of the tile in LDS, and of the one in registers
+  auto load = [&](const Place& at) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      // (rows of this load: 16-row group i * 4 * RPL + wave * RPL lies in, the same for the whole wave)
+      const int row0 = (i * kAttendWaves + wave) * RPL;
+      const char* k = row_at<UNI, ES>(kb, at.byte, row0 / 16 * 16, row0 + lane / LPR, a.stride_token) + (lane % LPR) * 16;
+      const char* v = row_at<UNI, ES>(vb, at.byte, row0 / 16 * 16, row0 + lane / LPR, a.stride_token) + (lane % LPR) * 16;
+      kr[i] = *reinterpret_cast<const u32x4*>(k);
+      vr[i] = *reinterpret_cast<const u32x4*>(v);
+    }
+    if (scaled && wave == 0) {
+      ks_mine = ksc[at.row];
+      vs_mine = vsc[at.row];
+    }
+  };
+  auto store = [&](const Place& at, int tile, int buf) {
+    const uint64_t okm = __ballot(at.ok);
+    const bool all = BT == 64 ? okm == ~0ull : (uint32_t)okm == ~0u;
+    const bool drafts = n > 1 && tile + BT > base;
+    if (!all || drafts) {
+      const int l = here(lane);
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int row = (i * kAttendWaves + wave) * RPL + l / LPR;
+        if (!(okm >> row & 1)) vr[i] = u32x4{0, 0, 0, 0};
+        if (drafts && tile + row >= base) odd |= clear_odd<FP8 ? TRI_KV_FP8_E4M3 : PT>(vr[i]);
+      }
+      if (odd) s_odd = 1;
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int row = (i * kAttendWaves + wave) * RPL + lane / LPR;
+      u32x4* kd = reinterpret_cast<u32x4*>(s_k[buf] + row * kKeyPitch + (lane % LPR) * (FP8 ? 32 : 16));
+      u32x4* vd = reinterpret_cast<u32x4*>(s_v[buf] + row * kValPitch + (lane % LPR) * (FP8 ? 32 : 16));
+      if constexpr (FP8) {
+        kd[0] = widen8<QT>(kr[i][0], kr[i][1]);
+        kd[1] = widen8<QT>(kr[i][2], kr[i][3]);
+        vd[0] = widen8<PT>(vr[i][0], vr[i][1]);
+        vd[1] = widen8<PT>(vr[i][2], vr[i][3]);
+      } else {
+        kd[0] = kr[i];
+        vd[0] = vr[i];
+      }
+    }
+    if (scaled && wave == 0 && lane < BT) {
+      s_scale[buf][0][lane] = ks_mine * a.scale_log2;
+      s_scale[buf][1][lane] = vs_mine;
+    }
+  };
+
+  u32x4 qf[RT][D / 32];
   uint64_t seen[RT];
+  float* scores[RT];
+  f32x4 o[RT][NT];
+  RowState st[RT];
   const uint64_t anc = n > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int m = m0 + rt * 16 + c16;
-    const int i = m < M ? m / a.G : 0, g = m < M ? m % a.G : 0;
-    seen[rt] = (uint64_t)shfl64((int64_t)anc, i);
-    const char* qp = reinterpret_cast<const char*>(a.q) + ((int64_t)(rows.first + i) * a.q_stride_row + (int64_t)(h * a.G + g) * a.q_stride_head) * 2;
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s) {
-      const int el = FP8 ? (s / 2) * 64 + q4 * 16 + (s & 1) * 8 : s * 32 + q4 * 8;
-      qf[rt][s] = m < M ? *reinterpret_cast<const uint4*>(qp + el * 2) : uint4{0, 0, 0, 0};
-    }
-  }
-
-  f32x4 o[RT][NT];
-  float top[RT], sum[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    top[rt] = -INFINITY;
-    sum[rt] = 0.f;
+    load_queries<FP8, D>(a, rows, h, m0 + rt * 16, M, lane, qf[rt]);
+    seen[rt] = (uint64_t)shfl64((int64_t)anc, min(m, M - 1) / a.G);
+    scores[rt] = a.scores && m < M ? a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + m) * a.score_pitch + q4 * 4 : nullptr;
+    st[rt] = RowState{-INFINITY, 0.f};
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Lane l holds the place of token l & 31 of a tile: list entry, then page, then byte offset, each asked for a tile
-  // ahead of the next (a wait for a young load would be a wait for every older one).
-  const int mine = lane & (kAttendTile - 1);
-  const int first_tile = begin + wave * kAttendTile;
-  constexpr int kStep = kAttendWaves * kAttendTile;
-  auto list_entry = [&](int tile) {
-    const int t = tile + mine;
-    return list && t < end ? list[t / a.block_size] : 0;
-  };
-  auto token_at = [&](int tile, int entry) {     // position in the sequence, or -1
-    const int t = tile + mine;
-    const int tok = list ? entry * a.block_size + t % a.block_size : t;
-    return t < end && entry >= 0 && tok < T ? tok : -1;
-  };
-  auto page_of = [&](int tok) {
-    if (tok < 0) return -1;
-    return table ? table[tok / a.block_size] : b;
-  };
-  struct Place {
-    int64_t byte, row;     // offset of the row, index of its scale
-    bool ok;
-  };
-  auto place_of = [&](int tok, int page) {
-    Place p;
-    p.ok = tok >= 0 && page >= 0 && page < a.num_blocks;
-    const int in = p.ok ? tok % a.block_size : 0;
-    const int64_t pg = p.ok ? page : 0;
-    p.byte = (pg * a.stride_block + (int64_t)in * a.stride_token) * ES;
-    p.row = (pg * a.block_size + in) * a.Hkv;
-    return p;
-  };
-
-  uint4 kr[2][KC], vr[NV];
-  float ks_mine = 1.f, vs_mine = 1.f;
-  auto load_keys = [&](const Place& p) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const char* src = kb + shfl64(p.byte, i * 16 + c16) + q4 * 16;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) kr[i][c] = *reinterpret_cast<const uint4*>(src + c * 64);
-    }
-    if (FP8 && vsc) {
-      ks_mine = ksc[p.row];
-      vs_mine = vsc[p.row];
-    }
-  };
-  auto load_values = [&](const Place& p) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      vr[i] = *reinterpret_cast<const uint4*>(vb + shfl64(p.byte, i * (kWave / LPR) + lane / LPR) + (lane % LPR) * 16);
-  };
-
-  unsigned char* const my_v = s_v + wave * kWaveBytes;
-  const LdsBytes my_lds = (LdsBytes)my_v;
-  Place now{}, next{};
+  // tile t in LDS, t + 1 in registers, pages of t + 2 and list entries of t + 3 on their way
   int next_tok = -1, next_page = -1, next2_entry = 0;
-  if (first_tile < end) {
-    const int t0 = token_at(first_tile, list_entry(first_tile));
-    next_tok = token_at(first_tile + kStep, list_entry(first_tile + kStep));
-    next_page = page_of(next_tok);
-    next2_entry = list_entry(first_tile + 2 * kStep);
-    now = place_of(t0, page_of(t0));
-    load_keys(now);
-    load_values(now);
-  }
-  for (int tile = first_tile; tile < end; tile += kStep) {
-    const bool more = tile + kStep < end;
-    const uint32_t okm = (uint32_t)__ballot(now.ok);
-    const bool drafts = n > 1 && tile + kAttendTile > base;
-
-    // ---- scores
-    f32x4 sc[RT][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sc[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) {
-        uint4 kf;
-        if constexpr (FP8) {
-          const uint4& w = kr[i][s / 2];
-          kf = (s & 1) ? widen8<QT>(w.z, w.w) : widen8<QT>(w.x, w.y);
-        } else {
-          kf = kr[i][s];
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sc[rt][i] = mfma_16x16x32<QT>(kf, qf[rt][s], sc[rt][i]);
-      }
-    }
-    if (FP8 && vsc && lane < kAttendTile) {
-      s_scale[wave][0][lane] = ks_mine;
-      s_scale[wave][1][lane] = vs_mine;
-    }
-    // ---- the next tile's keys into the registers of this one's, this one's values into LDS
-    if (more) {
-      next = place_of(next_tok, next_page);
-      next_tok = token_at(tile + 2 * kStep, next2_entry);
-      next_page = page_of(next_tok);
-      next2_entry = list_entry(tile + 3 * kStep);
-      load_keys(next);
-    }
-    bool odd_values = false;                    // an infinity or a NaN among the values of new tokens
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int row = i * (kWave / LPR) + lane / LPR;
-      uint4 w[2] = {vr[i], uint4{0, 0, 0, 0}};
-      if constexpr (FP8) {
-        w[0] = widen8<PT>(vr[i].x, vr[i].y);
-        w[1] = widen8<PT>(vr[i].z, vr[i].w);
-      }
-      if (okm != 0xffffffffu && !(okm >> row & 1)) w[0] = w[1] = uint4{0, 0, 0, 0};      // 0 * what lies behind the end could be NaN
-      if (drafts) {
-#pragma unroll
-        for (int j = 0; j < (FP8 ? 2 : 1); ++j)
-          odd_values |= not_finite2<PT>(w[j].x) || not_finite2<PT>(w[j].y) || not_finite2<PT>(w[j].z) || not_finite2<PT>(w[j].w);
-      }
-      uint4* dst = reinterpret_cast<uint4*>(my_v + row * kPitch + (lane % LPR) * (FP8 ? 32 : 16));
-      dst[0] = w[0];
-      if (FP8) dst[1] = w[1];
-    }
-    if (more) load_values(next);
-
-    // ---- softmax: a lane holds tokens i * 16 + q4 * 4 + r of row c16
-    const bool masked = okm != 0xffffffffu || drafts;
-    float ks[2][4], vs[2][4];
-    if (FP8 && vsc) {
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          ks[i][r] = s_scale[wave][0][i * 16 + q4 * 4 + r] * a.scale_log2;
-          vs[i][r] = s_scale[wave][1][i * 16 + q4 * 4 + r];
-        }
-    }
-    uint4 pf[RT];
-    float p[RT][2][4];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float best = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = sc[rt][i][r] * (FP8 && vsc ? ks[i][r] : a.scale_log2);
-          if (masked) {
-            const int j = i * 16 + q4 * 4 + r;
-            const int d = tile + j - base;
-            const bool sees = (okm >> j & 1) && (!drafts || d < 0 || (seen[rt] >> (d & 63) & 1));
-            x = sees ? x : -INFINITY;
-          }
-          sc[rt][i][r] = x;
-          best = fmaxf(best, x);
-        }
-      if (a.scores) {
-        const int m = m0 + rt * 16 + c16;
-        if (m < M) {
-          float* dst = a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + m) * a.score_pitch + tile + q4 * 4;
-          *reinterpret_cast<f32x4*>(dst) = sc[rt][0];
-          *reinterpret_cast<f32x4*>(dst + 16) = sc[rt][1];
-        }
-      }
-      best = fmaxf(best, __shfl_xor(best, 16));
-      best = fmaxf(best, __shfl_xor(best, 32));
-      const float now_top = fmaxf(top[rt], best);
-      const float safe = now_top == -INFINITY ? 0.f : now_top;
-      const float alpha = rescale(top[rt], safe);
-      top[rt] = now_top;
-      float part = 0.f;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[rt][i][r] = exp2f(sc[rt][i][r] - safe);
-          part += p[rt][i][r];
-        }
-      sum[rt] = sum[rt] * alpha + part;
-      if (__ballot(alpha != 1.f)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[rt][t] *= alpha;
-      }
-      if (FP8 && vsc) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) p[rt][i][r] *= vs[i][r];
-      }
-      // The weights are rounded to 16 bits for the second product (the sum above adds them unrounded): errors of half
-      // a step each and of either sign, below the one rounding of the output.
-      pf[rt] = uint4{Half<PT>::pack(p[rt][0][0], p[rt][0][1]), Half<PT>::pack(p[rt][0][2], p[rt][0][3]),
-                     Half<PT>::pack(p[rt][1][0], p[rt][1][1]), Half<PT>::pack(p[rt][1][2], p[rt][1][3])};
-    }
-    // ---- O^T += V^T P^T
-    if (!__ballot(odd_values)) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const LdsBytes at = my_lds + (q4 * 4 + (c16 >> 2)) * kPitch + t * 32 + (c16 & 3) * 8;
-        const uint2 lo = lds_read_transposed(at), hi = lds_read_transposed(at + 16 * kPitch);
-        const uint4 vf{lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma_16x16x32<PT>(vf, pf[rt], o[rt][t]);
-      }
-    } else {
-      // An infinity or a NaN in a new token's values reaches the rows that see the token and no others (0 * inf would
-      // put it into all of them): token by token on the vector unit.
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            for (int qq = 0; qq < 4; ++qq) {
-              const int j = i * 16 + qq * 4 + r, d = tile + j - base;
-              const float w = __shfl(p[rt][i][r], qq * 16 + c16);
-              const bool sees = (okm >> j & 1) && (d < 0 || (seen[rt] >> (d & 63) & 1));
-              const uint16_t* row = reinterpret_cast<const uint16_t*>(my_v + j * kPitch);
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float v = Half<PT>::value(row[t * 16 + q4 * 4 + e]);
-                  if (sees) o[rt][t][e] += w * v;
-                }
-            }
-    }
-    __builtin_amdgcn_wave_barrier();
-    now = next;
-  }
-
-  // ---- the four waves meet
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    sum[rt] += __shfl_xor(sum[rt], 16);
-    sum[rt] += __shfl_xor(sum[rt], 32);
-    if (q4 == 0) {
-      s_ml[wave][rt * 16 + c16][0] = top[rt];
-      s_ml[wave][rt * 16 + c16][1] = sum[rt];
-    }
+  if (threadIdx.x == 0) s_odd = 0;
+  if (begin < end) {
+    const int tok = walk.token(begin, walk.entry(begin));
+    next_tok = walk.token(begin + BT, walk.entry(begin + BT));
+    const int page = walk.page(tok);
+    next_page = walk.page(next_tok);
+    next2_entry = walk.entry(begin + 2 * BT);
+    p[0] = walk.place(tok, page);
+    load(p[0]);
+    __syncthreads();
+    store(p[0], begin, 0);
+    p[1] = walk.place(next_tok, next_page);
+    next_tok = walk.token(begin + 2 * BT, next2_entry);
+    next_page = walk.page(next_tok);
+    next2_entry = walk.entry(begin + 3 * BT);
+    if (begin + BT < end) load(p[1]);
   }
   __syncthreads();
-  f32x4* const box = reinterpret_cast<f32x4*>(s_v);       // [wave][NT][64]: 4 * D / 16 * 1 KB, no more than the value tiles
-  static_assert(kAttendWaves * NT * kWave * 16 <= kAttendWaves * kWaveBytes, "the exchange fits the value tiles");
+  for (int tile = begin, buf = 0; tile < end; tile += BT, buf ^= 1) {
+    if (m0 < M) {
+      const uint64_t okm_all = __ballot(p[0].ok);
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    float all = -INFINITY;
+      for (int sub = 0; sub < BT / 32; ++sub) {
+        const int first = tile + sub * 32;
+        const uint32_t okm = (uint32_t)(okm_all >> (sub * 32));
+        const bool drafts = n > 1 && first + 32 > base;
+        const bool masked = okm != 0xffffffffu || drafts;
+        f32x4 sc[RT][2];
 #pragma unroll
-    for (int w = 0; w < kAttendWaves; ++w) all = fmaxf(all, s_ml[w][rt * 16 + c16][0]);
-    const float mine_f = rescale(top[rt], all);
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) box[(wave * NT + t) * kWave + lane] = o[rt][t] * mine_f;
-    __syncthreads();
-    for (int it = threadIdx.x; it < NT * kWave; it += kAttendThreads) {
-      const int t = it / kWave, l = it % kWave, row = rt * 16 + (l & 15), m = m0 + row;
-      if (m >= M) continue;
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      float total = 0.f, big = -INFINITY;
+          for (int rt = 0; rt < RT; ++rt) sc[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+          const unsigned char* src = s_k[buf] + (sub * 32 + i * 16 + c16) * kKeyPitch;
 #pragma unroll
-      for (int w = 0; w < kAttendWaves; ++w) big = fmaxf(big, s_ml[w][row][0]);
+          for (int s = 0; s < D / 32; ++s) {
+            const int el = FP8 ? (s / 2) * 64 + q4 * 16 + (s & 1) * 8 : s * 32 + q4 * 8;
+            const u32x4 kf = *reinterpret_cast<const u32x4*>(src + el * 2);
 #pragma unroll
-      for (int w = 0; w < kAttendWaves; ++w) {
-        v += box[(w * NT + t) * kWave + l];
-        total += rescale(s_ml[w][row][0], big) * s_ml[w][row][1];
-      }
-      const int d = t * 16 + (l >> 4) * 4;
-      if (a.nsplit > 1) {
-        const int64_t at = (((int64_t)b * a.Hkv + h) * a.nsplit + split) * a.max_rows * a.G + m;
-        *reinterpret_cast<f32x4*>(a.part_out + at * D + d) = v;
-        if (d == 0) {
-          a.part_ml[at * 2] = big;
-          a.part_ml[at * 2 + 1] = total;
+            for (int rt = 0; rt < RT; ++rt) sc[rt][i] = mfma<QT>(kf, qf[rt][s], sc[rt][i]);
+          }
         }
-      } else {
-        const int64_t i = rows.first + m / a.G;
-        const int hq = h * a.G + m % a.G;
-        // (a row that saw nothing: zeros and -inf)
-        const float inv = total == 0.f ? 0.f : a.v_scale / total;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + i * a.out_stride_row + (int64_t)hq * a.out_stride_head + d;
-        *reinterpret_cast<uint2*>(dst) = uint2{Half<QT>::pack(v[0] * inv, v[1] * inv), Half<QT>::pack(v[2] * inv, v[3] * inv)};
-        if (d == 0) {
-          const float l2 = total == 0.f ? -INFINITY : big + log2f(total);
-          if (a.lse) a.lse[i * a.Hq + hq] = l2 * 0.69314718055994530942f;
-          if (a.lse2) a.lse2[i * a.Hq + hq] = l2;
+        u32x4 pf[RT];
+        f32x4 ks[2] = {}, vs[2] = {};
+        if (scaled) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[buf][0][sub * 32 + i * 16 + q4 * 4]);
+            vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[buf][1][sub * 32 + i * 16 + q4 * 4]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ks[i] = f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+            vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
+          }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          pf[rt] = softmax32<PT, FP8, NT>(sc[rt], st[rt], o[rt], a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen[rt], lane,
+                                          scores[rt] ? scores[rt] + first : nullptr);
+        const LdsBytes at = (LdsBytes)s_v[buf] + (sub * 32 + q4 * 4 + (c16 >> 2)) * kValPitch + (c16 & 3) * 8;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const u32x2 lo = lds_read_transposed(at + t * 32), hi = lds_read_transposed(at + t * 32 + 16 * kValPitch);
+          const u32x4 vf{lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma<PT>(vf, pf[rt], o[rt][t]);
         }
       }
     }
+    if (tile + BT < end) {
+      store(p[1], tile + BT, buf ^ 1);
+      p[0] = p[1];
+      p[1] = walk.place(next_tok, next_page);
+      next_tok = walk.token(tile + 3 * BT, next2_entry);
+      next_page = walk.page(next_tok);
+      next2_entry = walk.entry(tile + 4 * BT);
+      if (tile + 2 * BT < end) load(p[1]);
+    }
     __syncthreads();
+  }
+  if (s_odd) add_odd_values<PT, FP8, NT, RT>(o, walk, vb, begin, end, base, seen, lane, 0, 1);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    st[rt].sum += __shfl_xor(st[rt].sum, 16);
+    st[rt].sum += __shfl_xor(st[rt].sum, 32);
+    const int m = m0 + rt * 16 + c16;
+    if (m >= M) continue;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) put_row<QT, D>(a, rows, b, h, split, m, t * 16 + q4 * 4, o[rt][t], st[rt].top, st[rt].sum);
   }
 }
 
-// Row tiles of an instance: as many as the rows of a KV head need, up to what the registers hold.
-template <int QT, bool FP8, int D>
+template <int QT, bool FP8, int D, bool UNI>
 hipError_t launch_attend_typed(const AttendLaunch& a, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv));
-  if (a.row_tiles == 1) hipLaunchKernelGGL((attend_kernel<QT, FP8, D, 1>), grid, dim3(kAttendThreads), 0, s, a);
-  else if (a.row_tiles == 2) hipLaunchKernelGGL((attend_kernel<QT, FP8, D, 2>), grid, dim3(kAttendThreads), 0, s, a);
+  const dim3 grid((unsigned)((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv)), block(kAttendThreads);
+  if (a.row_tiles == 0) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI>), grid, block, 0, s, a);
+  else if (a.row_tiles == 1) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 1, UNI>), grid, block, 0, s, a);
+  else if (a.row_tiles == 2) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 2, UNI>), grid, block, 0, s, a);
   else if constexpr (D <= 128) {
     if (a.row_tiles != 4) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((attend_kernel<QT, FP8, D, 4>), grid, dim3(kAttendThreads), 0, s, a);
+    hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 4, UNI>), grid, block, 0, s, a);
   } else return hipErrorInvalidValue;
   return hipGetLastError();
 }
 
-template <int D>
+template <int QT, int D>
 hipError_t launch_attend_dim(const AttendLaunch& a, hipStream_t s) {
-  const bool fp8 = a.kv_dtype == TRI_KV_FP8_E4M3;
-  if (a.q_dtype == TRI_KV_BF16) return fp8 ? launch_attend_typed<TRI_KV_BF16, true, D>(a, s) : launch_attend_typed<TRI_KV_BF16, false, D>(a, s);
-  return fp8 ? launch_attend_typed<TRI_KV_FP16, true, D>(a, s) : launch_attend_typed<TRI_KV_FP16, false, D>(a, s);
+  const bool uni = a.block_size % 16 == 0;
+  if (a.kv_dtype == TRI_KV_FP8_E4M3) return uni ? launch_attend_typed<QT, true, D, true>(a, s) : launch_attend_typed<QT, true, D, false>(a, s);
+  return uni ? launch_attend_typed<QT, false, D, true>(a, s) : launch_attend_typed<QT, false, D, false>(a, s);
 }
 
 }  // namespace

@@ -923,6 +923,9 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
     return fail(TRI_ERR_INVALID_ARGUMENT, "out_stride_head %lld < head_dim", (long long)p->out_stride_head);
   if (!is_finite(p->scale) || !is_finite(p->k_scale) || !is_finite(p->v_scale) || !is_finite(p->scale * p->k_scale * 1.44269504f))
     return fail(TRI_ERR_INVALID_ARGUMENT, "scale, k_scale and v_scale must be finite");
+  // (in-block offsets of the rows a wave reads together are 32-bit)
+  if (kv->stride_token < 0 || kv->stride_token >= (1 << 25))
+    return fail(TRI_ERR_UNSUPPORTED, "stride_token %lld", (long long)kv->stride_token);
   if (p->weight_mode != 0 && p->weight_mode != 1) return fail(TRI_ERR_INVALID_ARGUMENT, "weight_mode %d", p->weight_mode);
   if (bp) {
     if (p->row_starts || p->parents || p->weights)
@@ -943,6 +946,9 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
     a.k_scale_layers = kv->k_scale_layers;
     a.v_scale_layers = kv->v_scale_layers;
   }
+  a.div_shift = 31;
+  while ((1ll << (a.div_shift - 31)) < a.block_size) ++a.div_shift;
+  a.div_factor = (uint32_t)(((1ull << a.div_shift) + a.block_size - 1) / a.block_size);
   a.block_table = batch->block_table; a.block_table_pitch = batch->block_table_pitch; a.seq_lens = batch->seq_lens;
   a.q = p->q; a.q_stride_row = p->q_stride_row; a.q_stride_head = p->q_stride_head;
   a.out = p->out; a.out_stride_row = p->out_stride_row; a.out_stride_head = p->out_stride_head; a.lse = p->lse;
@@ -957,8 +963,8 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   int64_t total = 0;
   for (int b = 0; b < a.B; ++b) total += std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest);
   const int rows = a.max_rows * a.G;
-  a.row_tiles = rows <= 16 ? 1 : rows <= 32 || a.D == 256 ? 2 : 4;
-  a.row_blocks = tri::ceil_div(rows, 16 * a.row_tiles);
+  a.row_tiles = rows <= 16 ? 0 : rows <= 64 ? 1 : rows <= 128 || a.D == 256 ? 2 : 4;
+  a.row_blocks = a.row_tiles ? tri::ceil_div(rows, 64 * a.row_tiles) : 1;
   const int64_t per = tri::ceil_div64(total * a.Hkv * a.row_blocks, kAttendWorkgroups);
   a.split_tokens = (int)std::min<int64_t>(tri::align_up(std::max<int64_t>(per, 1), kAttendStep), tri::align_up(longest, kAttendStep));
   a.nsplit = (int)tri::ceil_div64(longest, a.split_tokens);
@@ -993,8 +999,7 @@ int do_attend(AttendPlan& d, void* ws, hipStream_t s) {
     a.part_out = at<float>(ws, d.part_out);
     a.part_ml = at<float>(ws, d.part_ml);
   }
-  int rc = launch_status(a.D == 64 ? tri::launch_attend_64(a, s) : a.D == 128 ? tri::launch_attend_128(a, s) : tri::launch_attend_256(a, s),
-                         "attend");
+  int rc = launch_status(tri::launch_attend(a, s), "attend");
   if (!rc && a.nsplit > 1) rc = launch_status(tri::launch_attend_join(a, s), "attend_join");
   return rc;
 }

@@ -256,6 +256,7 @@ hipError_t launch_dense_gather(const DenseLaunch& d, hipStream_t s);
 // Attention over one layer of the paged cache (tri_attend_device.h, tri_attend.hip).
 struct AttendLaunch {
   int B, Hkv, G, Hq, D, block_size, kv_dtype, q_dtype, layer, Tmax, num_blocks;
+  uint32_t div_factor; int div_shift;                      // division by block_size
   int64_t stride_block, stride_token, stride_head;         // elements
   const void* const* k_layers;
   const void* const* v_layers;
@@ -277,7 +278,7 @@ struct AttendLaunch {
   const int32_t* list;
   int list_k, list_pitch;
   // how the work is cut
-  int row_tiles, row_blocks, nsplit, split_tokens;
+  int row_tiles, row_blocks, nsplit, split_tokens;         // row_tiles 0: the kernel for up to 16 rows
   // workspace
   float* part_out;                                         // [B][Hkv][nsplit][max_rows * G][D], not normalised (nsplit > 1)
   float* part_ml;                                          // the same rows' maximum (base 2) and sum
@@ -285,9 +286,13 @@ struct AttendLaunch {
   float* scores;                                           // [B][Hkv][max_rows * G][score_pitch] base 2, or NULL
   int64_t score_pitch;
 };
-hipError_t launch_attend_64(const AttendLaunch& a, hipStream_t s);
-hipError_t launch_attend_128(const AttendLaunch& a, hipStream_t s);
-hipError_t launch_attend_256(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_64_bf16(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_64_fp16(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_128_bf16(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_128_fp16(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_256_bf16(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend_256_fp16(const AttendLaunch& a, hipStream_t s);
+hipError_t launch_attend(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_join(const AttendLaunch& a, hipStream_t s);
 // weights: the layer's [num_blocks][block_size][Hkv]; set: written, not added to.
 hipError_t launch_attend_weights(const AttendLaunch& a, float* weights, int set, hipStream_t s);
