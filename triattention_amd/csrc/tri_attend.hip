@@ -23,15 +23,31 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendLaunch a) {
   const int d = (threadIdx.x % kLanes) * 4;
   f32x4 v = {0.f, 0.f, 0.f, 0.f};
   float top = -INFINITY, total = 0.f;
-  for (int s = 0; s < live; ++s) {
-    const int64_t row = first + (int64_t)s * rows_max;
-    const f32x2 ml = *reinterpret_cast<const f32x2*>(a.part_ml + row * 2);
-    const f32x4 o = *reinterpret_cast<const f32x4*>(a.part_out + row * D + d);
-    const float now = fmaxf(top, ml[0]);
-    const float old_f = rescale(top, now), new_f = rescale(ml[0], now);
-    v = v * old_f + o * new_f;
-    total = total * old_f + ml[1] * new_f;
+  constexpr int kAtOnce = 8;                 // splits asked for together
+  for (int s0 = 0; s0 < live; s0 += kAtOnce) {
+    f32x2 ml[kAtOnce];
+    f32x4 o[kAtOnce];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int64_t row = first + (int64_t)min(s0 + u, live - 1) * rows_max;
+      ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + row * 2);
+      o[u] = *reinterpret_cast<const f32x4*>(a.part_out + row * D + d);
+    }
+    float now = top;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) now = fmaxf(now, ml[u][0]);
+    const float old_f = rescale(top, now);
+    v *= old_f;
+    total *= old_f;
     top = now;
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      const float f = s0 + u < live ? rescale(ml[u][0], now) : 0.f;
+      if (f != 0.f) {
+        v += o[u] * f;
+        total += ml[u][1] * f;
+      }
+    }
   }
   const int64_t i = rows.first + m / a.G;
   const int hq = h * a.G + m % a.G;
@@ -46,32 +62,52 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendLaunch a) {
 }
 
 // weight[token][head] (+)= sum over the rows of the head of 2^(s - lse): every token and head by one thread, rows in order.
-// A lane is a token (the scores lie token by token), a wave takes every fourth head; the four bytes a lane writes are
-// joined with those of the other heads in L2.
+// A lane is a token (the scores lie token by token), a wave takes four heads, whose weights it reads and writes as one
+// piece (VEC).  Reads a score once, weights once, writes them once.
+template <bool VEC>
 __global__ __launch_bounds__(256) void attend_weights_kernel(AttendLaunch a, float* weights, int set) {
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int chunks = ceil_div(a.Tmax, kWave);
-  const int b = blockIdx.x / chunks;
+  const int lane = threadIdx.x % kWave;
+  const int quads = ceil_div(a.Hkv, 4), chunks = ceil_div(a.Tmax, kWave);
+  int64_t unit = (int64_t)blockIdx.x * (256 / kWave) + threadIdx.x / kWave;
+  const int h0 = (int)(unit % quads) * 4;
+  unit /= quads;
+  const int t = (int)(unit % chunks) * kWave + lane;
+  const int64_t b = unit / chunks;
+  if (b >= a.B) return;
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
-  const int t = blockIdx.x % chunks * kWave + lane;
   if (t >= T) return;
-  const RowRange rows = rows_of(a, b);
-  const int page = a.block_table ? a.block_table[(int64_t)b * a.block_table_pitch + t / a.block_size] : b;
+  const RowRange rows = rows_of(a, (int)b);
+  const int page = a.block_table ? a.block_table[b * a.block_table_pitch + t / a.block_size] : (int)b;
   if (page < 0 || page >= a.num_blocks) return;
-  float* const w = weights + ((int64_t)page * a.block_size + t % a.block_size) * a.Hkv;
+  float* const w = weights + ((int64_t)page * a.block_size + t % a.block_size) * a.Hkv + h0;
   const bool fresh = set || t >= T - rows.n;      // the rows' own tokens: nothing has been added for them yet
-  for (int h = wave; h < a.Hkv; h += 4) {
-    const float* s = a.scores + ((int64_t)b * a.Hkv + h) * a.max_rows * a.G * a.score_pitch + t;
-    float sum = 0.f;
-    for (int i = 0; i < rows.n; ++i) {
-      const float* lse = a.lse2 + (int64_t)(rows.first + i) * a.Hq + h * a.G;
-      for (int g = 0; g < a.G; ++g) {
-        const float l = lse[g];
-        if (l != -INFINITY) sum += pow2(s[(int64_t)(i * a.G + g) * a.score_pitch] - l);
+  f32x4 had = {0.f, 0.f, 0.f, 0.f};
+  if (!fresh) {
+    if (VEC) had = *reinterpret_cast<const f32x4*>(w);
+    else
+      for (int e = 0; e < 4; ++e) had[e] = h0 + e < a.Hkv ? w[e] : 0.f;
+  }
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  const int64_t per_head = (int64_t)a.max_rows * a.G * a.score_pitch;
+  const float* s = a.scores + (b * a.Hkv + h0) * per_head + t;
+  for (int i = 0; i < rows.n; ++i) {
+    const float* lse = a.lse2 + (int64_t)(rows.first + i) * a.Hq + h0 * a.G;
+#pragma unroll 4
+    for (int g = 0; g < a.G; ++g) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int ee = VEC ? e : min(e, a.Hkv - 1 - h0);
+        const float l = lse[ee * a.G + g];
+        // (a row without tokens, lse -inf: nothing)
+        sum[e] += pow2(s[ee * per_head + (int64_t)(i * a.G + g) * a.score_pitch] - (l == -INFINITY ? INFINITY : l));
       }
     }
-    w[h] = fresh ? sum : w[h] + sum;
   }
+  sum += had;
+  if (VEC) *reinterpret_cast<f32x4*>(w) = sum;
+  else
+    for (int e = 0; e < 4; ++e)
+      if (h0 + e < a.Hkv) w[e] = sum[e];
 }
 
 template <int QT>
@@ -100,7 +136,12 @@ hipError_t launch_attend_join(const AttendLaunch& a, hipStream_t s) {
 }
 
 hipError_t launch_attend_weights(const AttendLaunch& a, float* weights, int set, hipStream_t s) {
-  hipLaunchKernelGGL(attend_weights_kernel, dim3((unsigned)((int64_t)ceil_div(a.Tmax, kWave) * a.B)), dim3(256), 0, s, a, weights, set);
+  const int64_t waves = (int64_t)a.B * ceil_div(a.Tmax, kWave) * ceil_div(a.Hkv, 4);
+  const dim3 grid((unsigned)ceil_div64(waves, 256 / kWave));
+  if (a.Hkv % 4 == 0 && reinterpret_cast<uintptr_t>(weights) % 16 == 0)
+    hipLaunchKernelGGL(attend_weights_kernel<true>, grid, dim3(256), 0, s, a, weights, set);
+  else
+    hipLaunchKernelGGL(attend_weights_kernel<false>, grid, dim3(256), 0, s, a, weights, set);
   return hipGetLastError();
 }
 

@@ -20,6 +20,8 @@
 // splits where there are few rows, joined by attend_join_kernel.
 #pragma once
 
+#include <type_traits>
+
 #include "tri_common.h"
 #include "tri_mma_device.h"
 #include "tri_score_device.h"
@@ -162,10 +164,11 @@ __device__ __forceinline__ int tokens_of(const AttendLaunch& a, int b, int T) {
   return min(a.list_k, ceil_div(T, a.block_size)) * a.block_size;
 }
 
-// Places of tokens: a lane holds one token of a tile -- list entry, then page, then byte offset, each asked for a tile ahead
-// of the next (a wait for a young load would be a wait for every older one).
+// Places of tokens: a lane holds one token of a tile -- list entry, then page, then row, each asked for a tile ahead of the
+// next (a wait for a young load would be a wait for every older one).  The loads themselves are never skipped: where
+// one path has fewer of them, every wait behind it would be for all.
 struct Place {
-  int64_t byte, row;     // offset of the row, index of its scale; 0 for a token that is not there
+  int page, in;          // physical block and token in it; 0 and 0 for a token that is not there
   bool ok;
 };
 template <int ES>
@@ -175,46 +178,49 @@ struct Walk {
   const int32_t* list;
   int b, T, end, mine;
   __device__ __forceinline__ Walk(const AttendLaunch& a_, int b_, int h, int T_, int end_, int mine_) : a(a_), b(b_), T(T_), end(end_), mine(mine_) {
-    table = a.block_table ? a.block_table + (int64_t)b * a.block_table_pitch : nullptr;
+    table = a.block_table ? a.block_table + (int64_t)b * a.block_table_pitch : a.seq_lens;      // (any readable word where there is no table)
     list = a.list ? a.list + ((int64_t)b * a.Hkv + h) * a.list_pitch : nullptr;
   }
   // (t >= 0; exact below 2^31: the factor is 2^div_shift / block_size rounded up, div_shift = 31 + log2 block_size rounded up)
   __device__ __forceinline__ int div(int t) const { return (int)((uint64_t)(uint32_t)t * a.div_factor >> a.div_shift); }
   __device__ __forceinline__ int mod(int t) const { return t - div(t) * a.block_size; }
   __device__ __forceinline__ int entry(int tile) const {
+    if (!list) return 0;
     const int t = tile + mine;
-    return list && t < end ? list[div(t)] : 0;
+    return list[t < end ? div(t) : 0];
   }
   __device__ __forceinline__ int token(int tile, int entry) const {     // position in the sequence, or -1
     const int t = tile + mine;
     const int tok = list ? entry * a.block_size + mod(t) : t;
-    return t < end && entry >= 0 && tok < T ? tok : -1;
+    return ((t < end) & (entry >= 0) & (tok < T)) ? tok : -1;
   }
   __device__ __forceinline__ int page(int tok) const {
-    if (tok < 0) return -1;
-    return table ? table[div(tok)] : b;
+    const int p = table[a.block_table ? div(max(tok, 0)) : 0];
+    return a.block_table ? p : b;
   }
   __device__ __forceinline__ Place place(int tok, int page) const {
     Place p;
-    p.ok = tok >= 0 && page >= 0 && page < a.num_blocks;
-    const int in = p.ok ? mod(tok) : 0;
-    const int64_t pg = p.ok ? page : 0;
-    p.byte = (pg * a.stride_block + (int64_t)in * a.stride_token) * ES;
-    p.row = (pg * a.block_size + in) * a.Hkv;
+    p.ok = (tok >= 0) & ((uint32_t)page < (uint32_t)a.num_blocks);
+    p.page = p.ok ? page : 0;
+    p.in = p.ok ? mod(tok) : 0;
     return p;
   }
+  __device__ __forceinline__ uint64_t byte(int page, int in) const {
+    return ((uint64_t)(uint32_t)page * (uint64_t)a.stride_block + (uint64_t)(uint32_t)in * (uint32_t)a.stride_token) * ES;
+  }
+  __device__ __forceinline__ int64_t scale_at(const Place& p) const { return ((int64_t)p.page * a.block_size + p.in) * a.Hkv; }
 };
 
-// Address of row `row` of a tile (lane row holds its place).  UNI: blocks of a multiple of 16 tokens, so that 16 tokens
+// Address of row `row` of a tile (lane `row` holds its place).  UNI: blocks of a multiple of 16 tokens, so that 16 tokens
 // in a row lie behind one another and their base is the same for the wave (row0: the first of the 16 that this
-// load takes rows of; it must be a constant).
+// load takes rows of, the same for the wave).
 template <bool UNI, int ES>
-__device__ __forceinline__ const char* row_at(const char* base, int64_t byte, int row0, int row, int64_t stride_token) {
+__device__ __forceinline__ GlobalBytes row_at(const Walk<ES>& walk, GlobalBytes base, const Place& p, int row0, int row) {
   if constexpr (UNI) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)byte, row0), hi = __builtin_amdgcn_readlane((int)(byte >> 32), row0);
-    return base + (int64_t)((uint64_t)hi << 32 | lo) + (uint32_t)((row - row0) * (int)stride_token * ES);
+    const int page = __builtin_amdgcn_readlane(p.page, row0), in = __builtin_amdgcn_readlane(p.in, row0);
+    return base + walk.byte(page, in) + (uint32_t)((row - row0) * (int)walk.a.stride_token * ES);
   } else {
-    return base + shfl64(byte, row);
+    return base + walk.byte(__shfl(p.page, row), __shfl(p.in, row));
   }
 }
 
@@ -235,14 +241,14 @@ __device__ __forceinline__ void load_queries(const AttendLaunch& a, const RowRan
 // product would put them into all of them, so there they are 0): rare, at the end, read from memory again.  Tokens from
 // first_tok to end of which every step-th piece of 32, from the piece-th on, is the caller's.
 template <int PT, bool FP8, int NT, int RT, int ES>
-__device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Walk<ES>& walk, const char* vb, int begin, int end, int base,
+__device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Walk<ES>& walk, GlobalBytes vb, int begin, int end, int base,
                                                const uint64_t (&seen)[RT], int lane, int piece, int step) {
 #pragma unroll 1
   for (int tok = max(begin, base); tok < end; ++tok) {
     if ((tok - begin) / kAttendTile % step != piece) continue;
     const Place p = walk.place(tok, walk.page(tok));
     if (!p.ok) continue;
-    const char* row = vb + p.byte;
+    const GlobalBytes row = vb + walk.byte(p.page, p.in);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -250,7 +256,7 @@ __device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Walk<ES
         const int d = t * 16 + (lane >> 4) * 4 + e;
         float v;
         if constexpr (FP8) v = __builtin_amdgcn_cvt_f32_fp8((int)(uint8_t)row[d], 0);
-        else v = Half<PT>::value(*reinterpret_cast<const uint16_t*>(row + d * ES));
+        else v = Half<PT>::value(*(const __attribute__((address_space(1))) uint16_t*)(row + d * ES));
         if (!(v - v == 0.f)) {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
@@ -350,7 +356,7 @@ __device__ __forceinline__ u32x4 softmax32(f32x4 (&sc)[2], RowState& st, f32x4 (
 
 // ---- up to 16 rows of a KV head
 template <int QT, bool FP8, int D, bool UNI>
-__global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 3) void attend_few_kernel(AttendLaunch a) {
+__global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) void attend_few_kernel(AttendLaunch a) {
   constexpr int PT = FP8 ? TRI_KV_BF16 : QT;              // fp8 rows with a scale of their own: the weight carries it, which fp16 has no room for
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int KC = D * ES / 64;                         // 16-byte pieces of a key in a lane
@@ -380,50 +386,40 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 3) void attend_few_k
   const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
   if (begin >= Tv && split > 0) return;
   const int base = T - n;                                 // first new token (negative: not all of them are in the cache)
-  const char* kb = reinterpret_cast<const char*>(a.k_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
-  const char* vb = reinterpret_cast<const char*>(a.v_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
+  const GlobalBytes kb = (GlobalBytes)a.k_layers[a.layer] + (int64_t)h * a.stride_head * ES;
+  const GlobalBytes vb = (GlobalBytes)a.v_layers[a.layer] + (int64_t)h * a.stride_head * ES;
   const bool scaled = FP8 && a.k_scale_layers;
-  const float* ksc = scaled ? a.k_scale_layers[a.layer] + h : nullptr;
-  const float* vsc = scaled ? a.v_scale_layers[a.layer] + h : nullptr;
+  const GlobalF32 ksc = scaled ? (GlobalF32)a.k_scale_layers[a.layer] + h : nullptr;
+  const GlobalF32 vsc = scaled ? (GlobalF32)a.v_scale_layers[a.layer] + h : nullptr;
+
+  // (the queries first: the loop's first wait for them is then none for the keys and values behind them)
+  u32x4 qf[D / 32];
+  load_queries<FP8, D>(a, rows, h, 0, M, lane, qf);
+  uint64_t seen[1] = {1};
+  if (n > 1) seen[0] = (uint64_t)shfl64((int64_t)ancestor_mask(a.parents, rows.first, n, lane), min(c16, M - 1) / a.G);
 
   const Walk<ES> walk(a, b, h, T, end, lane & (kAttendTile - 1));
   const int first_tile = begin + wave * kAttendTile;
   u32x4 kr[2][KC], vr[NV];
   float ks_mine = 0.f, vs_mine = 0.f;
   auto load_keys = [&](const Place& p) {
+    if (scaled) {
+      ks_mine = ksc[walk.scale_at(p)];
+      vs_mine = vsc[walk.scale_at(p)];
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const char* src = row_at<UNI, ES>(kb, p.byte, i * 16, i * 16 + c16, a.stride_token) + q4 * 16;
+      const GlobalBytes src = row_at<UNI, ES>(walk, kb, p, i * 16, i * 16 + c16) + q4 * 16;
 #pragma unroll
-      for (int c = 0; c < KC; ++c) kr[i][c] = *reinterpret_cast<const u32x4*>(src + c * 64);
-    }
-    if (scaled) {
-      ks_mine = ksc[p.row];
-      vs_mine = vsc[p.row];
+      for (int c = 0; c < KC; ++c) kr[i][c] = *(GlobalU4)(src + c * 64);
     }
   };
   auto load_values = [&](const Place& p) {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      vr[i] = *reinterpret_cast<const u32x4*>(row_at<UNI, ES>(vb, p.byte, i * RPL / 16 * 16, i * RPL + lane / LPR, a.stride_token) + (lane % LPR) * 16);
+      vr[i] = *(GlobalU4)(row_at<UNI, ES>(walk, vb, p, i * RPL / 16 * 16, i * RPL + lane / LPR) + (lane % LPR) * 16);
   };
 
-  Place now{}, next{};
-  int next_tok = -1, next_page = -1, next2_entry = 0;
-  if (first_tile < end) {
-    const int tok = walk.token(first_tile, walk.entry(first_tile));
-    next_tok = walk.token(first_tile + kStep, walk.entry(first_tile + kStep));
-    const int page = walk.page(tok);
-    next_page = walk.page(next_tok);
-    next2_entry = walk.entry(first_tile + 2 * kStep);
-    now = walk.place(tok, page);
-    load_keys(now);
-    load_values(now);
-  }
-  u32x4 qf[D / 32];
-  load_queries<FP8, D>(a, rows, h, 0, M, lane, qf);
-  uint64_t seen[1] = {1};
-  if (n > 1) seen[0] = (uint64_t)shfl64((int64_t)ancestor_mask(a.parents, rows.first, n, lane), min(c16, M - 1) / a.G);
   float* const scores = a.scores && c16 < M ? a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + c16) * a.score_pitch + q4 * 4 : nullptr;
 
   f32x4 o[1][NT];
@@ -433,8 +429,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 3) void attend_few_k
   for (int t = 0; t < NT; ++t) o[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   unsigned char* const my_v = s_v + wave * kWaveBytes;
   const LdsBytes my_lds = (LdsBytes)my_v + (q4 * 4 + (c16 >> 2)) * kPitch + (c16 & 3) * 8;
-  for (int tile = first_tile; tile < end; tile += kStep) {
-    const bool more = tile + kStep < end;
+  Place now{}, next{};
+  int next_tok = -1, next_page = -1, next2_entry = 0;
+  // One tile; the last one has no next (a body of its own: see the loads above).
+  auto step = [&](int tile, auto has_next) {
+    constexpr bool more = decltype(has_next)::value;
     const uint32_t okm = (uint32_t)__ballot(now.ok);
     const bool drafts = n > 1 && tile + kAttendTile > base;
 
@@ -459,7 +458,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 3) void attend_few_k
     }
     __builtin_amdgcn_sched_barrier(0);
     // the next tile's keys into the registers of this one's, this one's values into LDS
-    if (more) {
+    if constexpr (more) {
       next = walk.place(next_tok, next_page);
       next_tok = walk.token(tile + 2 * kStep, next2_entry);
       next_page = walk.page(next_tok);
@@ -486,7 +485,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 3) void attend_few_k
         dst[0] = vr[i];
       }
     }
-    if (more) load_values(next);
+    if constexpr (more) load_values(next);
     __builtin_amdgcn_sched_barrier(0);
     const bool masked = okm != 0xffffffffu || drafts;
     u32x4 pf;
@@ -510,6 +509,22 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : 3) void attend_few_k
     }
     __builtin_amdgcn_wave_barrier();
     now = next;
+  };
+  if (first_tile < end) {
+    const int tok = walk.token(first_tile, walk.entry(first_tile));
+    next_tok = walk.token(first_tile + kStep, walk.entry(first_tile + kStep));
+    const int page = walk.page(tok);
+    next_page = walk.page(next_tok);
+    next2_entry = walk.entry(first_tile + 2 * kStep);
+    __builtin_amdgcn_sched_barrier(0);
+    now = walk.place(tok, page);
+    load_keys(now);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(now);
+    __builtin_amdgcn_sched_barrier(0);
+    int tile = first_tile;
+    for (; tile + kStep < end; tile += kStep) step(tile, std::true_type{});
+    if (tile < end) step(tile, std::false_type{});
   }
   if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, walk, vb, begin, end, base, seen, lane, wave, kAttendWaves);
 
@@ -581,11 +596,11 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
   const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
   if (begin >= Tv && split > 0) return;
   const int base = T - n;
-  const char* kb = reinterpret_cast<const char*>(a.k_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
-  const char* vb = reinterpret_cast<const char*>(a.v_layers[a.layer]) + (int64_t)h * a.stride_head * ES;
+  const GlobalBytes kb = (GlobalBytes)a.k_layers[a.layer] + (int64_t)h * a.stride_head * ES;
+  const GlobalBytes vb = (GlobalBytes)a.v_layers[a.layer] + (int64_t)h * a.stride_head * ES;
   const bool scaled = FP8 && a.k_scale_layers;
-  const float* ksc = scaled ? a.k_scale_layers[a.layer] + h : nullptr;
-  const float* vsc = scaled ? a.v_scale_layers[a.layer] + h : nullptr;
+  const GlobalF32 ksc = scaled ? (GlobalF32)a.k_scale_layers[a.layer] + h : nullptr;
+  const GlobalF32 vsc = scaled ? (GlobalF32)a.v_scale_layers[a.layer] + h : nullptr;
 
   const Walk<ES> walk(a, b, h, T, end, lane & (BT - 1));
   u32x4 kr[NL], vr[NL];
@@ -596,14 +611,14 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
     for (int i = 0; i < NL; ++i) {
       // (rows of this load: 16-row group i * 4 * RPL + wave * RPL lies in, the same for the whole wave)
       const int row0 = (i * kAttendWaves + wave) * RPL;
-      const char* k = row_at<UNI, ES>(kb, at.byte, row0 / 16 * 16, row0 + lane / LPR, a.stride_token) + (lane % LPR) * 16;
-      const char* v = row_at<UNI, ES>(vb, at.byte, row0 / 16 * 16, row0 + lane / LPR, a.stride_token) + (lane % LPR) * 16;
-      kr[i] = *reinterpret_cast<const u32x4*>(k);
-      vr[i] = *reinterpret_cast<const u32x4*>(v);
+      const GlobalBytes k = row_at<UNI, ES>(walk, kb, at, row0 / 16 * 16, row0 + lane / LPR) + (lane % LPR) * 16;
+      const GlobalBytes v = row_at<UNI, ES>(walk, vb, at, row0 / 16 * 16, row0 + lane / LPR) + (lane % LPR) * 16;
+      kr[i] = *(GlobalU4)k;
+      vr[i] = *(GlobalU4)v;
     }
     if (scaled && wave == 0) {
-      ks_mine = ksc[at.row];
-      vs_mine = vsc[at.row];
+      ks_mine = ksc[walk.scale_at(at)];
+      vs_mine = vsc[walk.scale_at(at)];
     }
   };
   auto store = [&](const Place& at, int tile, int buf) {

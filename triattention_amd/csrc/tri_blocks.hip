@@ -105,8 +105,10 @@ __device__ __forceinline__ double dpp64(double v) {
 constexpr int kScoreBlocks = 64;       // blocks of a (sequence, KV head) per workgroup
 constexpr int kHeadsAtOnce = 4;
 
-// D / 8 lanes a block, 8 elements each, the queries of up to four heads in registers.  Products are exact in 32 bits, sums are
-// 64-bit: which blocks are read must not depend on the order of a sum.
+// D / 8 lanes a block, 8 elements each, the queries of up to four heads in registers: a positive element of a query meets the
+// largest key, a negative one the least.  Products and sums are 64-bit: which blocks are read must not depend on the
+// order of a sum.  Bound by reading the bounds and, from four heads on, by the 64-bit products of every head
+// (selection, conversion and product are three instructions an element).
 template <int BT, int QT, int D>
 __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreLaunch a) {
   constexpr int LPB = D / 8, kBlocks = 256 / LPB;
@@ -131,12 +133,19 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreLaunch a) {
 #pragma unroll
   for (int i = 0; i < kScoreBlocks / kBlocks; ++i) { best[i] = -INFINITY; total[i] = 0.; }
   for (int g0 = 0; g0 < a.G; g0 += kHeadsAtOnce) {
-    float q[kHeadsAtOnce][8];
+    float q[8];
+    double q64[kHeadsAtOnce][8];
+    bool up[kHeadsAtOnce][8];
 #pragma unroll
     for (int g = 0; g < kHeadsAtOnce; ++g) {
       const int gg = min(g0 + g, a.G - 1);
       const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)b * a.q_stride_row + (int64_t)(h * a.G + gg) * a.q_stride_head + sub * 8;
-      unpack8<QT>(*reinterpret_cast<const uint4*>(src), q[g]);
+      unpack8<QT>(*reinterpret_cast<const uint4*>(src), q);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        q64[g][e] = (double)q[e];
+        up[g][e] = q[e] > 0.f;
+      }
     }
 #pragma unroll
     for (int i = 0; i < kScoreBlocks / kBlocks; ++i) {
@@ -152,7 +161,7 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreLaunch a) {
       for (int g = 0; g < kHeadsAtOnce; ++g) {
         double s = 0.;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s += (double)high_of(q[g][e] * low[e], q[g][e] * high[e]);
+        for (int e = 0; e < 8; ++e) s = __builtin_fma(q64[g][e], (double)(up[g][e] ? high[e] : low[e]), s);
         s += dpp64<kDppXor1>(s);
         s += dpp64<kDppXor2>(s);
         s += dpp64<kDppHalfMirror>(s);

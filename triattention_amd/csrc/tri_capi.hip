@@ -971,7 +971,7 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = tri::align_up(off + bytes, 256); return o; };
   const int64_t parts = a.nsplit > 1 ? (int64_t)a.B * a.Hkv * a.nsplit * rows : 0;
-  if ((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) > INT_MAX ||
+  if ((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) * tri::ceil_div(a.Hkv, 4) > INT_MAX ||
       (int64_t)a.B * a.Hkv * rows > INT_MAX)
     return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d rows and %d KV heads in one call", a.B, a.max_rows, a.Hkv);
   a.score_pitch = tri::align_up(a.Tmax, 32);
@@ -1017,7 +1017,7 @@ int fill_evict(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_
   if (kv->num_layers > 1 && p->weights_stride_layer < (int64_t)p->num_blocks * kv->block_size * kv->num_kv_heads)
     return fail(TRI_ERR_INVALID_ARGUMENT, "weights_stride_layer %lld is less than a layer", (long long)p->weights_stride_layer);
   const int64_t width = std::max(batch->max_seq_len, batch->max_budget);
-  if (tri::ceil_div64(width * kv->num_kv_heads, 256) * batch->num_seqs * kv->num_layers > INT_MAX)
+  if (tri::ceil_div64(width, 256) * tri::ceil_div(kv->num_kv_heads, 4) * batch->num_seqs * kv->num_layers > INT_MAX)
     return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d layers in one call", batch->num_seqs, batch->max_seq_len, kv->num_layers);
   a.B = batch->num_seqs; a.L = kv->num_layers; a.Hkv = kv->num_kv_heads; a.block_size = kv->block_size;
   a.Tmax = batch->max_seq_len; a.max_budget = batch->max_budget; a.num_blocks = p->num_blocks;
