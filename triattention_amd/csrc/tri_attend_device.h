@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / kWave;
+constexpr int kDies = 8;
 constexpr int kAttendTile = 32;       // tokens of one product with V
 
 template <int T>
@@ -156,6 +157,30 @@ __device__ __forceinline__ RowRange rows_of(const AttendLaunch& a, int b) {
   first = min(max(first, 0), a.num_rows);
   end = min(max(end, first), a.num_rows);
   return {first, min(end - first, a.max_rows)};
+}
+
+// What a workgroup works on: a split of a sequence (the unit), one KV head and block of rows of it (inner).  Workgroups go to the
+// eight dies in turn; with by_xcd all inner ones of a unit go to one of them, where they find the unit's pages in its
+// translation cache and, the blocks of rows, its K and V in L2.
+struct Work {
+  int b, split, h, rb;
+};
+__device__ __forceinline__ bool work_of(const AttendLaunch& a, Work& w) {
+  const int inner_n = a.Hkv * a.row_blocks;
+  int unit, inner;
+  if (a.by_xcd) {
+    const int l = blockIdx.x / kDies;
+    inner = l % inner_n;
+    unit = l / inner_n * kDies + blockIdx.x % kDies;
+  } else {
+    inner = blockIdx.x % inner_n;
+    unit = blockIdx.x / inner_n;
+  }
+  w.h = inner % a.Hkv;
+  w.rb = inner / a.Hkv;
+  w.split = unit % a.nsplit;
+  w.b = unit / a.nsplit;
+  return w.b < a.B;
 }
 
 // Tokens the call reads of a sequence, in the order it reads them: its cache, or the blocks of its list one after the other.
@@ -294,64 +319,85 @@ __device__ __forceinline__ void put_row(const AttendLaunch& a, const RowRange& r
   }
 }
 
-// The softmax of 32 tokens of one row a lane: sc holds q . k of tokens (i * 16 + (lane >> 4) * 4 + r) and becomes the weights
-// 2^(x - top); returns them packed for the product with V, which vs scales (fp8 rows with scales of their own).
-// The weights are rounded to 16 bits there while the sum adds them unrounded: errors of half a step each and of either
-// sign, below the one rounding of the output.
+// Running maximum (base 2, behind the true one by at most kSlack) and sum of a row.
 struct RowState {
   float top, sum;
 };
-template <int PT, bool SCALED, int NT>
-__device__ __forceinline__ u32x4 softmax32(f32x4 (&sc)[2], RowState& st, f32x4 (&o)[NT], float scale, const f32x4 (&ks)[2], const f32x4 (&vs)[2],
-                                           bool masked, bool drafts, uint32_t okm, int first, uint64_t seen, int lane, float* scores) {
-  float best = -INFINITY;
+// How far a score may lie above the maximum that weights are taken against before O is rescaled: weights stay below 2^8, far
+// inside either type, and a rescaling (a read and a write of all of O) is rare after the first tokens, where a new maximum is not.
+constexpr float kSlack = 8.f;
+
+// Which of 32 tokens a row sees (bit j: token first + j counted from the first new one): those that are there and, of the new
+// ones, itself and its ancestors.
+__device__ __forceinline__ uint32_t seen_of(uint32_t okm, bool drafts, int first, uint64_t seen) {
+  if (!drafts) return okm;
+  return okm & (first >= 0 ? (uint32_t)(seen >> (first & 63)) : (uint32_t)(seen << (-first & 63)) | ((1u << (-first & 31)) - 1));
+}
+
+// The softmax of 32 tokens for RT rows a lane: sc holds q . k of tokens i * 16 + (lane >> 4) * 4 + r; pf receives the weights
+// 2^(x - top) packed for the product with V (vs scales them: fp8 rows with scales of their own).  They are rounded to 16 bits
+// there while the sum adds them unrounded: errors of half a step each and of either sign, below the one rounding of the output.
+template <int PT, bool SCALED, int RT, int NT>
+__device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT], f32x4 (&o)[RT][NT], u32x4 (&pf)[RT], float scale,
+                                          const f32x4 (&ks)[2], const f32x4 (&vs)[2], bool masked, bool drafts, uint32_t okm, int first,
+                                          const uint64_t (&seen)[RT], int lane, float* const (&scores)[RT], int at) {
+  float best[RT];
+  bool grows = false;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) sc[i] *= SCALED ? ks[i] : f32x4{scale, scale, scale, scale};
-  if (masked) {
-    const int l = here(lane);
+  for (int rt = 0; rt < RT; ++rt) {
+    if (SCALED) {
+      sc[rt][0] *= ks[0];
+      sc[rt][1] *= ks[1];
+    }
+    if (masked) {
+      const uint32_t vis = seen_of(okm, drafts, first, seen[rt]) >> (here(lane) >> 4) * 4;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[rt][i][r] = vis >> (i * 16 + r) & 1 ? sc[rt][i][r] : -INFINITY;
+    }
+    best[rt] = fmaxf(fmaxf(fmaxf(sc[rt][0][0], sc[rt][0][1]), fmaxf(sc[rt][0][2], sc[rt][0][3])),
+                     fmaxf(fmaxf(sc[rt][1][0], sc[rt][1][1]), fmaxf(sc[rt][1][2], sc[rt][1][3])));
+    if (scores[rt]) {
+      *reinterpret_cast<f32x4*>(scores[rt] + at) = sc[rt][0] * scale;
+      *reinterpret_cast<f32x4*>(scores[rt] + at + 16) = sc[rt][1] * scale;
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) best[rt] = fmaxf(best[rt], __shfl_xor(best[rt], 16));
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    best[rt] = fmaxf(best[rt], __shfl_xor(best[rt], 32)) * scale;
+    grows |= best[rt] > st[rt].top + kSlack;
+  }
+  if (__ballot(grows)) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float top = best[rt] > st[rt].top + kSlack ? best[rt] : st[rt].top;
+      const float alpha = rescale(st[rt].top, top);
+      st[rt].top = top;
+      st[rt].sum *= alpha;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[rt][t] *= alpha;
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float down = st[rt].top == -INFINITY ? 0.f : -st[rt].top;
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int j = i * 16 + (l >> 4) * 4 + r, d = first + j;
-        const bool sees = (okm >> j & 1) && (!drafts || d < 0 || (seen >> (d & 63) & 1));
-        sc[i][r] = sees ? sc[i][r] : -INFINITY;
+        sc[rt][i][r] = pow2(__builtin_fmaf(sc[rt][i][r], scale, down));
+        part += sc[rt][i][r];
       }
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) best = fmaxf(best, sc[i][r]);
-  if (scores) {
-    *reinterpret_cast<f32x4*>(scores) = sc[0];
-    *reinterpret_cast<f32x4*>(scores + 16) = sc[1];
-  }
-  best = fmaxf(best, __shfl_xor(best, 16));
-  best = fmaxf(best, __shfl_xor(best, 32));
-  if (__ballot(best > st.top)) {
-    const float top = fmaxf(st.top, best);
-    const float alpha = rescale(st.top, top);
-    st.top = top;
-    st.sum *= alpha;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) o[t] *= alpha;
-  }
-  const float safe = st.top == -INFINITY ? 0.f : st.top;
-  float part = 0.f;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      sc[i][r] = pow2(sc[i][r] - safe);
-      part += sc[i][r];
+      if (SCALED) sc[rt][i] *= vs[i];
     }
-  st.sum += part;
-  if (SCALED) {
-    sc[0] *= vs[0];
-    sc[1] *= vs[1];
+    st[rt].sum += part;
+    pf[rt] = u32x4{Half<PT>::pack(sc[rt][0][0], sc[rt][0][1]), Half<PT>::pack(sc[rt][0][2], sc[rt][0][3]),
+                   Half<PT>::pack(sc[rt][1][0], sc[rt][1][1]), Half<PT>::pack(sc[rt][1][2], sc[rt][1][3])};
   }
-  return u32x4{Half<PT>::pack(sc[0][0], sc[0][1]), Half<PT>::pack(sc[0][2], sc[0][3]), Half<PT>::pack(sc[1][0], sc[1][1]),
-               Half<PT>::pack(sc[1][2], sc[1][3])};
 }
 
 // ---- up to 16 rows of a KV head
@@ -373,10 +419,9 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c16 = lane & 15, q4 = lane >> 4;
-  int idx = blockIdx.x;
-  const int h = idx % a.Hkv; idx /= a.Hkv;
-  const int split = idx % a.nsplit;
-  const int b = idx / a.nsplit;
+  Work work;
+  if (!work_of(a, work)) return;
+  const int b = work.b, split = work.split, h = work.h;
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   const RowRange rows = rows_of(a, b);
@@ -420,11 +465,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
       vr[i] = *(GlobalU4)(row_at<UNI, ES>(walk, vb, p, i * RPL / 16 * 16, i * RPL + lane / LPR) + (lane % LPR) * 16);
   };
 
-  float* const scores = a.scores && c16 < M ? a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + c16) * a.score_pitch + q4 * 4 : nullptr;
+  float* const scores[1] = {a.scores && c16 < M ? a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + c16) * a.score_pitch + q4 * 4 : nullptr};
 
   f32x4 o[1][NT];
   bool odd = false;
-  RowState st{-INFINITY, 0.f};
+  RowState st[1] = {{-INFINITY, 0.f}};
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   unsigned char* const my_v = s_v + wave * kWaveBytes;
@@ -437,10 +482,10 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     const uint32_t okm = (uint32_t)__ballot(now.ok);
     const bool drafts = n > 1 && tile + kAttendTile > base;
 
-    f32x4 sc[2];
+    f32x4 sc[1][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      sc[0][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < D / 32; ++s) {
         u32x4 kf;
@@ -449,11 +494,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
         } else {
           kf = kr[i][s];
         }
-        sc[i] = mfma<QT>(kf, qf[s], sc[i]);
+        sc[0][i] = mfma<QT>(kf, qf[s], sc[0][i]);
       }
     }
     if (scaled && lane < kAttendTile) {
-      s_scale[wave][0][lane] = ks_mine * a.scale_log2;
+      s_scale[wave][0][lane] = ks_mine;
       s_scale[wave][1][lane] = vs_mine;
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -488,7 +533,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     if constexpr (more) load_values(next);
     __builtin_amdgcn_sched_barrier(0);
     const bool masked = okm != 0xffffffffu || drafts;
-    u32x4 pf;
+    u32x4 pf[1];
     f32x4 ks[2] = {}, vs[2] = {};
     if (scaled) {
       __builtin_amdgcn_wave_barrier();
@@ -497,15 +542,15 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
         ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][0][i * 16 + q4 * 4]);
         vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][1][i * 16 + q4 * 4]);
       }
-      pf = softmax32<PT, true, NT>(sc, st, o[0], 0.f, ks, vs, masked, drafts, okm, tile - base, seen[0], lane, scores ? scores + tile : nullptr);
+      softmax32<PT, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
     } else {
-      pf = softmax32<PT, false, NT>(sc, st, o[0], a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen[0], lane, scores ? scores + tile : nullptr);
+      softmax32<PT, false, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const u32x2 lo = lds_read_transposed(my_lds + t * 32), hi = lds_read_transposed(my_lds + t * 32 + 16 * kPitch);
-      o[0][t] = mfma<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[0][t]);
+      o[0][t] = mfma<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[0], o[0][t]);
     }
     __builtin_amdgcn_wave_barrier();
     now = next;
@@ -529,11 +574,11 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, walk, vb, begin, end, base, seen, lane, wave, kAttendWaves);
 
   // the four waves meet
-  st.sum += __shfl_xor(st.sum, 16);
-  st.sum += __shfl_xor(st.sum, 32);
+  st[0].sum += __shfl_xor(st[0].sum, 16);
+  st[0].sum += __shfl_xor(st[0].sum, 32);
   if (q4 == 0) {
-    s_ml[wave][c16][0] = st.top;
-    s_ml[wave][c16][1] = st.sum;
+    s_ml[wave][c16][0] = st[0].top;
+    s_ml[wave][c16][1] = st[0].sum;
   }
   __syncthreads();
   f32x4* const box = reinterpret_cast<f32x4*>(s_v);       // [wave][NT][64]
@@ -541,7 +586,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   float all = -INFINITY;
 #pragma unroll
   for (int w = 0; w < kAttendWaves; ++w) all = fmaxf(all, s_ml[w][c16][0]);
-  const float mine = rescale(st.top, all);
+  const float mine = rescale(st[0].top, all);
 #pragma unroll
   for (int t = 0; t < NT; ++t) box[(wave * NT + t) * kWave + lane] = o[0][t] * mine;
   __syncthreads();
@@ -561,19 +606,19 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   }
 }
 
-// ---- more rows: RT tiles of 16 rows a wave, four waves, K and V of BT tokens in LDS for all of them
-template <int QT, bool FP8, int D, int RT, bool UNI>
-__global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunch a) {
+// ---- more rows: RT tiles of 16 rows a wave, W waves, K and V of BT tokens in LDS for all of them
+template <int QT, bool FP8, int D, int RT, int W, bool UNI>
+__global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch a) {
   constexpr int PT = FP8 ? TRI_KV_BF16 : QT;
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int BT = D == 256 ? 32 : 64;                  // tokens of a tile
   constexpr int LPR = D * ES / 16;                        // lanes that load one row
   constexpr int RPL = kWave / LPR;                        // rows of a wave's load
-  constexpr int NL = BT / (RPL * kAttendWaves);           // loads of a lane for K, and for V
+  constexpr int NL = BT / (RPL * W) > 0 ? BT / (RPL * W) : 1;      // loads of a lane for K, and for V
   constexpr int NT = D / 16;
   constexpr int kKeyPitch = D * 2 + 16;                   // 16 rows, 16 bytes of each, reach all banks
   constexpr int kValPitch = D * 2 + 32;                   // 8 rows, 32 bytes of each
-  static_assert(RPL <= 16 && NL >= 1, "a wave's load stays within 16 rows");
+  static_assert(RPL <= 16 && BT % RPL == 0, "a wave's load stays within 16 rows");
   __shared__ __align__(16) unsigned char s_k[2][BT * kKeyPitch];
   __shared__ __align__(16) unsigned char s_v[2][BT * kValPitch];
   __shared__ __align__(16) float s_scale[2][2][BT];
@@ -581,17 +626,16 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c16 = lane & 15, q4 = lane >> 4;
-  int idx = blockIdx.x;
-  const int h = idx % a.Hkv; idx /= a.Hkv;
-  const int rb = idx % a.row_blocks; idx /= a.row_blocks;
-  const int split = idx % a.nsplit;
-  const int b = idx / a.nsplit;
+  Work work;
+  if (!work_of(a, work)) return;
+  const int b = work.b, split = work.split, h = work.h, rb = work.rb;
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   const RowRange rows = rows_of(a, b);
   const int n = rows.n, M = n * a.G;
-  if (rb * RT * 16 * kAttendWaves >= M) return;
-  const int m0 = (rb * kAttendWaves + wave) * RT * 16;
+  if (rb * RT * 16 * W >= M) return;
+  const int m0 = (rb * W + wave) * RT * 16;
+  const bool loads = wave * RPL < BT;                     // (small rows: a load of every wave would be more than a tile)
   const int Tv = tokens_of(a, b, T);
   const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
   if (begin >= Tv && split > 0) return;
@@ -607,10 +651,11 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
   float ks_mine = 0.f, vs_mine = 0.f;
   Place p[2] = {};                       // of the tile in LDS, and of the one in registers
   auto load = [&](const Place& at) {
+    if (!loads) return;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       // (rows of this load: 16-row group i * 4 * RPL + wave * RPL lies in, the same for the whole wave)
-      const int row0 = (i * kAttendWaves + wave) * RPL;
+      const int row0 = (i * W + wave) * RPL;
       const GlobalBytes k = row_at<UNI, ES>(walk, kb, at, row0 / 16 * 16, row0 + lane / LPR) + (lane % LPR) * 16;
       const GlobalBytes v = row_at<UNI, ES>(walk, vb, at, row0 / 16 * 16, row0 + lane / LPR) + (lane % LPR) * 16;
       kr[i] = *(GlobalU4)k;
@@ -622,6 +667,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
     }
   };
   auto store = [&](const Place& at, int tile, int buf) {
+    if (!loads) return;
     const uint64_t okm = __ballot(at.ok);
     const bool all = BT == 64 ? okm == ~0ull : (uint32_t)okm == ~0u;
     const bool drafts = n > 1 && tile + BT > base;
@@ -630,7 +676,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
       bool odd = false;
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int row = (i * kAttendWaves + wave) * RPL + l / LPR;
+        const int row = (i * W + wave) * RPL + l / LPR;
         if (!(okm >> row & 1)) vr[i] = u32x4{0, 0, 0, 0};
         if (drafts && tile + row >= base) odd |= clear_odd<FP8 ? TRI_KV_FP8_E4M3 : PT>(vr[i]);
       }
@@ -638,7 +684,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
     }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int row = (i * kAttendWaves + wave) * RPL + lane / LPR;
+      const int row = (i * W + wave) * RPL + lane / LPR;
       u32x4* kd = reinterpret_cast<u32x4*>(s_k[buf] + row * kKeyPitch + (lane % LPR) * (FP8 ? 32 : 16));
       u32x4* vd = reinterpret_cast<u32x4*>(s_v[buf] + row * kValPitch + (lane % LPR) * (FP8 ? 32 : 16));
       if constexpr (FP8) {
@@ -652,7 +698,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
       }
     }
     if (scaled && wave == 0 && lane < BT) {
-      s_scale[buf][0][lane] = ks_mine * a.scale_log2;
+      s_scale[buf][0][lane] = ks_mine;
       s_scale[buf][1][lane] = vs_mine;
     }
   };
@@ -727,15 +773,9 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ks[i] = f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
-            vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
-          }
+          for (int i = 0; i < 2; ++i) ks[i] = vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
         }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          pf[rt] = softmax32<PT, FP8, NT>(sc[rt], st[rt], o[rt], a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen[rt], lane,
-                                          scores[rt] ? scores[rt] + first : nullptr);
+        softmax32<PT, FP8, RT, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
         const LdsBytes at = (LdsBytes)s_v[buf] + (sub * 32 + q4 * 4 + (c16 >> 2)) * kValPitch + (c16 & 3) * 8;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -771,13 +811,14 @@ __global__ __launch_bounds__(kAttendThreads) void attend_rows_kernel(AttendLaunc
 
 template <int QT, bool FP8, int D, bool UNI>
 hipError_t launch_attend_typed(const AttendLaunch& a, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv)), block(kAttendThreads);
-  if (a.row_tiles == 0) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI>), grid, block, 0, s, a);
-  else if (a.row_tiles == 1) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 1, UNI>), grid, block, 0, s, a);
-  else if (a.row_tiles == 2) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 2, UNI>), grid, block, 0, s, a);
+  const int64_t units = (int64_t)a.B * a.nsplit;
+  const dim3 grid((unsigned)((a.by_xcd ? align_up(units, kDies) : units) * a.row_blocks * a.Hkv));
+  if (a.row_tiles == 0) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI>), grid, dim3(kAttendThreads), 0, s, a);
+  else if (a.row_tiles == 4) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 1, 4, UNI>), grid, dim3(4 * kWave), 0, s, a);
+  else if (a.row_tiles == 8) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 1, 8, UNI>), grid, dim3(8 * kWave), 0, s, a);
   else if constexpr (D <= 128) {
-    if (a.row_tiles != 4) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 4, UNI>), grid, block, 0, s, a);
+    if (a.row_tiles != 16) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 2, 8, UNI>), grid, dim3(8 * kWave), 0, s, a);
   } else return hipErrorInvalidValue;
   return hipGetLastError();
 }

@@ -892,7 +892,12 @@ struct AttendPlan {
 };
 
 constexpr int kMaxNewTokens = 64;          // a word of ancestors
-constexpr int kAttendWorkgroups = 768;     // three for every CU: what is aimed at where the tokens allow it
+// Workgroups of an attention kernel that a CU holds, by its registers.
+int attend_workgroups_per_cu(int row_tiles, int D) {
+  if (row_tiles == 0) return D == 64 ? 4 : D == 128 ? 2 : 1;
+  if (row_tiles == 4) return D == 64 ? 4 : 2;
+  return 1;
+}
 constexpr int kAttendStep = 128;           // tokens the waves of a workgroup take at a time
 
 bool is_finite(float x) { return x - x == 0.f; }
@@ -923,6 +928,7 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
     return fail(TRI_ERR_INVALID_ARGUMENT, "out_stride_head %lld < head_dim", (long long)p->out_stride_head);
   if (!is_finite(p->scale) || !is_finite(p->k_scale) || !is_finite(p->v_scale) || !is_finite(p->scale * p->k_scale * 1.44269504f))
     return fail(TRI_ERR_INVALID_ARGUMENT, "scale, k_scale and v_scale must be finite");
+  if (!(p->scale * p->k_scale > 0.f)) return fail(TRI_ERR_INVALID_ARGUMENT, "scale * k_scale must be positive");
   // (in-block offsets of the rows a wave reads together are 32-bit)
   if (kv->stride_token < 0 || kv->stride_token >= (1 << 25))
     return fail(TRI_ERR_UNSUPPORTED, "stride_token %lld", (long long)kv->stride_token);
@@ -963,15 +969,26 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   int64_t total = 0;
   for (int b = 0; b < a.B; ++b) total += std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest);
   const int rows = a.max_rows * a.G;
-  a.row_tiles = rows <= 16 ? 0 : rows <= 64 ? 1 : rows <= 128 || a.D == 256 ? 2 : 4;
-  a.row_blocks = a.row_tiles ? tri::ceil_div(rows, 64 * a.row_tiles) : 1;
-  const int64_t per = tri::ceil_div64(total * a.Hkv * a.row_blocks, kAttendWorkgroups);
-  a.split_tokens = (int)std::min<int64_t>(tri::align_up(std::max<int64_t>(per, 1), kAttendStep), tri::align_up(longest, kAttendStep));
+  a.row_tiles = rows <= 16 ? 0 : rows <= 64 ? 4 : rows <= 128 || a.D == 256 ? 8 : 16;
+  a.row_blocks = a.row_tiles ? tri::ceil_div(rows, 16 * a.row_tiles) : 1;
+  // A split is as long as lets every workgroup run at once: on from the mean over what the chip holds, until the splits
+  // of all sequences fit (each sequence's last one is short).
+  const int64_t holds = 256 * attend_workgroups_per_cu(a.row_tiles, a.D);
+  const int64_t inner = (int64_t)a.Hkv * a.row_blocks, most = tri::align_up(longest, kAttendStep);
+  int64_t split = std::min<int64_t>(tri::align_up(std::max<int64_t>(tri::ceil_div64(total * inner, holds), 1), kAttendStep), most);
+  for (; split < most; split += kAttendStep) {
+    int64_t count = 0;
+    for (int b = 0; b < a.B; ++b)
+      count += std::max<int64_t>(1, tri::ceil_div64(std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest), split));
+    if (count * inner <= holds) break;
+  }
+  a.split_tokens = (int)split;
   a.nsplit = (int)tri::ceil_div64(longest, a.split_tokens);
+  a.by_xcd = a.row_blocks > 1 && (int64_t)a.B * a.nsplit >= 32;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = tri::align_up(off + bytes, 256); return o; };
   const int64_t parts = a.nsplit > 1 ? (int64_t)a.B * a.Hkv * a.nsplit * rows : 0;
-  if ((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) * tri::ceil_div(a.Hkv, 4) > INT_MAX ||
+  if (((int64_t)a.B * a.nsplit + 7) * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) * tri::ceil_div(a.Hkv, 4) > INT_MAX ||
       (int64_t)a.B * a.Hkv * rows > INT_MAX)
     return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d rows and %d KV heads in one call", a.B, a.max_rows, a.Hkv);
   a.score_pitch = tri::align_up(a.Tmax, 32);
