@@ -5,121 +5,174 @@
 namespace tri {
 namespace {
 
-// out = sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) L_s over the splits that hold tokens of the sequence, in the order of the
-// splits.  D / 4 lanes a row; reads nsplit * (D + 2) * 4 bytes of a row once, bound by that or, mostly, by its latency.
-template <int QT, int D>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendLaunch a) {
-  constexpr int kLanes = D / 4, kRows = 256 / kLanes;
+constexpr int kThreads = 256;
+constexpr int kWideSplits = 8;      // more splits than that: several lanes side by side over them, where rows are few
+constexpr int kWideRows = 1024;
+
+struct Joined {
+  f32x4 v;
+  float top, total;
+};
+__device__ __forceinline__ void join_two(Joined& a, const Joined& b) {
+  const float top = fmaxf(a.top, b.top), fa = rescale(a.top, top), fb = rescale(b.top, top);
+  // (a part of factor 0 has no tokens: its values are not looked at)
+  a.v = (fa == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a.v * fa) + (fb == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : b.v * fb);
+  a.total = a.total * fa + b.total * fb;
+  a.top = top;
+}
+
+// out = sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) L_s over the splits that hold tokens of the sequence, in a fixed order.
+// D / 4 lanes take a row, PARTS of them side by side every PARTS-th split.  Reads nsplit * (D + 2) * 4 bytes of a row
+// once; bound by their latency.
+template <int QT, int D, int PARTS>
+__device__ __forceinline__ void join_rows(const AttendLaunch& a, int64_t group) {
+  constexpr int kLanes = D / 4, kRows = kThreads / kLanes / PARTS;
+  constexpr int kAtOnce = PARTS > 1 ? 4 : 8;         // splits asked for together
+  __shared__ Joined s_part[PARTS > 1 ? PARTS : 1][kRows][kLanes];
   const int rows_max = a.max_rows * a.G;
-  const int64_t at = (int64_t)blockIdx.x * kRows + threadIdx.x / kLanes;
-  if (at >= (int64_t)a.B * a.Hkv * rows_max) return;
-  const int m = (int)(at % rows_max);
-  const int h = (int)(at / rows_max % a.Hkv), b = (int)(at / rows_max / a.Hkv);
+  const int lane = threadIdx.x % kLanes, part = threadIdx.x / kLanes % PARTS, mine = threadIdx.x / kLanes / PARTS;
+  const int64_t at = group * kRows + mine;
+  const bool in = at < (int64_t)a.B * a.Hkv * rows_max;
+  const int m = in ? (int)(at % rows_max) : 0;
+  const int h = in ? (int)(at / rows_max % a.Hkv) : 0, b = in ? (int)(at / rows_max / a.Hkv) : 0;
   const RowRange rows = rows_of(a, b);
-  if (m >= rows.n * a.G) return;
+  const bool live_row = in && m < rows.n * a.G;
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   const int live = max(1, ceil_div(tokens_of(a, b, T), a.split_tokens));
   const int64_t first = ((int64_t)b * a.Hkv + h) * a.nsplit * rows_max + m;
-  const int d = (threadIdx.x % kLanes) * 4;
-  f32x4 v = {0.f, 0.f, 0.f, 0.f};
-  float top = -INFINITY, total = 0.f;
-  constexpr int kAtOnce = 8;                 // splits asked for together
-  for (int s0 = 0; s0 < live; s0 += kAtOnce) {
-    f32x2 ml[kAtOnce];
-    f32x4 o[kAtOnce];
+  const int d = lane * 4;
+  Joined j{{0.f, 0.f, 0.f, 0.f}, -INFINITY, 0.f};
+  if (live_row) {
+    for (int s0 = part; s0 < live; s0 += kAtOnce * PARTS) {
+      f32x2 ml[kAtOnce];
+      f32x4 o[kAtOnce];
 #pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const int64_t row = first + (int64_t)min(s0 + u, live - 1) * rows_max;
-      ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + row * 2);
-      o[u] = *reinterpret_cast<const f32x4*>(a.part_out + row * D + d);
-    }
-    float now = top;
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) now = fmaxf(now, ml[u][0]);
-    const float old_f = rescale(top, now);
-    v *= old_f;
-    total *= old_f;
-    top = now;
-#pragma unroll
-    for (int u = 0; u < kAtOnce; ++u) {
-      const float f = s0 + u < live ? rescale(ml[u][0], now) : 0.f;
-      if (f != 0.f) {
-        v += o[u] * f;
-        total += ml[u][1] * f;
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int64_t row = first + (int64_t)min(s0 + u * PARTS, live - 1) * rows_max;
+        ml[u] = *reinterpret_cast<const f32x2*>(a.part_ml + row * 2);
+        o[u] = *reinterpret_cast<const f32x4*>(a.part_out + row * D + d);
       }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u)
+        if (s0 + u * PARTS < live) join_two(j, Joined{o[u], ml[u][0], ml[u][1]});
     }
   }
+  if (PARTS > 1) {
+    s_part[part][mine][lane] = j;
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll 4
+    for (int p = 1; p < PARTS; ++p) join_two(j, s_part[p][mine][lane]);
+  }
+  if (!live_row) return;
   const int64_t i = rows.first + m / a.G;
   const int hq = h * a.G + m % a.G;
-  const float inv = total == 0.f ? 0.f : a.v_scale / total;
+  const float inv = j.total == 0.f ? 0.f : a.v_scale / j.total;
   uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + i * a.out_stride_row + (int64_t)hq * a.out_stride_head + d;
-  *reinterpret_cast<uint2*>(dst) = uint2{Half<QT>::pack(v[0] * inv, v[1] * inv), Half<QT>::pack(v[2] * inv, v[3] * inv)};
-  if (d == 0) {
-    const float l2 = lse_of(top, total);
-    if (a.lse) a.lse[i * a.Hq + hq] = l2 * 0.69314718055994530942f;
-    if (a.lse2) a.lse2[i * a.Hq + hq] = l2;
-  }
+  *reinterpret_cast<uint2*>(dst) = uint2{Half<QT>::pack(j.v[0] * inv, j.v[1] * inv), Half<QT>::pack(j.v[2] * inv, j.v[3] * inv)};
+  if (d == 0 && a.lse) a.lse[i * a.Hq + hq] = lse_of(j.top, j.total) * 0.69314718055994530942f;
 }
 
 // weight[token][head] (+)= sum over the rows of the head of 2^(s - lse): every token and head by one thread, rows in order.
 // A lane is a token (the scores lie token by token), a wave takes four heads, whose weights it reads and writes as one
-// piece (VEC).  Reads a score once, weights once, writes them once.
+// piece (VEC), and sixteen rows at a time: four lanes find the lse of a row, from its splits where the sequence is
+// cut.  Reads a score once, weights once, writes them once.
 template <bool VEC>
-__global__ __launch_bounds__(256) void attend_weights_kernel(AttendLaunch a, float* weights, int set) {
+__device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weights, int set, int64_t group) {
+  __shared__ float s_lse[kThreads / kWave][16];
   const int lane = threadIdx.x % kWave;
   const int quads = ceil_div(a.Hkv, 4), chunks = ceil_div(a.Tmax, kWave);
-  int64_t unit = (int64_t)blockIdx.x * (256 / kWave) + threadIdx.x / kWave;
+  int64_t unit = group * (kThreads / kWave) + threadIdx.x / kWave;
   const int h0 = (int)(unit % quads) * 4;
   unit /= quads;
-  const int t = (int)(unit % chunks) * kWave + lane;
+  const int t0 = (int)(unit % chunks) * kWave;
   const int64_t b = unit / chunks;
   if (b >= a.B) return;
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
-  if (t >= T) return;
+  if (t0 >= T) return;
   const RowRange rows = rows_of(a, (int)b);
+  const int t = min(t0 + lane, T - 1);
   const int page = a.block_table ? a.block_table[b * a.block_table_pitch + t / a.block_size] : (int)b;
-  if (page < 0 || page >= a.num_blocks) return;
-  float* const w = weights + ((int64_t)page * a.block_size + t % a.block_size) * a.Hkv + h0;
+  const bool ok = t0 + lane < T && page >= 0 && page < a.num_blocks;
+  float* const w = weights + (ok ? ((int64_t)page * a.block_size + t % a.block_size) * a.Hkv + h0 : 0);
   const bool fresh = set || t >= T - rows.n;      // the rows' own tokens: nothing has been added for them yet
-  f32x4 had = {0.f, 0.f, 0.f, 0.f};
-  if (!fresh) {
-    if (VEC) had = *reinterpret_cast<const f32x4*>(w);
-    else
-      for (int e = 0; e < 4; ++e) had[e] = h0 + e < a.Hkv ? w[e] : 0.f;
-  }
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  const int64_t per_head = (int64_t)a.max_rows * a.G * a.score_pitch;
-  const float* s = a.scores + (b * a.Hkv + h0) * per_head + t;
-  for (int i = 0; i < rows.n; ++i) {
-    const float* lse = a.lse2 + (int64_t)(rows.first + i) * a.Hq + h0 * a.G;
+  if (ok && !fresh) {
+    if (VEC) sum = *reinterpret_cast<const f32x4*>(w);
+    else
+      for (int e = 0; e < 4; ++e) sum[e] = h0 + e < a.Hkv ? w[e] : 0.f;
+  }
+  f32x4 more = {0.f, 0.f, 0.f, 0.f};
+  const int per_head = rows.n * a.G, heads = min(4, a.Hkv - h0), rows_max = a.max_rows * a.G;
+  const int live = max(1, ceil_div(T, a.split_tokens));
+  for (int r0 = 0; r0 < heads * per_head; r0 += 16) {
+    const int r = min(r0 + (lane & 15), heads * per_head - 1), h = h0 + r / per_head, m = r % per_head;
+    float l;
+    if (a.nsplit > 1) {
+      const float* ml = a.part_ml + (((b * a.Hkv + h) * a.nsplit) * rows_max + m) * 2;
+      float top = -INFINITY, total = 0.f;
 #pragma unroll 4
-    for (int g = 0; g < a.G; ++g) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int ee = VEC ? e : min(e, a.Hkv - 1 - h0);
-        const float l = lse[ee * a.G + g];
-        // (a row without tokens, lse -inf: nothing)
-        sum[e] += pow2(s[ee * per_head + (int64_t)(i * a.G + g) * a.score_pitch] - (l == -INFINITY ? INFINITY : l));
+      for (int s = lane >> 4; s < live; s += 4) {
+        const f32x2 x = *reinterpret_cast<const f32x2*>(ml + (int64_t)s * rows_max * 2);
+        const float now = fmaxf(top, x[0]);
+        total = total * rescale(top, now) + x[1] * rescale(x[0], now);
+        top = now;
       }
+#pragma unroll
+      for (int step = 16; step <= 32; step *= 2) {
+        const float other = __shfl_xor(top, step), now = fmaxf(top, other);
+        total = total * rescale(top, now) + __shfl_xor(total, step) * rescale(other, now);
+        top = now;
+      }
+      l = lse_of(top, total);
+    } else {
+      l = a.lse2[(int64_t)(rows.first + m / a.G) * a.Hq + h * a.G + m % a.G];
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (lane < 16) s_lse[threadIdx.x / kWave][lane] = l == -INFINITY ? INFINITY : l;             // (a row without tokens adds nothing)
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float* s = a.scores + (b * a.Hkv + min(h0 + e, a.Hkv - 1)) * rows_max * a.score_pitch + t;
+      const int from = max(r0, e * per_head), to = min(min(r0 + 16, heads * per_head), (e + 1) * per_head);
+#pragma unroll 4
+      for (int x = from; x < to; ++x)
+        more[e] += pow2(s[(int64_t)(x - e * per_head) * a.score_pitch] - s_lse[threadIdx.x / kWave][x - r0]);
     }
   }
-  sum += had;
+  sum += more;
+  if (!ok) return;
   if (VEC) *reinterpret_cast<f32x4*>(w) = sum;
   else
     for (int e = 0; e < 4; ++e)
       if (h0 + e < a.Hkv) w[e] = sum[e];
 }
 
-template <int QT>
-hipError_t launch_join_typed(const AttendLaunch& a, hipStream_t s) {
-  const int64_t rows = (int64_t)a.B * a.Hkv * a.max_rows * a.G;
-  auto go = [&](auto kernel, int per) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div64(rows, per)), dim3(256), 0, s, a);
+// The splits joined and the weights added up, in one launch: both start from what attend_kernel left.
+template <int QT, int D, int PARTS, bool VEC>
+__global__ __launch_bounds__(kThreads) void attend_finish_kernel(AttendLaunch a, int join_groups, float* weights, int set) {
+  if ((int)blockIdx.x < join_groups) join_rows<QT, D, PARTS>(a, blockIdx.x);
+  else add_weights<VEC>(a, weights, set, blockIdx.x - join_groups);
+}
+
+template <int QT, int D>
+hipError_t launch_finish_typed(const AttendLaunch& a, float* weights, int set, hipStream_t s) {
+  constexpr int kRows = kThreads / (D / 4);
+  const int64_t rows = a.nsplit > 1 ? (int64_t)a.B * a.Hkv * a.max_rows * a.G : 0;
+  // Many splits of few rows: a workgroup a row, its lanes side by side over the splits (56 rows of 32 splits 7.2 -> 5.5 us;
+  // not 3840 rows of 16, 8.1 -> 15.4).
+  const bool wide = a.nsplit > kWideSplits && rows <= kWideRows;
+  const int64_t joins = wide ? rows : ceil_div64(rows, kRows);
+  const int64_t adds = weights ? ceil_div64((int64_t)a.B * ceil_div(a.Tmax, kWave) * ceil_div(a.Hkv, 4), kThreads / kWave) : 0;
+  if (joins + adds == 0) return hipSuccess;
+  if (joins + adds > INT32_MAX) return hipErrorInvalidValue;
+  const bool vec = a.Hkv % 4 == 0 && reinterpret_cast<uintptr_t>(weights) % 16 == 0;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(joins + adds)), dim3(kThreads), 0, s, a, (int)joins, weights, set);
     return hipGetLastError();
   };
-  if (a.D == 64) return go(attend_join_kernel<QT, 64>, 16);
-  if (a.D == 128) return go(attend_join_kernel<QT, 128>, 8);
-  return go(attend_join_kernel<QT, 256>, 4);
+  if (wide) return vec ? go(attend_finish_kernel<QT, D, kRows, true>) : go(attend_finish_kernel<QT, D, kRows, false>);
+  return vec ? go(attend_finish_kernel<QT, D, 1, true>) : go(attend_finish_kernel<QT, D, 1, false>);
 }
 
 }  // namespace
@@ -131,18 +184,11 @@ hipError_t launch_attend(const AttendLaunch& a, hipStream_t s) {
   return bf16 ? launch_attend_256_bf16(a, s) : launch_attend_256_fp16(a, s);
 }
 
-hipError_t launch_attend_join(const AttendLaunch& a, hipStream_t s) {
-  return a.q_dtype == TRI_KV_BF16 ? launch_join_typed<TRI_KV_BF16>(a, s) : launch_join_typed<TRI_KV_FP16>(a, s);
-}
-
-hipError_t launch_attend_weights(const AttendLaunch& a, float* weights, int set, hipStream_t s) {
-  const int64_t waves = (int64_t)a.B * ceil_div(a.Tmax, kWave) * ceil_div(a.Hkv, 4);
-  const dim3 grid((unsigned)ceil_div64(waves, 256 / kWave));
-  if (a.Hkv % 4 == 0 && reinterpret_cast<uintptr_t>(weights) % 16 == 0)
-    hipLaunchKernelGGL(attend_weights_kernel<true>, grid, dim3(256), 0, s, a, weights, set);
-  else
-    hipLaunchKernelGGL(attend_weights_kernel<false>, grid, dim3(256), 0, s, a, weights, set);
-  return hipGetLastError();
+hipError_t launch_attend_finish(const AttendLaunch& a, float* weights, int set, hipStream_t s) {
+  const bool bf16 = a.q_dtype == TRI_KV_BF16;
+  if (a.D == 64) return bf16 ? launch_finish_typed<TRI_KV_BF16, 64>(a, weights, set, s) : launch_finish_typed<TRI_KV_FP16, 64>(a, weights, set, s);
+  if (a.D == 128) return bf16 ? launch_finish_typed<TRI_KV_BF16, 128>(a, weights, set, s) : launch_finish_typed<TRI_KV_FP16, 128>(a, weights, set, s);
+  return bf16 ? launch_finish_typed<TRI_KV_BF16, 256>(a, weights, set, s) : launch_finish_typed<TRI_KV_FP16, 256>(a, weights, set, s);
 }
 
 }  // namespace tri

@@ -703,6 +703,18 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     }
   };
 
+  // tile t in LDS, t + 1 in registers, pages of t + 2 and list entries of t + 3 on their way
+  int next_tok = -1, next_page = -1, next2_entry = 0;
+  if (threadIdx.x == 0) s_odd = 0;
+  if (begin < end) {
+    const int tok = walk.token(begin, walk.entry(begin));
+    next_tok = walk.token(begin + BT, walk.entry(begin + BT));
+    const int page = walk.page(tok);
+    next_page = walk.page(next_tok);
+    next2_entry = walk.entry(begin + 2 * BT);
+    p[0] = walk.place(tok, page);
+    load(p[0]);
+  }
   u32x4 qf[RT][D / 32];
   uint64_t seen[RT];
   float* scores[RT];
@@ -720,18 +732,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     for (int t = 0; t < NT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // tile t in LDS, t + 1 in registers, pages of t + 2 and list entries of t + 3 on their way
-  int next_tok = -1, next_page = -1, next2_entry = 0;
-  if (threadIdx.x == 0) s_odd = 0;
+  __syncthreads();          // (s_odd)
   if (begin < end) {
-    const int tok = walk.token(begin, walk.entry(begin));
-    next_tok = walk.token(begin + BT, walk.entry(begin + BT));
-    const int page = walk.page(tok);
-    next_page = walk.page(next_tok);
-    next2_entry = walk.entry(begin + 2 * BT);
-    p[0] = walk.place(tok, page);
-    load(p[0]);
-    __syncthreads();
     store(p[0], begin, 0);
     p[1] = walk.place(next_tok, next_page);
     next_tok = walk.token(begin + 2 * BT, next2_entry);
@@ -746,6 +748,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
 #pragma unroll
       for (int sub = 0; sub < BT / 32; ++sub) {
         const int first = tile + sub * 32;
+        if (sub > 0 && first >= end) continue;           // (nothing there, and rows of scores are whole pieces of 32 tokens)
         const uint32_t okm = (uint32_t)(okm_all >> (sub * 32));
         const bool drafts = n > 1 && first + 32 > base;
         const bool masked = okm != 0xffffffffu || drafts;

@@ -57,7 +57,7 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(BoundsLaunch a, int b
   if (b >= a.B || piece >= a.Hkv * (a.D / 8)) return;
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   if (a.new_tokens > 0) j += max(T - a.new_tokens, 0) / a.block_size;
-  const int t0 = j * a.block_size, count = min(a.block_size, T - t0);
+  const int count = min(a.block_size, T - j * a.block_size);
   if (count <= 0) return;
   const int page = a.block_table ? a.block_table[b * a.block_table_pitch + j] : (int)b;
   if (page < 0 || page >= a.num_blocks) return;
@@ -67,26 +67,40 @@ __global__ __launch_bounds__(256) void block_bounds_kernel(BoundsLaunch a, int b
   float low[8], high[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) { low[e] = INFINITY; high[e] = -INFINITY; }
-#pragma unroll 8
-  for (int t = 0; t < count; ++t) {
-    float x[8];
-    const char* row = src + (int64_t)t * a.stride_token * ES;
-    if constexpr (DT == TRI_KV_FP8_E4M3) {
-      const uint2 w = *reinterpret_cast<const uint2*>(row);
-      x[0] = fp8_byte<0>(w.x); x[1] = fp8_byte<1>(w.x); x[2] = fp8_byte<2>(w.x); x[3] = fp8_byte<3>(w.x);
-      x[4] = fp8_byte<0>(w.y); x[5] = fp8_byte<1>(w.y); x[6] = fp8_byte<2>(w.y); x[7] = fp8_byte<3>(w.y);
-      if (sc) {
-        const float f = sc[(int64_t)t * a.Hkv];
+  constexpr int kAtOnce = 16;         // tokens asked for together (the last one again where the block has fewer)
+  for (int t0 = 0; t0 < count; t0 += kAtOnce) {
+    uint4 w[kAtOnce];
+    float f[kAtOnce];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= f;
+    for (int u = 0; u < kAtOnce; ++u) {
+      const int t = min(t0 + u, count - 1);
+      const char* row = src + (int64_t)t * a.stride_token * ES;
+      if constexpr (DT == TRI_KV_FP8_E4M3) {
+        const uint2 x = *reinterpret_cast<const uint2*>(row);
+        w[u] = uint4{x.x, x.y, 0, 0};
+        f[u] = sc ? sc[(int64_t)t * a.Hkv] : 1.f;
+      } else {
+        w[u] = *reinterpret_cast<const uint4*>(row);
       }
-    } else {
-      unpack8<DT>(*reinterpret_cast<const uint4*>(row), x);
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      low[e] = low_of(low[e], x[e]);
-      high[e] = high_of(high[e], x[e]);
+    for (int u = 0; u < kAtOnce; ++u) {
+      float x[8];
+      if constexpr (DT == TRI_KV_FP8_E4M3) {
+        x[0] = fp8_byte<0>(w[u].x); x[1] = fp8_byte<1>(w[u].x); x[2] = fp8_byte<2>(w[u].x); x[3] = fp8_byte<3>(w[u].x);
+        x[4] = fp8_byte<0>(w[u].y); x[5] = fp8_byte<1>(w[u].y); x[6] = fp8_byte<2>(w[u].y); x[7] = fp8_byte<3>(w[u].y);
+        if (sc) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= f[u];
+        }
+      } else {
+        unpack8<DT>(w[u], x);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        low[e] = low_of(low[e], x[e]);
+        high[e] = high_of(high[e], x[e]);
+      }
     }
   }
   uint16_t* dst = reinterpret_cast<uint16_t*>(a.bounds) + (int64_t)l * a.bounds_stride_layer + ((int64_t)page * a.Hkv + h) * 2 * a.D + d;
@@ -127,19 +141,35 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreLaunch a) {
     }
     for (int i = taken + threadIdx.x; i < a.top; i += 256) a.blocks[row * a.top + i] = -1;
   }
-  const int sub = threadIdx.x % LPB;
-  float best[kScoreBlocks / kBlocks];
-  double total[kScoreBlocks / kBlocks];
+  const int sub = threadIdx.x % LPB, slot = threadIdx.x / LPB;
+  const bool b0 = (sub ^ sub >> 2) & 1, b1 = (sub >> 1 ^ sub >> 2) & 1;      // (the same in the lanes that the half mirror pairs)
+  constexpr int kEach = kScoreBlocks / kBlocks;
+  float best[kEach];
+  double total[kEach];
+  uint4 low_w[kEach], high_w[kEach];
+  bool ok[kEach];
+  int page[kEach];
 #pragma unroll
-  for (int i = 0; i < kScoreBlocks / kBlocks; ++i) { best[i] = -INFINITY; total[i] = 0.; }
+  for (int i = 0; i < kEach; ++i) {
+    const int j = min(chunk * kScoreBlocks + i * kBlocks + slot, max(count - 1, 0));
+    page[i] = a.block_table ? a.block_table[(int64_t)b * a.block_table_pitch + j] : b;
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    best[i] = -INFINITY;
+    total[i] = 0.;
+    ok[i] = page[i] >= 0 && page[i] < a.num_blocks;
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(a.bounds) + ((int64_t)(ok[i] ? page[i] : 0) * a.Hkv + h) * 2 * D + sub * 8;
+    low_w[i] = *reinterpret_cast<const uint4*>(src);
+    high_w[i] = *reinterpret_cast<const uint4*>(src + D);
+  }
   for (int g0 = 0; g0 < a.G; g0 += kHeadsAtOnce) {
-    float q[8];
     double q64[kHeadsAtOnce][8];
     bool up[kHeadsAtOnce][8];
 #pragma unroll
     for (int g = 0; g < kHeadsAtOnce; ++g) {
-      const int gg = min(g0 + g, a.G - 1);
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)b * a.q_stride_row + (int64_t)(h * a.G + gg) * a.q_stride_head + sub * 8;
+      float q[8];
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)b * a.q_stride_row + (int64_t)(h * a.G + min(g0 + g, a.G - 1)) * a.q_stride_head + sub * 8;
       unpack8<QT>(*reinterpret_cast<const uint4*>(src), q);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -148,38 +178,40 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreLaunch a) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < kScoreBlocks / kBlocks; ++i) {
-      const int j = chunk * kScoreBlocks + i * kBlocks + threadIdx.x / LPB;
-      if (j >= count) continue;
-      const int page = a.block_table ? a.block_table[(int64_t)b * a.block_table_pitch + j] : b;
-      const bool ok = page >= 0 && page < a.num_blocks;
-      const uint16_t* src = reinterpret_cast<const uint16_t*>(a.bounds) + ((int64_t)(ok ? page : 0) * a.Hkv + h) * 2 * D + sub * 8;
+    for (int i = 0; i < kEach; ++i) {
       float low[8], high[8];
-      unpack8<BT>(*reinterpret_cast<const uint4*>(src), low);
-      unpack8<BT>(*reinterpret_cast<const uint4*>(src + D), high);
+      unpack8<BT>(low_w[i], low);
+      unpack8<BT>(high_w[i], high);
+      double s[kHeadsAtOnce];
 #pragma unroll
       for (int g = 0; g < kHeadsAtOnce; ++g) {
-        double s = 0.;
+        s[g] = 0.;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = __builtin_fma(q64[g][e], (double)(up[g][e] ? high[e] : low[e]), s);
-        s += dpp64<kDppXor1>(s);
-        s += dpp64<kDppXor2>(s);
-        s += dpp64<kDppHalfMirror>(s);
-        if (LPB >= 16) s += dpp64<kDppRor8>(s);
-        if (LPB >= 32) s += __shfl_xor(s, 16);
-        if (!ok) s = -INFINITY;
-        if (g0 + g < a.G) {
-          total[i] += s;
-          best[i] = high_of((float)s, best[i]);
-        }
+        for (int e = 0; e < 8; ++e) s[g] = __builtin_fma(q64[g][e], (double)(up[g][e] ? high[e] : low[e]), s[g]);
       }
+      // Over the block's lanes: the first two exchanges leave head 2 * b0 + b1 to a lane, the others add up.
+      double s0 = (b0 ? s[2] : s[0]) + dpp64<kDppXor1>(b0 ? s[0] : s[2]);
+      double s1 = (b0 ? s[3] : s[1]) + dpp64<kDppXor1>(b0 ? s[1] : s[3]);
+      double mine = (b1 ? s1 : s0) + dpp64<kDppXor2>(b1 ? s0 : s1);
+      mine += dpp64<kDppHalfMirror>(mine);
+      if (LPB >= 16) mine += dpp64<kDppRor8>(mine);
+      if (LPB >= 32) mine += __shfl_xor(mine, 16);
+      const bool in = g0 + (b0 ? 2 : 0) + (b1 ? 1 : 0) < a.G;
+      total[i] += in ? mine : 0.;
+      best[i] = in ? high_of((float)mine, best[i]) : best[i];
     }
   }
 #pragma unroll
-  for (int i = 0; i < kScoreBlocks / kBlocks; ++i) {
-    const int j = chunk * kScoreBlocks + i * kBlocks + threadIdx.x / LPB;
+  for (int i = 0; i < kEach; ++i) {
+    // (the four lanes at the front hold the heads)
+    best[i] = high_of(best[i], dpp<kDppXor1>(best[i]));
+    best[i] = high_of(best[i], dpp<kDppXor2>(best[i]));
+    total[i] += dpp64<kDppXor1>(total[i]);
+    total[i] += dpp64<kDppXor2>(total[i]);
+    const int j = chunk * kScoreBlocks + i * kBlocks + slot;
     if (j >= count || sub != 0) continue;
     float s = a.group_max ? best[i] : (float)(total[i] / a.G);
+    if (!ok[i]) s = -INFINITY;
     // (a NaN in a query or a key must come out of the attention as it would without the selection: its block is read)
     if (j < a.sinks || j >= count - a.recent || __builtin_isnan(s)) s = INFINITY;
     a.scores[row * a.max_count + j] = s;

@@ -898,7 +898,6 @@ int attend_workgroups_per_cu(int row_tiles, int D) {
   if (row_tiles == 4) return D == 64 ? 4 : 2;
   return 1;
 }
-constexpr int kAttendStep = 128;           // tokens the waves of a workgroup take at a time
 
 bool is_finite(float x) { return x - x == 0.f; }
 
@@ -974,9 +973,10 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   // A split is as long as lets every workgroup run at once: on from the mean over what the chip holds, until the splits
   // of all sequences fit (each sequence's last one is short).
   const int64_t holds = 256 * attend_workgroups_per_cu(a.row_tiles, a.D);
-  const int64_t inner = (int64_t)a.Hkv * a.row_blocks, most = tri::align_up(longest, kAttendStep);
-  int64_t split = std::min<int64_t>(tri::align_up(std::max<int64_t>(tri::ceil_div64(total * inner, holds), 1), kAttendStep), most);
-  for (; split < most; split += kAttendStep) {
+  constexpr int step = 128;      // whole tiles of every kernel (a single tile a workgroup saves the attention nothing and costs the join)
+  const int64_t inner = (int64_t)a.Hkv * a.row_blocks, most = tri::align_up(longest, step);
+  int64_t split = std::min<int64_t>(tri::align_up(std::max<int64_t>(tri::ceil_div64(total * inner, holds), 1), step), most);
+  for (; split < most; split += step) {
     int64_t count = 0;
     for (int b = 0; b < a.B; ++b)
       count += std::max<int64_t>(1, tri::ceil_div64(std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest), split));
@@ -1010,15 +1010,18 @@ int check_attend_pointers(const tri_attend_params* p, const AttendPlan& d, void*
   return check_workspace(need, ws, ws_bytes);
 }
 
-int do_attend(AttendPlan& d, void* ws, hipStream_t s) {
+int do_attend(AttendPlan& d, void* ws, float* weights, int weight_mode, hipStream_t s) {
   tri::AttendLaunch& a = d.a;
   if (a.nsplit > 1) {
     a.part_out = at<float>(ws, d.part_out);
     a.part_ml = at<float>(ws, d.part_ml);
   }
-  int rc = launch_status(tri::launch_attend(a, s), "attend");
-  if (!rc && a.nsplit > 1) rc = launch_status(tri::launch_attend_join(a, s), "attend_join");
-  return rc;
+  if (weights) {
+    a.lse2 = at<float>(ws, d.lse2);
+    a.scores = at<float>(ws, d.scores);
+  }
+  const int rc = launch_status(tri::launch_attend(a, s), "attend");
+  return rc ? rc : launch_status(tri::launch_attend_finish(a, weights, weight_mode, s), "attend_finish");
 }
 
 int fill_evict(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, int32_t* keep, tri::EvictLaunch& a) {
@@ -1077,14 +1080,7 @@ int tri_attend_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_
   if (!rc) rc = check_attend_pointers(p, d, ws, ws_bytes);
   if (rc) return rc;
   if (p->num_rows == 0) return TRI_OK;
-  hipStream_t s = (hipStream_t)stream;
-  if (p->weights) {
-    d.a.lse2 = at<float>(ws, d.lse2);
-    d.a.scores = at<float>(ws, d.scores);
-  }
-  rc = do_attend(d, ws, s);
-  if (rc || !p->weights) return rc;
-  return launch_status(tri::launch_attend_weights(d.a, p->weights, p->weight_mode, s), "attend_weights");
+  return do_attend(d, ws, p->weights, p->weight_mode, (hipStream_t)stream);
 }
 
 int tri_block_bounds(const tri_kv_layout* kv, const tri_batch* batch, int32_t num_blocks, int32_t new_tokens, void* bounds,
@@ -1148,7 +1144,7 @@ int tri_attend_blocks(const tri_kv_layout* kv, const tri_batch* batch, const tri
                      "topk_rows");
   if (rc) return rc;
   d.a.list = bp->blocks; d.a.list_k = bp->top_blocks; d.a.list_pitch = bp->top_blocks;
-  return do_attend(d, ws, s);
+  return do_attend(d, ws, nullptr, 0, s);
 }
 
 uint64_t tri_evict_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p) {

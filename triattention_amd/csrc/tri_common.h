@@ -282,7 +282,7 @@ struct AttendLaunch {
   // workspace
   float* part_out;                                         // [B][Hkv][nsplit][max_rows * G][D], not normalised (nsplit > 1)
   float* part_ml;                                          // the same rows' maximum (base 2) and sum
-  float* lse2;                                             // [num_rows][Hq], base 2, or NULL
+  float* lse2;                                             // [num_rows][Hq], base 2, or NULL (nsplit 1 with weights)
   float* scores;                                           // [B][Hkv][max_rows * G][score_pitch] base 2, or NULL
   int64_t score_pitch;
 };
@@ -293,9 +293,9 @@ hipError_t launch_attend_128_fp16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_256_bf16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_256_fp16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend(const AttendLaunch& a, hipStream_t s);
-hipError_t launch_attend_join(const AttendLaunch& a, hipStream_t s);
-// weights: the layer's [num_blocks][block_size][Hkv]; set: written, not added to.
-hipError_t launch_attend_weights(const AttendLaunch& a, float* weights, int set, hipStream_t s);
+// What follows it: the splits joined (nsplit > 1) and, with weights (the layer's [num_blocks][block_size][Hkv]), the
+// weights added to them (set: written).
+hipError_t launch_attend_finish(const AttendLaunch& a, float* weights, int set, hipStream_t s);
 
 // Bounds of a block's keys and the scores that choose blocks by them (tri_blocks.hip).
 struct BoundsLaunch {

@@ -704,14 +704,15 @@ class _on_device:
     """Makes a cache's device the current one for the calls of a block (kernels go to the current stream of the
     current device)."""
 
+    __slots__ = ("index", "back")
+
     def __init__(self, device):
         self.index = device.index
-        self.back = None
 
     def __enter__(self):
         now = torch.cuda.current_device()
-        if self.index is not None and self.index != now:
-            self.back = now
+        self.back = None if self.index is None or self.index == now else now
+        if self.back is not None:
             torch.cuda.set_device(self.index)
 
     def __exit__(self, *exc):
@@ -736,51 +737,78 @@ def _scratch(kv: PagedKV, nbytes: int, what: str):
     return buf, at + (-at) % 256
 
 
-def _layer_weights(kv: PagedKV, weights: torch.Tensor) -> torch.Tensor:
-    shape = (kv.num_layers, kv.num_blocks, kv.block_size, kv.num_kv_heads)
-    if tuple(_on(kv, "weights", weights, torch.float32).shape) != shape or not weights[0].is_contiguous():
-        raise ValueError(f"weights must be fp32 {shape}, contiguous within a layer")
-    return weights
+def _layer_address(kv: PagedKV, name: str, t: torch.Tensor, dtype, row: tuple, layer: int) -> int:
+    """Address of one layer of a [layers, blocks, *row] tensor beside the cache, contiguous within a layer."""
+    shape = (kv.num_layers, kv.num_blocks, *row)
+    _on(kv, name, t, dtype)
+    strides, want = t.stride(), 1
+    ok = t.shape == shape
+    for k in range(len(shape) - 1, 0, -1):
+        ok = ok and (strides[k] == want or shape[k] == 1)
+        want *= shape[k]
+    if not ok or (kv.num_layers > 1 and strides[0] < want):
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {shape}, contiguous within a layer")
+    return t.data_ptr() + layer * strides[0] * t.element_size()
+
+
+def _weights_address(kv: PagedKV, weights: torch.Tensor, layer: int = 0) -> int:
+    return _layer_address(kv, "weights", weights, torch.float32, (kv.block_size, kv.num_kv_heads), layer)
+
+
+def _bounds_address(kv: PagedKV, bounds: torch.Tensor, layer: int = 0) -> int:
+    return _layer_address(kv, "bounds", bounds, _bounds_dtype(kv), (kv.num_kv_heads, 2, kv.head_dim), layer)
+
+
+def _bounds_dtype(kv: PagedKV):
+    return torch.bfloat16 if _DTYPES[kv.dtype] == KV_FP8_E4M3 else kv.dtype
 
 
 def _check_attention_batch(kv: PagedKV, batch: StepBatch) -> None:
-    if batch.device != kv.device and torch.device(batch.device) != kv.device:
-        raise ValueError(f"the batch lies on {batch.device}, the cache on {kv.device}")
-    batch.check_capacity(kv.block_size)
+    if batch.seq_lens.device != kv.device:
+        raise ValueError(f"the batch lies on {batch.seq_lens.device}, the cache on {kv.device}")
     if kv.ks_ptrs is not None and kv.vs_ptrs is None and not hasattr(kv, "_unit"):
         raise ValueError("an fp8 cache has scales for K and V rows, or for neither")
-    if batch.block_table is None and (batch.max_seq_len > kv.block_size or batch.num_seqs > kv.num_blocks):
+    if batch.block_table is not None:
+        pitch = batch.struct.block_table_pitch
+        if -(-batch.max_seq_len // kv.block_size) > pitch:
+            raise IndexError(f"sequence of {batch.max_seq_len} tokens needs more than {pitch} blocks of {kv.block_size}")
+    elif batch.max_seq_len > kv.block_size or batch.num_seqs > kv.num_blocks:
         raise ValueError("without a block table a sequence is one block of the cache")
 
 
-def _attend_params(kv: PagedKV, batch: StepBatch, q, layer, row_starts, parents, max_rows, scale, k_scale, v_scale, out, want_lse):
+def _attend_params(kv: PagedKV, batch: StepBatch, q, layer, row_starts, parents, max_rows, scale, k_scale, v_scale, out, want_lse,
+                   weights=None, weight_set=0):
     """(parameters, out, lse) of an attention call after the checks that need the tensors."""
     _check_attention_batch(kv, batch)
     if kv.v_ptrs is None:
         raise ValueError("attention needs the values of the cache")
     _on(kv, "q", q)
-    if q.ndim != 3 or q.dtype not in (torch.bfloat16, torch.float16) or int(q.shape[2]) != kv.head_dim or q.stride(2) != 1:
-        raise ValueError(f"q must be a bf16 or fp16 [rows, heads, {kv.head_dim}] tensor with contiguous head_dim")
+    dtype, shape = q.dtype, q.shape
+    if len(shape) != 3 or dtype not in (torch.bfloat16, torch.float16) or shape[2] != kv.head_dim:
+        raise ValueError(f"q must be a bf16 or fp16 tensor [rows, heads, {kv.head_dim}]")
     if not 0 <= layer < kv.num_layers:
         raise IndexError(f"layer {layer} of {kv.num_layers}")
-    rows, heads = int(q.shape[0]), int(q.shape[1])
+    rows, heads, _ = shape
     if row_starts is not None:
         _on(kv, "row_starts", row_starts, torch.int32)
-        if tuple(row_starts.shape) != (batch.num_seqs + 1,) or not row_starts.is_contiguous():
+        if row_starts.shape != (batch.num_seqs + 1,) or not row_starts.is_contiguous():
             raise ValueError(f"row_starts must be a contiguous tensor of {batch.num_seqs + 1} entries")
         if parents is not None:
             _on(kv, "parents", parents, torch.int32)
-            if tuple(parents.shape) != (rows,) or not parents.is_contiguous():
+            if parents.shape != (rows,) or not parents.is_contiguous():
                 raise ValueError(f"parents must be a contiguous tensor of {rows} entries")
     if out is None:
-        out = torch.empty((rows, heads, kv.head_dim), dtype=q.dtype, device=kv.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != kv.device or out.stride(2) != 1:
-        raise ValueError("out must have q's shape and type on the cache's device, with contiguous head_dim")
+        out = torch.empty(shape, dtype=dtype, device=kv.device)
+    elif out.shape != shape or out.dtype != dtype or out.device != kv.device:
+        raise ValueError("out must have q's shape and type, on the cache's device")
+    qs, os = q.stride(), out.stride()
+    if qs[2] != 1 or os[2] != 1:
+        raise ValueError("head_dim must be contiguous in q and out")
     lse = torch.empty((rows, heads), dtype=torch.float32, device=kv.device) if want_lse else None
-    p = AttendParams(layer=layer, num_q_heads=heads, num_rows=rows, max_rows=max_rows, q_dtype=_DTYPES[q.dtype],
-                     num_blocks=kv.num_blocks, q=_ptr(q), q_stride_row=q.stride(0), q_stride_head=q.stride(1), out=_ptr(out),
-                     out_stride_row=out.stride(0), out_stride_head=out.stride(1), lse=_ptr(lse), row_starts=_ptr(row_starts),
-                     parents=_ptr(parents), scale=kv.head_dim ** -0.5 if scale is None else scale, k_scale=k_scale, v_scale=v_scale)
+    # (in the order of the fields: by name they cost some microseconds of a call whose kernels take ten)
+    p = AttendParams(layer, heads, rows, max_rows, _DTYPES[dtype], kv.num_blocks, q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0],
+                     os[1], _ptr(lse), _ptr(row_starts), _ptr(parents), kv.head_dim ** -0.5 if scale is None else scale, k_scale,
+                     v_scale, weights, weight_set)
     return p, out, lse
 
 
@@ -808,29 +836,19 @@ def attend_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, *, layer: int =
     lib = _lib.load()
     if weight_mode not in ("add", "set"):
         raise ValueError(f"weight_mode must be 'add' or 'set', got {weight_mode!r}")
-    p, out, lse = _attend_params(kv, batch, q, layer, row_starts, parents, max_rows, scale, k_scale, v_scale, out, want_lse)
-    if weights is not None:
-        p.weights = _ptr(_layer_weights(kv, weights)[layer])
-        p.weight_mode = int(weight_mode == "set")
+    p, out, lse = _attend_params(kv, batch, q, layer, row_starts, parents, max_rows, scale, k_scale, v_scale, out, want_lse,
+                                 None if weights is None else _weights_address(kv, weights, layer), int(weight_mode == "set"))
     with _on_device(kv.device):
-        nbytes = int(lib.tri_attend_workspace_bytes(C.byref(kv.struct), C.byref(batch.struct), C.byref(p)))
+        kvs, bs, ps = C.byref(kv.struct), C.byref(batch.struct), C.byref(p)
+        nbytes = lib.tri_attend_workspace_bytes(kvs, bs, ps)
         buf, at = _scratch(kv, nbytes, "attention call")
-        _lib.check(lib.tri_attend_paged(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), at, nbytes, _stream()))
+        _lib.check(lib.tri_attend_paged(kvs, bs, ps, at, nbytes, _stream()))
     return out, lse
 
 
 def block_bounds(kv: PagedKV) -> torch.Tensor:
     """An array for ``update_block_bounds``: [layers, blocks, Hkv, 2, D] of the cache's type (fp8 caches: bf16)."""
-    dtype = torch.bfloat16 if _DTYPES[kv.dtype] == KV_FP8_E4M3 else kv.dtype
-    return torch.zeros(kv.num_layers, kv.num_blocks, kv.num_kv_heads, 2, kv.head_dim, dtype=dtype, device=kv.device)
-
-
-def _checked_bounds(kv: PagedKV, bounds: torch.Tensor) -> torch.Tensor:
-    dtype = torch.bfloat16 if _DTYPES[kv.dtype] == KV_FP8_E4M3 else kv.dtype
-    shape = (kv.num_layers, kv.num_blocks, kv.num_kv_heads, 2, kv.head_dim)
-    if tuple(_on(kv, "bounds", bounds, dtype).shape) != shape or not bounds[0].is_contiguous():
-        raise ValueError(f"bounds must be {dtype} {shape}, contiguous within a layer")
-    return bounds
+    return torch.zeros(kv.num_layers, kv.num_blocks, kv.num_kv_heads, 2, kv.head_dim, dtype=_bounds_dtype(kv), device=kv.device)
 
 
 def update_block_bounds(kv: PagedKV, batch: StepBatch, bounds: torch.Tensor, *, new_tokens: int | None = None) -> torch.Tensor:
@@ -838,12 +856,12 @@ def update_block_bounds(kv: PagedKV, batch: StepBatch, bounds: torch.Tensor, *, 
     all its blocks; after a prompt or a compaction), every layer, into ``bounds`` (``tri_block_bounds``)."""
     lib = _lib.load()
     _check_attention_batch(kv, batch)
-    _checked_bounds(kv, bounds)
+    at = _bounds_address(kv, bounds)
     if new_tokens is not None and new_tokens < 1:
         raise ValueError(f"new_tokens must be positive or None, got {new_tokens}")
     with _on_device(kv.device):
-        _lib.check(lib.tri_block_bounds(C.byref(kv.struct), C.byref(batch.struct), kv.num_blocks, new_tokens or 0, _ptr(bounds),
-                                        int(bounds.stride(0)), _stream()))
+        _lib.check(lib.tri_block_bounds(C.byref(kv.struct), C.byref(batch.struct), kv.num_blocks, new_tokens or 0, at,
+                                        bounds.stride(0), _stream()))
     return bounds
 
 
@@ -859,15 +877,15 @@ def attend_blocks(kv: PagedKV, batch: StepBatch, q: torch.Tensor, bounds: torch.
     lib = _lib.load()
     if group_reduce not in ("max", "mean"):
         raise ValueError(f"group_reduce must be 'max' or 'mean', got {group_reduce!r}")
-    _checked_bounds(kv, bounds)
     p, out, lse = _attend_params(kv, batch, q, layer, None, None, 1, scale, k_scale, v_scale, out, want_lse)
     blocks = torch.empty((batch.num_seqs, kv.num_kv_heads, max(top_blocks, 0)), dtype=torch.int32, device=kv.device)
-    bp = BlockParams(bounds=_ptr(bounds[layer]), top_blocks=top_blocks, sink_blocks=sink_blocks, recent_blocks=recent_blocks,
-                     group_reduce=REDUCE_MAX if group_reduce == "max" else REDUCE_MEAN, blocks=_ptr(blocks))
+    bp = BlockParams(_bounds_address(kv, bounds, layer), top_blocks, sink_blocks, recent_blocks,
+                     REDUCE_MAX if group_reduce == "max" else REDUCE_MEAN, blocks.data_ptr())
     with _on_device(kv.device):
-        nbytes = int(lib.tri_attend_blocks_workspace_bytes(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), C.byref(bp)))
+        kvs, bs, ps, bps = C.byref(kv.struct), C.byref(batch.struct), C.byref(p), C.byref(bp)
+        nbytes = lib.tri_attend_blocks_workspace_bytes(kvs, bs, ps, bps)
         buf, at = _scratch(kv, nbytes, "attention call")
-        _lib.check(lib.tri_attend_blocks(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), C.byref(bp), at, nbytes, _stream()))
+        _lib.check(lib.tri_attend_blocks(kvs, bs, ps, bps, at, nbytes, _stream()))
     return out, lse, blocks
 
 
@@ -884,7 +902,7 @@ def _evict_params(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: Evic
     if batch.budgets is None:
         raise ValueError("batch has no budgets")
     _check_attention_batch(kv, batch)
-    _layer_weights(kv, weights)
+    at = _weights_address(kv, weights)
     if ev.layer_reduce not in ("mean", "max", None):
         raise ValueError(f"layer_reduce must be 'mean', 'max' or None, got {ev.layer_reduce!r}")
     if ev.protect_prefill and batch.prefill_lens is None:
@@ -897,8 +915,7 @@ def _evict_params(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: Evic
         raise ValueError(f"keep must be a contiguous int32 tensor with {rows} x {batch.max_budget} entries")
     lr = REDUCE_NONE if ev.layer_reduce is None else (REDUCE_MAX if ev.layer_reduce == "max" else REDUCE_MEAN)
     return EvictParams(num_blocks=kv.num_blocks, window_size=int(ev.window_size), protect_prefill=int(ev.protect_prefill),
-                       layer_reduce=lr, shared=int(ev.shared), weights=_ptr(weights),
-                       weights_stride_layer=int(weights.stride(0))), keep, rows
+                       layer_reduce=lr, shared=int(ev.shared), weights=at, weights_stride_layer=weights.stride(0)), keep, rows
 
 
 def select_by_weight(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: EvictConfig, *, want_scores: bool = False,
