@@ -10,7 +10,7 @@
 // S^T = K Q^T on the matrix cores (16 tokens x 16 rows x 32 elements) leaves in a lane the scores of one row (lane & 15) for
 // tokens (lane >> 4) * 4 + r: exactly the order in which the B operand of O^T = V^T P^T wants them, if the 32 tokens of that
 // product are numbered (lane >> 4) * 8 + j = token (j & 4) * 4 + (lane >> 4) * 4 + (j & 3).  So the weights never leave
-// their lane, a row's maximum is two exchanges between lanes, and the rescaling of O is a multiplication inside a lane.
+// their lane, and the rescaling of O is a multiplication inside a lane.
 // V^T comes out of LDS by the transposing read (16 lanes, 4 tokens x 16 elements).
 //
 // Up to 16 rows (attend_few_kernel) the four waves of a workgroup take tiles of 32 tokens in turn, keys straight from
@@ -32,6 +32,7 @@ namespace {
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / kWave;
 constexpr int kDies = 8;
+constexpr int kWaitLoads = 0x0f70;    // s_waitcnt vmcnt(0), the other counters left alone
 constexpr int kAttendTile = 32;       // tokens of one product with V
 
 template <int T>
@@ -189,65 +190,134 @@ __device__ __forceinline__ int tokens_of(const AttendLaunch& a, int b, int T) {
   return min(a.list_k, ceil_div(T, a.block_size)) * a.block_size;
 }
 
-// Places of tokens: a lane holds one token of a tile -- list entry, then page, then row, each asked for a tile ahead of the
-// next (a wait for a young load would be a wait for every older one).  The loads themselves are never skipped: where
-// one path has fewer of them, every wait behind it would be for all.
-struct Place {
-  int page, in;          // physical block and token in it; 0 and 0 for a token that is not there
-  bool ok;
-};
-template <int ES>
-struct Walk {
+// Where the tokens of a tile lie: list entry, then page, then row, each asked for a tile ahead of the next (a wait for a young
+// load would be a wait for every older one), by loads that are never skipped (where one path has fewer of them,
+// every wait behind it would be for all).
+struct Seq {
   const AttendLaunch& a;
   const int32_t* table;
   const int32_t* list;
-  int b, T, end, mine;
-  __device__ __forceinline__ Walk(const AttendLaunch& a_, int b_, int h, int T_, int end_, int mine_) : a(a_), b(b_), T(T_), end(end_), mine(mine_) {
+  int b, T, end, blocks;                     // blocks: that hold the sequence's tokens
+  __device__ __forceinline__ Seq(const AttendLaunch& a_, int b_, int h, int T_, int end_) : a(a_), b(b_), T(T_), end(end_) {
     table = a.block_table ? a.block_table + (int64_t)b * a.block_table_pitch : a.seq_lens;      // (any readable word where there is no table)
     list = a.list ? a.list + ((int64_t)b * a.Hkv + h) * a.list_pitch : nullptr;
+    blocks = div(T + a.block_size - 1);
   }
   // (t >= 0; exact below 2^31: the factor is 2^div_shift / block_size rounded up, div_shift = 31 + log2 block_size rounded up)
   __device__ __forceinline__ int div(int t) const { return (int)((uint64_t)(uint32_t)t * a.div_factor >> a.div_shift); }
   __device__ __forceinline__ int mod(int t) const { return t - div(t) * a.block_size; }
+  __device__ __forceinline__ uint64_t byte(int page, int in, int es) const {
+    return ((uint64_t)(uint32_t)page * (uint64_t)a.stride_block + (uint64_t)(uint32_t)in * (uint32_t)a.stride_token) * es;
+  }
+};
+
+// The tile of TOK tokens that comes next, STEP tokens apart; ok: which of its tokens there are.  Here for blocks of any size: a
+// lane holds one token of the tile.
+template <bool UNI, int ES, int TOK, int STEP>
+struct Finder {
+  const Seq& q;
+  int mine, page = 0, in = 0;                // of the lane's token; 0 and 0 for one that is not there
+  uint64_t ok = 0;
+  int next_tok = -1, next_page = -1, next2_entry = 0;
+  __device__ __forceinline__ Finder(const Seq& q_, int lane) : q(q_), mine(lane & (TOK - 1)) {}
   __device__ __forceinline__ int entry(int tile) const {
-    if (!list) return 0;
+    if (!q.list) return 0;
     const int t = tile + mine;
-    return list[t < end ? div(t) : 0];
+    return q.list[t < q.end ? q.div(t) : 0];
   }
   __device__ __forceinline__ int token(int tile, int entry) const {     // position in the sequence, or -1
     const int t = tile + mine;
-    const int tok = list ? entry * a.block_size + mod(t) : t;
-    return ((t < end) & (entry >= 0) & (tok < T)) ? tok : -1;
+    const int tok = q.list ? entry * q.a.block_size + q.mod(t) : t;
+    return ((t < q.end) & ((uint32_t)entry < (uint32_t)q.blocks) & (tok < q.T)) ? tok : -1;
   }
-  __device__ __forceinline__ int page(int tok) const {
-    const int p = table[a.block_table ? div(max(tok, 0)) : 0];
-    return a.block_table ? p : b;
+  __device__ __forceinline__ int page_of(int tok) const {
+    const int p = q.table[q.a.block_table ? q.div(max(tok, 0)) : 0];
+    return q.a.block_table ? p : q.b;
   }
-  __device__ __forceinline__ Place place(int tok, int page) const {
-    Place p;
-    p.ok = (tok >= 0) & ((uint32_t)page < (uint32_t)a.num_blocks);
-    p.page = p.ok ? page : 0;
-    p.in = p.ok ? mod(tok) : 0;
-    return p;
+  __device__ __forceinline__ void begin(int tile) {
+    next_tok = token(tile, entry(tile));
+    next_page = page_of(next_tok);
+    next2_entry = entry(tile + STEP);
   }
-  __device__ __forceinline__ uint64_t byte(int page, int in) const {
-    return ((uint64_t)(uint32_t)page * (uint64_t)a.stride_block + (uint64_t)(uint32_t)in * (uint32_t)a.stride_token) * ES;
+  __device__ __forceinline__ void take(int tile) {       // the places of `tile`; the next one's are asked for
+    const bool there = (next_tok >= 0) & ((uint32_t)next_page < (uint32_t)q.a.num_blocks);
+    page = there ? next_page : 0;
+    in = there ? q.mod(next_tok) : 0;
+    ok = __ballot(there);
+    if (TOK < 64) ok &= 0xffffffffu;
+    next_tok = token(tile + STEP, next2_entry);
+    next_page = page_of(next_tok);
+    next2_entry = entry(tile + 2 * STEP);
   }
-  __device__ __forceinline__ int64_t scale_at(const Place& p) const { return ((int64_t)p.page * a.block_size + p.in) * a.Hkv; }
+  __device__ __forceinline__ GlobalBytes row(GlobalBytes base, int, int r) const {
+    return base + q.byte(__shfl(page, r), __shfl(in, r), ES);
+  }
+  __device__ __forceinline__ int64_t scale_at(int) const { return ((int64_t)page * q.a.block_size + in) * q.a.Hkv; }
 };
 
-// Address of row `row` of a tile (lane `row` holds its place).  UNI: blocks of a multiple of 16 tokens, so that 16 tokens
-// in a row lie behind one another and their base is the same for the wave (row0: the first of the 16 that this
-// load takes rows of, the same for the wave).
-template <bool UNI, int ES>
-__device__ __forceinline__ GlobalBytes row_at(const Walk<ES>& walk, GlobalBytes base, const Place& p, int row0, int row) {
-  if constexpr (UNI) {
-    const int page = __builtin_amdgcn_readlane(p.page, row0), in = __builtin_amdgcn_readlane(p.in, row0);
-    return base + walk.byte(page, in) + (uint32_t)((row - row0) * (int)walk.a.stride_token * ES);
-  } else {
-    return base + walk.byte(__shfl(p.page, row), __shfl(p.in, row));
+// Blocks of a multiple of 16 tokens: 16 tokens in a row lie behind one another, so a tile is TOK / 16 places; lane g (and every
+// TOK / 16-th behind it) looks up the g-th.  A load of rows asks for the place of its own group alone, on the scalar unit, and
+// which tokens there are takes one comparison where all are.  (Scalar loads of the tables do worse: every wait for LDS
+// is then one for them too.)
+template <int ES, int TOK, int STEP>
+struct Finder<true, ES, TOK, STEP> {
+  static constexpr int kGroups = TOK / 16;
+  const Seq& q;
+  int ahead, now = 0, page = 0;
+  uint64_t ok = 0;
+  int next_entry = 0, next_page = 0, next2_entry = 0;       // of the lane's group
+  __device__ __forceinline__ Finder(const Seq& q_, int lane) : q(q_), ahead((lane & (kGroups - 1)) * 16) {}
+  __device__ __forceinline__ int entry(int tile) const {
+    if (!q.list) return 0;
+    const int t = tile + ahead;
+    return q.list[t < q.end ? q.div(t) : 0];
   }
-}
+  __device__ __forceinline__ int page_of(int tile, int entry) const {
+    const int t = tile + ahead;
+    const int p = q.table[!q.a.block_table ? 0 : q.list ? ((uint32_t)entry < (uint32_t)q.blocks ? entry : 0) : t < q.end ? q.div(t) : 0];
+    return q.a.block_table ? p : q.b;
+  }
+  __device__ __forceinline__ void begin(int tile) {
+    next_entry = entry(tile);
+    next_page = page_of(tile, next_entry);
+    next2_entry = entry(tile + STEP);
+  }
+  __device__ __forceinline__ void take(int tile) {
+    now = tile;
+    page = next_page;
+    bool whole = (uint32_t)page < (uint32_t)q.a.num_blocks;
+    if (q.list) whole &= ((uint32_t)next_entry < (uint32_t)q.blocks) & ((next_entry + 1) * q.a.block_size <= q.T);
+    constexpr uint64_t all = TOK < 64 ? 0xffffffffu : ~0ull;
+    ok = all;
+    if (tile + TOK > q.end || ~__ballot(whole)) {
+      ok = 0;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        const int t = tile + 16 * g, e = __builtin_amdgcn_readlane(next_entry, g), p = __builtin_amdgcn_readlane(page, g);
+        const int left = min(q.end - t, q.T - (q.list ? e * q.a.block_size + q.mod(t) : t));        // tokens from the group's first to the end
+        const bool there = (left > 0) & ((uint32_t)e < (uint32_t)q.blocks) & ((uint32_t)p < (uint32_t)q.a.num_blocks);
+        ok |= (uint64_t)(there ? (left >= 16 ? 0xffffu : (1u << left) - 1) : 0) << (16 * g);
+      }
+    }
+    next_entry = next2_entry;
+    next_page = page_of(tile + STEP, next_entry);
+    next2_entry = entry(tile + 2 * STEP);
+  }
+  // row0: the first row of the wave's load, all of whose rows lie in one group.  (A place that is not there: a row of another
+  // block, or of block 0.)
+  __device__ __forceinline__ GlobalBytes row(GlobalBytes base, int row0, int r) const {
+    const int g = row0 / 16;
+    int p = __builtin_amdgcn_readlane(page, g);
+    p = (uint32_t)p < (uint32_t)q.a.num_blocks ? p : 0;
+    return base + q.byte(p, q.mod(now + g * 16), ES) + (uint32_t)((r - g * 16) * (int)q.a.stride_token * ES);
+  }
+  __device__ __forceinline__ int64_t scale_at(int l) const {
+    const int g = (l & (TOK - 1)) / 16;
+    int p = __shfl(page, g);
+    p = (uint32_t)p < (uint32_t)q.a.num_blocks ? p : 0;
+    return ((int64_t)p * q.a.block_size + q.mod(now + g * 16) + (l & 15)) * q.a.Hkv;
+  }
+};
 
 // Queries of row c16 of 16 rows from m0 on: elements as the keys are loaded (fp8: 16 in a piece, two steps of 8).
 template <bool FP8, int D>
@@ -265,15 +335,16 @@ __device__ __forceinline__ void load_queries(const AttendLaunch& a, const RowRan
 // Infinities and NaNs among the values of new tokens reach the rows that see the token and no others (0 * inf in the matrix
 // product would put them into all of them, so there they are 0): rare, at the end, read from memory again.  Tokens from
 // first_tok to end of which every step-th piece of 32, from the piece-th on, is the caller's.
-template <int PT, bool FP8, int NT, int RT, int ES>
-__device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Walk<ES>& walk, GlobalBytes vb, int begin, int end, int base,
+template <int PT, bool FP8, int NT, int RT>
+__device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Seq& q, GlobalBytes vb, int begin, int base,
                                                const uint64_t (&seen)[RT], int lane, int piece, int step) {
+  constexpr int ES = FP8 ? 1 : 2;
 #pragma unroll 1
-  for (int tok = max(begin, base); tok < end; ++tok) {
+  for (int tok = max(begin, base); tok < q.end; ++tok) {
     if ((tok - begin) / kAttendTile % step != piece) continue;
-    const Place p = walk.place(tok, walk.page(tok));
-    if (!p.ok) continue;
-    const GlobalBytes row = vb + walk.byte(p.page, p.in);
+    const int page = q.a.block_table ? q.table[q.div(tok)] : q.b;
+    if (page < 0 || page >= q.a.num_blocks) continue;
+    const GlobalBytes row = vb + q.byte(page, q.mod(tok), ES);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -319,9 +390,20 @@ __device__ __forceinline__ void put_row(const AttendLaunch& a, const RowRange& r
   }
 }
 
-// Running maximum (base 2, behind the true one by at most kSlack) and sum of a row.
+// Where the scores of a wave's rows go, where weights are wanted.
+struct ScoreRows {
+  float* head;           // of the (sequence, KV head), or NULL
+  int64_t pitch;
+  int m0, M;
+};
+__device__ __forceinline__ ScoreRows score_rows(const AttendLaunch& a, int b, int h, int m0, int M) {
+  return {a.scores ? a.scores + ((int64_t)b * a.Hkv + h) * a.max_rows * a.G * a.score_pitch : nullptr, a.score_pitch, m0, M};
+}
+
+// Running maximum (base 2, behind the true one by at most kSlack) and sum of a row, with what every 32 tokens ask of the maximum:
+// the product above which it has to grow, and what is added to the exponents.
 struct RowState {
-  float top, sum;
+  float top = -INFINITY, sum = 0.f, grow = -INFINITY, down = 0.f;
 };
 // How far a score may lie above the maximum that weights are taken against before O is rescaled: weights stay below 2^8, far
 // inside either type, and a rescaling (a read and a write of all of O) is rare after the first tokens, where a new maximum is not.
@@ -340,7 +422,7 @@ __device__ __forceinline__ uint32_t seen_of(uint32_t okm, bool drafts, int first
 template <int PT, bool SCALED, int RT, int NT>
 __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT], f32x4 (&o)[RT][NT], u32x4 (&pf)[RT], float scale,
                                           const f32x4 (&ks)[2], const f32x4 (&vs)[2], bool masked, bool drafts, uint32_t okm, int first,
-                                          const uint64_t (&seen)[RT], int lane, float* const (&scores)[RT], int at) {
+                                          const uint64_t (&seen)[RT], int lane, const ScoreRows& scores, int at) {
   float best[RT];
   bool grows = false;
 #pragma unroll
@@ -358,38 +440,40 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
     }
     best[rt] = fmaxf(fmaxf(fmaxf(sc[rt][0][0], sc[rt][0][1]), fmaxf(sc[rt][0][2], sc[rt][0][3])),
                      fmaxf(fmaxf(sc[rt][1][0], sc[rt][1][1]), fmaxf(sc[rt][1][2], sc[rt][1][3])));
-    if (scores[rt]) {
-      *reinterpret_cast<f32x4*>(scores[rt] + at) = sc[rt][0] * scale;
-      *reinterpret_cast<f32x4*>(scores[rt] + at + 16) = sc[rt][1] * scale;
+    grows |= best[rt] > st[rt].grow;
+    if (scores.head) {
+      const int l = here(lane), m = scores.m0 + rt * 16 + (l & 15);
+      float* dst = scores.head + m * scores.pitch + at + (l >> 4) * 4;
+      if (m < scores.M) {
+        *reinterpret_cast<f32x4*>(dst) = sc[rt][0] * scale;
+        *reinterpret_cast<f32x4*>(dst + 16) = sc[rt][1] * scale;
+      }
     }
   }
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) best[rt] = fmaxf(best[rt], __shfl_xor(best[rt], 16));
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    best[rt] = fmaxf(best[rt], __shfl_xor(best[rt], 32)) * scale;
-    grows |= best[rt] > st[rt].top + kSlack;
-  }
+  // (the four lanes of a row only speak to each other where one of them has outgrown the maximum)
   if (__ballot(grows)) {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const float top = best[rt] > st[rt].top + kSlack ? best[rt] : st[rt].top;
+      float high = fmaxf(best[rt], __shfl_xor(best[rt], 16));
+      high = fmaxf(high, __shfl_xor(high, 32));
+      const float top = high > st[rt].grow ? high * scale : st[rt].top;
       const float alpha = rescale(st[rt].top, top);
       st[rt].top = top;
       st[rt].sum *= alpha;
+      st[rt].grow = (top + kSlack) / scale;
+      st[rt].down = top == -INFINITY ? 0.f : -top;
 #pragma unroll
       for (int t = 0; t < NT; ++t) o[rt][t] *= alpha;
     }
   }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const float down = st[rt].top == -INFINITY ? 0.f : -st[rt].top;
     float part = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        sc[rt][i][r] = pow2(__builtin_fmaf(sc[rt][i][r], scale, down));
+        sc[rt][i][r] = pow2(__builtin_fmaf(sc[rt][i][r], scale, st[rt].down));
         part += sc[rt][i][r];
       }
       if (SCALED) sc[rt][i] *= vs[i];
@@ -443,43 +527,43 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   uint64_t seen[1] = {1};
   if (n > 1) seen[0] = (uint64_t)shfl64((int64_t)ancestor_mask(a.parents, rows.first, n, lane), min(c16, M - 1) / a.G);
 
-  const Walk<ES> walk(a, b, h, T, end, lane & (kAttendTile - 1));
+  const Seq seq(a, b, h, T, end);
+  Finder<UNI, ES, kAttendTile, kStep> find(seq, lane);
   const int first_tile = begin + wave * kAttendTile;
   u32x4 kr[2][KC], vr[NV];
   float ks_mine = 0.f, vs_mine = 0.f;
-  auto load_keys = [&](const Place& p) {
+  auto load_keys = [&] {
     if (scaled) {
-      ks_mine = ksc[walk.scale_at(p)];
-      vs_mine = vsc[walk.scale_at(p)];
+      ks_mine = ksc[find.scale_at(lane)];
+      vs_mine = vsc[find.scale_at(lane)];
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const GlobalBytes src = row_at<UNI, ES>(walk, kb, p, i * 16, i * 16 + c16) + q4 * 16;
+      const GlobalBytes src = find.row(kb, i * 16, i * 16 + c16) + q4 * 16;
 #pragma unroll
       for (int c = 0; c < KC; ++c) kr[i][c] = *(GlobalU4)(src + c * 64);
     }
   };
-  auto load_values = [&](const Place& p) {
+  auto load_values = [&] {
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      vr[i] = *(GlobalU4)(row_at<UNI, ES>(walk, vb, p, i * RPL / 16 * 16, i * RPL + lane / LPR) + (lane % LPR) * 16);
+      vr[i] = *(GlobalU4)(find.row(vb, i * RPL, i * RPL + lane / LPR) + (lane % LPR) * 16);
   };
 
-  float* const scores[1] = {a.scores && c16 < M ? a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + c16) * a.score_pitch + q4 * 4 : nullptr};
+  const ScoreRows scores = score_rows(a, b, h, 0, M);
 
   f32x4 o[1][NT];
   bool odd = false;
-  RowState st[1] = {{-INFINITY, 0.f}};
+  RowState st[1];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   unsigned char* const my_v = s_v + wave * kWaveBytes;
   const LdsBytes my_lds = (LdsBytes)my_v + (q4 * 4 + (c16 >> 2)) * kPitch + (c16 & 3) * 8;
-  Place now{}, next{};
-  int next_tok = -1, next_page = -1, next2_entry = 0;
+  uint32_t ok_now = 0;
   // One tile; the last one has no next (a body of its own: see the loads above).
   auto step = [&](int tile, auto has_next) {
     constexpr bool more = decltype(has_next)::value;
-    const uint32_t okm = (uint32_t)__ballot(now.ok);
+    const uint32_t okm = ok_now;
     const bool drafts = n > 1 && tile + kAttendTile > base;
 
     f32x4 sc[1][2];
@@ -504,11 +588,9 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     __builtin_amdgcn_sched_barrier(0);
     // the next tile's keys into the registers of this one's, this one's values into LDS
     if constexpr (more) {
-      next = walk.place(next_tok, next_page);
-      next_tok = walk.token(tile + 2 * kStep, next2_entry);
-      next_page = walk.page(next_tok);
-      next2_entry = walk.entry(tile + 3 * kStep);
-      load_keys(next);
+      find.take(tile + kStep);
+      ok_now = (uint32_t)find.ok;
+      load_keys();
     }
     if (okm != 0xffffffffu || drafts) {
       // What lies behind the end is 0 in the product (0 * what is there could be NaN), and so are a new token's infinities.
@@ -530,7 +612,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
         dst[0] = vr[i];
       }
     }
-    if constexpr (more) load_values(next);
+    if constexpr (more) load_values();
     __builtin_amdgcn_sched_barrier(0);
     const bool masked = okm != 0xffffffffu || drafts;
     u32x4 pf[1];
@@ -553,25 +635,21 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
       o[0][t] = mfma<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[0], o[0][t]);
     }
     __builtin_amdgcn_wave_barrier();
-    now = next;
   };
   if (first_tile < end) {
-    const int tok = walk.token(first_tile, walk.entry(first_tile));
-    next_tok = walk.token(first_tile + kStep, walk.entry(first_tile + kStep));
-    const int page = walk.page(tok);
-    next_page = walk.page(next_tok);
-    next2_entry = walk.entry(first_tile + 2 * kStep);
+    find.begin(first_tile);
+    find.take(first_tile);
+    ok_now = (uint32_t)find.ok;
     __builtin_amdgcn_sched_barrier(0);
-    now = walk.place(tok, page);
-    load_keys(now);
+    load_keys();
     __builtin_amdgcn_sched_barrier(0);
-    load_values(now);
+    load_values();
     __builtin_amdgcn_sched_barrier(0);
     int tile = first_tile;
     for (; tile + kStep < end; tile += kStep) step(tile, std::true_type{});
     if (tile < end) step(tile, std::false_type{});
   }
-  if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, walk, vb, begin, end, base, seen, lane, wave, kAttendWaves);
+  if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, seq, vb, begin, base, seen, lane, wave, kAttendWaves);
 
   // the four waves meet
   st[0].sum += __shfl_xor(st[0].sum, 16);
@@ -635,7 +713,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   const int n = rows.n, M = n * a.G;
   if (rb * RT * 16 * W >= M) return;
   const int m0 = (rb * W + wave) * RT * 16;
-  const bool loads = wave * RPL < BT;                     // (small rows: a load of every wave would be more than a tile)
+  const bool loads = RPL * W <= BT || wave * RPL < BT;    // (small rows: a load of every wave would be more than a tile)
   const int Tv = tokens_of(a, b, T);
   const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
   if (begin >= Tv && split > 0) return;
@@ -646,29 +724,27 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   const GlobalF32 ksc = scaled ? (GlobalF32)a.k_scale_layers[a.layer] + h : nullptr;
   const GlobalF32 vsc = scaled ? (GlobalF32)a.v_scale_layers[a.layer] + h : nullptr;
 
-  const Walk<ES> walk(a, b, h, T, end, lane & (BT - 1));
+  const Seq seq(a, b, h, T, end);
+  Finder<UNI, ES, BT, BT> find(seq, lane);
   u32x4 kr[NL], vr[NL];
   float ks_mine = 0.f, vs_mine = 0.f;
-  Place p[2] = {};                       // of the tile in LDS, and of the one in registers
-  auto load = [&](const Place& at) {
+  uint64_t ok_now = 0;                   // tokens of the tile at work that are there
+  auto load = [&] {
     if (!loads) return;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      // (rows of this load: 16-row group i * 4 * RPL + wave * RPL lies in, the same for the whole wave)
-      const int row0 = (i * W + wave) * RPL;
-      const GlobalBytes k = row_at<UNI, ES>(walk, kb, at, row0 / 16 * 16, row0 + lane / LPR) + (lane % LPR) * 16;
-      const GlobalBytes v = row_at<UNI, ES>(walk, vb, at, row0 / 16 * 16, row0 + lane / LPR) + (lane % LPR) * 16;
-      kr[i] = *(GlobalU4)k;
-      vr[i] = *(GlobalU4)v;
+      const int row0 = (i * W + wave) * RPL;              // (the load's rows: all in one group of 16, the same for the whole wave)
+      kr[i] = *(GlobalU4)(find.row(kb, row0, row0 + lane / LPR) + (lane % LPR) * 16);
+      vr[i] = *(GlobalU4)(find.row(vb, row0, row0 + lane / LPR) + (lane % LPR) * 16);
     }
     if (scaled && wave == 0) {
-      ks_mine = ksc[walk.scale_at(at)];
-      vs_mine = vsc[walk.scale_at(at)];
+      ks_mine = ksc[find.scale_at(lane)];
+      vs_mine = vsc[find.scale_at(lane)];
     }
   };
-  auto store = [&](const Place& at, int tile, int buf) {
+  auto store = [&](int tile, int buf) {
+    const uint64_t okm = find.ok;
     if (!loads) return;
-    const uint64_t okm = __ballot(at.ok);
     const bool all = BT == 64 ? okm == ~0ull : (uint32_t)okm == ~0u;
     const bool drafts = n > 1 && tile + BT > base;
     if (!all || drafts) {
@@ -704,20 +780,15 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   };
 
   // tile t in LDS, t + 1 in registers, pages of t + 2 and list entries of t + 3 on their way
-  int next_tok = -1, next_page = -1, next2_entry = 0;
   if (threadIdx.x == 0) s_odd = 0;
   if (begin < end) {
-    const int tok = walk.token(begin, walk.entry(begin));
-    next_tok = walk.token(begin + BT, walk.entry(begin + BT));
-    const int page = walk.page(tok);
-    next_page = walk.page(next_tok);
-    next2_entry = walk.entry(begin + 2 * BT);
-    p[0] = walk.place(tok, page);
-    load(p[0]);
+    find.begin(begin);
+    find.take(begin);
+    load();
   }
   u32x4 qf[RT][D / 32];
   uint64_t seen[RT];
-  float* scores[RT];
+  const ScoreRows scores = score_rows(a, b, h, m0, M);
   f32x4 o[RT][NT];
   RowState st[RT];
   const uint64_t anc = n > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
@@ -726,81 +797,117 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     const int m = m0 + rt * 16 + c16;
     load_queries<FP8, D>(a, rows, h, m0 + rt * 16, M, lane, qf[rt]);
     seen[rt] = (uint64_t)shfl64((int64_t)anc, min(m, M - 1) / a.G);
-    scores[rt] = a.scores && m < M ? a.scores + (((int64_t)b * a.Hkv + h) * a.max_rows * a.G + m) * a.score_pitch + q4 * 4 : nullptr;
-    st[rt] = RowState{-INFINITY, 0.f};
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[rt][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
   __syncthreads();          // (s_odd)
+  // The queries are waited for here: left to the loop, the wait for them would be one for the next tile's rows in every turn.
+  __builtin_amdgcn_s_waitcnt(kWaitLoads);
+  // (The next tile is asked for in any case, see Seq: behind the end that is some row of the pool, one tile a workgroup.)
   if (begin < end) {
-    store(p[0], begin, 0);
-    p[1] = walk.place(next_tok, next_page);
-    next_tok = walk.token(begin + 2 * BT, next2_entry);
-    next_page = walk.page(next_tok);
-    next2_entry = walk.entry(begin + 3 * BT);
-    if (begin + BT < end) load(p[1]);
+    store(begin, 0);
+    ok_now = find.ok;
+    find.take(begin + BT);
+    load();
   }
   __syncthreads();
-  for (int tile = begin, buf = 0; tile < end; tile += BT, buf ^= 1) {
-    if (m0 < M) {
-      const uint64_t okm_all = __ballot(p[0].ok);
+
+  u32x4 kf[2][D / 32], pf[RT];
+  u32x2 vlo[NT], vhi[NT];
+  f32x4 sc[RT][2];
+  auto read_keys = [&](int sub, int buf) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned char* src = s_k[buf] + (sub * 32 + i * 16 + c16) * kKeyPitch;
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) {
+        const int el = FP8 ? (s / 2) * 64 + q4 * 16 + (s & 1) * 8 : s * 32 + q4 * 8;
+        kf[i][s] = *reinterpret_cast<const u32x4*>(src + el * 2);
+      }
+    }
+  };
+  auto read_values = [&](int sub, int buf, int from, int to) {
+    const LdsBytes at = (LdsBytes)s_v[buf] + (sub * 32 + q4 * 4 + (c16 >> 2)) * kValPitch + (c16 & 3) * 8;
+#pragma unroll
+    for (int t = from; t < to; ++t) {
+      vlo[t] = lds_read_transposed(at + t * 32);
+      vhi[t] = lds_read_transposed(at + t * 32 + 16 * kValPitch);
+    }
+  };
+  auto times_keys = [&] {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) sc[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt][i] = mfma<QT>(kf[i][s], qf[rt][s], sc[rt][i]);
+    }
+  };
+  auto times_values = [&] {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const u32x4 vf{vlo[t][0], vlo[t][1], vhi[t][0], vhi[t][1]};
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma<PT>(vf, pf[rt], o[rt][t]);
+    }
+  };
+  auto softmax = [&](int first, int sub, int buf) {
+    const uint32_t okm = (uint32_t)(ok_now >> (sub * 32));
+    const bool drafts = n > 1 && first + 32 > base;
+    const bool masked = okm != 0xffffffffu || drafts;
+    f32x4 ks[2] = {}, vs[2] = {};
+    if (scaled) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[buf][0][sub * 32 + i * 16 + q4 * 4]);
+        vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[buf][1][sub * 32 + i * 16 + q4 * 4]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ks[i] = vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
+    }
+    softmax32<PT, FP8, RT, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
+  };
+  const bool busy = m0 < M;
+  // A tile, while the next one goes from registers to LDS and the one behind it is asked for.
+  auto step = [&](int tile, int buf, auto has_next) {
+    constexpr bool more = decltype(has_next)::value;
+    uint64_t ok_after = 0;
+    if (more) {
+      store(tile + BT, buf ^ 1);
+      ok_after = find.ok;
+      find.take(tile + 2 * BT);
+      load();
+    }
+    if (busy) {
 #pragma unroll
       for (int sub = 0; sub < BT / 32; ++sub) {
         const int first = tile + sub * 32;
-        if (sub > 0 && first >= end) continue;           // (nothing there, and rows of scores are whole pieces of 32 tokens)
-        const uint32_t okm = (uint32_t)(okm_all >> (sub * 32));
-        const bool drafts = n > 1 && first + 32 > base;
-        const bool masked = okm != 0xffffffffu || drafts;
-        f32x4 sc[RT][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) sc[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-          const unsigned char* src = s_k[buf] + (sub * 32 + i * 16 + c16) * kKeyPitch;
-#pragma unroll
-          for (int s = 0; s < D / 32; ++s) {
-            const int el = FP8 ? (s / 2) * 64 + q4 * 16 + (s & 1) * 8 : s * 32 + q4 * 8;
-            const u32x4 kf = *reinterpret_cast<const u32x4*>(src + el * 2);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) sc[rt][i] = mfma<QT>(kf, qf[rt][s], sc[rt][i]);
-          }
-        }
-        u32x4 pf[RT];
-        f32x4 ks[2] = {}, vs[2] = {};
-        if (scaled) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[buf][0][sub * 32 + i * 16 + q4 * 4]);
-            vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[buf][1][sub * 32 + i * 16 + q4 * 4]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) ks[i] = vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
-        }
-        softmax32<PT, FP8, RT, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
-        const LdsBytes at = (LdsBytes)s_v[buf] + (sub * 32 + q4 * 4 + (c16 >> 2)) * kValPitch + (c16 & 3) * 8;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const u32x2 lo = lds_read_transposed(at + t * 32), hi = lds_read_transposed(at + t * 32 + 16 * kValPitch);
-          const u32x4 vf{lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma<PT>(vf, pf[rt], o[rt][t]);
-        }
+        if (!more && sub > 0 && first >= end) continue;  // (nothing there, and rows of scores are whole pieces of 32 tokens)
+        // (values asked for before the softmax, which hides their way out of LDS)
+        constexpr int kEarly = NT * RT <= 8 ? NT : NT / 2;
+        read_keys(sub, buf);
+        __builtin_amdgcn_sched_barrier(0);
+        times_keys();
+        __builtin_amdgcn_sched_barrier(0);
+        read_values(sub, buf, 0, kEarly);
+        __builtin_amdgcn_sched_barrier(0);
+        softmax(first, sub, buf);
+        __builtin_amdgcn_sched_barrier(0);
+        read_values(sub, buf, kEarly, NT);
+        times_values();
       }
     }
-    if (tile + BT < end) {
-      store(p[1], tile + BT, buf ^ 1);
-      p[0] = p[1];
-      p[1] = walk.place(next_tok, next_page);
-      next_tok = walk.token(tile + 3 * BT, next2_entry);
-      next_page = walk.page(next_tok);
-      next2_entry = walk.entry(tile + 4 * BT);
-      if (tile + 2 * BT < end) load(p[1]);
-    }
-    __syncthreads();
-  }
-  if (s_odd) add_odd_values<PT, FP8, NT, RT>(o, walk, vb, begin, end, base, seen, lane, 0, 1);
+    ok_now = ok_after;
+    if (more) __syncthreads();
+  };
+  int tile = begin, buf = 0;
+  for (; tile + BT < end; tile += BT, buf ^= 1) step(tile, buf, std::true_type{});
+  if (tile < end) step(tile, buf, std::false_type{});
+  if (s_odd) add_odd_values<PT, FP8, NT, RT>(o, seq, vb, begin, base, seen, lane, 0, 1);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     st[rt].sum += __shfl_xor(st[rt].sum, 16);
