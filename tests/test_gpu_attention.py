@@ -222,6 +222,46 @@ def test_long_and_split_sequences():
         _check_weights(case, weights, before, want, "add")
 
 
+@pytest.mark.parametrize("dim,rows,types", [
+    (64, 1, dict()), (64, 3, dict(dtype=FP8, row_scales=True)), (128, 1, dict(dtype=FP16)), (128, 4, dict()),
+    (128, 2, dict(dtype=FP8, query=FP16, row_scales=True)), (256, 1, dict(dtype=FP8)), (256, 2, dict()),
+])
+def test_many_tokens_and_heads(dim, rows, types):
+    """So many that a wave has a KV head to itself: empty sequences, short ones and those of several splits, some pages bad."""
+    lens = [9000, 1, 0, 700, 33, 12500, 4, 2048, 9985, 31]
+    case = Case(lens, q_heads=32, kv_heads=16, dim=dim, rows=[min(rows, t) for t in lens], seed=dim + rows, **types)
+    case.tables[0][100], case.tables[0][101], case.tables[3][-1] = -1, case.pool, 1 << 30
+    kv, batch = case.device()
+    before = _weights(case)
+    weights = before.to(DEV)
+    print(f"many dim={dim} rows={rows} {types}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, parents=case.dev_parents, max_rows=rows,
+                                weights=weights, want_lse=True)
+    want = case.expected()
+    _check_rows(case, out, lse, want)
+    _check_weights(case, weights, before, want, "add")
+
+
+def test_blocks_of_many_heads():
+    """Lists of blocks long enough that a wave has a KV head, and so a list, to itself: all blocks chosen is all of the cache."""
+    case = Case([600 - 7 * i for i in range(56)], q_heads=32, kv_heads=32, dim=64, block=32, seed=5)
+    kv, batch = case.device()
+    bounds = ops.update_block_bounds(kv, batch, ops.block_bounds(kv))
+    print("blocks of many heads", flush=True)
+    q = case.q.to(DEV)
+    out, lse, blocks = ops.attend_blocks(kv, batch, q, bounds, top_blocks=19, want_lse=True)
+    _check_rows(case, out, lse, case.expected())
+    assert blocks[0].tolist() == [list(range(19))] * 32
+    # ten of them: the same blocks in a call of its own for each sequence, which shares the heads' tokens among waves
+    out, lse, blocks = ops.attend_blocks(kv, batch, q, bounds, top_blocks=10, want_lse=True)
+    for b in (0, 20, 55):
+        one = ops.StepBatch(torch.device(DEV), [case.lens[b]], block_tables=torch.tensor([case.tables[b]], dtype=torch.int32, device=DEV))
+        alone, lse1, blocks1 = ops.attend_blocks(kv, one, q[b:b + 1], bounds, top_blocks=10, want_lse=True)
+        assert torch.equal(blocks1[0], blocks[b])
+        assert float((lse1[0] - lse[b]).abs().max()) < 1e-4
+        assert float((alone[0].float() - out[b].float()).abs().max()) <= 2.0 ** -6 * float(alone.float().abs().max())
+
+
 # ----------------------------------------------------------------------------------- trees
 @pytest.mark.parametrize("dim,heads,rows,types", [
     (128, (8, 2), [4, 1, 0, 7], dict()), (128, (8, 2), [16, 3, 20, 5], dict()), (128, (8, 1), [16, 9, 1, 0], dict()),

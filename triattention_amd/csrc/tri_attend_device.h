@@ -15,9 +15,9 @@
 //
 // Up to 16 rows (attend_few_kernel) the four waves of a workgroup take tiles of 32 tokens in turn, keys straight from
 // memory into the operand's registers, and meet once at the end: such a call is bound by reading K and V, and what
-// counts is how many bytes are asked for at a time.  Beyond that (attend_rows_kernel) every wave has rows of its own and
+// counts is how many bytes are asked for at a time; in long sequences they take a KV head each instead.  Beyond that (attend_rows_kernel) every wave has rows of its own and
 // the workgroup shares the tiles through LDS: a tile is read from memory once for up to 256 rows.  A sequence is cut into
-// splits where there are few rows, joined by attend_join_kernel.
+// splits, as many as the chip has room for at once, joined by attend_finish_kernel.
 #pragma once
 
 #include <type_traits>
@@ -167,7 +167,7 @@ struct Work {
   int b, split, h, rb;
 };
 __device__ __forceinline__ bool work_of(const AttendLaunch& a, Work& w) {
-  const int inner_n = a.Hkv * a.row_blocks;
+  const int heads = a.Hkv / a.heads_per_group, inner_n = heads * a.row_blocks;
   int unit, inner;
   if (a.by_xcd) {
     const int l = blockIdx.x / kDies;
@@ -177,8 +177,8 @@ __device__ __forceinline__ bool work_of(const AttendLaunch& a, Work& w) {
     inner = blockIdx.x % inner_n;
     unit = blockIdx.x / inner_n;
   }
-  w.h = inner % a.Hkv;
-  w.rb = inner / a.Hkv;
+  w.h = inner % heads * a.heads_per_group;
+  w.rb = inner / heads;
   w.split = unit % a.nsplit;
   w.b = unit / a.nsplit;
   return w.b < a.B;
@@ -485,7 +485,7 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
 }
 
 // ---- up to 16 rows of a KV head
-template <int QT, bool FP8, int D, bool UNI>
+template <int QT, bool FP8, int D, bool UNI, bool HEADS>
 __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) void attend_few_kernel(AttendLaunch a) {
   constexpr int PT = FP8 ? TRI_KV_BF16 : QT;              // fp8 rows with a scale of their own: the weight carries it, which fp16 has no room for
   constexpr int ES = FP8 ? 1 : 2;
@@ -496,7 +496,8 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   constexpr int NT = D / 16;
   constexpr int kPitch = D * 2 + 32;                      // bytes of a value row in LDS: eight rows reach all banks
   constexpr int kWaveBytes = kAttendTile * kPitch;
-  constexpr int kStep = kAttendWaves * kAttendTile;
+  constexpr int kParts = HEADS ? 1 : kAttendWaves;        // waves that share a head's tokens
+  constexpr int kStep = kParts * kAttendTile;
   __shared__ __align__(16) unsigned char s_v[kAttendWaves * kWaveBytes];
   __shared__ __align__(16) float s_scale[kAttendWaves][2][kAttendTile];
   __shared__ float s_ml[kAttendWaves][16][2];
@@ -505,7 +506,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   const int c16 = lane & 15, q4 = lane >> 4;
   Work work;
   if (!work_of(a, work)) return;
-  const int b = work.b, split = work.split, h = work.h;
+  const int b = work.b, split = work.split, h = work.h + (HEADS ? wave : 0), part = HEADS ? 0 : wave;
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   const RowRange rows = rows_of(a, b);
@@ -529,7 +530,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
 
   const Seq seq(a, b, h, T, end);
   Finder<UNI, ES, kAttendTile, kStep> find(seq, lane);
-  const int first_tile = begin + wave * kAttendTile;
+  const int first_tile = begin + part * kAttendTile;
   u32x4 kr[2][KC], vr[NV];
   float ks_mine = 0.f, vs_mine = 0.f;
   auto load_keys = [&] {
@@ -649,11 +650,17 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     for (; tile + kStep < end; tile += kStep) step(tile, std::true_type{});
     if (tile < end) step(tile, std::false_type{});
   }
-  if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, seq, vb, begin, base, seen, lane, wave, kAttendWaves);
+  if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, seq, vb, begin, base, seen, lane, part, kParts);
 
-  // the four waves meet
   st[0].sum += __shfl_xor(st[0].sum, 16);
   st[0].sum += __shfl_xor(st[0].sum, 32);
+  if constexpr (HEADS) {
+    if (c16 >= M) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) put_row<QT, D>(a, rows, b, h, split, c16, t * 16 + q4 * 4, o[0][t], st[0].top, st[0].sum);
+    return;
+  }
+  // the four waves meet
   if (q4 == 0) {
     s_ml[wave][c16][0] = st[0].top;
     s_ml[wave][c16][1] = st[0].sum;
@@ -922,8 +929,9 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
 template <int QT, bool FP8, int D, bool UNI>
 hipError_t launch_attend_typed(const AttendLaunch& a, hipStream_t s) {
   const int64_t units = (int64_t)a.B * a.nsplit;
-  const dim3 grid((unsigned)((a.by_xcd ? align_up(units, kDies) : units) * a.row_blocks * a.Hkv));
-  if (a.row_tiles == 0) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI>), grid, dim3(kAttendThreads), 0, s, a);
+  const dim3 grid((unsigned)((a.by_xcd ? align_up(units, kDies) : units) * a.row_blocks * (a.Hkv / a.heads_per_group)));
+  if (a.heads_per_group > 1) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI, true>), grid, dim3(kAttendThreads), 0, s, a);
+  else if (a.row_tiles == 0) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI, false>), grid, dim3(kAttendThreads), 0, s, a);
   else if (a.row_tiles == 4) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 1, 4, UNI>), grid, dim3(4 * kWave), 0, s, a);
   else if (a.row_tiles == 8) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 1, 8, UNI>), grid, dim3(8 * kWave), 0, s, a);
   else if constexpr (D <= 128) {

@@ -973,16 +973,30 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   // A split is as long as lets every workgroup run at once: on from the mean over what the chip holds, until the splits
   // of all sequences fit (each sequence's last one is short).
   const int64_t holds = 256 * attend_workgroups_per_cu(a.row_tiles, a.D);
-  constexpr int step = 128;      // whole tiles of every kernel (a single tile a workgroup saves the attention nothing and costs the join)
-  const int64_t inner = (int64_t)a.Hkv * a.row_blocks, most = tri::align_up(longest, step);
-  int64_t split = std::min<int64_t>(tri::align_up(std::max<int64_t>(tri::ceil_div64(total * inner, holds), 1), step), most);
-  for (; split < most; split += step) {
-    int64_t count = 0;
-    for (int b = 0; b < a.B; ++b)
-      count += std::max<int64_t>(1, tri::ceil_div64(std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest), split));
-    if (count * inner <= holds) break;
+  auto length = [&](int64_t inner, int step) {
+    const int64_t most = tri::align_up(longest, step);
+    int64_t split = std::min<int64_t>(tri::align_up(std::max<int64_t>(tri::ceil_div64(total * inner, holds), 1), step), most);
+    for (; split < most; split += step) {
+      int64_t count = 0;
+      for (int b = 0; b < a.B; ++b)
+        count += std::max<int64_t>(1, tri::ceil_div64(std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest), split));
+      if (count * inner <= holds) break;
+    }
+    return (int)split;
+  };
+  // Few rows of long sequences: a workgroup takes four KV heads, a wave each.  Its waves then read neighbouring rows, a token's
+  // heads lie side by side, and have nothing to join: 16 x 16384 tokens of fp8 114 us against 125 with four waves to a head, 24
+  // ragged ones of up to 8192 with 64 dimensions 48 against 55.  The splits are a quarter as long, which has to leave a wave
+  // enough to do: at 128 tokens a split 1 x 32768 of 128 dimensions take 42 us against 37, at 256 the two are level (rows of up
+  // to 128 bytes gain from 128 tokens on: 41 us against 45 for 64 x 1024).
+  a.heads_per_group = 1;
+  const int row_bytes = a.D * (a.kv_dtype == TRI_KV_FP8_E4M3 ? 1 : 2);
+  if (a.row_tiles == 0 && a.Hkv % 4 == 0 && a.block_size % 16 == 0) {
+    a.split_tokens = length(a.Hkv / 4, 32);
+    if (a.split_tokens >= (row_bytes <= 128 ? 128 : 256)) a.heads_per_group = 4;
   }
-  a.split_tokens = (int)split;
+  // (128: whole tiles of every kernel; a single tile a workgroup saves the attention nothing and costs the join)
+  if (a.heads_per_group == 1) a.split_tokens = length((int64_t)a.Hkv * a.row_blocks, 128);
   a.nsplit = (int)tri::ceil_div64(longest, a.split_tokens);
   a.by_xcd = a.row_blocks > 1 && (int64_t)a.B * a.nsplit >= 32;
   int64_t off = 0;

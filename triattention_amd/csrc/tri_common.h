@@ -279,6 +279,7 @@ struct AttendLaunch {
   int list_k, list_pitch;
   // how the work is cut
   int row_tiles, row_blocks, nsplit, split_tokens, by_xcd;         // row_tiles: tiles of 16 rows a workgroup has; 0: the kernel for up to 16 rows
+  int heads_per_group;                                     // KV heads of a workgroup
   // workspace
   float* part_out;                                         // [B][Hkv][nsplit][max_rows * G][D], not normalised (nsplit > 1)
   float* part_ml;                                          // the same rows' maximum (base 2) and sum
