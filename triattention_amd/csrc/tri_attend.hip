@@ -1,4 +1,4 @@
-// What follows attend_kernel (tri_attend_device.h): the splits of a sequence joined, and the weights its tokens received
+// What follows the attention itself (tri_attend_device.h): the splits of a sequence joined, and the weights its tokens received
 // added up beside the cache.
 #include "tri_attend_device.h"
 
@@ -148,7 +148,7 @@ __device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weight
       if (h0 + e < a.Hkv) w[e] = sum[e];
 }
 
-// The splits joined and the weights added up, in one launch: both start from what attend_kernel left.
+// The splits joined and the weights added up, in one launch: both start from what the attention left.
 template <int QT, int D, int PARTS, bool VEC>
 __global__ __launch_bounds__(kThreads) void attend_finish_kernel(AttendLaunch a, int join_groups, float* weights, int set) {
   if ((int)blockIdx.x < join_groups) join_rows<QT, D, PARTS>(a, blockIdx.x);
