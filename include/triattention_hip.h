@@ -384,10 +384,11 @@ typedef struct tri_attend_params {
                                    NULL: one row per sequence */
   const int32_t* parents;       /* [num_rows] of every row, counted from the sequence's first row: the row it follows; any value
                                    outside [0, own index): it follows the last token before the new ones.  NULL: each follows the one before it */
-  float scale, k_scale, v_scale;
+  float scale, k_scale, v_scale; /* scale * k_scale positive */
   float* weights;               /* the layer's accumulated weights [num_blocks][block_size][num_kv_heads] (the place of a slot's
                                    weight is that of an fp8 slot's scale), or NULL: every slot the rows see receives the sum of
-                                   their softmax weights over rows and query heads of its KV head */
+                                   their softmax weights over rows and query heads of its KV head.  No two sequences
+                                   of the call may then share a block (each would read and write its weights) */
   int32_t weight_mode;          /* 0: added, for the new tokens' own slots written; 1: written for every token of a sequence */
 } tri_attend_params;
 uint64_t tri_attend_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p);
@@ -419,7 +420,7 @@ int tri_attend_blocks(const tri_kv_layout* kv, const tri_batch* batch, const tri
 /* Eviction by the weights tri_attend_paged adds up, in place of the calibrated scores: per sequence and KV head the budget
  * tokens of the largest weight (mean over layers summed in 64 bits, or maximum; layer_reduce -1: a keep set per layer), the
  * last window_size tokens and, with protect_prefill, those before prefill_lens always among the first choices; ties keep
- * the lowest token.  keep: int32 [rows][max_budget] as tri_select's, -1 behind a sequence's budget; final_scores (may be
+ * the lowest token, a NaN counts as more than any number.  keep: int32 [rows][max_budget] as tri_select's, -1 behind a sequence's budget; final_scores (may be
  * NULL): [rows][max_seq_len], +inf where guarded, -inf behind the sequence.  tri_evict_step also moves K, V, their scales
  * and the weights of the kept tokens into the first slots (tri_compact_paged); its block table must be valid. */
 typedef struct tri_evict_params {

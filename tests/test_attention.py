@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import time
 
 import pytest
 import torch
@@ -74,6 +75,7 @@ def test_attention_plans_are_made_without_a_device():
     ({}, {}, dict(parents=8), _lib.TRI_ERR_INVALID_ARGUMENT, b"parents"),
     ({}, {}, dict(q_stride_row=8 * 128 + 4), _lib.TRI_ERR_INVALID_ARGUMENT, b"strides"),
     ({}, {}, dict(out_stride_head=64), _lib.TRI_ERR_INVALID_ARGUMENT, b"out_stride_head"),
+    ({}, {}, dict(out_stride_row=64), _lib.TRI_ERR_INVALID_ARGUMENT, b"out_stride_row"),
     ({}, {}, dict(scale=math.nan), _lib.TRI_ERR_INVALID_ARGUMENT, b"finite"),
     ({}, {}, dict(scale=0.0), _lib.TRI_ERR_INVALID_ARGUMENT, b"positive"),
     ({}, {}, dict(scale=-1.0), _lib.TRI_ERR_INVALID_ARGUMENT, b"positive"),
@@ -89,6 +91,23 @@ def test_attention_refuses(layout, batch, params, code, word):
     assert word in lib.tri_last_error()
     if "q" not in params and "out" not in params:
         assert lib.tri_attend_workspace_bytes(*args) == 0
+
+
+def test_plans_of_many_sequences_stay_small_and_are_made_quickly():
+    """A long sequence among many short ones is cut, the partial results stay within 512 MiB, and no number of sequences makes the host search long."""
+    lib = _lib.load()
+    for num, rows in ((600, 1), (600, 64), (4096, 1)):
+        lens = [100 + i % 7 for i in range(num - 1)] + [120000]
+        host = (C.c_int32 * num)(*lens)
+        batch = _batch(num_seqs=num, max_seq_len=max(lens), block_table_pitch=7500, seq_lens_host=C.cast(host, C.c_void_p))
+        p = _attend(num_rows=num * rows, max_rows=rows, row_starts=8)
+        args = C.byref(_layout()), C.byref(batch), C.byref(p)
+        nbytes = lib.tri_attend_workspace_bytes(*args)
+        assert 0 < nbytes <= (512 << 20) + 1024, (num, rows, nbytes)
+        start = time.perf_counter()
+        for _ in range(100):
+            lib.tri_attend_workspace_bytes(*args)
+        assert time.perf_counter() - start < 1.0
 
 
 def test_attention_refuses_a_missing_small_or_unaligned_workspace():

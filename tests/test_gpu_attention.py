@@ -731,6 +731,57 @@ def test_lengths_on_the_device_below_and_above_the_host_s():
     assert torch.equal(again, out) and torch.equal(lse2, lse)
 
 
+@pytest.mark.parametrize("heads", [(4, 2), (40, 2)])
+def test_fewer_tokens_than_rows(heads):
+    """Lengths on the device below the number of rows: the rows are those of the newest tokens, the first of them have none."""
+    case = Case([3, 1, 40, 0], q_heads=heads[0], kv_heads=heads[1], rows=[7, 4, 9, 5], parents="chain", seed=15)
+    kv, batch = case.device(host_lens=[48] * 4)
+    before = _weights(case)
+    weights = before.to(DEV)
+    print(f"fewer tokens than rows {heads}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, parents=case.dev_parents, max_rows=9,
+                                weights=weights, want_lse=True)
+    want = case.expected()
+    _check_rows(case, out, lse, want)
+    _check_weights(case, weights, before, want, "add")
+
+
+@pytest.mark.parametrize("heads", [(6, 3), (16, 4)])
+def test_a_long_sequence_among_many_short_ones(heads):
+    case = Case([1 + 5 * i % 37 for i in range(150)] + [5003], q_heads=heads[0], kv_heads=heads[1], dim=256, seed=heads[1])
+    kv, batch = case.device()
+    before = _weights(case)
+    weights = before.to(DEV)
+    print(f"one long {heads}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), weights=weights, want_lse=True)
+    want = case.expected()
+    _check_rows(case, out, lse, want)
+    _check_weights(case, weights, before, want, "add")
+
+
+def test_weights_that_are_no_numbers_are_kept_first():
+    """NaN weights, more than the budget in one head: the lists stay ascending positions, the rows they name are moved."""
+    case = Case([200, 90], seed=3, garbage=None)
+    kv, batch = case.device(budgets=[60, 30])
+    before = _weights(case)
+    odd = [(case.tables[0][t // 16], t % 16) for t in range(0, 200, 2)]
+    for p, o in odd:
+        before[0, p, o, 1] = math.nan
+    before[0, case.tables[1][2], 5, 0] = math.nan
+    weights = before.to(DEV)
+    print("NaN weights", flush=True)
+    keep = ops.evict_step(kv, batch, weights, ops.EvictConfig(window_size=8)).cpu()
+    for b, h, t, n in ((0, 0, 200, 60), (0, 1, 200, 60), (1, 0, 90, 30), (1, 1, 90, 30)):
+        row = keep[b * 2 + h, :n]
+        assert bool((row[1:] > row[:-1]).all()) and int(row[0]) >= 0 and int(row[-1]) < t
+        for j, i in enumerate(row.tolist()):
+            src, dst = (case.tables[b][i // 16], i % 16, h), (case.tables[b][j // 16], j % 16, h)
+            assert torch.equal(case.k[0][dst].cpu(), case.cache[0][0][src])
+            assert torch.equal(weights[0][dst].cpu().view(torch.int32), before[0][src].view(torch.int32))
+    assert all(i % 2 == 0 for i in keep[1, :60].tolist())
+    assert 2 * 16 + 5 in keep[2, :30].tolist()
+
+
 def test_refusals_of_the_python_layer():
     case = Case([30, 20], layers=2, seed=1)
     kv, batch = case.device(budgets=[10, 10])

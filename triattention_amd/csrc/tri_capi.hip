@@ -925,6 +925,8 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
     return fail(TRI_ERR_INVALID_ARGUMENT, "strides of q and out must be multiples of 8 elements (16 bytes)");
   if (p->num_q_heads > 1 && p->out_stride_head < kv->head_dim)
     return fail(TRI_ERR_INVALID_ARGUMENT, "out_stride_head %lld < head_dim", (long long)p->out_stride_head);
+  if (p->num_rows > 1 && p->out_stride_row < kv->head_dim)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "out_stride_row %lld < head_dim", (long long)p->out_stride_row);
   if (!is_finite(p->scale) || !is_finite(p->k_scale) || !is_finite(p->v_scale) || !is_finite(p->scale * p->k_scale * 1.44269504f))
     return fail(TRI_ERR_INVALID_ARGUMENT, "scale, k_scale and v_scale must be finite");
   if (!(p->scale * p->k_scale > 0.f)) return fail(TRI_ERR_INVALID_ARGUMENT, "scale * k_scale must be positive");
@@ -970,19 +972,23 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   const int rows = a.max_rows * a.G;
   a.row_tiles = rows <= 16 ? 0 : rows <= 64 ? 4 : rows <= 128 || a.D == 256 ? 8 : 16;
   a.row_blocks = a.row_tiles ? tri::ceil_div(rows, 16 * a.row_tiles) : 1;
-  // A split is as long as lets every workgroup run at once: on from the mean over what the chip holds, until the splits
-  // of all sequences fit (each sequence's last one is short).
+  // A split is as long as lets every workgroup run at once (each sequence's last one is short); with more sequences than that
+  // allows, what a workgroup has to do on the mean, so that a long one among short ones is still cut.
   const int64_t holds = 256 * attend_workgroups_per_cu(a.row_tiles, a.D);
   auto length = [&](int64_t inner, int step) {
-    const int64_t most = tri::align_up(longest, step);
-    int64_t split = std::min<int64_t>(tri::align_up(std::max<int64_t>(tri::ceil_div64(total * inner, holds), 1), step), most);
-    for (; split < most; split += step) {
+    const int64_t most = tri::align_up(longest, step), cap = holds / inner;
+    int64_t lo = std::min<int64_t>(tri::align_up(std::max<int64_t>(tri::ceil_div64(total * inner, holds), 1), step), most);
+    if (cap <= a.B) return (int)lo;
+    int64_t hi = std::min(tri::align_up(std::max<int64_t>(tri::ceil_div64(total, cap - a.B), 1), step), most);      // (surely fits)
+    while (lo < hi) {
+      const int64_t mid = lo + (hi - lo) / step / 2 * step;
       int64_t count = 0;
       for (int b = 0; b < a.B; ++b)
-        count += std::max<int64_t>(1, tri::ceil_div64(std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest), split));
-      if (count * inner <= holds) break;
+        count += std::max<int64_t>(1, tri::ceil_div64(std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest), mid));
+      if (count <= cap) hi = mid;
+      else lo = mid + step;
     }
-    return (int)split;
+    return (int)hi;
   };
   // Few rows of long sequences: a workgroup takes four KV heads, a wave each.  Its waves then read neighbouring rows, a token's
   // heads lie side by side, and have nothing to join: 16 x 16384 tokens of fp8 114 us against 125 with four waves to a head, 24
@@ -997,6 +1003,9 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   }
   // (128: whole tiles of every kernel; a single tile a workgroup saves the attention nothing and costs the join)
   if (a.heads_per_group == 1) a.split_tokens = length((int64_t)a.Hkv * a.row_blocks, 128);
+  // (the partial results of all splits: at most 512 MiB, of one split where that alone is more)
+  const int64_t part_bytes = (int64_t)a.B * a.Hkv * rows * (a.D + 2) * 4, parts_most = std::max<int64_t>((512ll << 20) / part_bytes, 1);
+  if (tri::ceil_div64(longest, a.split_tokens) > parts_most) a.split_tokens = (int)tri::align_up(tri::ceil_div64(longest, parts_most), 128);
   a.nsplit = (int)tri::ceil_div64(longest, a.split_tokens);
   a.by_xcd = a.row_blocks > 1 && (int64_t)a.B * a.nsplit >= 32;
   int64_t off = 0;
