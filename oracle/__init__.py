@@ -33,6 +33,9 @@ selection.topk_ascending     full sort on tiny inputs
 compaction.*                 golden vectors from the reference's
                              ``compact_request_kv_in_place(_per_head)``;
                              brute-force row loops; multiset preservation
+attention.*                  (no counterpart in the reference) torch softmax over the
+                             visible tokens, full sort; otherwise the definitions
+                             themselves
 ===========================  ==================================================
 
 fp8 (e4m3 + per-token-head scale) keys have no counterpart in the reference;

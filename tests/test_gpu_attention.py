@@ -696,6 +696,45 @@ def test_captured_steps_replay_with_new_lengths_and_share_nothing():
             assert torch.equal(w_after, weights) and torch.equal(b_after, bounds)
 
 
+@pytest.mark.parametrize("types", [dict(), dict(dtype=FP8, row_scales=True)], ids=["bf16", "fp8"])
+def test_captured_eviction_replays_with_new_weights_and_lengths(types):
+    """evict_step in a graph: every replay, on other weights and lengths, is the eager call on the same cache."""
+    case = Case([300, 90, 45], layers=2, seed=9, garbage=None, **types)
+    kv, batch = case.device(budgets=[64, 40, 45])
+    ev = ops.EvictConfig(window_size=16)
+    state = [*case.k, *case.v, *(case.ks or []), *(case.vs or [])]
+    fresh = [x.clone() for x in state]
+    weights = _weights(case).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.evict_step(kv, batch, weights, ev)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep = ops.evict_step(kv, batch, weights, ev)
+    raw = lambda x: x.view(torch.uint8) if x.dtype == FP8 else x           # noqa: E731
+    for rep, lens in enumerate(([300, 90, 45], [70, 90, 44], [1, 50, 0], [299, 40, 45])):
+        print(f"eviction replay {rep} {lens}", flush=True)
+        new = _weights(case, seed=20 + rep).to(DEV)
+        batch.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+
+        def restore():
+            for x, y in zip(state, fresh):
+                raw(x).copy_(raw(y))
+            weights.copy_(new)
+
+        restore()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [raw(x).clone() for x in state] + [weights.clone(), keep.clone()]
+        restore()
+        eager = ops.evict_step(kv, batch, weights, ev)
+        for x, y in zip(got, [raw(x) for x in state] + [weights, eager]):
+            assert torch.equal(x, y), rep
+
+
 def test_another_stream_and_two_calls_at_once():
     """Calls on two streams at the same time give what they give one after the other."""
     case = Case([700, 300, 41], seed=12)

@@ -15,8 +15,9 @@
 //
 // Up to 16 rows (attend_few_kernel) the four waves of a workgroup take tiles of 32 tokens in turn, keys straight from
 // memory into the operand's registers, and meet once at the end: such a call is bound by reading K and V, and what
-// counts is how many bytes are asked for at a time; in long sequences they take a KV head each instead.  Beyond that (attend_rows_kernel) every wave has rows of its own and
-// the workgroup shares the tiles through LDS: a tile is read from memory once for up to 256 rows.  A sequence is cut into
+// counts is how many bytes are asked for at a time; in long sequences they take a KV head each instead.  Beyond that
+// (attend_rows_kernel) every wave has rows of its own and the workgroup shares the tiles through LDS: a tile is read from
+// memory once for up to 256 rows.  A sequence is cut into
 // splits, as many as the chip has room for at once, joined by attend_finish_kernel.
 #pragma once
 
@@ -485,6 +486,12 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
 }
 
 // ---- up to 16 rows of a KV head
+// Bound by reading K and V.  Keys go from memory into the operand's registers (a lane's 16 bytes are a piece of it), values
+// through LDS, which transposes them; the next tile's are asked for as soon as this one's registers are free, so that two
+// workgroups a CU (four of 64 dimensions) have 128 KiB on their way (fp8: 64).
+// 16 x 2176 tokens of 8 x 128 bf16 with four query heads each 35 us (4.0 TB/s), 16 x 16384 of fp8 with HEADS 130 us (K, V and
+// the scores written for the weights: 4.4 TB/s), without weights 114 (4.7), where a copy reaches 5.1; 160 tokens 7 us.
+// HEADS: a wave has a KV head to itself, four neighbours in a workgroup, and nothing is joined here.
 template <int QT, bool FP8, int D, bool UNI, bool HEADS>
 __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) void attend_few_kernel(AttendLaunch a) {
   constexpr int PT = FP8 ? TRI_KV_BF16 : QT;              // fp8 rows with a scale of their own: the weight carries it, which fp16 has no room for
@@ -692,6 +699,12 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
 }
 
 // ---- more rows: RT tiles of 16 rows a wave, W waves, K and V of BT tokens in LDS for all of them
+// Bound by turns: the matrix cores work a third of the time, the softmax's vector instructions and LDS reads about as long
+// each, and two waves a SIMD overlap little of it (phases a barrier apart, so that one wave's softmax would meet the other's
+// products, were slower: 137 us and more against 112).  Two row tiles to a wave halve what it reads of LDS a row, and eight
+// waves what is read of memory (with the slack in rescaling, 257 -> 111 us for the call below when they came).  The next tile
+// waits in registers while this one is worked on.  2 x 32768 tokens with 60 rows of 4 query heads, 8 x 128 fp16: 93 us, 690
+// TFLOP/s of the 1200 a large product reaches; 8 x 4096 with up to 32 rows of 8: 50 us; 1217 tokens with 16 rows: 12 us.
 template <int QT, bool FP8, int D, int RT, int W, bool UNI>
 __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch a) {
   constexpr int PT = FP8 ? TRI_KV_BF16 : QT;
