@@ -1,5 +1,7 @@
 // What follows the attention itself (tri_attend_device.h): the splits of a sequence joined, and the weights its tokens received
 // added up beside the cache.
+#include <algorithm>
+
 #include "tri_attend_device.h"
 
 namespace tri {
@@ -76,24 +78,29 @@ __device__ __forceinline__ void join_rows(const AttendLaunch& a, int64_t group) 
 // weight[token][head] (+)= sum over the rows of the head of 2^(s - lse): every token and head by one thread, rows in order.
 // A lane is a token (the scores lie token by token), a wave takes four heads, whose weights it reads and writes as one
 // piece (VEC), and sixteen rows at a time: four lanes find the lse of a row, from its splits where the sequence is
-// cut.  Reads a score once, weights once, writes them once.
-template <bool VEC>
+// cut.  Where the four heads have more rows than sixteen, the workgroup's waves take four pieces of one sequence's tokens and find
+// the lse of 64 rows TOGETHER (a wave would read as much for them as of scores: 24 ragged sequences of 64 query heads 22 ->
+// 17 us; with sixteen rows three waves would wait for one, 18 -> 21).  Reads a score once, weights once, writes them once.
+template <bool VEC, bool TOGETHER>
 __device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weights, int set, int64_t group) {
-  __shared__ float s_lse[kThreads / kWave][16];
-  const int lane = threadIdx.x % kWave;
-  const int quads = ceil_div(a.Hkv, 4), chunks = ceil_div(a.Tmax, kWave);
-  int64_t unit = group * (kThreads / kWave) + threadIdx.x / kWave;
+  constexpr int kWaves = kThreads / kWave, kSpan = TOGETHER ? kThreads : kWave, kRows = kSpan / 4;
+  __shared__ float s_lse[kThreads / 4];
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  const int of_unit = TOGETHER ? 0 : wave * kRows;          // the unit's part of s_lse
+  const int quads = ceil_div(a.Hkv, 4), spans = ceil_div(a.Tmax, kSpan);
+  int64_t unit = TOGETHER ? group : group * kWaves + wave;
   const int h0 = (int)(unit % quads) * 4;
   unit /= quads;
-  const int t0 = (int)(unit % chunks) * kWave;
-  const int64_t b = unit / chunks;
+  const int t0 = (int)(unit % spans) * kSpan;
+  const int64_t b = unit / spans;
   if (b >= a.B) return;
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   if (t0 >= T) return;
+  const int mine = t0 + (TOGETHER ? (int)threadIdx.x : lane);
   const RowRange rows = rows_of(a, (int)b);
-  const int t = min(t0 + lane, T - 1);
+  const int t = min(mine, T - 1);
   const int page = a.block_table ? a.block_table[b * a.block_table_pitch + t / a.block_size] : (int)b;
-  const bool ok = t0 + lane < T && page >= 0 && page < a.num_blocks;
+  const bool ok = mine < T && page >= 0 && page < a.num_blocks;
   float* const w = weights + (ok ? ((int64_t)page * a.block_size + t % a.block_size) * a.Hkv + h0 : 0);
   const bool fresh = set || t >= T - rows.n;      // the rows' own tokens: nothing has been added for them yet
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
@@ -105,8 +112,9 @@ __device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weight
   f32x4 more = {0.f, 0.f, 0.f, 0.f};
   const int per_head = rows.n * a.G, heads = min(4, a.Hkv - h0), rows_max = a.max_rows * a.G;
   const int live = max(1, ceil_div(T, a.split_tokens));
-  for (int r0 = 0; r0 < heads * per_head; r0 += 16) {
-    const int r = min(r0 + (lane & 15), heads * per_head - 1), h = h0 + r / per_head, m = r % per_head;
+  const int all = heads * per_head;
+  for (int r0 = 0; r0 < all; r0 += kRows) {
+    const int r = min(r0 + (TOGETHER ? wave * 16 : 0) + (lane & 15), all - 1), h = h0 + r / per_head, m = r % per_head;
     float l;
     if (a.nsplit > 1) {
       const float* ml = a.part_ml + (((b * a.Hkv + h) * a.nsplit) * rows_max + m) * 2;
@@ -128,16 +136,20 @@ __device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weight
     } else {
       l = a.lse2[(int64_t)(rows.first + m / a.G) * a.Hq + h * a.G + m % a.G];
     }
-    __builtin_amdgcn_wave_barrier();
-    if (lane < 16) s_lse[threadIdx.x / kWave][lane] = l == -INFINITY ? INFINITY : l;             // (a row without tokens adds nothing)
-    __builtin_amdgcn_wave_barrier();
+    auto meet = [] {
+      if (TOGETHER) __syncthreads();
+      else __builtin_amdgcn_wave_barrier();
+    };
+    meet();
+    if (lane < 16) s_lse[wave * 16 + lane] = l == -INFINITY ? INFINITY : l;             // (a row without tokens adds nothing)
+    meet();
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float* s = a.scores + (b * a.Hkv + min(h0 + e, a.Hkv - 1)) * rows_max * a.score_pitch + t;
-      const int from = max(r0, e * per_head), to = min(min(r0 + 16, heads * per_head), (e + 1) * per_head);
+      const int from = max(r0, e * per_head), to = min(min(r0 + kRows, all), (e + 1) * per_head);
 #pragma unroll 4
       for (int x = from; x < to; ++x)
-        more[e] += pow2(s[(int64_t)(x - e * per_head) * a.score_pitch] - s_lse[threadIdx.x / kWave][x - r0]);
+        more[e] += pow2(s[(int64_t)(x - e * per_head) * a.score_pitch] - s_lse[of_unit + x - r0]);
     }
   }
   sum += more;
@@ -149,11 +161,11 @@ __device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weight
 }
 
 // The splits joined and the weights added up, in one launch: both start from what the attention left.  3 to 10 us, with the
-// weights of 16 x 16384 tokens of 32 query heads 18 (34 MB of scores, 8 of weights twice), of 24 ragged sequences of 64 heads 22.
-template <int QT, int D, int PARTS, bool VEC>
+// weights of 16 x 16384 tokens of 32 query heads 18 (34 MB of scores, 8 of weights twice), of 24 ragged sequences of 64 heads 17.
+template <int QT, int D, int PARTS, bool VEC, bool TOGETHER>
 __global__ __launch_bounds__(kThreads) void attend_finish_kernel(AttendLaunch a, int join_groups, float* weights, int set) {
   if ((int)blockIdx.x < join_groups) join_rows<QT, D, PARTS>(a, blockIdx.x);
-  else add_weights<VEC>(a, weights, set, blockIdx.x - join_groups);
+  else add_weights<VEC, TOGETHER>(a, weights, set, blockIdx.x - join_groups);
 }
 
 template <int QT, int D>
@@ -164,7 +176,9 @@ hipError_t launch_finish_typed(const AttendLaunch& a, float* weights, int set, h
   // not 3840 rows of 16, 8.1 -> 15.4).
   const bool wide = a.nsplit > kWideSplits && rows <= kWideRows;
   const int64_t joins = wide ? rows : ceil_div64(rows, kRows);
-  const int64_t adds = weights ? ceil_div64((int64_t)a.B * ceil_div(a.Tmax, kWave) * ceil_div(a.Hkv, 4), kThreads / kWave) : 0;
+  const bool together = weights && (int64_t)std::min(a.Hkv, 4) * a.max_rows * a.G > 16;
+  const int64_t quads = (int64_t)a.B * ceil_div(a.Hkv, 4);
+  const int64_t adds = !weights ? 0 : together ? quads * ceil_div(a.Tmax, kThreads) : ceil_div64(quads * ceil_div(a.Tmax, kWave), kThreads / kWave);
   if (joins + adds == 0) return hipSuccess;
   if (joins + adds > INT32_MAX) return hipErrorInvalidValue;
   const bool vec = a.Hkv % 4 == 0 && reinterpret_cast<uintptr_t>(weights) % 16 == 0;
@@ -172,8 +186,15 @@ hipError_t launch_finish_typed(const AttendLaunch& a, float* weights, int set, h
     hipLaunchKernelGGL(kernel, dim3((unsigned)(joins + adds)), dim3(kThreads), 0, s, a, (int)joins, weights, set);
     return hipGetLastError();
   };
-  if (wide) return vec ? go(attend_finish_kernel<QT, D, kRows, true>) : go(attend_finish_kernel<QT, D, kRows, false>);
-  return vec ? go(attend_finish_kernel<QT, D, 1, true>) : go(attend_finish_kernel<QT, D, 1, false>);
+  auto pick = [&](auto parts, auto four) {
+    constexpr int P = decltype(parts)::value;
+    constexpr bool V = decltype(four)::value;
+    return together ? go(attend_finish_kernel<QT, D, P, V, true>) : go(attend_finish_kernel<QT, D, P, V, false>);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Wide = std::integral_constant<int, kRows>;
+  if (wide) return vec ? pick(Wide{}, std::true_type{}) : pick(Wide{}, std::false_type{});
+  return vec ? pick(One{}, std::true_type{}) : pick(One{}, std::false_type{});
 }
 
 }  // namespace
