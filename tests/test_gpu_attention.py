@@ -284,6 +284,29 @@ def test_trees(dim, heads, rows, types):
     _check_weights(case, weights, before, want, "add")
 
 
+@pytest.mark.parametrize("dim,heads,rows,block,types", [
+    (128, (32, 2), [5, 0, 64, 9], 24, dict()), (64, (24, 8), [40, 64, 0, 1], 3, dict(dtype=FP16)),
+    (256, (9, 1), [8, 3, 30, 0], 16, dict(dtype=FP8, row_scales=True)), (128, (33, 1), [1, 1, 1, 1], 64, dict(dtype=FP8, query=FP16)),
+    (256, (6, 3), [64, 2, 50, 7], 20, dict(dtype=FP16)),
+])
+@pytest.mark.parametrize("mode", ["add", "set"])
+def test_weights_of_many_rows(dim, heads, rows, block, types, mode):
+    """More rows of a KV head than leave their scores behind: short sequences, fewer tokens than rows, none, bad pages, blocks of
+    any size."""
+    lens = [290, 50, 71, 3]
+    case = Case(lens, q_heads=heads[0], kv_heads=heads[1], dim=dim, rows=rows, block=block, seed=dim + rows[0], **types)
+    case.tables[0][1], case.tables[1][-1] = case.pool, -3
+    kv, batch = case.device(host_lens=[300] * 4) if block == 20 else case.device()
+    before = _weights(case)
+    weights = before.to(DEV)
+    print(f"weights of many rows dim={dim} heads={heads} rows={rows} block={block} {types} {mode}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, parents=case.dev_parents, max_rows=max(rows),
+                                weights=weights, weight_mode=mode, want_lse=True)
+    want = case.expected()
+    _check_rows(case, out, lse, want)
+    _check_weights(case, weights, before, want, mode)
+
+
 def test_trees_without_parents_are_chains_and_may_fill_the_cache():
     """parents=None: each row follows the one before it.  Sequences that hold nothing but their new tokens."""
     case = Case([12, 64, 3, 200], rows=[12, 64, 3, 33], parents="chain", seed=5)

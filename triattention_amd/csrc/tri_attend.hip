@@ -72,7 +72,11 @@ __device__ __forceinline__ void join_rows(const AttendLaunch& a, int64_t group) 
   const float inv = j.total == 0.f ? 0.f : a.v_scale / j.total;
   uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + i * a.out_stride_row + (int64_t)hq * a.out_stride_head + d;
   *reinterpret_cast<uint2*>(dst) = uint2{Half<QT>::pack(j.v[0] * inv, j.v[1] * inv), Half<QT>::pack(j.v[2] * inv, j.v[3] * inv)};
-  if (d == 0 && a.lse) a.lse[i * a.Hq + hq] = lse_of(j.top, j.total) * 0.69314718055994530942f;
+  if (d == 0) {
+    const float l2 = lse_of(j.top, j.total);
+    if (a.lse) a.lse[i * a.Hq + hq] = l2 * 0.69314718055994530942f;
+    if (a.lse2) a.lse2[i * a.Hq + hq] = l2;
+  }
 }
 
 // weight[token][head] (+)= sum over the rows of the head of 2^(s - lse): every token and head by one thread, rows in order.

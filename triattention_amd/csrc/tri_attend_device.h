@@ -393,9 +393,9 @@ __device__ __forceinline__ void put_row(const AttendLaunch& a, const RowRange& r
 
 // Where the scores of a wave's rows go, where weights are wanted.
 struct ScoreRows {
-  float* head;           // of the (sequence, KV head), or NULL
-  int64_t pitch;
-  int m0, M;
+  float* head = nullptr;           // of the (sequence, KV head), or NULL
+  int64_t pitch = 0;
+  int m0 = 0, M = 0;
 };
 __device__ __forceinline__ ScoreRows score_rows(const AttendLaunch& a, int b, int h, int m0, int M) {
   return {a.scores ? a.scores + ((int64_t)b * a.Hkv + h) * a.max_rows * a.G * a.score_pitch : nullptr, a.score_pitch, m0, M};
@@ -420,7 +420,7 @@ __device__ __forceinline__ uint32_t seen_of(uint32_t okm, bool drafts, int first
 // The softmax of 32 tokens for RT rows a lane: sc holds q . k of tokens i * 16 + (lane >> 4) * 4 + r; pf receives the weights
 // 2^(x - top) packed for the product with V (vs scales them: fp8 rows with scales of their own).  They are rounded to 16 bits
 // there while the sum adds them unrounded: errors of half a step each and of either sign, below the one rounding of the output.
-template <int PT, bool SCALED, int RT, int NT>
+template <int PT, bool SCALED, bool SCORES, int RT, int NT>
 __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT], f32x4 (&o)[RT][NT], u32x4 (&pf)[RT], float scale,
                                           const f32x4 (&ks)[2], const f32x4 (&vs)[2], bool masked, bool drafts, uint32_t okm, int first,
                                           const uint64_t (&seen)[RT], int lane, const ScoreRows& scores, int at) {
@@ -442,7 +442,7 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
     best[rt] = fmaxf(fmaxf(fmaxf(sc[rt][0][0], sc[rt][0][1]), fmaxf(sc[rt][0][2], sc[rt][0][3])),
                      fmaxf(fmaxf(sc[rt][1][0], sc[rt][1][1]), fmaxf(sc[rt][1][2], sc[rt][1][3])));
     grows |= best[rt] > st[rt].grow;
-    if (scores.head) {
+    if (SCORES && scores.head) {
       const int l = here(lane), m = scores.m0 + rt * 16 + (l & 15);
       float* dst = scores.head + m * scores.pitch + at + (l >> 4) * 4;
       if (m < scores.M) {
@@ -632,9 +632,9 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
         ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][0][i * 16 + q4 * 4]);
         vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][1][i * 16 + q4 * 4]);
       }
-      softmax32<PT, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
+      softmax32<PT, true, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
     } else {
-      softmax32<PT, false, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
+      softmax32<PT, false, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -808,7 +808,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   }
   u32x4 qf[RT][D / 32];
   uint64_t seen[RT];
-  const ScoreRows scores = score_rows(a, b, h, m0, M);
+  constexpr bool kScores = RT * W == 4;                   // (of more rows the weights come from the keys once more)
+  const ScoreRows scores = kScores ? score_rows(a, b, h, m0, M) : ScoreRows{};
   f32x4 o[RT][NT];
   RowState st[RT];
   const uint64_t anc = n > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
@@ -889,7 +890,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
 #pragma unroll
       for (int i = 0; i < 2; ++i) ks[i] = vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
     }
-    softmax32<PT, FP8, RT, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
+    softmax32<PT, FP8, kScores, RT, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
   };
   const bool busy = m0 < M;
   // A tile, while the next one goes from registers to LDS and the one behind it is asked for.
@@ -939,8 +940,141 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   }
 }
 
+// ---- the weights of many rows, from their lse
+// weight[token] (+)= sum over rows of 2^(scale q . k - lse): the scores a second time, where leaving them behind takes 8 bytes a row
+// and token, written and read, and the keys are read once however many rows there are.  A wave has 64 tokens of a KV head, their keys in
+// the operand's registers, and goes through all rows; a lane sums its rows' weights of its tokens, and the sixteen
+// lanes of a token's rows meet once at the end: no order of anything to depend on.  Bound by reading the keys, of many rows by the
+// exponentials: 2 x 32768 tokens of 8 x 128 bf16, 64 rows of four query heads, 187 us with the attention (120 of it) against 387 from scores.
+constexpr int kWeighTokens = kWave;
+template <int QT, bool FP8, int D, bool UNI>
+__global__ __launch_bounds__(kAttendThreads, 2) void weigh_rows_kernel(AttendLaunch a) {
+  constexpr int ES = FP8 ? 1 : 2;
+  constexpr int TOK = kWeighTokens, NG = TOK / 16;        // tokens of a wave, groups of the product
+  __shared__ __align__(16) float s_token[kAttendWaves][TOK];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c16 = lane & 15, q4 = lane >> 4;
+  const int h = blockIdx.x % a.Hkv, spans = ceil_div(a.Tmax, TOK * kAttendWaves);
+  const int unit = blockIdx.x / a.Hkv, b = unit / spans, t0 = (unit % spans * kAttendWaves + wave) * TOK;
+  const int T = min(max(a.seq_lens[b], 0), a.Tmax);
+  if (t0 >= T) return;
+  const RowRange rows = rows_of(a, b);
+  const int n = rows.n, M = n * a.G, base = T - n;
+  const GlobalBytes kb = (GlobalBytes)a.k_layers[a.layer] + (int64_t)h * a.stride_head * ES;
+  const bool scaled = FP8 && a.k_scale_layers;
+
+  const Seq seq(a, b, h, T, T);
+  Finder<UNI, ES, TOK, TOK> find(seq, lane);
+  find.begin(t0);
+  find.take(t0);
+  u32x4 kf[NG][D / 32];
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    const GlobalBytes src = find.row(kb, i * 16, i * 16 + c16) + q4 * 16;
+#pragma unroll
+    for (int c = 0; c < D * ES / 64; ++c) {
+      const u32x4 w = *(GlobalU4)(src + c * 64);
+      if constexpr (FP8) {
+        kf[i][2 * c] = widen8<QT>(w[0], w[1]);
+        kf[i][2 * c + 1] = widen8<QT>(w[2], w[3]);
+      } else {
+        kf[i][c] = w;
+      }
+    }
+  }
+  // the lane's token at the end
+  const int t = min(t0 + lane, T - 1), page = seq.a.block_table ? seq.table[seq.div(t)] : b;
+  const bool there = t0 + lane < T && page >= 0 && page < a.num_blocks;
+  float* const w = a.weights + (there ? ((int64_t)page * a.block_size + seq.mod(t)) * a.Hkv + h : 0);
+  const float before = a.weight_set || !there || t >= base ? 0.f : *w;
+  f32x4 ks[NG], sum[NG];
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    ks[i] = f32x4{a.scale_log2, a.scale_log2, a.scale_log2, a.scale_log2};
+    sum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (scaled) {
+    const GlobalF32 ksc = (GlobalF32)a.k_scale_layers[a.layer] + h;
+    s_token[wave][lane] = ksc[find.scale_at(lane)];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < NG; ++i) ks[i] *= *reinterpret_cast<const f32x4*>(&s_token[wave][i * 16 + q4 * 4]);
+    __builtin_amdgcn_wave_barrier();
+  }
+  const uint64_t anc = n > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
+  const bool drafts = n > 1 && t0 + TOK > base;
+
+  // a row's queries, lse (infinite where it adds nothing) and new tokens it sees; asked for one tile of rows ahead
+  u32x4 q_next[D / 32];
+  float lse_next;
+  uint64_t seen_next;
+  auto ask = [&](int m0) {
+    const int m = min(m0 + c16, M - 1), i = m / a.G;
+    const int64_t row = rows.first + i;
+    const int hq = h * a.G + m - i * a.G;
+    const GlobalBytes qp = (GlobalBytes)a.q + (row * a.q_stride_row + hq * a.q_stride_head) * 2;
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) {
+      const int el = FP8 ? (s / 2) * 64 + q4 * 16 + (s & 1) * 8 : s * 32 + q4 * 8;
+      q_next[s] = *(GlobalU4)(qp + el * 2);
+    }
+    lse_next = ((GlobalF32)a.lse2)[row * a.Hq + hq];
+    seen_next = (uint64_t)shfl64((int64_t)anc, i);
+  };
+  if (M > 0) ask(0);
+  for (int m0 = 0; m0 < M; m0 += 16) {
+    u32x4 qf[D / 32];
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s) qf[s] = q_next[s];
+    const float lse = m0 + c16 >= M || lse_next == -INFINITY ? INFINITY : lse_next;
+    const uint64_t seen = seen_next;
+    ask(m0 + 16);
+    f32x4 sc[NG];
+#pragma unroll
+    for (int i = 0; i < NG; ++i) sc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < D / 32; ++s)
+#pragma unroll
+      for (int i = 0; i < NG; ++i) sc[i] = mfma<QT>(kf[i][s], qf[s], sc[i]);
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sc[i][r] = __builtin_fmaf(sc[i][r], ks[i][r], -lse);
+    if (drafts) {
+#pragma unroll
+      for (int p = 0; p < NG / 2; ++p) {
+        const int first = t0 + p * 32 - base;
+        const uint32_t vis = seen_of(~0u, first > -32, first, seen) >> (here(lane) >> 4) * 4;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[p * 2 + i][r] = vis >> (i * 16 + r) & 1 ? sc[p * 2 + i][r] : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[i][r] += pow2(sc[i][r]);
+  }
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+#pragma unroll
+    for (int step = 1; step < 16; step *= 2)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum[i][r] += __shfl_xor(sum[i][r], step);
+    if (c16 == 0) *reinterpret_cast<f32x4*>(&s_token[wave][i * 16 + q4 * 4]) = sum[i];
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (there) *w = before + s_token[wave][lane];
+}
+
 template <int QT, bool FP8, int D, bool UNI>
 hipError_t launch_attend_typed(const AttendLaunch& a, hipStream_t s) {
+  if (a.weigh) {
+    const int span = kWeighTokens * kAttendWaves;
+    hipLaunchKernelGGL((weigh_rows_kernel<QT, FP8, D, UNI>), dim3((unsigned)(a.B * ceil_div(a.Tmax, span) * a.Hkv)), dim3(kAttendThreads), 0, s, a);
+    return hipGetLastError();
+  }
   const int64_t units = (int64_t)a.B * a.nsplit;
   const dim3 grid((unsigned)((a.by_xcd ? align_up(units, kDies) : units) * a.row_blocks * (a.Hkv / a.heads_per_group)));
   if (a.heads_per_group > 1) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI, true>), grid, dim3(kAttendThreads), 0, s, a);

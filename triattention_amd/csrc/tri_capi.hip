@@ -889,6 +889,7 @@ struct AttendPlan {
   // block selection
   int64_t block_scores, counts;
   int max_count;
+  bool weigh_again;
 };
 
 constexpr int kMaxNewTokens = 64;          // a word of ancestors
@@ -1011,14 +1012,18 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = tri::align_up(off + bytes, 256); return o; };
   const int64_t parts = a.nsplit > 1 ? (int64_t)a.B * a.Hkv * a.nsplit * rows : 0;
-  if (((int64_t)a.B * a.nsplit + 7) * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) * tri::ceil_div(a.Hkv, 4) > INT_MAX ||
+  if (((int64_t)a.B * a.nsplit + 7) * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) * a.Hkv > INT_MAX ||
       (int64_t)a.B * a.Hkv * rows > INT_MAX)
     return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d rows and %d KV heads in one call", a.B, a.max_rows, a.Hkv);
   a.score_pitch = tri::align_up(a.Tmax, 32);
   d.part_out = take(parts * a.D * 4);
   d.part_ml = take(parts * 8);
+  // Weights of few rows come from their scores, which the attention leaves (8 bytes a row and token, written and read), of many
+  // from the keys once more: 2 x 32768 tokens of 8 x 128 bf16, 20 rows a KV head 94 us from scores and 104 from keys, 32 rows
+  // 105 and 104, 128 rows 231 and 141, of fp8 32 rows 75 and 78, 64 rows 107 and 91; rows of 256 dimensions, 64 of them, 115 and 120.
+  d.weigh_again = p->weights && rows > (a.D == 256 ? 64 : 32);
   d.lse2 = take(p->weights ? (int64_t)a.num_rows * a.Hq * 4 : 0);
-  d.scores = take(p->weights ? (int64_t)a.B * a.Hkv * rows * a.score_pitch * 4 : 0);
+  d.scores = take(p->weights && !d.weigh_again ? (int64_t)a.B * a.Hkv * rows * a.score_pitch * 4 : 0);
   d.block_scores = take(bp ? (int64_t)a.B * a.Hkv * d.max_count * 4 : 0);
   d.counts = take(bp ? (int64_t)a.B * 8 : 0);
   d.total = std::max<int64_t>(off, 256);
@@ -1039,12 +1044,16 @@ int do_attend(AttendPlan& d, void* ws, float* weights, int weight_mode, hipStrea
     a.part_out = at<float>(ws, d.part_out);
     a.part_ml = at<float>(ws, d.part_ml);
   }
-  if (weights) {
-    a.lse2 = at<float>(ws, d.lse2);
-    a.scores = at<float>(ws, d.scores);
-  }
-  const int rc = launch_status(tri::launch_attend(a, s), "attend");
-  return rc ? rc : launch_status(tri::launch_attend_finish(a, weights, weight_mode, s), "attend_finish");
+  const bool again = d.weigh_again;
+  if (again || (weights && a.nsplit == 1)) a.lse2 = at<float>(ws, d.lse2);
+  if (weights && !again) a.scores = at<float>(ws, d.scores);
+  int rc = launch_status(tri::launch_attend(a, s), "attend");
+  if (!rc) rc = launch_status(tri::launch_attend_finish(a, again ? nullptr : weights, weight_mode, s), "attend_finish");
+  if (rc || !again) return rc;
+  a.weigh = 1;
+  a.weights = weights;
+  a.weight_set = weight_mode;
+  return launch_status(tri::launch_attend(a, s), "weigh_rows");
 }
 
 int fill_evict(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, int32_t* keep, tri::EvictLaunch& a) {

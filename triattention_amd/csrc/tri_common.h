@@ -283,9 +283,13 @@ struct AttendLaunch {
   // workspace
   float* part_out;                                         // [B][Hkv][nsplit][max_rows * G][D], not normalised (nsplit > 1)
   float* part_ml;                                          // the same rows' maximum (base 2) and sum
-  float* lse2;                                             // [num_rows][Hq], base 2, or NULL (nsplit 1 with weights)
+  float* lse2;                                             // [num_rows][Hq], base 2, or NULL
   float* scores;                                           // [B][Hkv][max_rows * G][score_pitch] base 2, or NULL
   int64_t score_pitch;
+  // the pass that finds the weights of many rows (launch_attend once more, when lse2 is there)
+  int weigh;
+  float* weights;                                          // the layer's [num_blocks][block_size][Hkv]
+  int weight_set;
 };
 hipError_t launch_attend_64_bf16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_64_fp16(const AttendLaunch& a, hipStream_t s);
@@ -294,8 +298,8 @@ hipError_t launch_attend_128_fp16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_256_bf16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_256_fp16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend(const AttendLaunch& a, hipStream_t s);
-// What follows it: the splits joined (nsplit > 1) and, with weights (the layer's [num_blocks][block_size][Hkv]), the
-// weights added to them (set: written).
+// What follows it: the splits joined (nsplit > 1) and, of few rows with weights (the layer's
+// [num_blocks][block_size][Hkv]), the weights added to them (set: written) from the scores the attention left.
 hipError_t launch_attend_finish(const AttendLaunch& a, float* weights, int set, hipStream_t s);
 
 // Bounds of a block's keys and the scores that choose blocks by them (tri_blocks.hip).

@@ -829,8 +829,8 @@ def attend_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, *, layer: int =
 
     ``weights`` (fp32 [layers, blocks, block_size, Hkv], beside the cache) receives the softmax weight of every cached token, summed over
     rows and the query heads of its KV head: added ("add"; the slots of the new tokens themselves are written) or written
-    ("set").  ``select_by_weight`` and ``evict_step`` go by them.  Sequences of such a call may not share blocks, and its scratch
-    holds four bytes per row, query head and token.
+    ("set").  ``select_by_weight`` and ``evict_step`` go by them.  Sequences of such a call may not share blocks; of
+    few rows its scratch holds the scores, four bytes per row, query head and token.
 
     ``scale`` (default head_dim ** -0.5) times ``k_scale`` must be positive.
 
