@@ -110,6 +110,17 @@ def test_plans_of_many_sequences_stay_small_and_are_made_quickly():
         assert time.perf_counter() - start < 1.0
 
 
+def test_tables_too_narrow_for_the_longest_sequence_are_refused():
+    lib = _lib.load()
+    kv, batch = C.byref(_layout()), C.byref(_batch(block_table_pitch=6))
+    for code in (lib.tri_attend_paged(kv, batch, C.byref(_attend()), 256, 1 << 40, None),
+                 lib.tri_attend_blocks(kv, batch, C.byref(_attend()), C.byref(_blocks()), 256, 1 << 40, None),
+                 lib.tri_block_bounds(kv, batch, 40, 0, 16, 40 * 4 * 256, None),
+                 lib.tri_select_by_weight(kv, batch, C.byref(_evict()), None, 8, 256, 1 << 40, None),
+                 lib.tri_evict_step(kv, batch, C.byref(_evict()), 8, 256, 1 << 40, None)):
+        assert code == _lib.TRI_ERR_INVALID_ARGUMENT and b"block_table_pitch" in lib.tri_last_error()
+
+
 def test_attention_refuses_a_missing_small_or_unaligned_workspace():
     lib = _lib.load()
     args = C.byref(_layout()), C.byref(_batch(max_seq_len=100000)), C.byref(_attend())

@@ -505,6 +505,10 @@ def test_bounds_follow_new_tokens_and_odd_keys_are_always_read():
             for j, p in enumerate(case.tables[b]):
                 want = full[j] if p in fresh else torch.full_like(full[j], 5.0)
                 assert torch.equal(got[layer, p], want), (layer, b, j)
+    # more new tokens than a sequence has: all of them
+    fresh = ops.update_block_bounds(kv, batch, torch.full_like(bounds, 5.0))
+    for most in (131, (1 << 31) - 1):
+        assert torch.equal(ops.update_block_bounds(kv, batch, torch.full_like(bounds, 5.0), new_tokens=most), fresh)
     # a NaN key: its block counts as the best one
     t = 70
     case.cache[0][0][case.tables[3][t // 16], t % 16, 1, 3] = math.nan

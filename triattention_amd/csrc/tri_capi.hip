@@ -82,6 +82,14 @@ int check_batch(const tri_batch* b, bool need_budget) {
   return TRI_OK;
 }
 
+// The calls that read a sequence's pages by themselves: the table has an entry for every block a sequence can have.
+int check_pages(const tri_kv_layout* kv, const tri_batch* b) {
+  if (b->block_table && (int64_t)b->block_table_pitch * kv->block_size < b->max_seq_len)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "block_table_pitch %d: %d blocks of %d tokens do not hold %d", b->block_table_pitch,
+                b->block_table_pitch, kv->block_size, b->max_seq_len);
+  return TRI_OK;
+}
+
 int check_score(const tri_kv_layout* kv, const tri_score_params* sp) {
   if (!sp) return fail(TRI_ERR_INVALID_ARGUMENT, "score params are NULL");
   if (sp->num_score_heads <= 0 || sp->num_score_heads % kv->num_kv_heads)
@@ -1059,6 +1067,7 @@ int do_attend(AttendPlan& d, void* ws, float* weights, int weight_mode, hipStrea
 int fill_evict(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, int32_t* keep, tri::EvictLaunch& a) {
   int rc = check_layout(kv, false);
   if (!rc) rc = check_batch(batch, true);
+  if (!rc) rc = check_pages(kv, batch);
   if (rc) return rc;
   if (!p) return fail(TRI_ERR_INVALID_ARGUMENT, "evict params are NULL");
   if (p->num_blocks <= 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_blocks %d", p->num_blocks);
@@ -1110,6 +1119,7 @@ int tri_attend_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_
   AttendPlan d;
   int rc = plan_attend(kv, batch, p, nullptr, d);
   if (!rc) rc = check_attend_pointers(p, d, ws, ws_bytes);
+  if (!rc) rc = check_pages(kv, batch);
   if (rc) return rc;
   if (p->num_rows == 0) return TRI_OK;
   return do_attend(d, ws, p->weights, p->weight_mode, (hipStream_t)stream);
@@ -1119,6 +1129,7 @@ int tri_block_bounds(const tri_kv_layout* kv, const tri_batch* batch, int32_t nu
                      int64_t bounds_stride_layer, void* stream) {
   int rc = check_layout(kv, false);
   if (!rc) rc = check_batch(batch, false);
+  if (!rc) rc = check_pages(kv, batch);
   if (rc) return rc;
   if (num_blocks <= 0 || new_tokens < 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_blocks %d, new_tokens %d", num_blocks, new_tokens);
   if (!bounds || !is_aligned(bounds, 16) || bounds_stride_layer % 8)
@@ -1130,7 +1141,7 @@ int tri_block_bounds(const tri_kv_layout* kv, const tri_batch* batch, int32_t nu
     return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d layers in one call", batch->num_seqs, batch->max_seq_len, kv->num_layers);
   tri::BoundsLaunch a{};
   a.B = batch->num_seqs; a.L = kv->num_layers; a.Hkv = kv->num_kv_heads; a.D = kv->head_dim; a.block_size = kv->block_size;
-  a.kv_dtype = kv->kv_dtype; a.Tmax = batch->max_seq_len; a.num_blocks = num_blocks; a.new_tokens = new_tokens;
+  a.kv_dtype = kv->kv_dtype; a.Tmax = batch->max_seq_len; a.num_blocks = num_blocks; a.new_tokens = std::min(new_tokens, batch->max_seq_len);
   a.stride_block = kv->stride_block; a.stride_token = kv->stride_token; a.stride_head = kv->stride_head;
   a.k_layers = kv->k_layers;
   if (kv->kv_dtype == TRI_KV_FP8_E4M3 && kv->v_scale_layers) a.k_scale_layers = kv->k_scale_layers;
@@ -1155,6 +1166,7 @@ int tri_attend_blocks(const tri_kv_layout* kv, const tri_batch* batch, const tri
   AttendPlan d;
   int rc = plan_attend(kv, batch, p, bp, d);
   if (!rc) rc = check_attend_pointers(p, d, ws, ws_bytes);
+  if (!rc) rc = check_pages(kv, batch);
   if (rc) return rc;
   if (!bp->bounds || !bp->blocks || !is_aligned(bp->bounds, 16))
     return fail(TRI_ERR_INVALID_ARGUMENT, "bounds / blocks is NULL or bounds not 16-byte aligned");
