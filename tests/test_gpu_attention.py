@@ -355,6 +355,36 @@ def test_odd_numbers_reach_only_the_rows_that_see_them(heads, types):
     assert clean > 0
 
 
+@pytest.mark.parametrize("heads,block", [((4, 2), 16), ((24, 2), 16), ((4, 2), 24), ((80, 2), 8), ((32, 16), 16)])
+@pytest.mark.parametrize("query", [BF16, FP16])
+def test_scales_that_are_no_numbers(heads, block, query):
+    """NaN in the scales of slots that no sequence owns (behind the ends, in bad pages' place, in blocks not used): nothing of it
+    is seen.  In a drafted token's: the rows that see it get NaN, others what they had."""
+    case = Case([50, 140, 33], q_heads=heads[0], kv_heads=heads[1], rows=[6, 9, 1], block=block, seed=41, dtype=FP8, query=query, row_scales=True)
+    case.parents = [-1, 0, 0, 1, 2, -1] + [-1, -1, 0, 1, 2, 3, 4, 1, 7] + [-1]
+    used = torch.zeros(case.pool, block, dtype=torch.bool)
+    for table, t in zip(case.tables, case.lens):
+        for i in range(t):
+            used[table[i // block], i % block] = True
+    for side in (0, 1):
+        case.scales[side][0][~used] = math.nan
+
+    def run():
+        kv, batch = case.device()
+        out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, parents=case.dev_parents, max_rows=9, want_lse=True)
+        return out, lse
+
+    print(f"scales that are no numbers {heads} {block} {query}", flush=True)
+    _check_rows(case, *run(), case.expected())
+    t = 140 - 9 + 3                                     # the second sequence's fourth draft: seen by itself, 5 and nobody else
+    case.scales[1][0][case.tables[1][t // block], t % block, 0] = math.nan
+    out, lse = run()
+    _check_rows(case, out, lse, case.expected())
+    g = heads[0] // heads[1]
+    odd = torch.isnan(out[6:15, :g].cpu()).all(-1).all(-1)
+    assert odd.tolist() == [False, False, False, True, False, True, False, False, False]
+
+
 @pytest.mark.parametrize("heads", [(4, 2), (20, 1)])
 def test_bad_pages_hold_no_tokens(heads):
     """Table entries outside the pool, first, last and in the middle: their tokens are seen by nobody and keep no weight."""

@@ -477,7 +477,12 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
         sc[rt][i][r] = pow2(__builtin_fmaf(sc[rt][i][r], scale, st[rt].down));
         part += sc[rt][i][r];
       }
-      if (SCALED) sc[rt][i] *= vs[i];
+      if (SCALED && masked) {           // (a new token's scale that is no number reaches the rows that see it)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[rt][i][r] = sc[rt][i][r] == 0.f ? 0.f : sc[rt][i][r] * vs[i][r];
+      } else if (SCALED) {
+        sc[rt][i] *= vs[i];
+      }
     }
     st[rt].sum += part;
     pf[rt] = u32x4{Half<PT>::pack(sc[rt][0][0], sc[rt][0][1]), Half<PT>::pack(sc[rt][0][2], sc[rt][0][3]),
@@ -591,7 +596,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     }
     if (scaled && lane < kAttendTile) {
       s_scale[wave][0][lane] = ks_mine;
-      s_scale[wave][1][lane] = vs_mine;
+      s_scale[wave][1][lane] = okm >> lane & 1 ? vs_mine : 0.f;       // (behind the end there may be anything)
     }
     __builtin_amdgcn_sched_barrier(0);
     // the next tile's keys into the registers of this one's, this one's values into LDS
@@ -795,7 +800,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     }
     if (scaled && wave == 0 && lane < BT) {
       s_scale[buf][0][lane] = ks_mine;
-      s_scale[buf][1][lane] = vs_mine;
+      s_scale[buf][1][lane] = okm >> lane & 1 ? vs_mine : 0.f;        // (behind the end there may be anything)
     }
   };
 
