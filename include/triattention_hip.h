@@ -363,8 +363,8 @@ int tri_compress_step_static(const tri_kv_layout* kv, const tri_batch* batch, co
  * their K and V rows are in the cache; each is a row of q.  A row sees every token before the new ones, itself and its
  * ancestors among the new ones.  out = softmax(scale * k_scale * q . k) v * v_scale, lse the natural logarithm of the
  * sum of exponentials.  A row that sees nothing (seq_lens 0), or nothing but scores of -inf, gets zeros and -inf.  Rows from row_starts[num_seqs] on
- * are left as they were, and so are their lse.  Scores and sums are held in fp32, weights rounded to 16 bits for the product
- * with V (bf16 for fp8 caches, else the cache's type).
+ * are left as they were, and so are their lse.  Scores and sums are held in fp32, weights rounded to the queries' type for the
+ * product with V (with fp16 and row scales after a common power of two).
  * A table entry outside [0, num_blocks) counts as a block without tokens.  Lengths above max_seq_len count as it, rows beyond
  * max_rows of a sequence are left out.  kv: bf16 or fp16 with queries of that type, fp8 (a scale per row where v_scale_layers is set,
  * none otherwise) with queries of either. */

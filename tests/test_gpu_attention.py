@@ -112,11 +112,11 @@ def _score_error(case, reach):
     return case.d * 2.0 ** -24 * case.scale * reach
 
 
-def _check_rows(case, out, lse, want, scale_v=1.0):
+def _check_rows(case, out, lse, want, scale_v=1.0, weight_eps=None, more=0.0):
     """out and lse of every row of every sequence within the bounds above."""
     out, lse = out.cpu(), lse.cpu()
     eps = EPS[case.query]
-    weight_eps = EPS[BF16] if case.cache[0][0].dtype == FP8 else eps
+    weight_eps = weight_eps or (EPS[BF16] if case.cache[0][0].dtype == FP8 else eps)
     for b, (o, z, _, mean_abs, reach) in enumerate(want):
         part = slice(case.starts[b], case.starts[b + 1])
         if part.start == part.stop:
@@ -135,7 +135,7 @@ def _check_rows(case, out, lse, want, scale_v=1.0):
         assert torch.equal(got[~finite & ~torch.isnan(o)], o[~finite & ~torch.isnan(o)])
         vmax = max(1e-30, float(mean_abs[torch.isfinite(mean_abs)].abs().max()) if mean_abs.numel() else 0)
         bound = ((weight_eps + 2 * err.unsqueeze(-1) + (t + 64) * 2.0 ** -24) * mean_abs + eps * o.abs()
-                 + t * 2.0 ** -25 * vmax * 8) * abs(scale_v) + 1e-30
+                 + t * 2.0 ** -25 * vmax * 8) * abs(scale_v) + 1e-30 + more
         if eps == EPS[FP16]:
             bound = bound + 2.0 ** -25           # (an output below the smallest normal number)
         off = (got - o * scale_v).abs()
@@ -196,6 +196,34 @@ def test_decoding_step_head_layouts(heads):
     want = case.expected()
     _check_rows(case, out, lse, want)
     _check_weights(case, weights, before, want, "add")
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,rows", [((8, 2), 1), ((40, 2), 1), ((8, 2), 9), ((16, 4), 40)])
+@pytest.mark.parametrize("scales", ["none", "rows", "growing", "apart", "zero"])
+def test_fp8_rows_with_fp16_queries_round_as_fp16(dim, heads, rows, scales):
+    """Weights are rounded to fp16 (half a step, 2^-11), whatever scales the rows bring along: growing ones, which O has to follow, ones far
+    apart and ones that are 0.  fp16 has 2^-25 absolutely for small weights: of the largest scale, times at most 448, a token."""
+    case = Case([70, 333, 1], q_heads=heads[0], kv_heads=heads[1], dim=dim, rows=[min(rows, 70), rows, 1], seed=dim + rows, dtype=FP8, query=FP16,
+                row_scales=scales != "none")
+    more = 0.0
+    if scales in ("growing", "apart", "zero"):
+        s = case.scales[1][0]
+        for table, t in zip(case.tables, case.lens):
+            for i in range(t):
+                at = (table[i // 16], i % 16)
+                if scales == "growing":
+                    s[at] *= 2.0 ** (i / 16 - 10)
+                elif scales == "apart":
+                    s[at] *= 2.0 ** ((i * 37 % 14) - 7)
+                elif i < 40:
+                    s[at] = 0.0
+        tops = [max(float(s[p].amax()) for p in table) for table in case.tables]
+        more = max(t * 2.0 ** -25 * 448 * top for t, top in zip(case.lens, tops))
+    kv, batch = case.device()
+    print(f"fp8 with fp16 queries dim={dim} heads={heads} rows={rows} {scales}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, parents=case.dev_parents, max_rows=rows, want_lse=True)
+    _check_rows(case, out, lse, case.expected(), weight_eps=EPS[FP16], more=more)
 
 
 @pytest.mark.parametrize("block", [1, 3, 8, 16, 24, 48, 128, 300])

@@ -420,6 +420,43 @@ __device__ __forceinline__ uint32_t seen_of(uint32_t okm, bool drafts, int first
 // The softmax of 32 tokens for RT rows a lane: sc holds q . k of tokens i * 16 + (lane >> 4) * 4 + r; pf receives the weights
 // 2^(x - top) packed for the product with V (vs scales them: fp8 rows with scales of their own).  They are rounded to 16 bits
 // there while the sum adds them unrounded: errors of half a step each and of either sign, below the one rounding of the output.
+// fp8 rows with scales of their own: the weight of a value carries its row's scale, which fp16 has no room for.  There all weights carry
+// a power of two as well, lift, that puts the largest scale so far between 1 and 2^6 (weights stay below 2^14) and that O is freed from
+// at the end.  fp16 loses up to 2^-25 of a weight there, against the 1 or more of the largest scale: no more than the output's own
+// rounding among scales within 2^14 of each other.  A larger scale rescales O, as a larger maximum does; lanes hold the scales
+// of 8 tokens, the lanes of all 32 meet where one of them asks for it.
+template <int QT, bool FP8>
+inline constexpr bool kLifts = FP8 && QT == TRI_KV_FP16;
+template <int RT, int NT>
+__device__ __forceinline__ void lift_scales(f32x4 (&vs)[2], float& lift, f32x4 (&o)[RT][NT]) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(vs[i][r]) < INFINITY ? fabsf(vs[i][r]) : 0.f);
+  // (the first scales set it too, however small)
+  if (__ballot(most * lift > 64.f || (lift == 0.f && most > 0.f))) {
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    const float now = ldexpf(1.f, min(-ilogbf(most), 120)), by = lift == 0.f ? 1.f : now / lift;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) o[rt][t] *= by;
+    lift = now;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) vs[i] *= lift;
+}
+template <int RT, int NT>
+__device__ __forceinline__ void free_of_lift(f32x4 (&o)[RT][NT], float lift) {
+  if (lift == 0.f) return;             // (no scale but 0, or none)
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[rt][t] *= 1.f / lift;
+}
+
 template <int PT, bool SCALED, bool SCORES, int RT, int NT>
 __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT], f32x4 (&o)[RT][NT], u32x4 (&pf)[RT], float scale,
                                           const f32x4 (&ks)[2], const f32x4 (&vs)[2], bool masked, bool drafts, uint32_t okm, int first,
@@ -499,7 +536,7 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
 // HEADS: a wave has a KV head to itself, four neighbours in a workgroup, and nothing is joined here.
 template <int QT, bool FP8, int D, bool UNI, bool HEADS>
 __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) void attend_few_kernel(AttendLaunch a) {
-  constexpr int PT = FP8 ? TRI_KV_BF16 : QT;              // fp8 rows with a scale of their own: the weight carries it, which fp16 has no room for
+  constexpr int PT = QT;                                  // type of the product with V
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int KC = D * ES / 64;                         // 16-byte pieces of a key in a lane
   constexpr int LPR = D * ES / 16;                        // lanes that load one value row
@@ -567,6 +604,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
 
   f32x4 o[1][NT];
   bool odd = false;
+  float lift = 0.f;
   RowState st[1];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -637,6 +675,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
         ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][0][i * 16 + q4 * 4]);
         vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][1][i * 16 + q4 * 4]);
       }
+      if constexpr (kLifts<QT, FP8>) lift_scales<1, NT>(vs, lift, o);
       softmax32<PT, true, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
     } else {
       softmax32<PT, false, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
@@ -662,6 +701,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     for (; tile + kStep < end; tile += kStep) step(tile, std::true_type{});
     if (tile < end) step(tile, std::false_type{});
   }
+  if constexpr (kLifts<QT, FP8>) free_of_lift<1, NT>(o, lift);
   if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, seq, vb, begin, base, seen, lane, part, kParts);
 
   st[0].sum += __shfl_xor(st[0].sum, 16);
@@ -712,7 +752,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
 // TFLOP/s of the 1200 a large product reaches; 8 x 4096 with up to 32 rows of 8: 50 us; 1217 tokens with 16 rows: 12 us.
 template <int QT, bool FP8, int D, int RT, int W, bool UNI>
 __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch a) {
-  constexpr int PT = FP8 ? TRI_KV_BF16 : QT;
+  constexpr int PT = QT;
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int BT = D == 256 ? 32 : 64;                  // tokens of a tile
   constexpr int LPR = D * ES / 16;                        // lanes that load one row
@@ -816,6 +856,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   constexpr bool kScores = RT * W == 4;                   // (of more rows the weights come from the keys once more)
   const ScoreRows scores = kScores ? score_rows(a, b, h, m0, M) : ScoreRows{};
   f32x4 o[RT][NT];
+  float lift = 0.f;
   RowState st[RT];
   const uint64_t anc = n > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
 #pragma unroll
@@ -895,6 +936,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
 #pragma unroll
       for (int i = 0; i < 2; ++i) ks[i] = vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
     }
+    if (kLifts<QT, FP8> && scaled) lift_scales<RT, NT>(vs, lift, o);
     softmax32<PT, FP8, kScores, RT, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
   };
   const bool busy = m0 < M;
@@ -933,6 +975,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   int tile = begin, buf = 0;
   for (; tile + BT < end; tile += BT, buf ^= 1) step(tile, buf, std::true_type{});
   if (tile < end) step(tile, buf, std::false_type{});
+  if constexpr (kLifts<QT, FP8>) free_of_lift<RT, NT>(o, lift);
   if (s_odd) add_odd_values<PT, FP8, NT, RT>(o, seq, vb, begin, base, seen, lane, 0, 1);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
