@@ -333,11 +333,11 @@ __device__ __forceinline__ void load_queries(const AttendLaunch& a, const RowRan
   }
 }
 
-// Infinities and NaNs among the values of new tokens reach the rows that see the token and no others (0 * inf in the matrix
+// Infinities and NaNs among the values (and value scales, vsc) of new tokens reach the rows that see the token and no others (0 * inf in the matrix
 // product would put them into all of them, so there they are 0): rare, at the end, read from memory again.  Tokens from
 // first_tok to end of which every step-th piece of 32, from the piece-th on, is the caller's.
 template <int PT, bool FP8, int NT, int RT>
-__device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Seq& q, GlobalBytes vb, int begin, int base,
+__device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Seq& q, GlobalBytes vb, GlobalF32 vsc, int begin, int base,
                                                const uint64_t (&seen)[RT], int lane, int piece, int step) {
   constexpr int ES = FP8 ? 1 : 2;
 #pragma unroll 1
@@ -346,6 +346,7 @@ __device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Seq& q,
     const int page = q.a.block_table ? q.table[q.div(tok)] : q.b;
     if (page < 0 || page >= q.a.num_blocks) continue;
     const GlobalBytes row = vb + q.byte(page, q.mod(tok), ES);
+    const float by = FP8 && vsc ? vsc[((int64_t)page * q.a.block_size + q.mod(tok)) * q.a.Hkv] : 1.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -354,14 +355,21 @@ __device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Seq& q,
         float v;
         if constexpr (FP8) v = __builtin_amdgcn_cvt_f32_fp8((int)(uint8_t)row[d], 0);
         else v = Half<PT>::value(*(const __attribute__((address_space(1))) uint16_t*)(row + d * ES));
-        if (!(v - v == 0.f)) {
+        if (!(v - v == 0.f) || !(by - by == 0.f)) {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
-            if (seen[rt] >> ((tok - base) & 63) & 1) o[rt][t][e] += v;
+            if (seen[rt] >> ((tok - base) & 63) & 1) o[rt][t][e] += v * by;
         }
       }
     }
   }
+}
+
+// A value's scale as it goes into the product: 0 behind the end, and where it is a new token's and no number (odd).
+__device__ __forceinline__ float scale_of(float vs, bool there, bool is_new, bool& odd) {
+  const bool out = is_new && there && !(vs - vs == 0.f);
+  odd |= out;
+  return there && !out ? vs : 0.f;
 }
 
 __device__ __forceinline__ float lse_of(float top, float total) { return total == 0.f ? -INFINITY : top + log2f(total); }
@@ -514,12 +522,7 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
         sc[rt][i][r] = pow2(__builtin_fmaf(sc[rt][i][r], scale, st[rt].down));
         part += sc[rt][i][r];
       }
-      if (SCALED && masked) {           // (a new token's scale that is no number reaches the rows that see it)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sc[rt][i][r] = sc[rt][i][r] == 0.f ? 0.f : sc[rt][i][r] * vs[i][r];
-      } else if (SCALED) {
-        sc[rt][i] *= vs[i];
-      }
+      if (SCALED) sc[rt][i] *= vs[i];
     }
     st[rt].sum += part;
     pf[rt] = u32x4{Half<PT>::pack(sc[rt][0][0], sc[rt][0][1]), Half<PT>::pack(sc[rt][0][2], sc[rt][0][3]),
@@ -634,7 +637,8 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     }
     if (scaled && lane < kAttendTile) {
       s_scale[wave][0][lane] = ks_mine;
-      s_scale[wave][1][lane] = okm >> lane & 1 ? vs_mine : 0.f;       // (behind the end there may be anything)
+      // (behind the end there may be anything)
+      s_scale[wave][1][lane] = scale_of(vs_mine, okm >> lane & 1, drafts && tile + lane >= base, odd);
     }
     __builtin_amdgcn_sched_barrier(0);
     // the next tile's keys into the registers of this one's, this one's values into LDS
@@ -702,7 +706,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     if (tile < end) step(tile, std::false_type{});
   }
   if constexpr (kLifts<QT, FP8>) free_of_lift<1, NT>(o, lift);
-  if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, seq, vb, begin, base, seen, lane, part, kParts);
+  if (__ballot(odd)) add_odd_values<PT, FP8, NT, 1>(o, seq, vb, vsc, begin, base, seen, lane, part, kParts);
 
   st[0].sum += __shfl_xor(st[0].sum, 16);
   st[0].sum += __shfl_xor(st[0].sum, 32);
@@ -840,7 +844,9 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     }
     if (scaled && wave == 0 && lane < BT) {
       s_scale[buf][0][lane] = ks_mine;
-      s_scale[buf][1][lane] = okm >> lane & 1 ? vs_mine : 0.f;        // (behind the end there may be anything)
+      bool odd = false;
+      s_scale[buf][1][lane] = scale_of(vs_mine, okm >> lane & 1, n > 1 && tile + lane >= base, odd);
+      if (odd) s_odd = 1;
     }
   };
 
@@ -976,7 +982,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   for (; tile + BT < end; tile += BT, buf ^= 1) step(tile, buf, std::true_type{});
   if (tile < end) step(tile, buf, std::false_type{});
   if constexpr (kLifts<QT, FP8>) free_of_lift<RT, NT>(o, lift);
-  if (s_odd) add_odd_values<PT, FP8, NT, RT>(o, seq, vb, begin, base, seen, lane, 0, 1);
+  if (s_odd) add_odd_values<PT, FP8, NT, RT>(o, seq, vb, vsc, begin, base, seen, lane, 0, 1);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     st[rt].sum += __shfl_xor(st[rt].sum, 16);
