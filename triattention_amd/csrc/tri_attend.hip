@@ -37,9 +37,9 @@ __device__ __forceinline__ void join_rows(const AttendLaunch& a, int64_t group) 
   const bool in = at < (int64_t)a.B * a.Hkv * rows_max;
   const int m = in ? (int)(at % rows_max) : 0;
   const int h = in ? (int)(at / rows_max % a.Hkv) : 0, b = in ? (int)(at / rows_max / a.Hkv) : 0;
-  const RowRange rows = rows_of(a, b);
-  const bool live_row = in && m < rows.n * a.G;
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
+  const RowRange rows = rows_of(a, b, T);
+  const bool live_row = in && m < rows.n * a.G;
   const int live = max(1, ceil_div(tokens_of(a, b, T), a.split_tokens));
   const int64_t first = ((int64_t)b * a.Hkv + h) * a.nsplit * rows_max + m;
   const int d = lane * 4;
@@ -101,12 +101,12 @@ __device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weight
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   if (t0 >= T) return;
   const int mine = t0 + (TOGETHER ? (int)threadIdx.x : lane);
-  const RowRange rows = rows_of(a, (int)b);
+  const RowRange rows = rows_of(a, (int)b, T);
   const int t = min(mine, T - 1);
   const int page = a.block_table ? a.block_table[b * a.block_table_pitch + t / a.block_size] : (int)b;
   const bool ok = mine < T && page >= 0 && page < a.num_blocks;
   float* const w = weights + (ok ? ((int64_t)page * a.block_size + t % a.block_size) * a.Hkv + h0 : 0);
-  const bool fresh = set || t >= T - rows.n;      // the rows' own tokens: nothing has been added for them yet
+  const bool fresh = set || t >= T - rows.fresh;  // new tokens: nothing has been added for them yet
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   if (ok && !fresh) {
     if (VEC) sum = *reinterpret_cast<const f32x4*>(w);

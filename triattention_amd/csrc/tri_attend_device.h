@@ -4,8 +4,8 @@
 //   s[m][t] = scale * q[m] . k[t]   where row m sees token t, else -inf
 //   out[m]  = sum_t 2^(s log2 e - M) v[t] / sum_t 2^(s log2 e - M),   M the running maximum
 //
-// Rows: a sequence has n new tokens, the last n of its cache; KV head h serves the M = n * G rows (token i, query head
-// h * G + g), m = i * G + g.  Row m sees every token before the new ones, and of those token i and its ancestors.
+// Rows: the new tokens of a sequence are the last of its cache, n of them have rows here; KV head h serves the M = n * G rows
+// (token i, query head h * G + g), m = i * G + g.  Row m sees every token before the new ones, and of those token i and its ancestors.
 //
 // S^T = K Q^T on the matrix cores (16 tokens x 16 rows x 32 elements) leaves in a lane the scores of one row (lane & 15) for
 // tokens (lane >> 4) * 4 + r: exactly the order in which the B operand of O^T = V^T P^T wants them, if the 32 tokens of that
@@ -150,15 +150,17 @@ __device__ __forceinline__ uint64_t ancestor_mask(const int32_t* parents, int fi
   return m;
 }
 
+// Rows of a sequence of T tokens: the first of them, how many are computed, and how many new tokens the sequence has, which is more where
+// there are rows beyond max_rows or beyond q's.  (No row that is computed sees a new token behind the 64th, so more of
+// them than T + 64 are that many.)
 struct RowRange {
-  int first, n;      // first row of the sequence and their number
+  int first, n, fresh;
 };
-__device__ __forceinline__ RowRange rows_of(const AttendLaunch& a, int b) {
-  if (!a.row_starts) return {b, 1};
-  int first = a.row_starts[b], end = a.row_starts[b + 1];
-  first = min(max(first, 0), a.num_rows);
-  end = min(max(end, first), a.num_rows);
-  return {first, min(end - first, a.max_rows)};
+__device__ __forceinline__ RowRange rows_of(const AttendLaunch& a, int b, int T) {
+  if (!a.row_starts) return {b, 1, 1};
+  const int64_t from = a.row_starts[b], to = a.row_starts[b + 1];
+  const int first = min(max((int)from, 0), a.num_rows), end = min(max((int)to, first), a.num_rows);
+  return {first, min(end - first, a.max_rows), (int)min(max(to - from, (int64_t)0), (int64_t)T + 64)};
 }
 
 // What a workgroup works on: a split of a sequence (the unit), one KV head and block of rows of it (inner).  Workgroups go to the
@@ -341,7 +343,7 @@ __device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Seq& q,
                                                const uint64_t (&seen)[RT], int lane, int piece, int step) {
   constexpr int ES = FP8 ? 1 : 2;
 #pragma unroll 1
-  for (int tok = max(begin, base); tok < q.end; ++tok) {
+  for (int tok = max(begin, base); tok < min(q.end, base + 64); ++tok) {
     if ((tok - begin) / kAttendTile % step != piece) continue;
     const int page = q.a.block_table ? q.table[q.div(tok)] : q.b;
     if (page < 0 || page >= q.a.num_blocks) continue;
@@ -358,7 +360,7 @@ __device__ __forceinline__ void add_odd_values(f32x4 (&o)[RT][NT], const Seq& q,
         if (!(v - v == 0.f) || !(by - by == 0.f)) {
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
-            if (seen[rt] >> ((tok - base) & 63) & 1) o[rt][t][e] += v * by;
+            if (seen[rt] >> (tok - base) & 1) o[rt][t][e] += v * by;
         }
       }
     }
@@ -422,6 +424,7 @@ constexpr float kSlack = 8.f;
 // ones, itself and its ancestors.
 __device__ __forceinline__ uint32_t seen_of(uint32_t okm, bool drafts, int first, uint64_t seen) {
   if (!drafts) return okm;
+  if (first >= 64) return 0;
   return okm & (first >= 0 ? (uint32_t)(seen >> (first & 63)) : (uint32_t)(seen << (-first & 63)) | ((1u << (-first & 31)) - 1));
 }
 
@@ -561,13 +564,13 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   const int b = work.b, split = work.split, h = work.h + (HEADS ? wave : 0), part = HEADS ? 0 : wave;
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
-  const RowRange rows = rows_of(a, b);
-  const int n = rows.n, M = n * a.G;
+  const RowRange rows = rows_of(a, b, T);
+  const int n = rows.n, fresh = rows.fresh, M = n * a.G;
   if (M == 0) return;
   const int Tv = tokens_of(a, b, T);
   const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
   if (begin >= Tv && split > 0) return;
-  const int base = T - n;                                 // first new token (negative: not all of them are in the cache)
+  const int base = T - fresh;                             // first new token (negative: not all of them are in the cache)
   const GlobalBytes kb = (GlobalBytes)a.k_layers[a.layer] + (int64_t)h * a.stride_head * ES;
   const GlobalBytes vb = (GlobalBytes)a.v_layers[a.layer] + (int64_t)h * a.stride_head * ES;
   const bool scaled = FP8 && a.k_scale_layers;
@@ -578,7 +581,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   u32x4 qf[D / 32];
   load_queries<FP8, D>(a, rows, h, 0, M, lane, qf);
   uint64_t seen[1] = {1};
-  if (n > 1) seen[0] = (uint64_t)shfl64((int64_t)ancestor_mask(a.parents, rows.first, n, lane), min(c16, M - 1) / a.G);
+  if (fresh > 1) seen[0] = (uint64_t)shfl64((int64_t)ancestor_mask(a.parents, rows.first, n, lane), min(c16, M - 1) / a.G);
 
   const Seq seq(a, b, h, T, end);
   Finder<UNI, ES, kAttendTile, kStep> find(seq, lane);
@@ -618,7 +621,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   auto step = [&](int tile, auto has_next) {
     constexpr bool more = decltype(has_next)::value;
     const uint32_t okm = ok_now;
-    const bool drafts = n > 1 && tile + kAttendTile > base;
+    const bool drafts = fresh > 1 && tile + kAttendTile > base;
 
     f32x4 sc[1][2];
 #pragma unroll
@@ -778,15 +781,15 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   const int b = work.b, split = work.split, h = work.h, rb = work.rb;
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
-  const RowRange rows = rows_of(a, b);
-  const int n = rows.n, M = n * a.G;
+  const RowRange rows = rows_of(a, b, T);
+  const int n = rows.n, fresh = rows.fresh, M = n * a.G;
   if (rb * RT * 16 * W >= M) return;
   const int m0 = (rb * W + wave) * RT * 16;
   const bool loads = RPL * W <= BT || wave * RPL < BT;    // (small rows: a load of every wave would be more than a tile)
   const int Tv = tokens_of(a, b, T);
   const int begin = split * a.split_tokens, end = min(begin + a.split_tokens, Tv);
   if (begin >= Tv && split > 0) return;
-  const int base = T - n;
+  const int base = T - fresh;
   const GlobalBytes kb = (GlobalBytes)a.k_layers[a.layer] + (int64_t)h * a.stride_head * ES;
   const GlobalBytes vb = (GlobalBytes)a.v_layers[a.layer] + (int64_t)h * a.stride_head * ES;
   const bool scaled = FP8 && a.k_scale_layers;
@@ -815,7 +818,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     const uint64_t okm = find.ok;
     if (!loads) return;
     const bool all = BT == 64 ? okm == ~0ull : (uint32_t)okm == ~0u;
-    const bool drafts = n > 1 && tile + BT > base;
+    const bool drafts = fresh > 1 && tile + BT > base;
     if (!all || drafts) {
       const int l = here(lane);
       bool odd = false;
@@ -845,7 +848,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     if (scaled && wave == 0 && lane < BT) {
       s_scale[buf][0][lane] = ks_mine;
       bool odd = false;
-      s_scale[buf][1][lane] = scale_of(vs_mine, okm >> lane & 1, n > 1 && tile + lane >= base, odd);
+      s_scale[buf][1][lane] = scale_of(vs_mine, okm >> lane & 1, fresh > 1 && tile + lane >= base, odd);
       if (odd) s_odd = 1;
     }
   };
@@ -864,7 +867,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   f32x4 o[RT][NT];
   float lift = 0.f;
   RowState st[RT];
-  const uint64_t anc = n > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
+  const uint64_t anc = fresh > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int m = m0 + rt * 16 + c16;
@@ -929,7 +932,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   };
   auto softmax = [&](int first, int sub, int buf) {
     const uint32_t okm = (uint32_t)(ok_now >> (sub * 32));
-    const bool drafts = n > 1 && first + 32 > base;
+    const bool drafts = fresh > 1 && first + 32 > base;
     const bool masked = okm != 0xffffffffu || drafts;
     f32x4 ks[2] = {}, vs[2] = {};
     if (scaled) {
@@ -1012,8 +1015,8 @@ __global__ __launch_bounds__(kAttendThreads, 2) void weigh_rows_kernel(AttendLau
   const int unit = blockIdx.x / a.Hkv, b = unit / spans, t0 = (unit % spans * kAttendWaves + wave) * TOK;
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
   if (t0 >= T) return;
-  const RowRange rows = rows_of(a, b);
-  const int n = rows.n, M = n * a.G, base = T - n;
+  const RowRange rows = rows_of(a, b, T);
+  const int n = rows.n, fresh = rows.fresh, M = n * a.G, base = T - fresh;
   const GlobalBytes kb = (GlobalBytes)a.k_layers[a.layer] + (int64_t)h * a.stride_head * ES;
   const bool scaled = FP8 && a.k_scale_layers;
 
@@ -1055,8 +1058,8 @@ __global__ __launch_bounds__(kAttendThreads, 2) void weigh_rows_kernel(AttendLau
     for (int i = 0; i < NG; ++i) ks[i] *= *reinterpret_cast<const f32x4*>(&s_token[wave][i * 16 + q4 * 4]);
     __builtin_amdgcn_wave_barrier();
   }
-  const uint64_t anc = n > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
-  const bool drafts = n > 1 && t0 + TOK > base;
+  const uint64_t anc = fresh > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
+  const bool drafts = fresh > 1 && t0 + TOK > base;
 
   // a row's queries, lse (infinite where it adds nothing) and new tokens it sees; asked for one tile of rows ahead
   u32x4 q_next[D / 32];

@@ -789,6 +789,8 @@ def _attend_params(kv: PagedKV, batch: StepBatch, q, layer, row_starts, parents,
     if not 0 <= layer < kv.num_layers:
         raise IndexError(f"layer {layer} of {kv.num_layers}")
     rows, heads, _ = shape
+    if max_rows is None:
+        max_rows = 1 if row_starts is None else min(max(rows, 1), 64)
     if row_starts is not None:
         _on(kv, "row_starts", row_starts, torch.int32)
         if row_starts.shape != (batch.num_seqs + 1,) or not row_starts.is_contiguous():
@@ -813,7 +815,7 @@ def _attend_params(kv: PagedKV, batch: StepBatch, q, layer, row_starts, parents,
 
 
 def attend_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, *, layer: int = 0, row_starts: torch.Tensor | None = None,
-                 parents: torch.Tensor | None = None, max_rows: int = 1, scale: float | None = None, k_scale: float = 1.0,
+                 parents: torch.Tensor | None = None, max_rows: int | None = None, scale: float | None = None, k_scale: float = 1.0,
                  v_scale: float = 1.0, weights: torch.Tensor | None = None, weight_mode: str = "add",
                  out: torch.Tensor | None = None, want_lse: bool = False):
     """Attention of the newest tokens of every sequence over one layer of the cache (``tri_attend_paged``).
@@ -821,7 +823,8 @@ def attend_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, *, layer: int =
     ``q`` [rows, Hq, D], after RoPE, of the cache's type (fp8 caches: bf16 or fp16).  The new tokens are the last ones of
     ``batch.seq_lens``, their keys and values are in the cache already.  Without ``row_starts`` there is one per
     sequence: a decoding step.  With it (int32 [sequences + 1] on the device, ascending) sequence b has the rows
-    ``row_starts[b]`` to ``row_starts[b + 1] - 1``, at most ``max_rows`` <= 64, and ``parents`` (int32 [rows]) says which earlier
+    ``row_starts[b]`` to ``row_starts[b + 1] - 1``, of which the first ``max_rows`` <= 64 are computed (None: as many as ``q`` has,
+    64 at most; the call is cut for them, so a program that knows fewer says so; those beyond are left as they were), and ``parents`` (int32 [rows]) says which earlier
     row of its sequence each follows, counted from the sequence's first (anything else, such as -1: the
     last token before them; None: each follows the one before): a tree of drafted tokens, or a short chunk of a
     prompt.  A row sees every token before the new ones, its ancestors and itself.  Rows behind ``row_starts[-1]`` are
