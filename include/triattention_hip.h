@@ -378,7 +378,7 @@ typedef struct tri_attend_params {
   int32_t num_blocks;           /* physical blocks of the cache */
   const void* q;                /* element (row, head, d) at q + row*q_stride_row + head*q_stride_head + d; 16-byte aligned rows */
   int64_t q_stride_row, q_stride_head;
-  void* out;                    /* q's type, likewise */
+  void* out;                    /* q's type, likewise; may be q itself (same strides), any other element of it may not be one of q's */
   int64_t out_stride_row, out_stride_head;
   float* lse;                   /* [num_rows][num_q_heads], or NULL */
   const int32_t* row_starts;    /* [num_seqs + 1] ascending: rows of sequence b are row_starts[b] to row_starts[b+1] - 1;
@@ -392,6 +392,7 @@ typedef struct tri_attend_params {
                                    of the call may then share a block (each would read and write its weights) */
   int32_t weight_mode;          /* 0: added, for the new tokens' own slots written; 1: written for every token of a sequence */
 } tri_attend_params;
+/* (of the call's own q and out, or of neither: with many rows and weights, out in q's memory takes a copy of q) */
 uint64_t tri_attend_workspace_bytes(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p);
 int tri_attend_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_attend_params* p, void* workspace,
                      uint64_t workspace_bytes, void* stream);

@@ -1,0 +1,26 @@
+"""The attention and eviction entry points without a GPU: plans and refusals of calls at the edge of what they allow."""
+from __future__ import annotations
+
+import ctypes as C
+
+from test_attention import _attend, _batch, _layout
+from triattention_amd import _lib
+
+
+def test_scratch_for_a_copy_of_q_where_out_lies_in_its_memory():
+    """Only where weights of many rows are wanted, by the elements that q and out span; without addresses as if they overlapped."""
+    lib = _lib.load()
+    rows, heads = 60, 64
+
+    def need(**kw):
+        p = _attend(num_q_heads=heads, num_rows=rows, max_rows=20, row_starts=8, q_stride_row=heads * 128, out_stride_row=heads * 128, **kw)
+        got = lib.tri_attend_workspace_bytes(C.byref(_layout()), C.byref(_batch()), C.byref(p))
+        assert got > 0
+        return got
+
+    size = rows * heads * 128 * 2
+    base = need(q=1 << 20, out=(1 << 20) + size, weights=16)
+    for q, out in ((1 << 20, 1 << 20), ((1 << 20) + size - 16, 1 << 20), (1 << 20, (1 << 20) + size - 16), (None, None)):
+        assert need(q=q, out=out, weights=16) == base + size
+    assert need(q=(1 << 20) + size, out=1 << 20, weights=16) == base
+    assert need(q=16, out=16) == need(q=1 << 20, out=(1 << 20) + size)

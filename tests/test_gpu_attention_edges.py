@@ -99,3 +99,62 @@ def test_without_max_rows_every_row_is_computed():
     print("no max_rows", flush=True)
     out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, parents=case.dev_parents, want_lse=True)
     _check_rows(case, out, lse, case.expected())
+
+
+# ------------------------------------------------------------------------ out in place of q
+@pytest.mark.parametrize("heads,dim,rows", [((8, 2), 64, [1, 1]), ((8, 1), 128, [4, 3]), ((32, 1), 128, [1, 1]), ((33, 1), 64, [1, 1]),
+                                            ((32, 2), 128, [9, 4]), ((9, 1), 256, [9, 2])])
+@pytest.mark.parametrize("layout", ["same", "beside", "shifted_rows"])
+def test_out_may_be_q(heads, dim, rows, layout):
+    """The same memory, or parts of one tensor with q and out in turn: what a call with memory of its own gives.  A copy of q
+    is what the weights of many rows then go by."""
+    case = Case([3000, 41], q_heads=heads[0], kv_heads=heads[1], dim=dim, rows=rows, seed=dim + heads[0])
+    kv, batch = case.device()
+    before = _weights(case)
+    weights = before.to(DEV)
+    args = dict(row_starts=case.dev_starts, parents=case.dev_parents, max_rows=max(rows), want_lse=True)
+    want, lse = ops.attend_paged(kv, batch, case.q.to(DEV), weights=weights, **args)
+    n = len(case.q)
+    if layout == "same":
+        q = out = case.q.to(DEV)
+    elif layout == "beside":                  # the rows of q and out in turn
+        room = torch.empty(n, 2, heads[0], dim, dtype=BF16, device=DEV)
+        q, out = room[:, 0], room[:, 1]
+    else:                                     # heads before rows, q's rows ahead of out's in every head
+        room = torch.empty(heads[0], 2 * n, dim, dtype=BF16, device=DEV)
+        q, out = room[:, :n].transpose(0, 1), room[:, n:].transpose(0, 1)
+    q.copy_(case.q)
+    again = before.to(DEV)
+    print(f"out in q's memory heads={heads} dim={dim} rows={rows} {layout}", flush=True)
+    got, lse2 = ops.attend_paged(kv, batch, q, weights=again, out=out, **args)
+    assert torch.equal(got, want) and torch.equal(lse, lse2)
+    assert torch.equal(again, weights)
+    _check_weights(case, again, before, case.expected(), "add")
+
+
+def test_out_in_q_s_memory_captured():
+    """The copy of q is of the call: every replay takes what then stands there."""
+    case = Case([700, 41], q_heads=32, kv_heads=2, rows=[9, 4], seed=2)
+    kv, batch = case.device()
+    args = dict(row_starts=case.dev_starts, parents=case.dev_parents, max_rows=9, want_lse=True)
+    buf = case.q.to(DEV)
+    weights = torch.zeros(1, case.pool, 16, 2, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ops.attend_paged(kv, batch, buf, weights=weights, out=buf, **args)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, lse = ops.attend_paged(kv, batch, buf, weights=weights, weight_mode="set", out=buf, **args)
+    for rep in range(3):
+        q = torch.randn(case.q.shape, device=DEV).to(BF16)
+        expect = torch.zeros_like(weights)
+        want, want_lse = ops.attend_paged(kv, batch, q, weights=expect, weight_mode="set", **args)
+        buf.copy_(q)
+        weights.zero_()
+        print(f"replay {rep}", flush=True)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(buf, want) and torch.equal(lse, want_lse) and torch.equal(weights, expect)

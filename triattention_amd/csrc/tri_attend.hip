@@ -201,7 +201,21 @@ hipError_t launch_finish_typed(const AttendLaunch& a, float* weights, int set, h
   return vec ? pick(One{}, std::true_type{}) : pick(One{}, std::false_type{});
 }
 
+// 16 bytes a thread.
+__global__ __launch_bounds__(kThreads) void copy_queries_kernel(AttendLaunch a, uint4* dst) {
+  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = i / (a.D / 8);
+  if (row >= (int64_t)a.num_rows * a.Hq) return;
+  const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + row / a.Hq * a.q_stride_row + row % a.Hq * a.q_stride_head + i % (a.D / 8) * 8;
+  dst[i] = *reinterpret_cast<const uint4*>(q);
+}
+
 }  // namespace
+
+hipError_t launch_copy_queries(const AttendLaunch& a, void* dst, hipStream_t s) {
+  const int64_t groups = ceil_div64((int64_t)a.num_rows * a.Hq * (a.D / 8), kThreads);
+  hipLaunchKernelGGL(copy_queries_kernel, dim3((unsigned)groups), dim3(kThreads), 0, s, a, reinterpret_cast<uint4*>(dst));
+  return hipGetLastError();
+}
 
 hipError_t launch_attend(const AttendLaunch& a, hipStream_t s) {
   const bool bf16 = a.q_dtype == TRI_KV_BF16;

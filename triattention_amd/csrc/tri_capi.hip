@@ -893,11 +893,11 @@ namespace {
 // How a call of attend_kernel is cut, and what it needs of the workspace.
 struct AttendPlan {
   tri::AttendLaunch a{};
-  int64_t part_out, part_ml, lse2, scores, total;
+  int64_t part_out, part_ml, lse2, scores, q_copy, total;
   // block selection
   int64_t block_scores, counts;
   int max_count;
-  bool weigh_again;
+  bool weigh_again, copies_q;
 };
 
 constexpr int kMaxNewTokens = 64;          // a word of ancestors
@@ -906,6 +906,16 @@ int attend_workgroups_per_cu(int row_tiles, int D) {
   if (row_tiles == 0) return D == 64 ? 4 : D == 128 ? 2 : 1;
   if (row_tiles == 4) return D == 64 ? 4 : 2;
   return 1;
+}
+
+// The bytes that rows of heads span.
+struct Span {
+  intptr_t from, to;
+};
+Span span_of(const void* p, int64_t rows, int64_t stride_row, int64_t heads, int64_t stride_head, int D) {
+  const int64_t r = (rows - 1) * stride_row, h = (heads - 1) * stride_head;
+  const intptr_t at = reinterpret_cast<intptr_t>(p);
+  return {at + (std::min<int64_t>(r, 0) + std::min<int64_t>(h, 0)) * 2, at + (std::max<int64_t>(r, 0) + std::max<int64_t>(h, 0) + D) * 2};
 }
 
 bool is_finite(float x) { return x - x == 0.f; }
@@ -1030,6 +1040,11 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   // from the keys once more: 2 x 32768 tokens of 8 x 128 bf16, 20 rows a KV head 94 us from scores and 104 from keys, 32 rows
   // 105 and 104, 128 rows 231 and 141, of fp8 32 rows 75 and 78, 64 rows 107 and 91; rows of 256 dimensions, 64 of them, 115 and 120.
   d.weigh_again = p->weights && rows > (a.D == 256 ? 64 : 32);
+  // (they read the queries again when out is written: out in q's memory is read from a copy)
+  const Span of_q = span_of(p->q, a.num_rows, a.q_stride_row, a.Hq, a.q_stride_head, a.D);
+  const Span of_out = span_of(p->out, a.num_rows, a.out_stride_row, a.Hq, a.out_stride_head, a.D);
+  d.copies_q = d.weigh_again && a.num_rows > 0 && of_q.from < of_out.to && of_out.from < of_q.to;
+  d.q_copy = take(d.copies_q ? (int64_t)a.num_rows * a.Hq * a.D * 2 : 0);
   d.lse2 = take(p->weights ? (int64_t)a.num_rows * a.Hq * 4 : 0);
   d.scores = take(p->weights && !d.weigh_again ? (int64_t)a.B * a.Hkv * rows * a.score_pitch * 4 : 0);
   d.block_scores = take(bp ? (int64_t)a.B * a.Hkv * d.max_count * 4 : 0);
@@ -1055,9 +1070,16 @@ int do_attend(AttendPlan& d, void* ws, float* weights, int weight_mode, hipStrea
   const bool again = d.weigh_again;
   if (again || (weights && a.nsplit == 1)) a.lse2 = at<float>(ws, d.lse2);
   if (weights && !again) a.scores = at<float>(ws, d.scores);
-  int rc = launch_status(tri::launch_attend(a, s), "attend");
+  int rc = TRI_OK;
+  if (d.copies_q) rc = launch_status(tri::launch_copy_queries(a, at<void>(ws, d.q_copy), s), "copy_queries");
+  if (!rc) rc = launch_status(tri::launch_attend(a, s), "attend");
   if (!rc) rc = launch_status(tri::launch_attend_finish(a, again ? nullptr : weights, weight_mode, s), "attend_finish");
   if (rc || !again) return rc;
+  if (d.copies_q) {
+    a.q = at<void>(ws, d.q_copy);
+    a.q_stride_row = (int64_t)a.Hq * a.D;
+    a.q_stride_head = a.D;
+  }
   a.weigh = 1;
   a.weights = weights;
   a.weight_set = weight_mode;

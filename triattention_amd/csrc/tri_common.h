@@ -298,6 +298,8 @@ hipError_t launch_attend_128_fp16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_256_bf16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend_256_fp16(const AttendLaunch& a, hipStream_t s);
 hipError_t launch_attend(const AttendLaunch& a, hipStream_t s);
+// The queries one behind the other, [num_rows][Hq][D], at dst.
+hipError_t launch_copy_queries(const AttendLaunch& a, void* dst, hipStream_t s);
 // What follows it: the splits joined (nsplit > 1) and, of few rows with weights (the layer's
 // [num_blocks][block_size][Hkv]), the weights added to them (set: written) from the scores the attention left.
 hipError_t launch_attend_finish(const AttendLaunch& a, float* weights, int set, hipStream_t s);

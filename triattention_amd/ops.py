@@ -835,7 +835,8 @@ def attend_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, *, layer: int =
     ("set").  ``select_by_weight`` and ``evict_step`` go by them.  Sequences of such a call may not share blocks; of
     few rows its scratch holds the scores, four bytes per row, query head and token.
 
-    ``scale`` (default head_dim ** -0.5) times ``k_scale`` must be positive.
+    ``scale`` (default head_dim ** -0.5) times ``k_scale`` must be positive.  ``out`` may be ``q`` itself; otherwise they have no element
+    in common.
 
     Lengths are read on the device: a program that replays a captured call may rewrite ``batch.seq_lens`` in place, up to
     the batch's ``max_seq_len``; a sequence of no tokens gives zeros.  Returns (out, lse or None)."""
