@@ -376,7 +376,7 @@ typedef struct tri_attend_params {
   int32_t max_rows;             /* 1 to 64: most rows of a sequence that are computed */
   int32_t q_dtype;              /* TRI_KV_BF16 or TRI_KV_FP16 */
   int32_t num_blocks;           /* physical blocks of the cache */
-  const void* q;                /* element (row, head, d) at q + row*q_stride_row + head*q_stride_head + d; 16-byte aligned rows */
+  const void* q;                /* (q and out may be NULL where num_rows is 0) element (row, head, d) at q + row*q_stride_row + head*q_stride_head + d; 16-byte aligned rows */
   int64_t q_stride_row, q_stride_head;
   void* out;                    /* q's type, likewise; may be q itself (same strides), any other element of it may not be one of q's */
   int64_t out_stride_row, out_stride_head;

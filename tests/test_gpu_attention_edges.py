@@ -158,3 +158,26 @@ def test_out_in_q_s_memory_captured():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(buf, want) and torch.equal(lse, want_lse) and torch.equal(weights, expect)
+
+
+# --------------------------------------------------------------------------------- no rows
+@pytest.mark.parametrize("heads,most", [((8, 2), 1), ((8, 2), 16), ((16, 1), 64)])
+@pytest.mark.parametrize("mode", ["add", "set"])
+def test_a_call_of_no_rows(heads, most, mode):
+    """Nothing to attend: no error; "set" writes a weight of nothing for every token, "add" adds it."""
+    case = Case([5000, 41, 0], q_heads=heads[0], kv_heads=heads[1], dim=64, rows=[0, 0, 0], seed=3)
+    kv, batch = case.device()
+    before = _weights(case)
+    weights = before.to(DEV)
+    print(f"no rows {heads} {most} {mode}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, max_rows=most, weights=weights, weight_mode=mode,
+                                want_lse=True)
+    assert out.shape == (0, heads[0], 64) and lse.shape == (0, heads[0])
+    expect = before.clone()
+    if mode == "set":
+        for b, t in enumerate(case.lens):
+            for i in range(t):
+                expect[0, case.tables[b][i // 16], i % 16] = 0
+    assert torch.equal(weights.cpu(), expect)
+    out, none = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, max_rows=most)
+    assert len(out) == 0 and none is None

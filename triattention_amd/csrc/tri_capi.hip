@@ -1054,7 +1054,7 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
 }
 
 int check_attend_pointers(const tri_attend_params* p, const AttendPlan& d, void* ws, uint64_t ws_bytes) {
-  if (!p->q || !p->out) return fail(TRI_ERR_INVALID_ARGUMENT, "q / out is NULL");
+  if (p->num_rows > 0 && (!p->q || !p->out)) return fail(TRI_ERR_INVALID_ARGUMENT, "q / out is NULL");
   if (!is_aligned(p->q, 16) || !is_aligned(p->out, 16)) return fail(TRI_ERR_INVALID_ARGUMENT, "q and out must be 16-byte aligned");
   tri::Workspace need{};
   need.total = d.total;
@@ -1143,7 +1143,7 @@ int tri_attend_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_
   if (!rc) rc = check_attend_pointers(p, d, ws, ws_bytes);
   if (!rc) rc = check_pages(kv, batch);
   if (rc) return rc;
-  if (p->num_rows == 0) return TRI_OK;
+  if (p->num_rows == 0 && !p->weights) return TRI_OK;
   return do_attend(d, ws, p->weights, p->weight_mode, (hipStream_t)stream);
 }
 
