@@ -422,8 +422,10 @@ int tri_attend_blocks(const tri_kv_layout* kv, const tri_batch* batch, const tri
 /* Eviction by the weights tri_attend_paged adds up, in place of the calibrated scores: per sequence and KV head the budget
  * tokens of the largest weight (mean over layers summed in 64 bits, or maximum; layer_reduce -1: a keep set per layer), the
  * last window_size tokens and, with protect_prefill, those before prefill_lens always among the first choices; ties keep
- * the lowest token, a NaN counts as more than any number.  keep: int32 [rows][max_budget] as tri_select's, -1 behind a sequence's budget; final_scores (may be
- * NULL): [rows][max_seq_len], +inf where guarded, -inf behind the sequence.  tri_evict_step also moves K, V, their scales
+ * the lowest token.  A NaN counts as more than any number, whatever its sign and the guards' +inf among them: more of them
+ * than a head's budget leave no room for guarded tokens.  An infinite weight is a guard's equal.
+ * keep: int32 [rows][max_budget] as tri_select's, -1 behind a sequence's budget; final_scores (may be NULL):
+ * [rows][max_seq_len], +inf where guarded, -inf behind the sequence.  tri_evict_step also moves K, V, their scales
  * and the weights of the kept tokens into the first slots (tri_compact_paged); its block table must be valid. */
 typedef struct tri_evict_params {
   int32_t num_blocks;

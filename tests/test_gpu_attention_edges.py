@@ -181,3 +181,44 @@ def test_a_call_of_no_rows(heads, most, mode):
     assert torch.equal(weights.cpu(), expect)
     out, none = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, max_rows=most)
     assert len(out) == 0 and none is None
+
+
+# ------------------------------------------------------------------------------- eviction
+@pytest.mark.parametrize("reduce,shared", [("mean", False), ("max", False), (None, False), ("mean", True), ("max", True)])
+def test_negative_nan_weights_are_kept_first_too(reduce, shared):
+    """A NaN counts as more than any number whatever its sign bit."""
+    case = Case([200], q_heads=8, kv_heads=4, layers=2, seed=3, garbage=None)
+    kv, batch = case.device(budgets=[20])
+    before = _weights(case)
+    odd = [4, 50, 51, 100]
+    for t in odd:
+        before[:, case.tables[0][t // 16], t % 16, 1] = torch.tensor(-0x400000, dtype=torch.int32).view(torch.float32)
+    assert int(before[0, case.tables[0][0], 4, 1:2].contiguous().view(torch.int32)[0]) == -0x400000
+    weights = before.to(DEV)
+    print(f"negative NaN {reduce} {shared}", flush=True)
+    keep, scores = ops.select_by_weight(kv, batch, weights, ops.EvictConfig(window_size=8, layer_reduce=reduce, shared=shared), want_scores=True)
+    keep, scores = keep.cpu(), scores.cpu()
+    for r in range(len(keep)):
+        if shared or r % 4 == 1:
+            assert set(odd) <= set(keep[r].tolist()), r
+            assert bool(torch.isnan(scores[r, odd]).all())
+        assert set(range(192, 200)) <= set(keep[r].tolist()), r
+
+
+def test_eviction_of_long_rows_keeps_what_the_definition_keeps_in_every_head():
+    """Rows longer than a tile of the weights' move, every head's list against the definition."""
+    case = Case([9000], q_heads=4, kv_heads=4, dim=64, layers=2, seed=2, garbage=None)
+    kv, batch = case.device(budgets=[5000])
+    before = _weights(case)
+    before[1, case.tables[0][7], 3, 2] = math.inf
+    weights = before.to(DEV)
+    print("evict long", flush=True)
+    keep = ops.evict_step(kv, batch, weights, ops.EvictConfig(window_size=0)).cpu()
+    slots = torch.tensor([case.tables[0][i // 16] * 16 + i % 16 for i in range(9000)])
+    flat = before.view(2, -1, 4)[:, slots]
+    mean = (flat.double().sum(0) / 2).float()
+    for h in range(4):
+        want = torch.sort(mean[:, h], descending=True, stable=True).indices[:5000].sort().values
+        assert torch.equal(keep[h].long(), want), h
+        assert torch.equal(weights.cpu().view(2, -1, 4)[:, slots[:5000], h], flat[:, want, h])
+    assert 7 * 16 + 3 in keep[2].tolist()

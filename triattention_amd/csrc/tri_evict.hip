@@ -77,9 +77,10 @@ __global__ __launch_bounds__(256) void weight_rows_kernel(EvictLaunch a, int wid
         for (int e = 0; e < min(kHeads, left); ++e) v[0] = larger(x[e], v[0]);
     }
   }
+  // (one NaN for all: the top-k orders by the bits, where those of negative sign lie below every number)
 #pragma unroll
   for (int e = 0; e < kHeads; ++e)
-    if (e < mine) out[(int64_t)e * a.Tmax] = v[e];
+    if (e < mine) out[(int64_t)e * a.Tmax] = __builtin_isnan(v[e]) ? __builtin_nanf("") : v[e];
 }
 
 // One workgroup per (sequence, layer) moves the weights of all heads as their rows move: slot j of head h receives the

@@ -899,7 +899,7 @@ def attend_blocks(kv: PagedKV, batch: StepBatch, q: torch.Tensor, bounds: torch.
 @dataclass
 class EvictConfig:
     """How ``select_by_weight`` / ``evict_step`` turn accumulated weights into keep sets."""
-    window_size: int = 128               # recent tokens that always stay
+    window_size: int = 128               # recent tokens that stay, ahead of every weight that is a finite number
     protect_prefill: bool = False        # those of the prompt (the batch's prefill_lens) as well
     layer_reduce: str | None = "mean"    # "max"; None: one keep set per layer
     shared: bool = False                 # one list for all KV heads (the largest of their weights)
