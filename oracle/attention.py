@@ -84,7 +84,8 @@ def choose_blocks(q: torch.Tensor, bounds: torch.Tensor, top: int, sinks: int, r
         x = q[k * g:(k + 1) * g].double()
         s = torch.maximum(x[:, None] * bounds[:, k, 0].double(), x[:, None] * bounds[:, k, 1].double()).sum(-1)
         s = (s.amax(0) if group_max else s.mean(0)).float()
-        s[torch.isnan(s)] = math.inf
+        most = torch.finfo(torch.float32).max
+        s = torch.where(torch.isnan(s), most, s).clamp(max=most)
         s[:sinks] = math.inf
         s[max(0, nb - recent):] = math.inf
         order = sorted(range(nb), key=lambda j: (-float(s[j]), j))

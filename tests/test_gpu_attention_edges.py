@@ -183,6 +183,23 @@ def test_a_call_of_no_rows(heads, most, mode):
     assert len(out) == 0 and none is None
 
 
+# -------------------------------------------------------------------------- chosen blocks
+def test_first_and_last_blocks_are_read_whatever_others_score():
+    """More blocks with a NaN or infinite key than are chosen: those asked for by place are among them all the same."""
+    case = Case([16 * 40], seed=1)
+    for j in range(2, 38):
+        case.cache[0][0][case.tables[0][j], 3, 0, 5] = math.nan
+        case.cache[0][0][case.tables[0][j], 3, 1] = math.inf * torch.sign(case.q[0, 4].float())
+    case.q[0, 4:] = case.q[0, 4]
+    kv, batch = case.device()
+    bounds = ops.update_block_bounds(kv, batch, ops.block_bounds(kv))
+    print("blocks by place", flush=True)
+    _, _, blocks = ops.attend_blocks(kv, batch, case.q.to(DEV), bounds, top_blocks=7, sink_blocks=1, recent_blocks=2)
+    want = oat.choose_blocks(case.q[0], oat.bounds_of(case.cache[0][0], case.tables[0], 640, BF16), 7, 1, 2, True)
+    assert want == [[0, 2, 3, 4, 5, 38, 39]] * 2
+    assert blocks[0].tolist() == want
+
+
 # ------------------------------------------------------------------------------- eviction
 @pytest.mark.parametrize("reduce,shared", [("mean", False), ("max", False), (None, False), ("mean", True), ("max", True)])
 def test_negative_nan_weights_are_kept_first_too(reduce, shared):

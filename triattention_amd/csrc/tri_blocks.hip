@@ -4,6 +4,7 @@
 //   score  = max (or mean) over the query heads of a KV head of  sum_d max(q[d] low[d], q[d] high[d])
 // which no q . k of the block exceeds.
 #include <algorithm>
+#include <cfloat>
 
 #include "tri_common.h"
 #include "tri_mma_device.h"
@@ -214,8 +215,10 @@ __global__ __launch_bounds__(256) void block_scores_kernel(BlockScoreLaunch a) {
     if (j >= count || sub != 0) continue;
     float s = a.group_max ? best[i] : (float)(total[i] / a.G);
     if (!ok[i]) s = -INFINITY;
-    // (a NaN in a query or a key must come out of the attention as it would without the selection: its block is read)
-    if (j < a.sinks || j >= count - a.recent || __builtin_isnan(s)) s = INFINITY;
+    // (a NaN in a query or a key should come out of the attention as it would without the selection: its block comes first, but for
+    // those asked for by their place)
+    if (__builtin_isnan(s) || s > FLT_MAX) s = FLT_MAX;
+    if (j < a.sinks || j >= count - a.recent) s = INFINITY;
     a.scores[row * a.max_count + j] = s;
   }
 }
