@@ -399,14 +399,16 @@ int tri_attend_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_
 
 /* Bounds of the keys of every block that holds one of the new_tokens last tokens of a sequence (0: of every block), all
  * layers: bounds[l*stride_layer + ((block*num_kv_heads + head)*2 + {0: least, 1: largest})*head_dim + d], in the cache's type
- * (fp8: bf16, of the scaled keys).  A NaN key makes its bounds NaN.  Blocks outside [0, num_blocks) are left out. */
+ * (fp8: bf16; with a scale per row the scaled keys rounded to nearest, so that a key may lie outside by half a step of
+ * bf16; keys lie within their bounds otherwise).  A NaN key makes its bounds NaN.  Blocks outside [0, num_blocks) are left out.
+ * Sequences that share a block have the same number of tokens in it (the bounds are those of either). */
 int tri_block_bounds(const tri_kv_layout* kv, const tri_batch* batch, int32_t num_blocks, int32_t new_tokens, void* bounds,
                      int64_t bounds_stride_layer, void* stream);
 
 /* tri_attend_paged for one new token per sequence, over the top_blocks blocks of each KV head that score highest: sum over d
- * of max(q*least, q*largest), the largest (or mean) over the query heads of the KV head.  The first sink_blocks and the last
- * recent_blocks blocks of a sequence are always among them; ties go to the lowest block, NaN and infinite scores count as
- * the largest finite one.  blocks receives int32 [num_seqs][num_kv_heads][top_blocks], logical blocks ascending, -1 behind the last.
+ * of max(q*least, q*largest), which no q . k of the block exceeds (but for that half step), the largest (or mean) over the
+ * query heads of the KV head.  The first sink_blocks and the last recent_blocks blocks of a sequence are always among
+ * them; ties go to the lowest block, NaN and infinite scores count as the largest finite one.  blocks receives int32 [num_seqs][num_kv_heads][top_blocks], logical blocks ascending, -1 behind the last.
  * row_starts, parents and weights of the attention parameters must be NULL. */
 typedef struct tri_block_params {
   const void* bounds;           /* the layer's part of tri_block_bounds' array */

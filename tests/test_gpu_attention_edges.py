@@ -200,6 +200,21 @@ def test_first_and_last_blocks_are_read_whatever_others_score():
     assert blocks[0].tolist() == want
 
 
+@pytest.mark.parametrize("types", [dict(), dict(dtype=FP16), dict(dtype=FP8), dict(dtype=FP8, row_scales=True)], ids=["bf16", "fp16", "fp8", "fp8_scaled"])
+@pytest.mark.parametrize("block", [1, 16])
+def test_keys_lie_within_their_block_s_bounds(types, block):
+    """Exactly, but for scaled fp8 keys: there the bounds are rounded to bf16, by at most half a step (2^-8 of the bound)."""
+    case = Case([333], block=block, seed=block, garbage=None, **types)
+    kv, batch = case.device()
+    print(f"bounds {types} {block}", flush=True)
+    bounds = ops.update_block_bounds(kv, batch, ops.block_bounds(kv)).cpu()
+    k, _ = oat.rows_of(case.cache[0][0], case.tables[0], 333, case.scales[0][0])
+    b = bounds[0, torch.tensor([case.tables[0][i // block] for i in range(333)])].double()
+    # (the scaled key itself is a product in fp32)
+    slack = (2.0 ** -8 + 2.0 ** -23) if types.get("row_scales") else 0.0
+    assert bool((k >= b[:, :, 0] - slack * b[:, :, 0].abs()).all()) and bool((k <= b[:, :, 1] + slack * b[:, :, 1].abs()).all())
+
+
 # ------------------------------------------------------------------------------- eviction
 @pytest.mark.parametrize("reduce,shared", [("mean", False), ("max", False), (None, False), ("mean", True), ("max", True)])
 def test_negative_nan_weights_are_kept_first_too(reduce, shared):

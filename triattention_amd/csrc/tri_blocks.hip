@@ -2,7 +2,9 @@
 //
 //   low[d] = min over the block's tokens of k[d],  high[d] = max
 //   score  = max (or mean) over the query heads of a KV head of  sum_d max(q[d] low[d], q[d] high[d])
-// which no q . k of the block exceeds.
+// which no q . k of the block exceeds, where the bounds are keys of the cache: bf16, fp16 and fp8 without scales of its rows.  Scaled fp8
+// keys are products in fp32, their bounds the nearest bf16 numbers: a key lies outside by half a step (2^-8 of the bound)
+// at most, and a q . k above the score by 2^-8 sum_d |q[d] bound[d]|, which is how far such scores tell blocks apart.
 #include <algorithm>
 #include <cfloat>
 

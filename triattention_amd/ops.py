@@ -860,7 +860,8 @@ def block_bounds(kv: PagedKV) -> torch.Tensor:
 
 def update_block_bounds(kv: PagedKV, batch: StepBatch, bounds: torch.Tensor, *, new_tokens: int | None = None) -> torch.Tensor:
     """Least and largest key per dimension of the blocks that hold the last ``new_tokens`` tokens of every sequence (None: of
-    all its blocks; after a prompt or a compaction), every layer, into ``bounds`` (``tri_block_bounds``)."""
+    all its blocks; after a prompt or a compaction), every layer, into ``bounds`` (``tri_block_bounds``).  Keys of an fp8
+    cache with a scale per row are rounded to the nearest bf16 there."""
     lib = _lib.load()
     _check_attention_batch(kv, batch)
     at = _bounds_address(kv, bounds)
@@ -876,7 +877,8 @@ def attend_blocks(kv: PagedKV, batch: StepBatch, q: torch.Tensor, bounds: torch.
                   sink_blocks: int = 1, recent_blocks: int = 1, group_reduce: str = "max", scale: float | None = None,
                   k_scale: float = 1.0, v_scale: float = 1.0, out: torch.Tensor | None = None, want_lse: bool = False):
     """A decoding step that reads, per KV head, the ``top_blocks`` blocks whose keys may score highest with its queries
-    (``tri_attend_blocks``): the upper bounds of q . k that ``update_block_bounds`` allows, the largest (``group_reduce``
+    (``tri_attend_blocks``): the upper bounds of q . k that ``update_block_bounds`` allows (fp8 caches with a scale per row: but
+    for the rounding of the bounds, 2^-8), the largest (``group_reduce``
     "mean": the mean) over the query heads of the KV head; the first ``sink_blocks`` and last ``recent_blocks`` blocks always.
 
     ``q`` [sequences, Hq, D].  Returns (out, lse or None, blocks int32 [sequences, Hkv, top_blocks]: logical
