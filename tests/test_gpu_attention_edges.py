@@ -183,6 +183,28 @@ def test_a_call_of_no_rows(heads, most, mode):
     assert len(out) == 0 and none is None
 
 
+# ------------------------------------------------------------- infinities and NaN in the cache
+@pytest.mark.parametrize("heads,lens", [((4, 1), [9000]), ((8, 2), [300]), ((40, 2), [9000])])
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_odd_values_are_seen_however_little_they_weigh(heads, lens, odd):
+    """A value that is no number, of a token whose weight is less than fp32 holds: not hidden, whichever workgroup or wave had it."""
+    case = Case(lens, q_heads=heads[0], kv_heads=heads[1], dim=64, seed=9)
+    t = lens[0]
+    g = heads[0] // heads[1]
+    case.q[:] = case.q[:, :1].abs() + 0.5                # (the same query for all heads)
+    for h in range(heads[1]):
+        case.cache[0][0][case.tables[0][0], 3, h] = case.q[0, h * g] * 40
+    at = t - 30
+    case.cache[1][0][case.tables[0][at // 16], at % 16, 0, 5] = odd
+    kv, batch = case.device()
+    print(f"odd value of no weight {heads} {odd}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), want_lse=True)
+    out = out.cpu().float()
+    assert bool((~torch.isfinite(out[0, :g, 5])).all())
+    out[0, :g, 5] = 0
+    assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
+
+
 # -------------------------------------------------------------------------- chosen blocks
 def test_first_and_last_blocks_are_read_whatever_others_score():
     """More blocks with a NaN or infinite key than are chosen: those asked for by place are among them all the same."""

@@ -17,8 +17,8 @@ struct Joined {
 };
 __device__ __forceinline__ void join_two(Joined& a, const Joined& b) {
   const float top = fmaxf(a.top, b.top), fa = rescale(a.top, top), fb = rescale(b.top, top);
-  // (a part of factor 0 has no tokens: its values are not looked at)
-  a.v = (fa == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : a.v * fa) + (fb == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : b.v * fb);
+  // (0 * NaN on purpose: a value that is no number shows, however the sequence is cut; a part without tokens holds zeros)
+  a.v = a.v * fa + b.v * fb;
   a.total = a.total * fa + b.total * fb;
   a.top = top;
 }
