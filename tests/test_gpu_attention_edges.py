@@ -205,6 +205,20 @@ def test_odd_values_are_seen_however_little_they_weigh(heads, lens, odd):
     assert bool(torch.isfinite(out).all()) and bool(torch.isfinite(lse).all())
 
 
+@pytest.mark.parametrize("query", [BF16, FP16])
+@pytest.mark.parametrize("heads,rows", [((4, 2), 1), ((40, 2), 1)])
+def test_infinite_value_scales(heads, rows, query):
+    """The only scale of a sequence, the first one and one among others."""
+    case = Case([1, 200, 200, 16], q_heads=heads[0], kv_heads=heads[1], dim=64, seed=8, dtype=FP8, query=query, row_scales=True)
+    for b, i in ((0, 0), (1, 0), (2, 77)):
+        case.scales[1][0][case.tables[b][i // 16], i % 16, 0] = math.inf
+    case.scales[1][0][torch.tensor(case.tables[3])] = 0.0
+    kv, batch = case.device()
+    print(f"infinite scales {heads} {query}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), want_lse=True)
+    _check_rows(case, out, lse, case.expected())
+
+
 # -------------------------------------------------------------------------- chosen blocks
 def test_first_and_last_blocks_are_read_whatever_others_score():
     """More blocks with a NaN or infinite key than are chosen: those asked for by place are among them all the same."""

@@ -456,8 +456,9 @@ __device__ __forceinline__ void lift_scales(f32x4 (&vs)[2], float& lift, f32x4 (
       for (int t = 0; t < NT; ++t) o[rt][t] *= by;
     lift = now;
   }
+  // (no lift yet: scales of 0, infinities and NaN alone, which go as they are)
 #pragma unroll
-  for (int i = 0; i < 2; ++i) vs[i] *= lift;
+  for (int i = 0; i < 2; ++i) vs[i] *= lift == 0.f ? 1.f : lift;
 }
 template <int RT, int NT>
 __device__ __forceinline__ void free_of_lift(f32x4 (&o)[RT][NT], float lift) {
