@@ -142,7 +142,7 @@ __device__ __forceinline__ void add_weights(const AttendLaunch& a, float* weight
     }
     auto meet = [] {
       if (TOGETHER) __syncthreads();
-      else __builtin_amdgcn_wave_barrier();
+      else order_lds_of_wave();
     };
     meet();
     if (lane < 16) s_lse[wave * 16 + lane] = l == -INFINITY ? INFINITY : l;             // (a row without tokens adds nothing)

@@ -672,12 +672,12 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
       }
     }
     if constexpr (more) load_values();
+    order_lds_of_wave();
     __builtin_amdgcn_sched_barrier(0);
     const bool masked = okm != 0xffffffffu || drafts;
     u32x4 pf[1];
     f32x4 ks[2] = {}, vs[2] = {};
     if (scaled) {
-      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         ks[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][0][i * 16 + q4 * 4]);
@@ -694,7 +694,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
       const u32x2 lo = lds_read_transposed(my_lds + t * 32), hi = lds_read_transposed(my_lds + t * 32 + 16 * kPitch);
       o[0][t] = mfma<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[0], o[0][t]);
     }
-    __builtin_amdgcn_wave_barrier();
+    order_lds_of_wave();             // (the next tile goes to the same places)
   };
   if (first_tile < end) {
     find.begin(first_tile);
@@ -1054,10 +1054,10 @@ __global__ __launch_bounds__(kAttendThreads, 2) void weigh_rows_kernel(AttendLau
   if (scaled) {
     const GlobalF32 ksc = (GlobalF32)a.k_scale_layers[a.layer] + h;
     s_token[wave][lane] = ksc[find.scale_at(lane)];
-    __builtin_amdgcn_wave_barrier();
+    order_lds_of_wave();
 #pragma unroll
     for (int i = 0; i < NG; ++i) ks[i] *= *reinterpret_cast<const f32x4*>(&s_token[wave][i * 16 + q4 * 4]);
-    __builtin_amdgcn_wave_barrier();
+    order_lds_of_wave();
   }
   const uint64_t anc = fresh > 1 ? ancestor_mask(a.parents, rows.first, n, lane) : 1ull;
   const bool drafts = fresh > 1 && t0 + TOK > base;
@@ -1122,7 +1122,7 @@ __global__ __launch_bounds__(kAttendThreads, 2) void weigh_rows_kernel(AttendLau
       for (int r = 0; r < 4; ++r) sum[i][r] += __shfl_xor(sum[i][r], step);
     if (c16 == 0) *reinterpret_cast<f32x4*>(&s_token[wave][i * 16 + q4 * 4]) = sum[i];
   }
-  __builtin_amdgcn_wave_barrier();
+  order_lds_of_wave();
   if (there) *w = before + s_token[wave][lane];
 }
 

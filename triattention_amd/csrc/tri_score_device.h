@@ -7,6 +7,11 @@
 namespace tri {
 namespace {
 
+// Between LDS stores of a wave and loads by which its lanes read each other's words, and between such loads and the stores
+// that reuse the words.  The hardware takes a wave's LDS operations in order, so this costs no instruction; the compiler
+// knows the addresses of one lane only and may otherwise move the one across the other.
+__device__ __forceinline__ void order_lds_of_wave() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+
 // cos and sin of a phase that is an fp32 value, evaluated in double and rounded to fp32 once:
 // the correctly rounded value of what torch.cos(t * omega) approximates in fp32
 // (core/scoring.py:322-324).  Four-term Cody-Waite reduction by pi/2 (33-bit pieces: n * piece
