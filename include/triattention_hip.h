@@ -365,7 +365,7 @@ int tri_compress_step_static(const tri_kv_layout* kv, const tri_batch* batch, co
  * sum of exponentials.  A row that sees nothing (seq_lens 0), or nothing but scores of -inf, gets zeros and -inf.  Rows from row_starts[num_seqs] on
  * are left as they were, and so are their lse.  Scores and sums are held in fp32, weights rounded to the queries' type for the
  * product with V (with fp16 and row scales after a common power of two).
- * A table entry outside [0, num_blocks) counts as a block without tokens.  Lengths above max_seq_len count as it.  Rows beyond
+ * A table entry outside [0, num_blocks) counts as a block without tokens; without a table sequence b is block b.  Lengths above max_seq_len count as it.  Rows beyond
  * max_rows of a sequence, and rows that row_starts names beyond num_rows, are left as they were; their tokens are new tokens
  * all the same, which the rows before them do not see and whose slots of weights are written.  kv: bf16 or fp16 with queries of that type, fp8 (a scale per row where v_scale_layers is set,
  * none otherwise) with queries of either. */

@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import ctypes as C
 
-from test_attention import _attend, _batch, _layout
+from test_attention import _attend, _batch, _blocks, _evict, _layout
 from triattention_amd import _lib
 
 
@@ -24,3 +24,15 @@ def test_scratch_for_a_copy_of_q_where_out_lies_in_its_memory():
         assert need(q=q, out=out, weights=16) == base + size
     assert need(q=(1 << 20) + size, out=1 << 20, weights=16) == base
     assert need(q=16, out=16) == need(q=1 << 20, out=(1 << 20) + size)
+
+
+def test_without_a_table_a_sequence_is_one_block():
+    lib = _lib.load()
+    kv, batch = C.byref(_layout()), C.byref(_batch(block_table=None, max_seq_len=17))
+    fits = C.byref(_batch(block_table=None, max_seq_len=16))
+    for code in (lib.tri_attend_paged(kv, batch, C.byref(_attend()), 256, 1 << 40, None),
+                 lib.tri_attend_blocks(kv, batch, C.byref(_attend()), C.byref(_blocks()), 256, 1 << 40, None),
+                 lib.tri_block_bounds(kv, batch, 40, 0, 16, 40 * 4 * 256, None),
+                 lib.tri_select_by_weight(kv, batch, C.byref(_evict()), None, 8, 256, 1 << 40, None)):
+        assert code == _lib.TRI_ERR_INVALID_ARGUMENT and b"block" in lib.tri_last_error()
+    assert lib.tri_attend_workspace_bytes(kv, fits, C.byref(_attend())) > 0

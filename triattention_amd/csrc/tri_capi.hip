@@ -82,8 +82,11 @@ int check_batch(const tri_batch* b, bool need_budget) {
   return TRI_OK;
 }
 
-// The calls that read a sequence's pages by themselves: the table has an entry for every block a sequence can have.
+// The calls that read a sequence's pages by themselves: the table has an entry for every block a sequence can have, and without one
+// a sequence is one block.
 int check_pages(const tri_kv_layout* kv, const tri_batch* b) {
+  if (!b->block_table && b->max_seq_len > kv->block_size)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "without a block table a sequence is one block: of %d tokens, not %d", kv->block_size, b->max_seq_len);
   if (b->block_table && (int64_t)b->block_table_pitch * kv->block_size < b->max_seq_len)
     return fail(TRI_ERR_INVALID_ARGUMENT, "block_table_pitch %d: %d blocks of %d tokens do not hold %d", b->block_table_pitch,
                 b->block_table_pitch, kv->block_size, b->max_seq_len);
