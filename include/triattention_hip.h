@@ -362,13 +362,17 @@ int tri_compress_step_static(const tri_kv_layout* kv, const tri_batch* batch, co
  * reference, which leaves attention to its engine).  The new tokens of a sequence are the last n of its seq_lens tokens,
  * their K and V rows are in the cache; each is a row of q.  A row sees every token before the new ones, itself and its
  * ancestors among the new ones.  out = softmax(scale * k_scale * q . k) v * v_scale, lse the natural logarithm of the
- * sum of exponentials.  A row that sees nothing (seq_lens 0), or nothing but scores of -inf, gets zeros and -inf.  Rows from row_starts[num_seqs] on
- * are left as they were, and so are their lse.  Scores and sums are held in fp32, weights rounded to the queries' type for the
- * product with V (with fp16 and row scales after a common power of two).
- * A table entry outside [0, num_blocks) counts as a block without tokens; without a table sequence b is block b.  Lengths above max_seq_len count as it.  Rows beyond
- * max_rows of a sequence, and rows that row_starts names beyond num_rows, are left as they were; their tokens are new tokens
- * all the same, which the rows before them do not see and whose slots of weights are written.  kv: bf16 or fp16 with queries of that type, fp8 (a scale per row where v_scale_layers is set,
- * none otherwise) with queries of either. */
+ * sum of exponentials.  A row that sees nothing (seq_lens 0), or nothing but scores of -inf, gets zeros and -inf.  Rows from
+ * row_starts[num_seqs] on are left as they were, and so are their lse.
+ * Scores and sums are held in fp32.  For the product with V a weight is two numbers of the queries' type (with fp16 and row
+ * scales after a common power of two), off by 2^-16 (bf16) or 2^-22 (fp16) of it; of more than 64 rows (new tokens times
+ * query heads) a KV head, of fp8 caches more than 16, it is one: 2^-8 or 2^-11.
+ * A table entry outside [0, num_blocks) counts as a block without tokens; without a table sequence b is block b.  Lengths
+ * above max_seq_len count as it.  Rows beyond max_rows of a sequence, and rows that row_starts names beyond num_rows, are
+ * left as they were; their tokens are new tokens all the same, which the rows before them do not see and whose slots of
+ * weights are written.
+ * kv: bf16 or fp16 with queries of that type, fp8 (a scale per row where v_scale_layers is set, none otherwise) with queries
+ * of either. */
 typedef struct tri_attend_params {
   int32_t layer;                /* of the layout */
   int32_t num_q_heads;          /* a multiple of num_kv_heads */

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from oracle import attention as oat
-from test_gpu_attention import BF16, DEV, FP8, FP16, Case, _check_rows, _check_weights, _weights
+from test_gpu_attention import BF16, DEV, EPS, FP8, FP16, Case, _check_rows, _check_weights, _weights
 from triattention_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -290,3 +290,25 @@ def test_eviction_of_long_rows_keeps_what_the_definition_keeps_in_every_head():
         assert torch.equal(keep[h].long(), want), h
         assert torch.equal(weights.cpu().view(2, -1, 4)[:, slots[:5000], h], flat[:, want, h])
     assert 7 * 16 + 3 in keep[2].tolist()
+
+
+# ------------------------------------------------------------- what weights are rounded to
+ROUNDING = [dict(), dict(dtype=FP16), dict(dtype=FP8), dict(dtype=FP8, row_scales=True), dict(dtype=FP8, query=FP16),
+            dict(dtype=FP8, query=FP16, row_scales=True)]
+
+
+@pytest.mark.parametrize("types", ROUNDING, ids=["bf16", "fp16", "fp8", "fp8_scaled", "fp8_fp16q", "fp8_fp16q_scaled"])
+@pytest.mark.parametrize("dim,heads,rows", [(64, (4, 2), 1), (128, (8, 2), 4), (256, (16, 1), 1), (64, (32, 16), 2), (128, (20, 1), 1), (64, (32, 2), 4),
+                                            (256, (8, 2), 9), (64, (32, 2), 7), (128, (40, 1), 3), (128, (32, 1), 8), (256, (32, 1), 5)])
+def test_weights_are_rounded_as_stated(types, dim, heads, rows):
+    """Two numbers of the queries' type: half a step of half a step.  One of them beyond 64 rows, and of fp8 beyond 16.  Tokens of like
+    weights and values of either sign, whose sums leave the rounding errors bare."""
+    case = Case([70, 1, 33, 150], q_heads=heads[0], kv_heads=heads[1], dim=dim, rows=[rows, 1, rows, rows], seed=dim + rows, q_scale=0.2, **types)
+    if heads == (32, 16):                     # (enough of them that a wave has a head to itself)
+        case = Case([9000 - 7 * i for i in range(4)], q_heads=32, kv_heads=16, dim=dim, rows=[rows] * 4, seed=dim + rows, q_scale=0.2, **types)
+    kv, batch = case.device()
+    print(f"rounding {types} dim={dim} heads={heads} rows={rows}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), row_starts=case.dev_starts, parents=case.dev_parents, max_rows=rows, want_lse=True)
+    step = EPS[case.query]
+    two = rows * heads[0] // heads[1] <= (16 if types.get("dtype") == FP8 else 64)
+    _check_rows(case, out, lse, case.expected(), weight_eps=step * step if two else step)

@@ -429,8 +429,14 @@ __device__ __forceinline__ uint32_t seen_of(uint32_t okm, bool drafts, int first
 }
 
 // The softmax of 32 tokens for RT rows a lane: sc holds q . k of tokens i * 16 + (lane >> 4) * 4 + r; pf receives the weights
-// 2^(x - top) packed for the product with V (vs scales them: fp8 rows with scales of their own).  They are rounded to 16 bits
-// there while the sum adds them unrounded: errors of half a step each and of either sign, below the one rounding of the output.
+// 2^(x - top) packed for the product with V (vs scales them: fp8 rows with scales of their own) in PIECES numbers of the
+// queries' type.  Two, the rounded weight and what that left of it, hold a bf16 weight to 2^-16 and an fp16 one to 2^-22; a single one
+// to 2^-8 and 2^-11, while the sum adds them unrounded: errors of either sign, which take outputs from 0.0017 to 0.0022 of their size
+// off the exact ones (fp16 0.0002 to 0.0003), most of it the rounding of the output in either case.  The second piece doubles
+// the products with V.  Up to 16 rows, where reading bounds, that costs nothing (16 x 2176: 45.0 us both; fp8 16 x 16384: 155), of 17
+// to 64 rows of 16-bit caches 1 to 2 % (8 x 8192 tokens, 64 rows: 66 -> 67).  With more rows, and of fp8 where
+// widening takes turns with the products, it would be felt: 2 x 32768 with 240 rows 101 -> 124 us, 8 x 4096 with 256 rows 55 -> 64, fp8
+// 8 x 8192 with 64 rows 53 -> 58: there weights are one number.
 // fp8 rows with scales of their own: the weight of a value carries its row's scale, which fp16 has no room for.  There all weights carry
 // a power of two as well, lift, that puts the largest scale so far between 1 and 2^6 (weights stay below 2^14) and that O is freed from
 // at the end.  fp16 loses up to 2^-25 of a weight there, against the 1 or more of the largest scale: no more than the output's own
@@ -469,8 +475,8 @@ __device__ __forceinline__ void free_of_lift(f32x4 (&o)[RT][NT], float lift) {
     for (int t = 0; t < NT; ++t) o[rt][t] *= 1.f / lift;
 }
 
-template <int PT, bool SCALED, bool SCORES, int RT, int NT>
-__device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT], f32x4 (&o)[RT][NT], u32x4 (&pf)[RT], float scale,
+template <int PT, bool SCALED, bool SCORES, int RT, int NT, int PIECES>
+__device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT], f32x4 (&o)[RT][NT], u32x4 (&pf)[PIECES][RT], float scale,
                                           const f32x4 (&ks)[2], const f32x4 (&vs)[2], bool masked, bool drafts, uint32_t okm, int first,
                                           const uint64_t (&seen)[RT], int lane, const ScoreRows& scores, int at) {
   float best[RT];
@@ -529,8 +535,21 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
       if (SCALED) sc[rt][i] *= vs[i];
     }
     st[rt].sum += part;
-    pf[rt] = u32x4{Half<PT>::pack(sc[rt][0][0], sc[rt][0][1]), Half<PT>::pack(sc[rt][0][2], sc[rt][0][3]),
-                   Half<PT>::pack(sc[rt][1][0], sc[rt][1][1]), Half<PT>::pack(sc[rt][1][2], sc[rt][1][3])};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float lo = sc[rt][i / 2][(i & 1) * 2], hi = sc[rt][i / 2][(i & 1) * 2 + 1];
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const uint32_t w = Half<PT>::pack(lo, hi);
+        pf[p][rt][i] = w;
+        lo -= Half<PT>::value((uint16_t)w);
+        hi -= Half<PT>::value((uint16_t)(w >> 16));
+        if (SCALED) {                  // (of an infinite scale nothing is left)
+          lo = fabsf(lo) < INFINITY ? lo : 0.f;
+          hi = fabsf(hi) < INFINITY ? hi : 0.f;
+        }
+      }
+    }
   }
 }
 
@@ -553,6 +572,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
   constexpr int kPitch = D * 2 + 32;                      // bytes of a value row in LDS: eight rows reach all banks
   constexpr int kWaveBytes = kAttendTile * kPitch;
   constexpr int kParts = HEADS ? 1 : kAttendWaves;        // waves that share a head's tokens
+  constexpr int kPieces = 2;                              // of a weight (see softmax32)
   constexpr int kStep = kParts * kAttendTile;
   __shared__ __align__(16) unsigned char s_v[kAttendWaves * kWaveBytes];
   __shared__ __align__(16) float s_scale[kAttendWaves][2][kAttendTile];
@@ -675,7 +695,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
     order_lds_of_wave();
     __builtin_amdgcn_sched_barrier(0);
     const bool masked = okm != 0xffffffffu || drafts;
-    u32x4 pf[1];
+    u32x4 pf[kPieces][1];
     f32x4 ks[2] = {}, vs[2] = {};
     if (scaled) {
 #pragma unroll
@@ -684,15 +704,16 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
         vs[i] = *reinterpret_cast<const f32x4*>(&s_scale[wave][1][i * 16 + q4 * 4]);
       }
       if constexpr (kLifts<QT, FP8>) lift_scales<1, NT>(vs, lift, o);
-      softmax32<PT, true, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
+      softmax32<PT, true, true, 1, NT, kPieces>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
     } else {
-      softmax32<PT, false, true, 1, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
+      softmax32<PT, false, true, 1, NT, kPieces>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, tile - base, seen, lane, scores, tile);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const u32x2 lo = lds_read_transposed(my_lds + t * 32), hi = lds_read_transposed(my_lds + t * 32 + 16 * kPitch);
-      o[0][t] = mfma<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[0], o[0][t]);
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) o[0][t] = mfma<PT>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[p][0], o[0][t]);
     }
     order_lds_of_wave();             // (the next tile goes to the same places)
   };
@@ -864,6 +885,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   u32x4 qf[RT][D / 32];
   uint64_t seen[RT];
   constexpr bool kScores = RT * W == 4;                   // (of more rows the weights come from the keys once more)
+  constexpr int kPieces = RT * W == 4 && !FP8 ? 2 : 1;    // (see softmax32)
   const ScoreRows scores = kScores ? score_rows(a, b, h, m0, M) : ScoreRows{};
   f32x4 o[RT][NT];
   float lift = 0.f;
@@ -890,7 +912,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
   }
   __syncthreads();
 
-  u32x4 kf[2][D / 32], pf[RT];
+  u32x4 kf[2][D / 32], pf[kPieces][RT];
   u32x2 vlo[NT], vhi[NT];
   f32x4 sc[RT][2];
   auto read_keys = [&](int sub, int buf) {
@@ -928,7 +950,9 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
     for (int t = 0; t < NT; ++t) {
       const u32x4 vf{vlo[t][0], vlo[t][1], vhi[t][0], vhi[t][1]};
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma<PT>(vf, pf[rt], o[rt][t]);
+      for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][t] = mfma<PT>(vf, pf[p][rt], o[rt][t]);
     }
   };
   auto softmax = [&](int first, int sub, int buf) {
@@ -947,7 +971,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
       for (int i = 0; i < 2; ++i) ks[i] = vs[i] = f32x4{1.f, 1.f, 1.f, 1.f};
     }
     if (kLifts<QT, FP8> && scaled) lift_scales<RT, NT>(vs, lift, o);
-    softmax32<PT, FP8, kScores, RT, NT>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
+    softmax32<PT, FP8, kScores, RT, NT, kPieces>(sc, st, o, pf, a.scale_log2, ks, vs, masked, drafts, okm, first - base, seen, lane, scores, first);
   };
   const bool busy = m0 < M;
   // A tile, while the next one goes from registers to LDS and the one behind it is asked for.
