@@ -312,3 +312,25 @@ def test_weights_are_rounded_as_stated(types, dim, heads, rows):
     step = EPS[case.query]
     two = rows * heads[0] // heads[1] <= (16 if types.get("dtype") == FP8 else 64)
     _check_rows(case, out, lse, case.expected(), weight_eps=step * step if two else step)
+
+
+# ----------------------------------------------------------- scratch of a long sequence among short ones
+@pytest.mark.parametrize("types", [dict(), dict(dtype=FP8, row_scales=True)], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("mode", ["add", "set"])
+def test_weights_of_a_long_sequence_among_many_short_ones(types, mode):
+    """Scores of all of them would take more than the cache: the weights come from the keys, of single rows too."""
+    lens = [20000] + [1 + 7 * i % 90 for i in range(899)]
+    heads = (64, 2)
+    case = Case(lens, q_heads=heads[0], kv_heads=heads[1], dim=64, seed=4, garbage=None, **types)
+    kv, batch = case.device()
+    before = _weights(case)
+    weights = before.to(DEV)
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    print(f"long among short {types} {mode}", flush=True)
+    out, lse = ops.attend_paged(kv, batch, case.q.to(DEV), weights=weights, weight_mode=mode, want_lse=True)
+    assert torch.cuda.max_memory_allocated() - held < 1 << 30
+    want = case.expected()
+    _check_rows(case, out, lse, want)
+    _check_weights(case, weights, before, want, mode)

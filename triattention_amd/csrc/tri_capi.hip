@@ -1042,14 +1042,20 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   // Weights of few rows come from their scores, which the attention leaves (8 bytes a row and token, written and read), of many
   // from the keys once more: 2 x 32768 tokens of 8 x 128 bf16, 20 rows a KV head 94 us from scores and 104 from keys, 32 rows
   // 105 and 104, 128 rows 231 and 141, of fp8 32 rows 75 and 78, 64 rows 107 and 91; rows of 256 dimensions, 64 of them, 115 and 120.
-  d.weigh_again = p->weights && rows > (a.D == 256 ? 64 : 32);
+  // Scores of all sequences lie as far apart as the longest one's, so a long one among many short ones would take scratch without
+  // end: beyond 2 GiB and all of the batch's K and V in this layer, which sequences of one length never need, the keys are read again
+  // too.  One of 60000 tokens among 299 of 300, 64 query heads over 8 of 128: 4.6 GB of scores for 0.6 GB of K and V, 255 us; from
+  // the keys 467.
+  const int64_t score_bytes = (int64_t)a.B * a.Hkv * rows * a.score_pitch * 4;
+  const int64_t cache_bytes = total * a.Hkv * a.D * 2 * elem_bytes(a.kv_dtype);
+  d.weigh_again = p->weights && (rows > (a.D == 256 ? 64 : 32) || score_bytes > std::max<int64_t>(2ll << 30, cache_bytes));
   // (they read the queries again when out is written: out in q's memory is read from a copy)
   const Span of_q = span_of(p->q, a.num_rows, a.q_stride_row, a.Hq, a.q_stride_head, a.D);
   const Span of_out = span_of(p->out, a.num_rows, a.out_stride_row, a.Hq, a.out_stride_head, a.D);
   d.copies_q = d.weigh_again && a.num_rows > 0 && of_q.from < of_out.to && of_out.from < of_q.to;
   d.q_copy = take(d.copies_q ? (int64_t)a.num_rows * a.Hq * a.D * 2 : 0);
   d.lse2 = take(p->weights ? (int64_t)a.num_rows * a.Hq * 4 : 0);
-  d.scores = take(p->weights && !d.weigh_again ? (int64_t)a.B * a.Hkv * rows * a.score_pitch * 4 : 0);
+  d.scores = take(p->weights && !d.weigh_again ? score_bytes : 0);
   d.block_scores = take(bp ? (int64_t)a.B * a.Hkv * d.max_count * 4 : 0);
   d.counts = take(bp ? (int64_t)a.B * 8 : 0);
   d.total = std::max<int64_t>(off, 256);

@@ -833,7 +833,8 @@ def attend_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, *, layer: int =
     ``weights`` (fp32 [layers, blocks, block_size, Hkv], beside the cache) receives the softmax weight of every cached token, summed over
     rows and the query heads of its KV head: added ("add"; the slots of the new tokens themselves are written) or written
     ("set").  ``select_by_weight`` and ``evict_step`` go by them.  Sequences of such a call may not share blocks; of
-    few rows its scratch holds the scores, four bytes per row, query head and token.
+    few rows its scratch holds the scores, four bytes per row, query head and token of the longest sequence, unless that is
+    more than 2 GiB and than the sequences' K and V in the layer.
 
     ``scale`` (default head_dim ** -0.5) times ``k_scale`` must be positive.  ``out`` may be ``q`` itself; otherwise they have no element
     in common.
