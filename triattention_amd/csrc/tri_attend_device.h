@@ -32,7 +32,6 @@ namespace {
 
 constexpr int kAttendThreads = 256;
 constexpr int kAttendWaves = kAttendThreads / kWave;
-constexpr int kDies = 8;
 constexpr int kWaitLoads = 0x0f70;    // s_waitcnt vmcnt(0), the other counters left alone
 constexpr int kAttendTile = 32;       // tokens of one product with V
 
@@ -163,28 +162,16 @@ __device__ __forceinline__ RowRange rows_of(const AttendLaunch& a, int b, int T)
   return {first, min(end - first, a.max_rows), (int)min(max(to - from, (int64_t)0), (int64_t)T + 64)};
 }
 
-// What a workgroup works on: a split of a sequence (the unit), one KV head and block of rows of it (inner).  Workgroups go to the
-// eight dies in turn; with by_xcd all inner ones of a unit go to one of them, where they find the unit's pages in its
-// translation cache and, the blocks of rows, its K and V in L2.
+// What a workgroup works on: a split of a sequence (the unit), one KV head and block of rows of it (inner).  (All blocks of rows of a
+// unit on one die, where its L2 has the unit's K and V, gave nothing: 2 x 32768 tokens, 512 rows a KV head 168 us either way, 16 x
+// 8192 with 320 rows 267.)
 struct Work {
   int b, split, h, rb;
 };
-__device__ __forceinline__ bool work_of(const AttendLaunch& a, Work& w) {
+__device__ __forceinline__ Work work_of(const AttendLaunch& a) {
   const int heads = a.Hkv / a.heads_per_group, inner_n = heads * a.row_blocks;
-  int unit, inner;
-  if (a.by_xcd) {
-    const int l = blockIdx.x / kDies;
-    inner = l % inner_n;
-    unit = l / inner_n * kDies + blockIdx.x % kDies;
-  } else {
-    inner = blockIdx.x % inner_n;
-    unit = blockIdx.x / inner_n;
-  }
-  w.h = inner % heads * a.heads_per_group;
-  w.rb = inner / heads;
-  w.split = unit % a.nsplit;
-  w.b = unit / a.nsplit;
-  return w.b < a.B;
+  const int inner = blockIdx.x % inner_n, unit = blockIdx.x / inner_n;
+  return {unit / a.nsplit, unit % a.nsplit, inner % heads * a.heads_per_group, inner / heads};
 }
 
 // Tokens the call reads of a sequence, in the order it reads them: its cache, or the blocks of its list one after the other.
@@ -580,8 +567,7 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c16 = lane & 15, q4 = lane >> 4;
-  Work work;
-  if (!work_of(a, work)) return;
+  const Work work = work_of(a);
   const int b = work.b, split = work.split, h = work.h + (HEADS ? wave : 0), part = HEADS ? 0 : wave;
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
@@ -798,8 +784,7 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int c16 = lane & 15, q4 = lane >> 4;
-  Work work;
-  if (!work_of(a, work)) return;
+  const Work work = work_of(a);
   const int b = work.b, split = work.split, h = work.h, rb = work.rb;
 
   const int T = min(max(a.seq_lens[b], 0), a.Tmax);
@@ -1158,7 +1143,7 @@ hipError_t launch_attend_typed(const AttendLaunch& a, hipStream_t s) {
     return hipGetLastError();
   }
   const int64_t units = (int64_t)a.B * a.nsplit;
-  const dim3 grid((unsigned)((a.by_xcd ? align_up(units, kDies) : units) * a.row_blocks * (a.Hkv / a.heads_per_group)));
+  const dim3 grid((unsigned)(units * a.row_blocks * (a.Hkv / a.heads_per_group)));
   if (a.heads_per_group > 1) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI, true>), grid, dim3(kAttendThreads), 0, s, a);
   else if (a.row_tiles == 0) hipLaunchKernelGGL((attend_few_kernel<QT, FP8, D, UNI, false>), grid, dim3(kAttendThreads), 0, s, a);
   else if (a.row_tiles == 4) hipLaunchKernelGGL((attend_rows_kernel<QT, FP8, D, 1, 4, UNI>), grid, dim3(4 * kWave), 0, s, a);

@@ -1029,11 +1029,10 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   const int64_t part_bytes = (int64_t)a.B * a.Hkv * rows * (a.D + 2) * 4, parts_most = std::max<int64_t>((512ll << 20) / part_bytes, 1);
   if (tri::ceil_div64(longest, a.split_tokens) > parts_most) a.split_tokens = (int)tri::align_up(tri::ceil_div64(longest, parts_most), 128);
   a.nsplit = (int)tri::ceil_div64(longest, a.split_tokens);
-  a.by_xcd = a.row_blocks > 1 && (int64_t)a.B * a.nsplit >= 32;
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = tri::align_up(off + bytes, 256); return o; };
   const int64_t parts = a.nsplit > 1 ? (int64_t)a.B * a.Hkv * a.nsplit * rows : 0;
-  if (((int64_t)a.B * a.nsplit + 7) * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) * a.Hkv > INT_MAX ||
+  if ((int64_t)a.B * a.nsplit * a.row_blocks * a.Hkv > INT_MAX || (int64_t)a.B * tri::ceil_div(a.Tmax, 64) * a.Hkv > INT_MAX ||
       (int64_t)a.B * a.Hkv * rows > INT_MAX)
     return fail(TRI_ERR_UNSUPPORTED, "%d sequences of %d rows and %d KV heads in one call", a.B, a.max_rows, a.Hkv);
   a.score_pitch = tri::align_up(a.Tmax, 32);

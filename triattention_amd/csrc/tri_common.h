@@ -278,7 +278,7 @@ struct AttendLaunch {
   const int32_t* list;
   int list_k, list_pitch;
   // how the work is cut
-  int row_tiles, row_blocks, nsplit, split_tokens, by_xcd;         // row_tiles: tiles of 16 rows a workgroup has; 0: the kernel for up to 16 rows
+  int row_tiles, row_blocks, nsplit, split_tokens;         // row_tiles: tiles of 16 rows a workgroup has; 0: the kernel for up to 16 rows
   int heads_per_group;                                     // KV heads of a workgroup
   // workspace
   float* part_out;                                         // [B][Hkv][nsplit][max_rows * G][D], not normalised (nsplit > 1)
