@@ -334,3 +334,29 @@ def test_weights_of_a_long_sequence_among_many_short_ones(types, mode):
     want = case.expected()
     _check_rows(case, out, lse, want)
     _check_weights(case, weights, before, want, mode)
+
+
+# -------------------------------------------------------------- sizes beyond 32 bits
+def test_sizes_beyond_32_bits_are_not_cut():
+    """A window of more tokens than there can be guards all; counts that no call can have are refused."""
+    case = Case([100, 40], seed=1, garbage=None)
+    kv, batch = case.device(budgets=[30, 20])
+    weights = _weights(case).to(DEV)
+    bounds = ops.block_bounds(kv)
+    q = case.q.to(DEV)
+    print("beyond 32 bits", flush=True)
+    for window in (100, (1 << 31) - 1, 1 << 31, (1 << 32) + 5, 1 << 40):
+        keep, _ = ops.select_by_weight(kv, batch, weights, ops.EvictConfig(window_size=window))
+        assert keep[0].tolist() == list(range(30)) and keep[2].tolist() == list(range(20)) + [-1] * 10
+    every = ops.update_block_bounds(kv, batch, bounds.clone())
+    for new in (100, 1 << 31, (1 << 32) + 1):
+        assert torch.equal(ops.update_block_bounds(kv, batch, bounds.clone(), new_tokens=new), every)
+    for args in (dict(top_blocks=(1 << 32) + 4), dict(top_blocks=4, sink_blocks=1 << 32), dict(top_blocks=4, recent_blocks=(1 << 32) + 1),
+                 dict(top_blocks=4, sink_blocks=-1, recent_blocks=3)):
+        with pytest.raises(ValueError):
+            ops.attend_blocks(kv, batch, q, bounds, **args)
+    for most in ((1 << 32) + 1, 0, -1, 65):
+        with pytest.raises(ValueError):
+            ops.attend_paged(kv, batch, q, row_starts=case.dev_starts, max_rows=most)
+    with pytest.raises(ValueError):
+        ops.select_by_weight(kv, batch, weights, ops.EvictConfig(window_size=-1))

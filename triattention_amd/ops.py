@@ -791,6 +791,8 @@ def _attend_params(kv: PagedKV, batch: StepBatch, q, layer, row_starts, parents,
     rows, heads, _ = shape
     if max_rows is None:
         max_rows = 1 if row_starts is None else min(max(rows, 1), 64)
+    elif not 1 <= max_rows <= 64:
+        raise ValueError(f"max_rows must be 1 to 64, got {max_rows}")
     if row_starts is not None:
         _on(kv, "row_starts", row_starts, torch.int32)
         if row_starts.shape != (batch.num_seqs + 1,) or not row_starts.is_contiguous():
@@ -868,8 +870,9 @@ def update_block_bounds(kv: PagedKV, batch: StepBatch, bounds: torch.Tensor, *, 
     at = _bounds_address(kv, bounds)
     if new_tokens is not None and new_tokens < 1:
         raise ValueError(f"new_tokens must be positive or None, got {new_tokens}")
+    recent = 0 if new_tokens is None else min(new_tokens, batch.max_seq_len)          # (more than that are all of them)
     with _on_device(kv.device):
-        _lib.check(lib.tri_block_bounds(C.byref(kv.struct), C.byref(batch.struct), kv.num_blocks, new_tokens or 0, at,
+        _lib.check(lib.tri_block_bounds(C.byref(kv.struct), C.byref(batch.struct), kv.num_blocks, recent, at,
                                         bounds.stride(0), _stream()))
     return bounds
 
@@ -887,8 +890,10 @@ def attend_blocks(kv: PagedKV, batch: StepBatch, q: torch.Tensor, bounds: torch.
     lib = _lib.load()
     if group_reduce not in ("max", "mean"):
         raise ValueError(f"group_reduce must be 'max' or 'mean', got {group_reduce!r}")
+    if not (0 < top_blocks < 1 << 31 and min(sink_blocks, recent_blocks) >= 0 and sink_blocks + recent_blocks <= top_blocks):
+        raise ValueError(f"{sink_blocks} sink and {recent_blocks} recent blocks of {top_blocks}")
     p, out, lse = _attend_params(kv, batch, q, layer, None, None, 1, scale, k_scale, v_scale, out, want_lse)
-    blocks = torch.empty((batch.num_seqs, kv.num_kv_heads, max(top_blocks, 0)), dtype=torch.int32, device=kv.device)
+    blocks = torch.empty((batch.num_seqs, kv.num_kv_heads, top_blocks), dtype=torch.int32, device=kv.device)
     bp = BlockParams(_bounds_address(kv, bounds, layer), top_blocks, sink_blocks, recent_blocks,
                      REDUCE_MAX if group_reduce == "max" else REDUCE_MEAN, blocks.data_ptr())
     with _on_device(kv.device):
@@ -924,7 +929,9 @@ def _evict_params(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: Evic
           or keep.device != kv.device):
         raise ValueError(f"keep must be a contiguous int32 tensor with {rows} x {batch.max_budget} entries")
     lr = REDUCE_NONE if ev.layer_reduce is None else (REDUCE_MAX if ev.layer_reduce == "max" else REDUCE_MEAN)
-    return EvictParams(num_blocks=kv.num_blocks, window_size=int(ev.window_size), protect_prefill=int(ev.protect_prefill),
+    if ev.window_size < 0:
+        raise ValueError(f"window_size must not be negative, got {ev.window_size}")
+    return EvictParams(num_blocks=kv.num_blocks, window_size=min(int(ev.window_size), batch.max_seq_len), protect_prefill=int(ev.protect_prefill),
                        layer_reduce=lr, shared=int(ev.shared), weights=at, weights_stride_layer=weights.stride(0)), keep, rows
 
 
