@@ -176,8 +176,10 @@ template <int QT, int D>
 hipError_t launch_finish_typed(const AttendLaunch& a, float* weights, int set, hipStream_t s) {
   constexpr int kRows = kThreads / (D / 4);
   const int64_t rows = a.nsplit > 1 ? (int64_t)a.B * a.Hkv * a.max_rows * a.G : 0;
-  // Many splits of few rows: a workgroup a row, its lanes side by side over the splits (56 rows of 32 splits 7.2 -> 5.5 us;
-  // not 3840 rows of 16, 8.1 -> 15.4).
+  // Many splits of few rows: a workgroup a row, its lanes side by side over the splits.  1 and 2 x 32768 tokens of 128 dimensions,
+  // without and with it: 128 rows 13.7 and 5.2 us, 640 8.1 and 5.7, 1024 8.4 and 6.9, 2048 6.8 and 8.5 (64 dimensions: 1024 7.9 and
+  // 5.8, 2048 8.4 and 9.2; 256: 10.5 and 9.5, 9.1 and 10.1).  Up to eight splits are asked for at once either way (4.2 and 4.2 us;
+  // 640 rows 4.2 and 5.2).
   const bool wide = a.nsplit > kWideSplits && rows <= kWideRows;
   const int64_t joins = wide ? rows : ceil_div64(rows, kRows);
   const bool together = weights && (int64_t)std::min(a.Hkv, 4) * a.max_rows * a.G > 16;

@@ -1,5 +1,6 @@
 // Attention of a few query rows per sequence over the paged cache (gfx950): one decoding step, a tree of drafted
-// tokens, or the blocks of a list.  Instantiated per head dimension in tri_attend_{64,128,256}.hip.
+// tokens, or the blocks of a list.  Instantiated per head dimension and type of the queries in
+// tri_attend_{64,128,256}_{bf16,fp16}.hip.
 //
 //   s[m][t] = scale * q[m] . k[t]   where row m sees token t, else -inf
 //   out[m]  = sum_t 2^(s log2 e - M) v[t] / sum_t 2^(s log2 e - M),   M the running maximum
@@ -544,7 +545,7 @@ __device__ __forceinline__ void softmax32(f32x4 (&sc)[RT][2], RowState (&st)[RT]
 // Bound by reading K and V.  Keys go from memory into the operand's registers (a lane's 16 bytes are a piece of it), values
 // through LDS, which transposes them; the next tile's are asked for as soon as this one's registers are free, so that two
 // workgroups a CU (four of 64 dimensions) have 128 KiB on their way (fp8: 64).
-// 16 x 2176 tokens of 8 x 128 bf16 with four query heads each 35 us (4.0 TB/s), 16 x 16384 of fp8 with HEADS 130 us (K, V and
+// 16 x 2176 tokens of 8 x 128 bf16 with four query heads each 36 us (4.0 TB/s), 16 x 16384 of fp8 with HEADS 131 us (K, V and
 // the scores written for the weights: 4.4 TB/s), without weights 114 (4.7), where a copy reaches 5.1; 160 tokens 7 us.
 // HEADS: a wave has a KV head to itself, four neighbours in a workgroup, and nothing is joined here.
 template <int QT, bool FP8, int D, bool UNI, bool HEADS>
@@ -763,8 +764,8 @@ __global__ __launch_bounds__(kAttendThreads, D == 256 ? 1 : D == 128 ? 2 : 4) vo
 // each, and two waves a SIMD overlap little of it (phases a barrier apart, so that one wave's softmax would meet the other's
 // products, were slower: 137 us and more against 112).  Two row tiles to a wave halve what it reads of LDS a row, and eight
 // waves what is read of memory (with the slack in rescaling, 257 -> 111 us for the call below when they came).  The next tile
-// waits in registers while this one is worked on.  2 x 32768 tokens with 60 rows of 4 query heads, 8 x 128 fp16: 93 us, 690
-// TFLOP/s of the 1200 a large product reaches; 8 x 4096 with up to 32 rows of 8: 50 us; 1217 tokens with 16 rows: 12 us.
+// waits in registers while this one is worked on.  2 x 32768 tokens with 60 rows of 4 query heads, 8 x 128 fp16: 88 to 92 us, 700
+// to 730 TFLOP/s of the 1200 a large product reaches; 8 x 4096 with up to 32 rows of 8: 48 us; 1217 tokens with 16 rows: 12 us.
 template <int QT, bool FP8, int D, int RT, int W, bool UNI>
 __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch a) {
   constexpr int PT = QT;
@@ -1012,7 +1013,8 @@ __global__ __launch_bounds__(W * kWave, 2) void attend_rows_kernel(AttendLaunch 
 // and token, written and read, and the keys are read once however many rows there are.  A wave has 64 tokens of a KV head, their keys in
 // the operand's registers, and goes through all rows; a lane sums its rows' weights of its tokens, and the sixteen
 // lanes of a token's rows meet once at the end: no order of anything to depend on.  Bound by reading the keys, of many rows by the
-// exponentials: 2 x 32768 tokens of 8 x 128 bf16, 64 rows of four query heads, 187 us with the attention (120 of it) against 387 from scores.
+// exponentials: 2 x 32768 tokens of 8 x 128 bf16, 64 rows of four query heads, 98 to 104 us of the 185 that the call takes with the
+// attention, 32 rows 64 of 136; 8 x 4096 with 32 rows of eight 49 of 105, 16 x 2176 of scaled fp8 with 32 of four 37 of 88.
 constexpr int kWeighTokens = kWave;
 template <int QT, bool FP8, int D, bool UNI>
 __global__ __launch_bounds__(kAttendThreads, 2) void weigh_rows_kernel(AttendLaunch a) {

@@ -992,6 +992,11 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   int64_t total = 0;
   for (int b = 0; b < a.B; ++b) total += std::min<int64_t>(batch->seq_lens_host ? batch->seq_lens_host[b] : a.Tmax, longest);
   const int rows = a.max_rows * a.G;
+  // Tiles of 16 rows a workgroup has room for: 8 x 4096 tokens of 8 x 128 bf16, a call with four, eight and sixteen of them: 80 rows
+  // 53, 41, 42 us; 128 rows 57, 46, 45; 160 rows 89, 70, 52; 256 rows 94, 74, 61; of 64 dimensions 128 rows 38, 30, 33, 256 rows
+  // 59, 47, 41.  Of up to 64 rows four leave the scores that weights come from and hold weights as two numbers (softmax32); calls that
+  // want neither would gain from eight, of which waves without rows still load (64 rows 42, 37, 41).  (256 dimensions have no sixteen:
+  // registers.)
   a.row_tiles = rows <= 16 ? 0 : rows <= 64 ? 4 : rows <= 128 || a.D == 256 ? 8 : 16;
   a.row_blocks = a.row_tiles ? tri::ceil_div(rows, 16 * a.row_tiles) : 1;
   // A split is as long as lets every workgroup run at once (each sequence's last one is short); with more sequences than that
@@ -1039,8 +1044,10 @@ int plan_attend(const tri_kv_layout* kv, const tri_batch* batch, const tri_atten
   d.part_out = take(parts * a.D * 4);
   d.part_ml = take(parts * 8);
   // Weights of few rows come from their scores, which the attention leaves (8 bytes a row and token, written and read), of many
-  // from the keys once more: 2 x 32768 tokens of 8 x 128 bf16, 20 rows a KV head 94 us from scores and 104 from keys, 32 rows
-  // 105 and 104, 128 rows 231 and 141, of fp8 32 rows 75 and 78, 64 rows 107 and 91; rows of 256 dimensions, 64 of them, 115 and 120.
+  // from the keys once more.  Calls on 2 x 32768 tokens of eight KV heads, from scores and from keys, us: 128 dimensions bf16, 16 rows
+  // a KV head 84 and 100, 24 rows 97 and 103, 32 rows 105 and 104, 64 rows 152 and 115; fp8 16 rows 59 and 69, 32 rows 76 and 78,
+  // 64 rows 111 and 91; 64 dimensions 16 rows 59 and 65, 24 rows 71 and 71, 32 rows 78 and 72 (fp8 with scales 76 and 76), 64 rows 103 and
+  // 79; 256 dimensions 32 rows 161 and 171, 48 rows 181 and 182, 64 rows 208 and 193.
   // Scores of all sequences lie as far apart as the longest one's, so a long one among many short ones would take scratch without
   // end: beyond 2 GiB and all of the batch's K and V in this layer, which sequences of one length never need, the keys are read again
   // too.  One of 60000 tokens among 299 of 300, 64 query heads over 8 of 128: 4.6 GB of scores for 0.6 GB of K and V, 255 us; from
