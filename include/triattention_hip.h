@@ -412,7 +412,7 @@ int tri_block_bounds(const tri_kv_layout* kv, const tri_batch* batch, int32_t nu
 /* tri_attend_paged for one new token per sequence, over the top_blocks blocks of each KV head that score highest: sum over d
  * of max(q*least, q*largest), which no q . k of the block exceeds (but for that half step), the largest (or mean) over the
  * query heads of the KV head.  The first sink_blocks and the last recent_blocks blocks of a sequence are always among
- * them; ties go to the lowest block, NaN and infinite scores count as the largest finite one.  blocks receives int32 [num_seqs][num_kv_heads][top_blocks], logical blocks ascending, -1 behind the last.
+ * them; ties go to the lowest block, scores of NaN and +inf count as the largest finite one.  blocks receives int32 [num_seqs][num_kv_heads][top_blocks], logical blocks ascending, -1 behind the last.
  * row_starts, parents and weights of the attention parameters must be NULL. */
 typedef struct tri_block_params {
   const void* bounds;           /* the layer's part of tri_block_bounds' array */
