@@ -445,6 +445,110 @@ int tri_select_by_weight(const tri_kv_layout* kv, const tri_batch* batch, const 
 int tri_evict_step(const tri_kv_layout* kv, const tri_batch* batch, const tri_evict_params* p, int32_t* keep, void* workspace,
                    uint64_t workspace_bytes, void* stream);
 
+/* The step around tri_attend_paged on the same cache: its new tokens' rows written before it, drafted tokens verified and
+ * accepted after it, cached rows read back (no counterpart in the reference, which leaves all of these to its engine).
+ * Rows, row_starts and sequences are those of tri_attend_paged without its limit of 64 rows, but for tri_verify_drafts and
+ * tri_accept_drafts: the rows of a sequence are the last n of its seq_lens tokens.  Rows that no sequence has (behind
+ * row_starts[num_seqs], or row_starts naming rows beyond num_rows) are left as they were. */
+typedef enum tri_real { TRI_REAL_BF16 = 0, TRI_REAL_FP16 = 1, TRI_REAL_FP32 = 2 } tri_real;
+
+/* Queries and keys of new tokens, normalised per head (y = x / sqrt(mean(x^2) + eps) * norm, where there is a norm) and
+ * rotated: the pairs (f, f + head_dim/2) (TRI_ROPE_HALF) or (2f, 2f + 1) (TRI_ROPE_INTERLEAVED) by the angle positions[axis of
+ * f][row] * inv_freq[f], times rotary_scale.  The queries go to out, keys and the values as they are into the slots of their tokens in one
+ * layer of the cache.  fp8 caches: with v_scale_layers a row's scale is max(largest finite |element| / 448, 2^-126) and is
+ * written with it; without, codes stand for code * k_scale (v_scale), numbers beyond 448 of those are the largest code; infinities and NaN become NaN
+ * either way.  Angles are 64-bit, norms and rotations 32-bit, and every output is rounded once, to nearest.
+ * A row whose sequence has fewer tokens than rows, or whose block lies outside [0, num_blocks), is not cached, its query is written all the same.
+ * Two rows of a call may not have the same slot. */
+typedef struct tri_write_params {
+  int32_t layer;                /* of the layout */
+  int32_t num_q_heads;          /* a multiple of num_kv_heads */
+  int32_t num_rows;
+  int32_t num_blocks;           /* physical blocks of the cache */
+  int32_t dtype;                /* of q, k, v and out: TRI_KV_BF16 or TRI_KV_FP16; the cache's, where it is not fp8 */
+  int32_t num_axes;             /* of positions, 1 or more */
+  int32_t positions_64;         /* 1: positions are int64, 0: int32 */
+  int32_t norm_fp32;            /* 1: q_norm and k_norm are fp32, 0: of dtype */
+  const void* q;                /* element (row, head, d) at q + row*q_stride_row + head*q_stride_head + d; 16-byte aligned rows */
+  const void* k;
+  const void* v;
+  int64_t q_stride_row, q_stride_head, k_stride_row, k_stride_head, v_stride_row, v_stride_head;
+  void* out;                    /* may be q itself (same strides); any other element of it may not be one of q's, k's or v's */
+  int64_t out_stride_row, out_stride_head;
+  const void* positions;        /* element (axis, row) at axis*position_stride + row */
+  int64_t position_stride;
+  const int32_t* freq_axes;     /* [head_dim/2]: the axis of each frequency (any number that is none counts as 0), or NULL: axis 0 */
+  const float* inv_freq;        /* [head_dim/2] */
+  const void* q_norm;           /* [head_dim], or NULL */
+  const void* k_norm;
+  const int32_t* row_starts;    /* [num_seqs + 1] ascending, or NULL: one row per sequence */
+  float eps, rotary_scale, k_scale, v_scale;
+} tri_write_params;
+int tri_write_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_write_params* p, void* stream);
+
+/* The rows of one layer as dense K and V: k_out and v_out [num_rows][num_kv_heads][head_dim], 16-byte aligned, of type
+ * out_dtype (tri_real): the cached number times its row's scale (where v_scale_layers is set) times k_scale (v_scale), rounded once.  Rows of
+ * tokens that the cache does not have (more rows than tokens, a block outside [0, num_blocks)) are zeros. */
+typedef struct tri_read_params {
+  int32_t layer, num_rows, num_blocks, out_dtype;
+  const int32_t* row_starts;    /* [num_seqs + 1] ascending */
+  void* k_out;
+  void* v_out;
+  float k_scale, v_scale;
+} tri_read_params;
+int tri_read_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_read_params* p, void* stream);
+
+/* Which drafted tokens the target accepts, from given random numbers.  Row 0 of a sequence is the last token decided; the other rows hold drafted
+ * tokens, each behind its parent (as in tri_attend_paged; a row whose parent is no row is never reached); target has
+ * what follows each row: logits, with p = softmax(logits / temperature), or probabilities, with p = those over their sum.
+ *  Without draft probabilities a token is drawn from p of every row, and from row 0 on the walk goes to the child (the first) that holds the drawn token,
+ * as long as there is one: next is the token drawn last.  With them (a chain): row i + 1 is accepted iff u * draft(token) < p(token) of row i, u its
+ * uniforms[.][0]; behind the last accepted row next is drawn from p, or where a row was rejected from max(p - draft, 0) over its sum (p,
+ * where that is 0).  A draw takes the least token whose running sum exceeds uniforms[row][1] of the whole.  A temperature that is not above 0:
+ * the largest logit, the first among equals, in place of every draw, and a draft is accepted iff it is that.  So next and the accepted
+ * tokens have the distribution of the target, whatever drafted them.
+ *  Weights and sums are 64-bit.  NaN logits count as -inf, probabilities that are no positive finite number as 0; a row without any
+ * weight draws -1.  Tokens outside [0, vocab) are never accepted.  Rows beyond max_rows of a sequence are not looked at.
+ * rows: int32 [num_seqs][max_rows], the accepted rows ascending, row 0 first, -1 behind them; counts: how many; next: the token
+ * behind them.  A sequence without rows: 0 and -1. */
+typedef struct tri_verify_params {
+  int32_t num_seqs, num_rows;
+  int32_t max_rows;             /* 1 to 64 */
+  int32_t vocab;
+  int32_t target_dtype;         /* tri_real; probabilities are TRI_REAL_FP32 */
+  int32_t target_probs;         /* 1: probabilities, 0: logits */
+  const void* target;           /* element (row, token) at target + row*target_stride + token, aligned to the element */
+  int64_t target_stride;
+  const int32_t* tokens;        /* [num_rows] */
+  const int32_t* row_starts;    /* [num_seqs + 1] ascending */
+  const int32_t* parents;       /* [num_rows], or NULL: each row follows the one before it */
+  const float* uniforms;        /* [num_rows][2], in [0, 1) */
+  const float* temperatures;    /* [num_seqs], or NULL: 1; NULL with probabilities */
+  const float* draft_probs;     /* the distribution that each row's token was drawn from (of row 0: not read), or NULL; NULL with parents */
+  int64_t draft_stride;
+  int32_t* rows;
+  int32_t* counts;
+  int32_t* next;
+} tri_verify_params;
+uint64_t tri_verify_workspace_bytes(const tri_verify_params* p);
+int tri_verify_drafts(const tri_verify_params* p, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* The accepted rows of every sequence one behind the other in the cache, every layer: of the n rows of a sequence, its last tokens, row rows[j] to
+ * the place of row j, j < counts: K, V, an fp8 row's scales and, where weights is set, the accumulated weights.  Lists ascend (one that does not, or
+ * names a row that the sequence has not, ends there).  new_lens (may be NULL; not the batch's seq_lens, which the call reads) receives
+ * seq_lens - n + counts.  Moves of a row from or to a block outside [0, num_blocks) are left out.  Sequences may not share the blocks of their new tokens. */
+typedef struct tri_accept_params {
+  int32_t num_blocks;
+  int32_t max_rows;             /* 1 to 64: entries of a list */
+  const int32_t* row_starts;    /* [num_seqs + 1] ascending */
+  const int32_t* rows;          /* [num_seqs][max_rows] */
+  const int32_t* counts;        /* [num_seqs] */
+  float* weights;               /* [num_layers][num_blocks][block_size][num_kv_heads], or NULL */
+  int64_t weights_stride_layer; /* floats */
+  int32_t* new_lens;            /* [num_seqs], or NULL */
+} tri_accept_params;
+int tri_accept_drafts(const tri_kv_layout* kv, const tri_batch* batch, const tri_accept_params* p, void* stream);
+
 /* Calibration: per-query-head frequency statistics of one layer's captured query states;
  * replaces the RoPE inversion and the per-head means of scripts/calibrate.py:196-224
  * (helpers :38-98; same arithmetic as triattention/methods/pruning_utils.py:40-98).

@@ -23,6 +23,7 @@ TRI_ERR_LAUNCH = -4
 
 KV_BF16, KV_FP16, KV_FP8_E4M3 = 0, 1, 2
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+REAL_BF16, REAL_FP16, REAL_FP32 = 0, 1, 2
 REDUCE_MEAN, REDUCE_MAX, REDUCE_NONE = 0, 1, -1
 
 # tri_tuning keys
@@ -39,6 +40,7 @@ EXPORTS = (
     "tri_compact_paged_full", "tri_compress_step", "tri_compress_step_static", "tri_qstats_workspace_bytes", "tri_qstats",
     "tri_attend_workspace_bytes", "tri_attend_paged", "tri_block_bounds", "tri_attend_blocks_workspace_bytes", "tri_attend_blocks",
     "tri_evict_workspace_bytes", "tri_select_by_weight", "tri_evict_step",
+    "tri_write_paged", "tri_read_paged", "tri_verify_workspace_bytes", "tri_verify_drafts", "tri_accept_drafts",
 )
 
 
@@ -115,6 +117,35 @@ class EvictParams(C.Structure):
                 ("shared", C.c_int32), ("weights", C.c_void_p), ("weights_stride_layer", C.c_int64)]
 
 
+class WriteParams(C.Structure):
+    _fields_ = (
+        [(n, C.c_int32) for n in ("layer", "num_q_heads", "num_rows", "num_blocks", "dtype", "num_axes", "positions_64", "norm_fp32")]
+        + [(n, C.c_void_p) for n in ("q", "k", "v")]
+        + [(n, C.c_int64) for n in ("q_stride_row", "q_stride_head", "k_stride_row", "k_stride_head", "v_stride_row", "v_stride_head")]
+        + [("out", C.c_void_p), ("out_stride_row", C.c_int64), ("out_stride_head", C.c_int64), ("positions", C.c_void_p),
+           ("position_stride", C.c_int64)]
+        + [(n, C.c_void_p) for n in ("freq_axes", "inv_freq", "q_norm", "k_norm", "row_starts")]
+        + [(n, C.c_float) for n in ("eps", "rotary_scale", "k_scale", "v_scale")])
+
+
+class ReadParams(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("layer", "num_rows", "num_blocks", "out_dtype")]
+                + [(n, C.c_void_p) for n in ("row_starts", "k_out", "v_out")] + [("k_scale", C.c_float), ("v_scale", C.c_float)])
+
+
+class VerifyParams(C.Structure):
+    _fields_ = (
+        [(n, C.c_int32) for n in ("num_seqs", "num_rows", "max_rows", "vocab", "target_dtype", "target_probs")]
+        + [("target", C.c_void_p), ("target_stride", C.c_int64)]
+        + [(n, C.c_void_p) for n in ("tokens", "row_starts", "parents", "uniforms", "temperatures", "draft_probs")]
+        + [("draft_stride", C.c_int64)] + [(n, C.c_void_p) for n in ("rows", "counts", "next")])
+
+
+class AcceptParams(C.Structure):
+    _fields_ = [("num_blocks", C.c_int32), ("max_rows", C.c_int32), ("row_starts", C.c_void_p), ("rows", C.c_void_p), ("counts", C.c_void_p),
+                ("weights", C.c_void_p), ("weights_stride_layer", C.c_int64), ("new_lens", C.c_void_p)]
+
+
 class TriError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(f"libtriattention_hip error {code}: {message}")
@@ -189,6 +220,12 @@ def load() -> C.CDLL:
     lib.tri_evict_workspace_bytes.restype = U64
     lib.tri_select_by_weight.argtypes = [KV, BT, EP, P, P, P, U64, P]
     lib.tri_evict_step.argtypes = [KV, BT, EP, P, P, U64, P]
+    lib.tri_write_paged.argtypes = [KV, BT, C.POINTER(WriteParams), P]
+    lib.tri_read_paged.argtypes = [KV, BT, C.POINTER(ReadParams), P]
+    lib.tri_verify_workspace_bytes.argtypes = [C.POINTER(VerifyParams)]
+    lib.tri_verify_workspace_bytes.restype = U64
+    lib.tri_verify_drafts.argtypes = [C.POINTER(VerifyParams), P, U64, P]
+    lib.tri_accept_drafts.argtypes = [KV, BT, C.POINTER(AcceptParams), P]
     for name in EXPORTS:
         fn = getattr(lib, name)
         if fn.restype is C.c_int and name not in ("tri_abi_version",):

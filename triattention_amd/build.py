@@ -19,7 +19,8 @@ LIB_NAME = "libtriattention_hip.so"
 LIB_PATH = PKG / LIB_NAME
 SOURCES = ["tri_capi.hip", "tri_score.hip", "tri_score_small.hip", "tri_fused.hip", "tri_fused_mfma.hip", "tri_select.hip", "tri_compact.hip", "tri_dense.hip",
            "tri_calib.hip", "tri_attend.hip", "tri_attend_64_bf16.hip", "tri_attend_64_fp16.hip",
-           "tri_attend_128_bf16.hip", "tri_attend_128_fp16.hip", "tri_attend_256_bf16.hip", "tri_attend_256_fp16.hip", "tri_blocks.hip", "tri_evict.hip"]
+           "tri_attend_128_bf16.hip", "tri_attend_128_fp16.hip", "tri_attend_256_bf16.hip", "tri_attend_256_fp16.hip", "tri_blocks.hip", "tri_evict.hip",
+           "tri_write.hip", "tri_verify.hip"]
 
 # Packed fp32 instructions are switched off on purpose: hipcc forms them from
 # ordinary float code and some forms have given wrong results on this hardware.

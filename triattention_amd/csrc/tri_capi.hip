@@ -1258,6 +1258,197 @@ int tri_evict_step(const tri_kv_layout* kv, const tri_batch* batch, const tri_ev
   return launch_status(tri::launch_move_weights(a, s), "move_weights");
 }
 
+namespace {
+
+// What the calls around attention have in common: the layout, the batch, its pages and the pool.
+int check_rows_call(const tri_kv_layout* kv, const tri_batch* batch, int32_t layer, int32_t num_blocks) {
+  int rc = check_layout(kv, true);
+  if (!rc) rc = check_batch(batch, false);
+  if (!rc) rc = check_pages(kv, batch);
+  if (rc) return rc;
+  if (layer < 0 || layer >= kv->num_layers) return fail(TRI_ERR_INVALID_ARGUMENT, "layer %d of %d", layer, kv->num_layers);
+  if (num_blocks <= 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_blocks %d", num_blocks);
+  if (kv->stride_token < 0 || kv->stride_token >= (1 << 25))
+    return fail(TRI_ERR_UNSUPPORTED, "stride_token %lld", (long long)kv->stride_token);
+  return TRI_OK;
+}
+
+// A tensor of rows of heads: aligned, and where it is written its rows and heads apart.
+int check_heads(const char* name, const void* p, int64_t stride_row, int64_t stride_head, int rows, int heads, int D, bool written) {
+  if (rows > 0 && !p) return fail(TRI_ERR_INVALID_ARGUMENT, "%s is NULL", name);
+  if (!is_aligned(p, 16) || stride_row % 8 || stride_head % 8)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "%s must be 16-byte aligned, its strides multiples of 8 elements", name);
+  if (written && ((heads > 1 && stride_head < D) || (rows > 1 && stride_row < D)))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "strides of %s are less than head_dim", name);
+  return TRI_OK;
+}
+
+struct VerifyPlan {
+  tri::VerifyLaunch a{};
+  int64_t part, state, rest, total;
+};
+
+int plan_verify(const tri_verify_params* p, VerifyPlan& d) {
+  if (!p) return fail(TRI_ERR_INVALID_ARGUMENT, "verify params are NULL");
+  if (p->num_seqs <= 0 || p->num_rows < 0) return fail(TRI_ERR_INVALID_ARGUMENT, "%d sequences, %d rows", p->num_seqs, p->num_rows);
+  if (p->max_rows < 1 || p->max_rows > kMaxNewTokens)
+    return fail(TRI_ERR_UNSUPPORTED, "max_rows %d not in [1, %d]", p->max_rows, kMaxNewTokens);
+  if (p->vocab <= 0) return fail(TRI_ERR_INVALID_ARGUMENT, "vocab %d", p->vocab);
+  // (places are counted to the end of a row's last piece in 32 bits)
+  if (p->vocab > INT_MAX - tri::kVerifyPiece) return fail(TRI_ERR_UNSUPPORTED, "vocab %d", p->vocab);
+  if (p->target_dtype < TRI_REAL_BF16 || p->target_dtype > TRI_REAL_FP32)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "target_dtype %d", p->target_dtype);
+  if (p->target_probs && p->target_dtype != TRI_REAL_FP32) return fail(TRI_ERR_UNSUPPORTED, "target_dtype %d (fp32 probabilities)", p->target_dtype);
+  if (p->target_probs && p->temperatures) return fail(TRI_ERR_INVALID_ARGUMENT, "temperatures are for logits: probabilities have theirs in them");
+  if (p->draft_probs && p->parents) return fail(TRI_ERR_UNSUPPORTED, "draft_probs are for chains: parents must be NULL");
+  if (p->num_rows > 1 && (p->target_stride < p->vocab || (p->draft_probs && p->draft_stride < p->vocab)))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "a row's stride is less than vocab %d", p->vocab);
+  tri::VerifyLaunch& a = d.a;
+  a.pieces = (int)tri::ceil_div64(p->vocab, tri::kVerifyPiece);
+  const int64_t most = std::max<int64_t>(p->num_rows, p->num_seqs);
+  if (most * a.pieces > INT_MAX || (int64_t)p->num_seqs * p->max_rows > INT_MAX)
+    return fail(TRI_ERR_UNSUPPORTED, "%d rows of %d logits in one call", p->num_rows, p->vocab);
+  a.B = p->num_seqs; a.num_rows = p->num_rows; a.max_rows = p->max_rows; a.vocab = p->vocab;
+  a.target_dtype = p->target_dtype; a.probs = p->target_probs ? 1 : 0;
+  a.target = p->target; a.target_stride = p->target_stride; a.tokens = p->tokens; a.row_starts = p->row_starts; a.parents = p->parents;
+  a.uniforms = p->uniforms; a.temperatures = p->temperatures; a.draft = p->draft_probs; a.draft_stride = p->draft_stride;
+  a.rows_out = p->rows; a.counts = p->counts; a.next = p->next;
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) { const int64_t o = off; off = tri::align_up(off + bytes, 256); return o; };
+  d.part = take((int64_t)p->num_rows * a.pieces * sizeof(tri::VerifyPart));
+  d.state = take(p->draft_probs ? (int64_t)p->num_seqs * sizeof(tri::VerifyState) : 0);
+  d.rest = take(p->draft_probs ? (int64_t)p->num_seqs * a.pieces * 8 : 0);
+  d.total = std::max<int64_t>(off, 256);
+  return TRI_OK;
+}
+
+}  // namespace
+
+int tri_write_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_write_params* p, void* stream) {
+  if (!p) return fail(TRI_ERR_INVALID_ARGUMENT, "write params are NULL");
+  int rc = check_rows_call(kv, batch, p->layer, p->num_blocks);
+  if (rc) return rc;
+  if (p->num_q_heads <= 0 || p->num_q_heads % kv->num_kv_heads)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "num_q_heads %d is not a multiple of num_kv_heads %d", p->num_q_heads, kv->num_kv_heads);
+  if (p->dtype != TRI_KV_BF16 && p->dtype != TRI_KV_FP16) return fail(TRI_ERR_UNSUPPORTED, "dtype %d (bf16 or fp16 rows)", p->dtype);
+  if (kv->kv_dtype != TRI_KV_FP8_E4M3 && p->dtype != kv->kv_dtype)
+    return fail(TRI_ERR_UNSUPPORTED, "rows of type %d into a cache of type %d", p->dtype, kv->kv_dtype);
+  if (p->num_rows < 0 || p->num_rows > INT_MAX / p->num_q_heads) return fail(TRI_ERR_INVALID_ARGUMENT, "num_rows %d", p->num_rows);
+  if (!p->row_starts && p->num_rows != batch->num_seqs)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "without row_starts there is one row per sequence (%d rows, %d sequences)", p->num_rows, batch->num_seqs);
+  const int D = kv->head_dim, n = p->num_rows;
+  rc = check_heads("q", p->q, p->q_stride_row, p->q_stride_head, n, p->num_q_heads, D, false);
+  if (!rc) rc = check_heads("k", p->k, p->k_stride_row, p->k_stride_head, n, kv->num_kv_heads, D, false);
+  if (!rc) rc = check_heads("v", p->v, p->v_stride_row, p->v_stride_head, n, kv->num_kv_heads, D, false);
+  if (!rc) rc = check_heads("out", p->out, p->out_stride_row, p->out_stride_head, n, p->num_q_heads, D, true);
+  if (rc) return rc;
+  if (!p->inv_freq || (n > 0 && !p->positions)) return fail(TRI_ERR_INVALID_ARGUMENT, "inv_freq / positions is NULL");
+  if (p->num_axes < 1 || (p->num_axes > 1 && p->position_stride < n))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "%d axes of positions, %lld apart", p->num_axes, (long long)p->position_stride);
+  if (!(p->eps >= 0.f) || !is_finite(p->eps) || !is_finite(p->rotary_scale))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, rotary_scale finite");
+  const bool row_scales = kv->kv_dtype == TRI_KV_FP8_E4M3 && kv->v_scale_layers;
+  const bool scaled = kv->kv_dtype == TRI_KV_FP8_E4M3 && !row_scales;
+  for (const float x : {p->k_scale, p->v_scale}) {
+    if (!scaled && x != 1.f) return fail(TRI_ERR_INVALID_ARGUMENT, "k_scale and v_scale are for fp8 caches without a scale per row");
+    if (!(x > 0.f) || !is_finite(x) || !is_finite(1.f / x)) return fail(TRI_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be positive, and so their reciprocals");
+  }
+  if (n == 0) return TRI_OK;
+  tri::WriteLaunch a{};
+  a.B = batch->num_seqs; a.Hq = p->num_q_heads; a.Hkv = kv->num_kv_heads; a.D = D; a.block_size = kv->block_size;
+  a.kv_dtype = kv->kv_dtype; a.q_dtype = p->dtype; a.rope_style = kv->rope_style; a.layer = p->layer; a.Tmax = batch->max_seq_len;
+  a.num_blocks = p->num_blocks; a.num_rows = n; a.num_axes = p->num_axes; a.positions_64 = p->positions_64; a.norm_fp32 = p->norm_fp32;
+  a.stride_block = kv->stride_block; a.stride_token = kv->stride_token; a.stride_head = kv->stride_head;
+  a.k_layers = const_cast<void* const*>(kv->k_layers); a.v_layers = const_cast<void* const*>(kv->v_layers);
+  if (row_scales) {
+    a.k_scale_layers = const_cast<float* const*>(kv->k_scale_layers);
+    a.v_scale_layers = const_cast<float* const*>(kv->v_scale_layers);
+  }
+  a.block_table = batch->block_table; a.block_table_pitch = batch->block_table_pitch; a.seq_lens = batch->seq_lens;
+  a.row_starts = p->row_starts; a.q = p->q; a.k = p->k; a.v = p->v; a.out = p->out;
+  a.q_stride_row = p->q_stride_row; a.q_stride_head = p->q_stride_head; a.k_stride_row = p->k_stride_row; a.k_stride_head = p->k_stride_head;
+  a.v_stride_row = p->v_stride_row; a.v_stride_head = p->v_stride_head; a.out_stride_row = p->out_stride_row; a.out_stride_head = p->out_stride_head;
+  a.positions = p->positions; a.position_stride = p->position_stride; a.freq_axes = p->freq_axes; a.inv_freq = p->inv_freq;
+  a.q_norm = p->q_norm; a.k_norm = p->k_norm; a.eps = p->eps; a.rotary_scale = p->rotary_scale;
+  a.k_inv_scale = 1.f / p->k_scale; a.v_inv_scale = 1.f / p->v_scale;
+  return launch_status(tri::launch_write_paged(a, (hipStream_t)stream), "write_paged");
+}
+
+int tri_read_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_read_params* p, void* stream) {
+  if (!p) return fail(TRI_ERR_INVALID_ARGUMENT, "read params are NULL");
+  const int rc = check_rows_call(kv, batch, p->layer, p->num_blocks);
+  if (rc) return rc;
+  if (!p->row_starts) return fail(TRI_ERR_INVALID_ARGUMENT, "row_starts is NULL");
+  if (p->out_dtype < TRI_REAL_BF16 || p->out_dtype > TRI_REAL_FP32) return fail(TRI_ERR_INVALID_ARGUMENT, "out_dtype %d", p->out_dtype);
+  if (p->num_rows < 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_rows %d", p->num_rows);
+  if (!is_finite(p->k_scale) || !is_finite(p->v_scale)) return fail(TRI_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be finite");
+  if (p->num_rows > 0 && (!p->k_out || !p->v_out)) return fail(TRI_ERR_INVALID_ARGUMENT, "k_out / v_out is NULL");
+  if (!is_aligned(p->k_out, 16) || !is_aligned(p->v_out, 16)) return fail(TRI_ERR_INVALID_ARGUMENT, "k_out and v_out must be 16-byte aligned");
+  if (p->num_rows == 0) return TRI_OK;
+  tri::ReadLaunch a{};
+  a.B = batch->num_seqs; a.Hkv = kv->num_kv_heads; a.D = kv->head_dim; a.block_size = kv->block_size; a.kv_dtype = kv->kv_dtype;
+  a.out_dtype = p->out_dtype; a.layer = p->layer; a.Tmax = batch->max_seq_len; a.num_blocks = p->num_blocks; a.num_rows = p->num_rows;
+  a.stride_block = kv->stride_block; a.stride_token = kv->stride_token; a.stride_head = kv->stride_head;
+  a.k_layers = kv->k_layers; a.v_layers = kv->v_layers;
+  if (kv->kv_dtype == TRI_KV_FP8_E4M3 && kv->v_scale_layers) {
+    a.k_scale_layers = kv->k_scale_layers;
+    a.v_scale_layers = kv->v_scale_layers;
+  }
+  a.block_table = batch->block_table; a.block_table_pitch = batch->block_table_pitch; a.seq_lens = batch->seq_lens;
+  a.row_starts = p->row_starts; a.k_out = p->k_out; a.v_out = p->v_out; a.k_scale = p->k_scale; a.v_scale = p->v_scale;
+  return launch_status(tri::launch_read_paged(a, (hipStream_t)stream), "read_paged");
+}
+
+uint64_t tri_verify_workspace_bytes(const tri_verify_params* p) {
+  VerifyPlan d;
+  return plan_verify(p, d) ? 0 : (uint64_t)d.total;
+}
+
+int tri_verify_drafts(const tri_verify_params* p, void* ws, uint64_t ws_bytes, void* stream) {
+  VerifyPlan d;
+  int rc = plan_verify(p, d);
+  if (rc) return rc;
+  if (!p->row_starts || !p->rows || !p->counts || !p->next) return fail(TRI_ERR_INVALID_ARGUMENT, "row_starts / rows / counts / next is NULL");
+  if (p->num_rows > 0 && (!p->target || !p->tokens || !p->uniforms)) return fail(TRI_ERR_INVALID_ARGUMENT, "target / tokens / uniforms is NULL");
+  if (!is_aligned(p->target, p->target_dtype == TRI_REAL_FP32 ? 4 : 2) || !is_aligned(p->draft_probs, 4))
+    return fail(TRI_ERR_INVALID_ARGUMENT, "target and draft_probs must be aligned to their elements");
+  tri::Workspace need{};
+  need.total = d.total;
+  rc = check_workspace(need, ws, ws_bytes);
+  if (rc) return rc;
+  d.a.part = at<tri::VerifyPart>(ws, d.part);
+  d.a.state = at<tri::VerifyState>(ws, d.state);
+  d.a.rest = at<double>(ws, d.rest);
+  return launch_status(tri::launch_verify_drafts(d.a, (hipStream_t)stream), "verify_drafts");
+}
+
+int tri_accept_drafts(const tri_kv_layout* kv, const tri_batch* batch, const tri_accept_params* p, void* stream) {
+  if (!p) return fail(TRI_ERR_INVALID_ARGUMENT, "accept params are NULL");
+  const int rc = check_rows_call(kv, batch, 0, p->num_blocks);
+  if (rc) return rc;
+  if (p->max_rows < 1 || p->max_rows > kMaxNewTokens)
+    return fail(TRI_ERR_UNSUPPORTED, "max_rows %d not in [1, %d]", p->max_rows, kMaxNewTokens);
+  if (!p->row_starts || !p->rows || !p->counts) return fail(TRI_ERR_INVALID_ARGUMENT, "row_starts / rows / counts is NULL");
+  if (p->new_lens == batch->seq_lens) return fail(TRI_ERR_INVALID_ARGUMENT, "new_lens is the batch's seq_lens, which the call reads");
+  if (p->weights && kv->num_layers > 1 && p->weights_stride_layer < (int64_t)p->num_blocks * kv->block_size * kv->num_kv_heads)
+    return fail(TRI_ERR_INVALID_ARGUMENT, "weights_stride_layer %lld is less than a layer", (long long)p->weights_stride_layer);
+  if ((int64_t)batch->num_seqs * kv->num_layers > INT_MAX / 2)
+    return fail(TRI_ERR_UNSUPPORTED, "%d sequences and %d layers in one call", batch->num_seqs, kv->num_layers);
+  tri::AcceptLaunch a{};
+  a.B = batch->num_seqs; a.L = kv->num_layers; a.Hkv = kv->num_kv_heads; a.D = kv->head_dim; a.elem_bytes = elem_bytes(kv->kv_dtype);
+  a.block_size = kv->block_size; a.Tmax = batch->max_seq_len; a.num_blocks = p->num_blocks; a.max_rows = p->max_rows;
+  a.stride_block = kv->stride_block; a.stride_token = kv->stride_token; a.stride_head = kv->stride_head;
+  a.k_layers = const_cast<void* const*>(kv->k_layers); a.v_layers = const_cast<void* const*>(kv->v_layers);
+  if (kv->kv_dtype == TRI_KV_FP8_E4M3 && kv->v_scale_layers) {
+    a.k_scale_layers = const_cast<float* const*>(kv->k_scale_layers);
+    a.v_scale_layers = const_cast<float* const*>(kv->v_scale_layers);
+  }
+  a.block_table = batch->block_table; a.block_table_pitch = batch->block_table_pitch; a.seq_lens = batch->seq_lens;
+  a.row_starts = p->row_starts; a.rows = p->rows; a.counts = p->counts; a.weights = p->weights;
+  a.weights_stride_layer = p->weights_stride_layer; a.lens_out = p->new_lens;
+  return launch_status(tri::launch_accept_rows(a, (hipStream_t)stream), "accept_rows");
+}
+
 uint64_t tri_qstats_workspace_bytes(int32_t num_heads, int32_t num_tokens, int32_t head_dim) {
   if (num_heads <= 0 || num_tokens <= 0 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) return 0;
   return (uint64_t)tri::qstats_workspace_bytes(num_heads, num_tokens, head_dim);

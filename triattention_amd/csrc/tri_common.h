@@ -348,6 +348,100 @@ struct EvictLaunch {
 hipError_t launch_weight_rows(const EvictLaunch& a, hipStream_t s);
 hipError_t launch_move_weights(const EvictLaunch& a, hipStream_t s);
 
+// New tokens' rows into one layer of the paged cache, and cached rows out of it (tri_write.hip).
+struct WriteLaunch {
+  int B, Hq, Hkv, D, block_size, kv_dtype, q_dtype, rope_style, layer, Tmax, num_blocks, num_rows;
+  int num_axes, positions_64, norm_fp32;
+  int waves_per_row;                                       // set by the launcher
+  int64_t stride_block, stride_token, stride_head;         // elements
+  void* const* k_layers;
+  void* const* v_layers;
+  float* const* k_scale_layers;                            // both NULL: rows without scales of their own
+  float* const* v_scale_layers;
+  const int32_t* block_table;                              // NULL: dense, physical block = sequence
+  int block_table_pitch;
+  const int32_t* seq_lens;
+  const int32_t* row_starts;                               // [B + 1], or NULL: row b
+  const void* q; const void* k; const void* v;
+  int64_t q_stride_row, q_stride_head, k_stride_row, k_stride_head, v_stride_row, v_stride_head;   // elements
+  void* out;
+  int64_t out_stride_row, out_stride_head;
+  const void* positions;                                   // [num_axes][position_stride]
+  int64_t position_stride;
+  const int32_t* freq_axes;                                // [D / 2], or NULL: axis 0
+  const float* inv_freq;
+  const void* q_norm; const void* k_norm;                  // [D], or NULL
+  float eps, rotary_scale, k_inv_scale, v_inv_scale;
+};
+hipError_t launch_write_paged(WriteLaunch a, hipStream_t s);
+struct ReadLaunch {
+  int B, Hkv, D, block_size, kv_dtype, out_dtype, layer, Tmax, num_blocks, num_rows;
+  int rows_per_wave;                                       // set by the launcher
+  int64_t stride_block, stride_token, stride_head;
+  const void* const* k_layers;
+  const void* const* v_layers;
+  const float* const* k_scale_layers;
+  const float* const* v_scale_layers;
+  const int32_t* block_table;
+  int block_table_pitch;
+  const int32_t* seq_lens;
+  const int32_t* row_starts;
+  void* k_out; void* v_out;                                // [num_rows][Hkv][D]
+  float k_scale, v_scale;
+};
+hipError_t launch_read_paged(ReadLaunch a, hipStream_t s);
+
+// Drafted tokens against the target's logits (tri_verify.hip).
+constexpr int kVerifyPiece = 2048;        // logits of a row that a wave sums
+struct VerifyPart {                       // of a piece: sum of the weights against the largest number, that one, where it is first
+  double sum;
+  float most;
+  int32_t where;
+};
+struct VerifyState {                      // of a sequence: its last accepted row's sum, largest number and place; rows accepted; 1: a row was rejected
+  double sum;
+  float most;
+  int32_t where, count, rest;
+};
+struct VerifyLaunch {
+  int B, num_rows, max_rows, vocab, target_dtype, probs, pieces;
+  const void* target;
+  int64_t target_stride;                                   // elements
+  const int32_t* tokens;
+  const int32_t* row_starts;
+  const int32_t* parents;                                  // NULL: a chain
+  const float* uniforms;                                   // [num_rows][2]
+  const float* temperatures;                               // [B], or NULL: 1
+  const float* draft;                                      // draft probabilities, or NULL
+  int64_t draft_stride;
+  int32_t* rows_out;                                       // [B][max_rows]
+  int32_t* counts;
+  int32_t* next;
+  // workspace
+  VerifyPart* part;                                        // [num_rows][pieces]
+  VerifyState* state;                                      // [B]
+  double* rest;                                            // [B][pieces]
+};
+hipError_t launch_verify_drafts(const VerifyLaunch& a, hipStream_t s);
+struct AcceptLaunch {
+  int B, L, Hkv, D, elem_bytes, block_size, Tmax, num_blocks, max_rows;
+  int64_t stride_block, stride_token, stride_head;         // elements
+  void* const* k_layers;
+  void* const* v_layers;
+  float* const* k_scale_layers;                            // both NULL: rows without scales of their own
+  float* const* v_scale_layers;
+  const int32_t* block_table;
+  int block_table_pitch;
+  const int32_t* seq_lens;
+  const int32_t* row_starts;
+  const int32_t* rows;                                     // [B][max_rows]
+  const int32_t* counts;
+  float* weights;                                          // [L][num_blocks][block_size][Hkv], or NULL
+  int64_t weights_stride_layer;
+  int32_t* lens_out;                                       // [B], or NULL
+};
+hipError_t launch_accept_rows(const AcceptLaunch& a, hipStream_t s);
+
 // Calibration statistics of one layer's captured queries (tri_calib.hip).
 struct QStatsLaunch {
   const void* q_rot;      // [H][T][D] through (stride_head, stride_token), 16-bit elements

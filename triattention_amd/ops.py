@@ -11,10 +11,12 @@ from typing import Sequence
 import torch
 
 from . import _lib
-from ._lib import (KV_BF16, KV_FP16, KV_FP8_E4M3, REDUCE_MAX, REDUCE_MEAN, REDUCE_NONE, ROPE_HALF,
-                   ROPE_INTERLEAVED, AttendParams, Batch, BlockParams, EvictParams, KvLayout, ScoreParams, SelectParams)
+from ._lib import (KV_BF16, KV_FP16, KV_FP8_E4M3, REAL_BF16, REAL_FP16, REAL_FP32, REDUCE_MAX, REDUCE_MEAN, REDUCE_NONE, ROPE_HALF,
+                   ROPE_INTERLEAVED, AcceptParams, AttendParams, Batch, BlockParams, EvictParams, KvLayout, ReadParams, ScoreParams,
+                   SelectParams, VerifyParams, WriteParams)
 
 _DTYPES = {torch.bfloat16: KV_BF16, torch.float16: KV_FP16}
+_REALS = {torch.bfloat16: REAL_BF16, torch.float16: REAL_FP16, torch.float32: REAL_FP32}
 _UNIT_SCALES: dict = {}
 
 
@@ -963,3 +965,194 @@ def evict_step(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: EvictCo
         buf, at = _scratch(kv, nbytes, "eviction")
         _lib.check(lib.tri_evict_step(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _ptr(keep), at, nbytes, _stream()))
     return keep
+
+
+def _check_rows(kv: PagedKV, name: str, t: torch.Tensor, dtype, heads: int | None, rows: int | None):
+    """Strides of a tensor of rows [rows, heads, head_dim] on the cache's device."""
+    shape, strides = t.shape, t.stride()
+    if (t.device != kv.device or t.dtype != dtype or len(shape) != 3 or shape[2] != kv.head_dim or strides[2] != 1
+            or (heads is not None and shape[1] != heads) or (rows is not None and shape[0] != rows)):
+        raise ValueError(f"{name} must be a {dtype} tensor [{'rows' if rows is None else rows}, {heads or 'heads'}, {kv.head_dim}] on {kv.device} "
+                         "with head_dim contiguous")
+    return strides
+
+
+def _check_vector(kv, name: str, t: torch.Tensor, dtype, shape: tuple) -> int:
+    if t.device != kv.device or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {kv.device}")
+    return t.data_ptr()
+
+
+def write_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                inv_freq: torch.Tensor, *, layer: int = 0, row_starts: torch.Tensor | None = None, freq_axes: torch.Tensor | None = None,
+                q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6, rotary_scale: float = 1.0,
+                k_scale: float = 1.0, v_scale: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """What comes before ``attend_paged``: queries and keys of the new tokens normalised per head (where there is a
+    norm) and rotated by their positions, keys and values written into their slots of one layer of the cache
+    (``tri_write_paged``).  Returns the rotated queries.
+
+    ``q`` [rows, Hq, D], ``k`` and ``v`` [rows, Hkv, D], bf16 or fp16 (of the cache's type, where it is not fp8), any strides of whole 16-byte
+    pieces: views of one projection's rows will do.  Rows as ``attend_paged``'s, without its limit of 64 a
+    sequence: the last tokens of ``batch.seq_lens``, one per sequence without ``row_starts``.
+
+    ``positions`` int32 or int64 [rows], or [axes, rows] with ``freq_axes`` (int32 [D / 2]: the axis each frequency goes by;
+    ``rope.section_axes`` makes it) for images and video.  ``inv_freq`` fp32 [D / 2], the pairs by the cache's ``rope_style``.
+    ``q_norm`` and ``k_norm`` [D], both of q's type or both fp32: y = x / sqrt(mean(x^2) + eps) * norm.  ``rotary_scale`` multiplies what is rotated.
+
+    An fp8 cache with a scale per row gets each row's: its largest finite magnitude / 448, at least 2^-126.  One without takes codes for code * ``k_scale``
+    (``v_scale``), as ``attend_paged`` reads them with these; larger numbers are the largest code.  Infinities and NaN become NaN
+    in either.  Everything is computed in 32 bits (angles in 64) and rounded once.
+
+    ``out`` may be ``q`` itself; otherwise it has no element in common with ``q``, ``k`` and ``v``.  Rows behind ``row_starts[-1]`` are left as they
+    were.  A captured call may be replayed with everything on the device rewritten in place."""
+    lib = _lib.load()
+    _check_attention_batch(kv, batch)
+    if kv.v_ptrs is None:
+        raise ValueError("write_paged needs the values of the cache")
+    dtype = q.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"q must be a bf16 or fp16 tensor [rows, heads, {kv.head_dim}]")
+    qs = _check_rows(kv, "q", q, dtype, None, None)
+    rows, heads, dim = q.shape
+    ks = _check_rows(kv, "k", k, dtype, kv.num_kv_heads, rows)
+    vs = _check_rows(kv, "v", v, dtype, kv.num_kv_heads, rows)
+    if out is None:
+        out = torch.empty((rows, heads, dim), dtype=dtype, device=kv.device)
+    os = _check_rows(kv, "out", out, dtype, heads, rows)
+    if not 0 <= layer < kv.num_layers:
+        raise IndexError(f"layer {layer} of {kv.num_layers}")
+    axes = positions.shape[0] if positions.ndim == 2 else 1
+    if (positions.device != kv.device or positions.dtype not in (torch.int32, torch.int64) or positions.shape[-1:] != (rows,)
+            or positions.ndim > 2 or axes < 1 or (rows > 1 and positions.stride(-1) != 1)):
+        raise ValueError(f"positions must be an int32 or int64 tensor [{rows}] or [axes, {rows}] on {kv.device}, the rows contiguous")
+    if axes > 1 and freq_axes is None:
+        raise ValueError("positions on several axes need freq_axes")
+    half = (dim // 2,)
+    norm = k_norm if q_norm is None else q_norm
+    norm_fp32 = norm is not None and norm.dtype == torch.float32
+    kind = torch.float32 if norm_fp32 else dtype
+    if row_starts is not None:
+        _check_vector(kv, "row_starts", row_starts, torch.int32, (batch.num_seqs + 1,))
+    # (in the order of the fields: by name they cost some microseconds of a call whose kernel takes a few)
+    p = WriteParams(layer, heads, rows, kv.num_blocks, _DTYPES[dtype], axes, positions.dtype == torch.int64, norm_fp32,
+                    q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], out.data_ptr(), os[0], os[1],
+                    positions.data_ptr(), positions.stride(0) if axes > 1 else 0,
+                    None if freq_axes is None else _check_vector(kv, "freq_axes", freq_axes, torch.int32, half),
+                    _check_vector(kv, "inv_freq", inv_freq, torch.float32, half),
+                    None if q_norm is None else _check_vector(kv, "q_norm", q_norm, kind, (dim,)),
+                    None if k_norm is None else _check_vector(kv, "k_norm", k_norm, kind, (dim,)), _ptr(row_starts), eps, rotary_scale, k_scale,
+                    v_scale)
+    with _on_device(kv.device):
+        _lib.check(lib.tri_write_paged(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _stream()))
+    return out
+
+
+def read_paged(kv: PagedKV, batch: StepBatch, row_starts: torch.Tensor, num_rows: int, *, layer: int = 0, dtype: torch.dtype | None = None,
+               k_scale: float = 1.0, v_scale: float = 1.0, out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """The last tokens of every sequence of one layer as dense K and V [num_rows, Hkv, D], each number times its row's scale
+    (fp8 caches that have them) and ``k_scale`` (``v_scale``), rounded once (``tri_read_paged``).
+
+    Sequence b has the rows ``row_starts[b]`` to ``row_starts[b + 1] - 1`` (int32 [sequences + 1] on the device, ascending): the running
+    sum of the lengths reads everything.  ``dtype`` bf16, fp16 or fp32 (None: the cache's; fp8: bf16).  Rows of tokens
+    that the cache does not have are zeros; rows behind ``row_starts[-1]`` are left as they were.  ``out``: contiguous tensors for K and V."""
+    lib = _lib.load()
+    _check_attention_batch(kv, batch)
+    if kv.v_ptrs is None:
+        raise ValueError("read_paged needs the values of the cache")
+    if not 0 <= layer < kv.num_layers:
+        raise IndexError(f"layer {layer} of {kv.num_layers}")
+    if not 0 <= num_rows < 1 << 31:
+        raise ValueError(f"num_rows {num_rows}")
+    if out is not None and dtype is None:
+        dtype = out[0].dtype
+    if dtype is None:
+        dtype = torch.bfloat16 if _DTYPES[kv.dtype] == KV_FP8_E4M3 else kv.dtype
+    if dtype not in _REALS:
+        raise TypeError(f"rows are read as bf16, fp16 or fp32, not {dtype}")
+    shape = (num_rows, kv.num_kv_heads, kv.head_dim)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=kv.device), torch.empty(shape, dtype=dtype, device=kv.device)
+    k_out, v_out = out
+    p = ReadParams(layer, num_rows, kv.num_blocks, _REALS[dtype], _check_vector(kv, "row_starts", row_starts, torch.int32, (batch.num_seqs + 1,)),
+                   _check_vector(kv, "out[0]", k_out, dtype, shape), _check_vector(kv, "out[1]", v_out, dtype, shape), k_scale, v_scale)
+    with _on_device(kv.device):
+        _lib.check(lib.tri_read_paged(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _stream()))
+    return k_out, v_out
+
+
+def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, row_starts: torch.Tensor, uniforms: torch.Tensor, *, max_rows: int | None = None,
+                  parents: torch.Tensor | None = None, draft_probs: torch.Tensor | None = None, temperatures: torch.Tensor | None = None,
+                  probs: bool = False):
+    """Which drafted tokens the target accepts, and the token that follows them, from given random numbers (``tri_verify_drafts``).
+
+    Rows as in ``attend_paged``: sequence b has ``row_starts[b]`` to ``row_starts[b + 1] - 1``, of which the first ``max_rows`` <= 64 are looked at; the first
+    is the last token decided, the others drafts behind their ``parents`` (None: each behind the one before).  ``target`` [rows, vocab] has what
+    follows each row: logits (bf16, fp16, fp32), p = softmax(logits / ``temperatures[b]``), or with ``probs`` fp32 probabilities.
+    ``tokens`` int32 [rows]; ``uniforms`` fp32 [rows, 2] in [0, 1).
+
+    Without ``draft_probs`` a token is drawn from every row's p, and the walk goes from the first row on to the child that holds it (the
+    first of several), as long as there is one.  With them (fp32 [rows, vocab]: what each row's token was drawn from; chains only) a row is accepted
+    iff uniforms[row, 0] * draft(token) < p(token), and after a rejection the next token comes from max(p - draft, 0).  Either way accepted and next
+    tokens have the target's distribution.  A draw: the least token whose running sum exceeds uniforms[row, 1] of the whole, in 64 bits.
+    A temperature of 0 takes the largest logit (the first of equals) instead.
+
+    Returns (rows int32 [sequences, max_rows]: accepted rows ascending, the first row first, -1 behind them; counts int32 [sequences];
+    next int32 [sequences], -1 for a sequence without rows, or where a row leaves nothing to draw).  ``accept_drafts`` takes rows and counts."""
+    lib = _lib.load()
+    if not target.is_cuda:
+        raise RuntimeError("verify_drafts needs device tensors (there is no CPU fallback)")
+    if target.ndim != 2 or target.dtype not in _REALS or (target.shape[1] > 1 and target.stride(1) != 1):
+        raise ValueError("target must be a bf16, fp16 or fp32 tensor [rows, vocab], the vocabulary contiguous")
+    if probs and target.dtype != torch.float32:
+        raise ValueError("probabilities must be fp32")
+    rows, vocab = target.shape
+    if row_starts.ndim != 1 or row_starts.shape[0] < 2:
+        raise ValueError("row_starts must have an entry for every sequence and one behind the last")
+    seqs = row_starts.shape[0] - 1
+    if max_rows is None:
+        max_rows = min(max(rows, 1), 64)
+    elif not 1 <= max_rows <= 64:
+        raise ValueError(f"max_rows must be 1 to 64, got {max_rows}")
+    if draft_probs is not None and (draft_probs.shape != target.shape or draft_probs.dtype != torch.float32 or draft_probs.device != target.device
+                                    or (vocab > 1 and draft_probs.stride(1) != 1)):
+        raise ValueError(f"draft_probs must be a fp32 tensor [{rows}, {vocab}] on {target.device}, the vocabulary contiguous")
+    # one allocation for the three answers
+    answer = torch.empty(seqs * (max_rows + 2), dtype=torch.int32, device=target.device)
+    at = answer.data_ptr()
+    p = VerifyParams(seqs, rows, max_rows, vocab, _REALS[target.dtype], probs, target.data_ptr(), target.stride(0),
+                     _check_vector(target, "tokens", tokens, torch.int32, (rows,)),
+                     _check_vector(target, "row_starts", row_starts, torch.int32, (seqs + 1,)),
+                     None if parents is None else _check_vector(target, "parents", parents, torch.int32, (rows,)),
+                     _check_vector(target, "uniforms", uniforms, torch.float32, (rows, 2)),
+                     None if temperatures is None else _check_vector(target, "temperatures", temperatures, torch.float32, (seqs,)),
+                     _ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0), at, at + 4 * seqs * max_rows,
+                     at + 4 * seqs * (max_rows + 1))
+    with _on_device(target.device):
+        ps = C.byref(p)
+        nbytes = lib.tri_verify_workspace_bytes(ps)
+        buf, ws = _scratch(target, nbytes, "verification")
+        _lib.check(lib.tri_verify_drafts(ps, ws, nbytes, _stream()))
+    n = seqs * max_rows
+    return answer[:n].view(seqs, max_rows), answer[n:n + seqs], answer[n + seqs:]
+
+
+def accept_drafts(kv: PagedKV, batch: StepBatch, row_starts: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor, *,
+                  weights: torch.Tensor | None = None) -> torch.Tensor:
+    """The accepted rows of every sequence moved one behind the other in every layer of the cache (``tri_accept_drafts``): K, V, an
+    fp8 row's scales and the accumulated ``weights``.  ``batch.seq_lens`` counts all drafted rows (the last tokens, by
+    ``row_starts``), ``rows`` and ``counts`` are ``verify_drafts``'.  Returns the new lengths, int32 [sequences]: the batch's less the rows that
+    were not accepted.  Block bounds of the blocks concerned are to be updated behind it."""
+    lib = _lib.load()
+    _check_attention_batch(kv, batch)
+    if kv.v_ptrs is None:
+        raise ValueError("accept_drafts needs the values of the cache")
+    n = batch.num_seqs
+    if rows.ndim != 2 or not 1 <= rows.shape[1] <= 64:
+        raise ValueError(f"rows must be an int32 tensor [{n}, 1 to 64]")
+    lens = torch.empty(n, dtype=torch.int32, device=kv.device)
+    p = AcceptParams(kv.num_blocks, rows.shape[1], _check_vector(kv, "row_starts", row_starts, torch.int32, (n + 1,)),
+                     _check_vector(kv, "rows", rows, torch.int32, (n, rows.shape[1])), _check_vector(kv, "counts", counts, torch.int32, (n,)),
+                     None if weights is None else _weights_address(kv, weights), 0 if weights is None else weights.stride(0), lens.data_ptr())
+    with _on_device(kv.device):
+        _lib.check(lib.tri_accept_drafts(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _stream()))
+    return lens

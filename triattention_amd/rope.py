@@ -9,7 +9,7 @@ model code is imported.
 from __future__ import annotations
 
 import math
-from typing import Any, Mapping
+from typing import Any, Mapping, Sequence
 
 import torch
 
@@ -56,6 +56,25 @@ def inv_freq_from_rope_config(head_dim: int, rope_theta: float | None,
         return llama3_inv_freq(head_dim, theta, float(rs["factor"]), float(rs["low_freq_factor"]),
                                float(rs["high_freq_factor"]), int(rs["original_max_position_embeddings"]))
     raise ValueError(f"unsupported rope_type {kind!r}: put inv_freq into the stats file's metadata")
+
+
+def section_axes(sections: Sequence[int], interleaved: bool = False) -> torch.Tensor:
+    """The position axis of every frequency, int32 [sum(sections)], for rotary positions with several axes (time, height and width
+    of images and video).  ``sections`` says how many frequencies each axis has; they follow one another, or with
+    ``interleaved`` take turns, frequency by frequency, an axis that has none left passing its turn to the first."""
+    counts = [int(x) for x in sections]
+    if not counts or min(counts) < 0 or sum(counts) == 0:
+        raise ValueError(f"sections must be counts of frequencies, got {list(sections)}")
+    if not interleaved:
+        return torch.repeat_interleave(torch.arange(len(counts), dtype=torch.int32), torch.tensor(counts))
+    axes, left = [], list(counts)
+    for f in range(sum(counts)):
+        axis = f % len(counts)
+        if left[axis] == 0:
+            axis = next(a for a, n in enumerate(left) if n)
+        axes.append(axis)
+        left[axis] -= 1
+    return torch.tensor(axes, dtype=torch.int32)
 
 
 def verify_rope_alignment(pruner_rotary: Any, model_rotary: Any, tolerance: float = 1e-5) -> None:
