@@ -1278,6 +1278,8 @@ int check_heads(const char* name, const void* p, int64_t stride_row, int64_t str
   if (rows > 0 && !p) return fail(TRI_ERR_INVALID_ARGUMENT, "%s is NULL", name);
   if (!is_aligned(p, 16) || stride_row % 8 || stride_head % 8)
     return fail(TRI_ERR_INVALID_ARGUMENT, "%s must be 16-byte aligned, its strides multiples of 8 elements", name);
+  // (the offsets of the heads that a wave has together are 32-bit)
+  if (stride_head < 0 || stride_head >= (1 << 27)) return fail(TRI_ERR_UNSUPPORTED, "stride of the heads of %s: %lld", name, (long long)stride_head);
   if (written && ((heads > 1 && stride_head < D) || (rows > 1 && stride_row < D)))
     return fail(TRI_ERR_INVALID_ARGUMENT, "strides of %s are less than head_dim", name);
   return TRI_OK;
@@ -1285,7 +1287,7 @@ int check_heads(const char* name, const void* p, int64_t stride_row, int64_t str
 
 struct VerifyPlan {
   tri::VerifyLaunch a{};
-  int64_t part, state, rest, total;
+  int64_t part, arrived, picked, rest, total;
 };
 
 int plan_verify(const tri_verify_params* p, VerifyPlan& d) {
@@ -1316,7 +1318,8 @@ int plan_verify(const tri_verify_params* p, VerifyPlan& d) {
   int64_t off = 0;
   auto take = [&](int64_t bytes) { const int64_t o = off; off = tri::align_up(off + bytes, 256); return o; };
   d.part = take((int64_t)p->num_rows * a.pieces * sizeof(tri::VerifyPart));
-  d.state = take(p->draft_probs ? (int64_t)p->num_seqs * sizeof(tri::VerifyState) : 0);
+  d.arrived = take((int64_t)p->num_seqs * 4);
+  d.picked = take(p->draft_probs ? 0 : (int64_t)p->num_seqs * p->max_rows * 4);
   d.rest = take(p->draft_probs ? (int64_t)p->num_seqs * a.pieces * 8 : 0);
   d.total = std::max<int64_t>(off, 256);
   return TRI_OK;
@@ -1347,6 +1350,7 @@ int tri_write_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_w
     return fail(TRI_ERR_INVALID_ARGUMENT, "%d axes of positions, %lld apart", p->num_axes, (long long)p->position_stride);
   if (!(p->eps >= 0.f) || !is_finite(p->eps) || !is_finite(p->rotary_scale))
     return fail(TRI_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, rotary_scale finite");
+  if (kv->stride_head < 0 || kv->stride_head >= (1 << 27)) return fail(TRI_ERR_UNSUPPORTED, "stride_head %lld", (long long)kv->stride_head);
   const bool row_scales = kv->kv_dtype == TRI_KV_FP8_E4M3 && kv->v_scale_layers;
   const bool scaled = kv->kv_dtype == TRI_KV_FP8_E4M3 && !row_scales;
   for (const float x : {p->k_scale, p->v_scale}) {
@@ -1417,7 +1421,8 @@ int tri_verify_drafts(const tri_verify_params* p, void* ws, uint64_t ws_bytes, v
   rc = check_workspace(need, ws, ws_bytes);
   if (rc) return rc;
   d.a.part = at<tri::VerifyPart>(ws, d.part);
-  d.a.state = at<tri::VerifyState>(ws, d.state);
+  d.a.arrived = at<int32_t>(ws, d.arrived);
+  d.a.picked = at<int32_t>(ws, d.picked);
   d.a.rest = at<double>(ws, d.rest);
   return launch_status(tri::launch_verify_drafts(d.a, (hipStream_t)stream), "verify_drafts");
 }

@@ -352,7 +352,7 @@ hipError_t launch_move_weights(const EvictLaunch& a, hipStream_t s);
 struct WriteLaunch {
   int B, Hq, Hkv, D, block_size, kv_dtype, q_dtype, rope_style, layer, Tmax, num_blocks, num_rows;
   int num_axes, positions_64, norm_fp32;
-  int waves_per_row;                                       // set by the launcher
+  int waves_per_row, stream_rows;                          // set by the launcher
   int64_t stride_block, stride_token, stride_head;         // elements
   void* const* k_layers;
   void* const* v_layers;
@@ -398,11 +398,6 @@ struct VerifyPart {                       // of a piece: sum of the weights agai
   float most;
   int32_t where;
 };
-struct VerifyState {                      // of a sequence: its last accepted row's sum, largest number and place; rows accepted; 1: a row was rejected
-  double sum;
-  float most;
-  int32_t where, count, rest;
-};
 struct VerifyLaunch {
   int B, num_rows, max_rows, vocab, target_dtype, probs, pieces;
   const void* target;
@@ -419,8 +414,9 @@ struct VerifyLaunch {
   int32_t* next;
   // workspace
   VerifyPart* part;                                        // [num_rows][pieces]
-  VerifyState* state;                                      // [B]
-  double* rest;                                            // [B][pieces]
+  int32_t* arrived;                                        // [B]: workgroups that have come to a sequence's end
+  int32_t* picked;                                         // [B][max_rows]: the token drawn from each row (no draft probabilities)
+  double* rest;                                            // [B][pieces]: sums of what a rejection leaves (draft probabilities)
 };
 hipError_t launch_verify_drafts(const VerifyLaunch& a, hipStream_t s);
 struct AcceptLaunch {

@@ -5,8 +5,8 @@
 // the last accepted row the next token is drawn from p, or where a row was rejected from max(p - q, 0) over its sum.  Without
 // them (chain or tree): every row's token is drawn from p (T = 0: the first largest), and the walk goes on to the child that holds it.
 // A draw is the least x whose running sum exceeds u times the whole.  Which token that is must not depend on the order of a sum:
-// exponentials and sums are 64-bit, off by some 2^-46 of the whole, and of 2^17 boundaries between tokens one lies that
-// near a random number once in 2^29 draws.
+// exponentials and sums are 64-bit, off by some 2^-43 of the whole, and of 2^17 boundaries between tokens one lies that
+// near a random number once in 2^25 draws.
 //
 //  verify_sums_kernel  : every row's pieces of 2048 logits, a wave each: largest, where, and the sum of w against that
 //  verify_walk_kernel  : (no draft probabilities) a workgroup per sequence: a wave draws a row's token, then the walk
@@ -22,100 +22,217 @@
 namespace tri {
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kPieceSteps = kVerifyPiece / (kWave * 8);
 constexpr int kVerifyThreads = 256;
 constexpr int kVerifyWaves = kVerifyThreads / kWave;
-constexpr int kWalkThreads = 1024;
+constexpr int kChainThreads = 512;
+constexpr int kChainWaves = kChainThreads / kWave;
 
-// 2^y for y <= 0 (anything below -1100, and NaN, gives 0): y = n + f, the Taylor series of 2^f up to f^11 on [-1/2, 1/2], whose next
-// term is 2^-47 of the result, and the exponent n.  Sixteen 64-bit instructions; the library's exponential has about twice that.
-__device__ __forceinline__ double pow2_64(double y) {
-  y = fmax(y, -1100.0);
-  const double n = __builtin_rint(y), f = y - n;
-  double p = 4.4455382718708113e-10;
-  p = __builtin_fma(p, f, 7.0549116208011234e-09);
-  p = __builtin_fma(p, f, 1.0178086009239700e-07);
-  p = __builtin_fma(p, f, 1.3215486790144310e-06);
-  p = __builtin_fma(p, f, 1.5252733804059841e-05);
-  p = __builtin_fma(p, f, 1.5403530393381610e-04);
-  p = __builtin_fma(p, f, 1.3333558146428443e-03);
-  p = __builtin_fma(p, f, 9.6181291076284772e-03);
-  p = __builtin_fma(p, f, 5.5504108664821580e-02);
-  p = __builtin_fma(p, f, 2.4022650695910072e-01);
-  p = __builtin_fma(p, f, 6.9314718055994531e-01);
-  p = __builtin_fma(p, f, 1.0);
-  return __builtin_ldexp(p, (int)n);
+// 2^y, y <= 0, never less than 2^-1000 (which NaN gives too): y = n + j / 32 + f, rounded by an addition; 2^f on [-1/64, 1/64] by its Chebyshev
+// interpolation of degree 4 (off by 2^-43.5 of it), 2^(j/32) out of LDS, n into the exponent.  Sixteen instructions for a logit, with
+// the series alone (degree 9) it would be twenty.  The table is 32 numbers because those lie in 64 different banks: lanes read the
+// same word or different banks.  The coefficients are kept from being constants that the compiler copies into vector registers before
+// every step: they are the products' scalar operand.
+constexpr double kLeastPower = -1000.0;
+constexpr int kPowers = 32;
+struct Powers {
+  const double* table;      // 2^(j/32) with j << 15 taken off its high word: what y's units of 1/32, shifted as far, add to it is n alone
+  double c[4];
+  __device__ __forceinline__ explicit Powers(const double* in_lds) : table(in_lds) {
+    const double exact[4] = {0.6931471805351095, 0.24022650695623157, 0.055504515573860415, 0.009618176115571158};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = exact[i];
+      asm("" : "+s"(c[i]));
+    }
+  }
+  // eight of them: the table's words are all asked for before the first is used
+  __device__ __forceinline__ void operator()(double (&y)[8]) const {
+    uint32_t units[8];
+    double power[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = fmax(y[e], kLeastPower);
+      const double shifted = y[e] + 211106232532992.0;      // 1.5 * 2^47: the sum's low bits are the units
+      units[e] = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
+      power[e] = table[units[e] % kPowers];
+      y[e] -= shifted - 211106232532992.0;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      double p = __builtin_fma(c[3], y[e], c[2]);
+      p = __builtin_fma(p, y[e], c[1]);
+      p = __builtin_fma(p, y[e], c[0]);
+      p = __builtin_fma(p, y[e], 1.0);
+      u32x2 words = __builtin_bit_cast(u32x2, power[e]);
+      words.y += units[e] << 15;
+      y[e] = p * __builtin_bit_cast(double, words);
+    }
+  }
+  __device__ __forceinline__ double operator()(double y) const {
+    double eight[8] = {y, 0, 0, 0, 0, 0, 0, 0};
+    (*this)(eight);
+    return eight[0];
+  }
+};
+// 2^(j/32), as the table holds them.
+__device__ const double kPowerTable[kPowers] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+__device__ __forceinline__ void make_powers(double* table) {
+  if (threadIdx.x < kPowers) {
+    u32x2 words = __builtin_bit_cast(u32x2, kPowerTable[threadIdx.x]);
+    words.y -= threadIdx.x << 15;
+    table[threadIdx.x] = __builtin_bit_cast(double, words);
+  }
 }
 
-// w of a logit against `most`, c = log2 e / T.  Infinite logits share everything, -inf has nothing.
-__device__ __forceinline__ double weight_of(float x, float most, double c) {
-  if (most == INFINITY) return x == INFINITY ? 1.0 : 0.0;
-  return x == -INFINITY ? 0.0 : pow2_64(((double)x - (double)most) * c);
+// w of eight logits against the largest one, c = log2 e / T: exactly nothing where it is below 2^-1000 of that, -inf or NaN.
+__device__ __forceinline__ void weights_of(const Powers& powers, const float (&x)[8], double most, double c, double (&w)[8]) {
+  double y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = y[e] = ((double)x[e] - most) * c;
+  powers(w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = y[e] > kLeastPower ? w[e] : 0.0;
+}
+__device__ __forceinline__ double weight_of(const Powers& powers, float x, double most, double c) {
+  const double y = ((double)x - most) * c, w = powers(y);
+  return y > kLeastPower ? w : 0.0;
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(1))) char* GlobalRows;
 typedef __attribute__((address_space(1))) u32x4* GlobalPiece;
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
 
-// The number a logit or probability counts as.  NaN logits are -inf; probabilities that are no positive finite number are 0.
-template <bool PROBS>
+// The number a logit or probability counts as.  Logits: NaN as -inf, +inf as the largest finite number, so that infinities share
+// everything.  Probabilities that are no positive finite number: 0.  Raw logits are taken as they are.
+enum Numbers { kRawLogits = 0, kLogits = 1, kProbs = 2 };
+template <int N>
 __device__ __forceinline__ float counted(float x) {
-  if constexpr (PROBS) return x > 0.f && x <= FLT_MAX ? x : 0.f;
-  else return x == x ? x : -INFINITY;
+  if constexpr (N == kProbs) return x <= FLT_MAX ? fmaxf(x, 0.f) : 0.f;
+  else if constexpr (N == kLogits) return x == x ? fminf(x, FLT_MAX) : -INFINITY;
+  else return x;
 }
-template <int RT, bool PROBS>
+template <int RT, int N>
 __device__ __forceinline__ float load_one(const void* row, int64_t i) {
-  if constexpr (RT == TRI_REAL_FP32) return counted<PROBS>(reinterpret_cast<const float*>(row)[i]);
-  else if constexpr (RT == TRI_REAL_FP16) return counted<PROBS>((float)reinterpret_cast<const _Float16*>(row)[i]);
-  else return counted<PROBS>(__uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16));
+  if constexpr (RT == TRI_REAL_FP32) return counted<N>(reinterpret_cast<const float*>(row)[i]);
+  else if constexpr (RT == TRI_REAL_FP16) return counted<N>((float)reinterpret_cast<const _Float16*>(row)[i]);
+  else return counted<N>(__uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(row)[i] << 16));
 }
-// Eight of them from element i on (rows lie at any element); behind the row what counts as nothing.
-template <int RT, bool PROBS>
-__device__ __forceinline__ void load_eight(const void* row, int i, int V, float (&x)[8]) {
+// Eight of them from element i on as they lie (rows begin at any element); behind the row what counts as nothing.
+template <int RT>
+struct Eight {
+  uint32_t word[RT == TRI_REAL_FP32 ? 8 : 4];
+};
+template <int RT, int N>
+__device__ __forceinline__ Eight<RT> load_eight(const void* row, int i, int V) {
+  Eight<RT> x;
   if (i + 8 <= V) {
-    if constexpr (RT == TRI_REAL_FP32) {
-      const u32x4u* p = reinterpret_cast<const u32x4u*>(reinterpret_cast<const float*>(row) + i);
-      const u32x4u a = p[0], b = p[1];
+    const u32x4u* p = reinterpret_cast<const u32x4u*>(reinterpret_cast<const char*>(row) + (int64_t)i * (RT == TRI_REAL_FP32 ? 4 : 2));
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = __uint_as_float(a[e]);
-        x[4 + e] = __uint_as_float(b[e]);
-      }
-    } else {
-      const u32x4u a = *reinterpret_cast<const u32x4u*>(reinterpret_cast<const uint16_t*>(row) + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if constexpr (RT == TRI_REAL_FP16) {
-          x[2 * e] = (float)__builtin_bit_cast(_Float16, (unsigned short)(a[e] & 0xffffu));
-          x[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(a[e] >> 16));
-        } else {
-          x[2 * e] = __uint_as_float(a[e] << 16);
-          x[2 * e + 1] = __uint_as_float(a[e] & 0xffff0000u);
-        }
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = counted<PROBS>(x[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = i + e < V ? load_one<RT, PROBS>(row, i + e) : (PROBS ? 0.f : -INFINITY);
+    for (int e = 0; e < (RT == TRI_REAL_FP32 ? 8 : 4); ++e) x.word[e] = p[e / 4][e % 4];
+    return x;
   }
+  if constexpr (RT == TRI_REAL_FP32) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x.word[e] = i + e < V ? reinterpret_cast<const uint32_t*>(row)[i + e] : N == kProbs ? 0u : 0xff800000u;
+  } else {
+    const uint32_t nothing = N == kProbs ? 0u : RT == TRI_REAL_FP16 ? 0xfc00u : 0xff80u;
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const uint32_t lo = i + e < V ? reinterpret_cast<const uint16_t*>(row)[i + e] : nothing;
+      const uint32_t hi = i + e + 1 < V ? reinterpret_cast<const uint16_t*>(row)[i + e + 1] : nothing;
+      x.word[e / 2] = lo | hi << 16;
+    }
+  }
+  return x;
+}
+struct Numbers8 {
+  float x[8];
+};
+template <int RT, int N>
+__device__ __forceinline__ Numbers8 numbers_of(const Eight<RT>& eight) {
+  Numbers8 n;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float x;
+    if constexpr (RT == TRI_REAL_FP32) x = __uint_as_float(eight.word[e]);
+    else if constexpr (RT == TRI_REAL_FP16) x = (float)__builtin_bit_cast(_Float16, (unsigned short)(eight.word[e / 2] >> e % 2 * 16));
+    else x = __uint_as_float(e % 2 ? eight.word[e / 2] & 0xffff0000u : eight.word[e / 2] << 16);
+    n.x[e] = counted<N>(x);
+  }
+  return n;
+}
+// A piece as a wave has it: step s is 512 numbers, eight a lane.
+template <int RT>
+struct Piece {
+  Eight<RT> step[kPieceSteps];
+};
+template <int RT, int N>
+__device__ __forceinline__ Piece<RT> load_piece(const VerifyLaunch& a, const void* row, int piece, int lane) {
+  Piece<RT> x;
+#pragma unroll
+  for (int s = 0; s < kPieceSteps; ++s)
+    x.step[s] = load_eight<RT, N>(row, (int)min((int64_t)piece * kVerifyPiece + s * kWave * 8 + lane * 8, (int64_t)a.vocab), a.vocab);
+  return x;
 }
 
-__device__ __forceinline__ double shfl_double(double v, int lane) { return __shfl(v, lane); }
-__device__ __forceinline__ double sum_of_wave(double v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) v += __shfl_xor(v, d);
-  return v;
+// Exchanges inside a wave without LDS: every 16 lanes by their row's permutations, the four rows by broadcasts or scalar registers.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, true);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// Inclusive running sum over the lanes.
-__device__ __forceinline__ double running_sum(double v, int lane) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const double below = __shfl_up(v, d);
-    if (lane >= d) v += below;
-  }
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double sum_of_wave(double v) {
+  v += moved<0xB1>(v);        // quad_perm [1, 0, 3, 2]
+  v += moved<0x4E>(v);        // quad_perm [2, 3, 0, 1]
+  v += moved<0x141>(v);       // row_half_mirror
+  v += moved<0x128>(v);       // row_ror:8
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+}
+template <int CTRL>
+__device__ __forceinline__ int moved_int(int v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+__device__ __forceinline__ float most_of_wave(float v) {
+  v = fmaxf(v, __int_as_float(moved_int<0xB1>(__float_as_int(v))));
+  v = fmaxf(v, __int_as_float(moved_int<0x4E>(__float_as_int(v))));
+  v = fmaxf(v, __int_as_float(moved_int<0x141>(__float_as_int(v))));
+  v = fmaxf(v, __int_as_float(moved_int<0x128>(__float_as_int(v))));
+  const auto of = [&](int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane)); };
+  return fmaxf(fmaxf(of(0), of(16)), fmaxf(of(32), of(48)));
+}
+__device__ __forceinline__ int least_of_wave(int v) {
+  v = min(v, moved_int<0xB1>(v));
+  v = min(v, moved_int<0x4E>(v));
+  v = min(v, moved_int<0x141>(v));
+  v = min(v, moved_int<0x128>(v));
+  const auto of = [&](int lane) { return __builtin_amdgcn_readlane(v, lane); };
+  return min(min(of(0), of(16)), min(of(32), of(48)));
+}
+// Inclusive running sum over the lanes: within rows of 16 by shifts, then each row's last lane into the rows behind it.
+__device__ __forceinline__ double running_sum(double v) {
+  v += moved<0x111>(v);
+  v += moved<0x112>(v);
+  v += moved<0x114>(v);
+  v += moved<0x118>(v);
+  v += moved<0x142, 0xa>(v);  // row_bcast:15 into rows 1 and 3
+  v += moved<0x143, 0xc>(v);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
@@ -138,53 +255,79 @@ __device__ __forceinline__ const void* row_of(const VerifyLaunch& a, int row) {
   return reinterpret_cast<const char*>(a.target) + row * a.target_stride * (RT == TRI_REAL_FP32 ? 4 : 2);
 }
 
+// A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunch a) {
+  __shared__ double table[kPowers];
   const int lane = threadIdx.x % kWave;
+  for (int64_t i = (int64_t)blockIdx.x * kVerifyThreads + threadIdx.x; i < a.B; i += (int64_t)gridDim.x * kVerifyThreads) a.arrived[i] = 0;
   const int64_t unit = (int64_t)blockIdx.x * kVerifyWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int row = (int)(unit / a.pieces), piece = (int)(unit % a.pieces);
+  constexpr int N = PROBS ? kProbs : kRawLogits;
+  Piece<RT> held;
+  if (row < a.num_rows) held = load_piece<RT, N>(a, row_of<RT, PROBS>(a, row), piece, lane);
+  make_powers(table);
+  __syncthreads();
   if (row >= a.num_rows) return;
-  const void* const src = row_of<RT, PROBS>(a, row);
-  float x[kPieceSteps][8];
-#pragma unroll
-  for (int s = 0; s < kPieceSteps; ++s) {
-    const int64_t i = (int64_t)piece * kVerifyPiece + s * kWave * 8 + lane * 8;
-    load_eight<RT, PROBS>(src, (int)min(i, (int64_t)a.vocab), a.vocab, x[s]);
-  }
-  const int b = sequence_of_row(a.row_starts, a.B, row, lane);
+  const int b = __builtin_amdgcn_readfirstlane(sequence_of_row(a.row_starts, a.B, row, lane));
   if (b < 0 || row - a.row_starts[b] >= a.max_rows) return;
   bool greedy;
   const double c = sharpness_of(a, b, greedy);
   float most = -INFINITY;
 #pragma unroll
-  for (int s = 0; s < kPieceSteps; ++s)
+  for (int s = 0; s < kPieceSteps; ++s) {
+    const Numbers8 n = numbers_of<RT, N>(held.step[s]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = fmaxf(most, x[s][e]);
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-  int where = INT32_MAX;
-#pragma unroll
-  for (int s = kPieceSteps - 1; s >= 0; --s)
-#pragma unroll
-    for (int e = 7; e >= 0; --e)
-      if (x[s][e] == most) where = s * kWave * 8 + lane * 8 + e;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) where = min(where, __shfl_xor(where, d));
+    for (int e = 0; e < 8; ++e) most = fmaxf(most, n.x[e]);
+  }
+  most = most_of_wave(most);
   double sum = 0.0;
-  if constexpr (PROBS) {
+  int where = 0;
+  if (greedy) {
+    where = INT32_MAX;
 #pragma unroll
-    for (int s = 0; s < kPieceSteps; ++s)
+    for (int s = kPieceSteps - 1; s >= 0; --s) {
+      const Numbers8 n = numbers_of<RT, N>(held.step[s]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += (double)x[s][e];
+      for (int e = 7; e >= 0; --e)
+        if (n.x[e] == most) where = s * kWave * 8 + lane * 8 + e;
+    }
+    where = most > -INFINITY ? least_of_wave(where) : 0;
+  } else if (PROBS || most == INFINITY) {
+    // (what counts as nothing weighs nothing, and beside infinities all else does)
+#pragma unroll
+    for (int s = 0; s < kPieceSteps; ++s) {
+      const Numbers8 n = numbers_of<RT, N>(held.step[s]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += PROBS ? (double)n.x[e] : n.x[e] == INFINITY ? 1.0 : 0.0;
+    }
     sum = sum_of_wave(sum);
-  } else if (!greedy && most > -INFINITY) {
+  } else if (most > -INFINITY) {
+    // (what weighs less than 2^-1000 counts as that here: the largest weighs 1)
+    const Powers powers(table);
+    const double top = most;
 #pragma unroll
-    for (int s = 0; s < kPieceSteps; ++s)
+    for (int s = 0; s < kPieceSteps; ++s) {
+      const Numbers8 n = numbers_of<RT, N>(held.step[s]);
+      double w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += weight_of(x[s][e], most, c);
+      for (int e = 0; e < 8; ++e) w[e] = ((double)n.x[e] - top) * c;
+      powers(w);
+      sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    }
     sum = sum_of_wave(sum);
   }
-  if (lane == 0) a.part[unit] = VerifyPart{sum, most, piece * kVerifyPiece + where};
+  if (lane == 0) a.part[unit] = VerifyPart{sum, PROBS ? most : fminf(most, FLT_MAX), piece * kVerifyPiece + where};
+}
+
+template <bool PROBS>
+__device__ __forceinline__ void weights_or_probs(const Powers& powers, const Numbers8& n, float most, double c, double (&w)[8]) {
+  if constexpr (PROBS) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = n.x[e];
+  } else {
+    weights_of(powers, n.x, most, c, w);
+  }
 }
 
 // A row's largest number, the first place that holds it (-1: every number is -inf) and the sum of its weights.
@@ -196,103 +339,87 @@ struct RowTotal {
 
 // The sum of a piece's weights against the row's largest number.
 template <bool PROBS>
-__device__ __forceinline__ double against(const VerifyPart& p, float most, double c) {
+__device__ __forceinline__ double against(const Powers& powers, const VerifyPart& p, float most, double c) {
   if constexpr (PROBS) return p.sum;
-  else return p.sum == 0.0 ? 0.0 : p.sum * weight_of(p.most, most, c);
+  else return p.sum == 0.0 ? 0.0 : p.sum * weight_of(powers, p.most, most, c);
 }
 
 template <bool PROBS>
-__device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, int row, double c, int lane) {
+__device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, const Powers& powers, int row, double c, int lane) {
   const VerifyPart* part = a.part + (int64_t)row * a.pieces;
   RowTotal t{0.0, -INFINITY, INT32_MAX};
-  for (int i = lane; i < a.pieces; i += kWave)
+  // (a row of up to 2^17 numbers: one piece a lane, read once)
+  VerifyPart mine{0.0, -INFINITY, INT32_MAX};
+  if (lane < a.pieces) mine = part[lane];
+  t.most = mine.most;
+  t.where = mine.where;
+  for (int i = lane + kWave; i < a.pieces; i += kWave)
     if (part[i].most > t.most) {
       t.most = part[i].most;
       t.where = part[i].where;
     }
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const float m = __shfl_xor(t.most, d);
-    const int w = __shfl_xor(t.where, d);
-    if (m > t.most || (m == t.most && w < t.where)) {
-      t.most = m;
-      t.where = w;
-    }
-  }
+  const float most = most_of_wave(t.most);
+  t.where = least_of_wave(t.most == most ? t.where : INT32_MAX);
+  t.most = most;
   if (t.most == -INFINITY) t.where = -1;
-  for (int i = lane; i < a.pieces; i += kWave) t.sum += against<PROBS>(part[i], t.most, c);
+  t.sum = against<PROBS>(powers, mine, t.most, c);
+  for (int i = lane + kWave; i < a.pieces; i += kWave) t.sum += against<PROBS>(powers, part[i], t.most, c);
   t.sum = sum_of_wave(t.sum);
   return t;
 }
 
-// The least place whose running sum exceeds u of the whole; piece_sum(i) is piece i's sum, weights(i, w) its eight weights from element i
-// on.  A wave's work: the pieces' sums tell the piece, whose weights are found anew.  Where rounding leaves nothing above the
+// The least place whose running sum exceeds u of the whole; piece_sum(i) is piece i's sum, weights(load(i), s, w) a lane's eight weights in
+// its step s.  A wave's work: the pieces' sums tell the piece, whose weights are found anew.  Where rounding leaves nothing above the
 // mark, and for u >= 1, the last place of any weight; -1 if there is none.
-template <class PieceSum, class Weights>
-__device__ __forceinline__ int draw(const VerifyLaunch& a, double whole, float u, int lane, PieceSum piece_sum, Weights weights) {
+template <class PieceSum, class Load, class Weights>
+__device__ __forceinline__ int draw(const VerifyLaunch& a, double whole, float u, int lane, PieceSum piece_sum, Load load, Weights weights) {
   const double mark = (u > 0.f ? (double)u : 0.0) * whole;
   double before = 0.0, start = 0.0;
   int piece = -1, last = -1;
   for (int i0 = 0; i0 < a.pieces && piece < 0; i0 += kWave) {
     const double v = i0 + lane < a.pieces ? piece_sum(i0 + lane) : 0.0;
-    const double upto = before + running_sum(v, lane);
+    const double upto = before + running_sum(v);
     const uint64_t some = __ballot(v > 0.0), over = __ballot(v > 0.0 && upto > mark);
     if (over) {
       const int at = __ffsll((unsigned long long)over) - 1;
       piece = i0 + at;
-      start = at ? shfl_double(upto, at - 1) : before;
+      start = at ? lane_of(upto, at - 1) : before;
     } else if (some) {
       last = i0 + 63 - __clzll((long long)some);
     }
-    before = shfl_double(upto, kWave - 1);
+    before = lane_of(upto, kWave - 1);
   }
   const bool found = piece >= 0;
   if (!found) {
     piece = last;
     if (piece < 0) return -1;
   }
+  const auto held = load(piece);
   int best = -1;
+#pragma unroll
   for (int s = 0; s < kPieceSteps; ++s) {
     const int i = piece * kVerifyPiece + s * kWave * 8 + lane * 8;
     double w[8], sum = 0.0;
-    weights(i, w);
-    int final = -1;
+    weights(held, s, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += w[e];
+    const double upto = running_sum(sum);
+    double running = start + (upto - sum);
+    int mine = -1, final = -1;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      sum += w[e];
-      if (w[e] > 0.0) final = i + e;
-    }
-    const double upto = running_sum(sum, lane);
-    if (found) {
-      double running = start + (upto - sum);
-      int mine = -1;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        running += w[e];
-        if (mine < 0 && w[e] > 0.0 && running > mark) mine = i + e;
+      running += w[e];
+      if (w[e] > 0.0) {
+        if (mine < 0 && running > mark) mine = i + e;
+        final = i + e;
       }
-      const uint64_t over = __ballot(mine >= 0);
-      if (over) return __shfl(mine, __ffsll((unsigned long long)over) - 1);
     }
-    const uint64_t some = __ballot(final >= 0);
-    if (some) best = __shfl(final, 63 - __clzll((long long)some));
-    start += shfl_double(upto, kWave - 1);
+    const uint64_t over = found ? __ballot(mine >= 0) : 0, some = __ballot(final >= 0);
+    if (over) return __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)over) - 1);
+    if (some) best = __builtin_amdgcn_readlane(final, 63 - __clzll((long long)some));
+    start += lane_of(upto, kWave - 1);
   }
   return best;
-}
-
-// A token drawn from a row's weights.
-template <int RT, bool PROBS>
-__device__ __forceinline__ int draw_from_row(const VerifyLaunch& a, int row, const RowTotal& t, double c, float u, int lane) {
-  const void* const src = row_of<RT, PROBS>(a, row);
-  const VerifyPart* part = a.part + (int64_t)row * a.pieces;
-  return draw(a, t.sum, u, lane, [&](int i) { return against<PROBS>(part[i], t.most, c); },
-              [&](int i, double (&w)[8]) {
-                float x[8];
-                load_eight<RT, PROBS>(src, min(i, a.vocab), a.vocab, x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = PROBS ? (double)x[e] : weight_of(x[e], t.most, c);
-              });
 }
 
 __device__ __forceinline__ void write_path(const VerifyLaunch& a, int b, int lane, int row, int count, int next) {
@@ -303,134 +430,185 @@ __device__ __forceinline__ void write_path(const VerifyLaunch& a, int b, int lan
   }
 }
 
-template <int RT, bool PROBS>
-__global__ __launch_bounds__(kWalkThreads) void verify_walk_kernel(VerifyLaunch a) {
-  __shared__ int picked[64];
-  const int b = blockIdx.x, lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  int first;
-  const int n = rows_of_sequence(a, b, first);
-  bool greedy;
-  const double c = sharpness_of(a, b, greedy);
-  for (int i = wave; i < n; i += kWalkThreads / kWave) {
-    const RowTotal t = total_of_row<PROBS>(a, first + i, c, lane);
-    const int token = greedy ? t.where : draw_from_row<RT, PROBS>(a, first + i, t, c, a.uniforms[2 * (int64_t)(first + i) + 1], lane);
-    if (lane == 0) picked[i] = token;
+// Whether this workgroup is the last of `groups` of sequence b to come here: what the others wrote before is then seen by its first wave.
+__device__ __forceinline__ bool last_to_arrive(const VerifyLaunch& a, int b, int groups) {
+  __shared__ int count;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+    count = __hip_atomic_fetch_add(a.arrived + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
-  if (wave) return;
-  // lane i is row i
-  int parent = -1, token = -1;
-  if (lane < n && lane > 0) {
-    parent = a.parents ? a.parents[first + lane] : lane - 1;
-    if (parent < 0 || parent >= lane) parent = -1;
-    token = a.tokens[first + lane];
+  if (count != groups - 1) return false;
+  if (threadIdx.x < kWave) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  return true;
+}
+
+template <int RT, bool PROBS>
+__global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunch a, int max_groups) {
+  constexpr int N = PROBS ? kProbs : kLogits;
+  __shared__ double table[kPowers];
+  const int b = blockIdx.x / max_groups, group = blockIdx.x % max_groups;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  int first;
+  const int n = rows_of_sequence(a, b, first), groups = max(1, ceil_div(n, kVerifyWaves));
+  if (group >= groups) return;
+  make_powers(table);
+  __syncthreads();
+  const Powers powers(table);
+  const int i = group * kVerifyWaves + wave;
+  int32_t* const picked = a.picked + (int64_t)b * a.max_rows;
+  if (i < n) {
+    bool greedy;
+    const double c = sharpness_of(a, b, greedy);
+    const float u = a.uniforms[2 * (int64_t)(first + i) + 1];
+    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, c, lane);
+    int token = t.where;
+    if (!greedy) {
+      const void* const src = row_of<RT, PROBS>(a, first + i);
+      const VerifyPart* const part = a.part + (int64_t)(first + i) * a.pieces;
+      token = draw(a, t.sum, u, lane, [&](int piece) { return against<PROBS>(powers, part[piece], t.most, c); },
+                   [&](int piece) { return load_piece<RT, N>(a, src, piece, lane); },
+                   [&](const Piece<RT>& held, int s, double (&w)[8]) { weights_or_probs<PROBS>(powers, numbers_of<RT, N>(held.step[s]), t.most, c, w); });
+    }
+    if (lane == 0) picked[i] = token;
   }
+  if (!last_to_arrive(a, b, groups) || wave) return;
+  // lane i is row i
+  int parent = -1, token = -1, want = -1;
+  if (lane < n) {
+    want = picked[lane];
+    if (lane > 0) {
+      parent = a.parents ? a.parents[first + lane] : lane - 1;
+      if (parent < 0 || parent >= lane) parent = -1;
+      token = a.tokens[first + lane];
+    }
+  }
+  // a row that may follow its parent; of those the walk takes the first behind where it stands
+  const int wanted = __shfl(want, max(parent, 0));
+  const bool follows = parent >= 0 && token == wanted && wanted >= 0;
   int here = 0, count = n > 0 ? 1 : 0, path = 0;
   while (n > 0) {
-    const int want = picked[here];
-    const uint64_t child = __ballot(parent == here && token == want && want >= 0);
+    const uint64_t child = __ballot(follows && parent == here);
     if (!child) break;
     here = __ffsll((unsigned long long)child) - 1;
     if (lane == count) path = here;
     ++count;
   }
-  write_path(a, b, lane, path, count, n > 0 ? picked[here] : -1);
+  write_path(a, b, lane, path, count, n > 0 ? __builtin_amdgcn_readlane(want, here) : -1);
 }
 
+// A piece of a row and of the draft probabilities of the row behind it, and what a rejection leaves of its tokens: max(w / E - q, 0).  Where the
+// token comes from the row itself, q is no pointer, and per_sum 1.
+template <int RT>
+struct Rest {
+  Piece<RT> row;
+  Piece<TRI_REAL_FP32> draft;
+};
+template <int RT, int N>
+__device__ __forceinline__ Rest<RT> load_rest(const VerifyLaunch& a, const void* row, const float* q, int piece, int lane) {
+  Rest<RT> x;
+  x.row = load_piece<RT, N>(a, row, piece, lane);
+  if (q) {
+    x.draft = load_piece<TRI_REAL_FP32, kProbs>(a, q, piece, lane);
+  } else {
+#pragma unroll
+    for (int s = 0; s < kPieceSteps; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x.draft.step[s].word[e] = 0;
+  }
+  return x;
+}
 template <int RT, bool PROBS>
-__global__ __launch_bounds__(kVerifyThreads) void verify_chain_kernel(VerifyLaunch a, int groups) {
+__device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& held, int s, float most, double per_sum, double c, double (&w)[8]) {
+  const Numbers8 q = numbers_of<TRI_REAL_FP32, kProbs>(held.draft.step[s]);
+  weights_or_probs<PROBS>(powers, numbers_of<RT, PROBS ? kProbs : kLogits>(held.row.step[s]), most, c, w);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(w[e], per_sum, -(double)q.x[e]), 0.0);
+}
+
+// Every workgroup of a sequence finds for itself which rows are accepted (a wave a row); where one is not, each takes some pieces of what
+// that leaves, and the last one draws from it.
+template <int RT, bool PROBS>
+__global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLaunch a, int groups) {
+  constexpr int N = PROBS ? kProbs : kLogits;
   __shared__ RowTotal totals[64];
   __shared__ int fits[64];
+  __shared__ double table[kPowers];
   const int b = blockIdx.x / groups, group = blockIdx.x % groups;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   int first;
   const int n = rows_of_sequence(a, b, first);
   bool greedy;
   const double c = sharpness_of(a, b, greedy);
-  for (int i = wave; i < n; i += kVerifyWaves) {
-    const RowTotal t = total_of_row<PROBS>(a, first + i, c, lane);
+  make_powers(table);
+  __syncthreads();
+  const Powers powers(table);
+  for (int i = wave; i < n; i += kChainWaves) {
+    // what the decision on the next row needs is asked for before the sums are joined
+    int token = -1;
+    float x = -INFINITY, q = 0.f, u = 0.f;
+    if (i + 1 < n) {
+      const int64_t next = first + i + 1;
+      token = a.tokens[next];
+      u = a.uniforms[2 * next];
+      if (!greedy && token >= 0 && token < a.vocab) {
+        x = load_one<RT, N>(row_of<RT, PROBS>(a, first + i), token);
+        q = counted<kProbs>(a.draft[next * a.draft_stride + token]);
+      }
+    }
+    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, c, lane);
+    bool ok = false;
+    if (greedy) {
+      ok = t.where >= 0 && token == t.where;
+    } else if (token >= 0 && token < a.vocab) {
+      const double w = PROBS ? (double)x : weight_of(powers, x, t.most, c);
+      ok = (u > 0.f ? (double)u : 0.0) * (double)q * t.sum < w;
+    }
     if (lane == 0) {
       totals[i] = t;
-      if (i + 1 < n) {
-        const int64_t next = first + i + 1;
-        const int token = a.tokens[next];
-        bool ok = false;
-        if (greedy) {
-          ok = t.where >= 0 && token == t.where;
-        } else if (token >= 0 && token < a.vocab) {
-          const float x = load_one<RT, PROBS>(row_of<RT, PROBS>(a, first + i), token);
-          const double w = PROBS ? (double)x : weight_of(x, t.most, c);
-          const float q = counted<true>(a.draft[next * a.draft_stride + token]), u = a.uniforms[2 * next];
-          ok = (u > 0.f ? (double)u : 0.0) * (double)q * t.sum < w;
-        }
-        fits[i + 1] = ok;
-      }
+      if (i + 1 < n) fits[i + 1] = ok;
     }
   }
   __syncthreads();
   const uint64_t refused = __ballot(lane > 0 && lane < n && !fits[lane]);
-  const int count = refused ? __ffsll((unsigned long long)refused) - 1 : n;
+  const int count = refused ? __ffsll((unsigned long long)refused) - 1 : n, row = first + count - 1;
   const RowTotal t = n > 0 ? totals[count - 1] : RowTotal{0.0, -INFINITY, -1};
-  const bool rest = refused && !greedy && t.sum > 0.0;
-  if (group == 0 && threadIdx.x == 0) a.state[b] = VerifyState{t.sum, t.most, t.where, count, rest};
-  const int piece = group * kVerifyWaves + wave;
-  if (!rest || piece >= a.pieces) return;
-  const void* const src = row_of<RT, PROBS>(a, first + count - 1);
-  const float* const q = a.draft + (int64_t)(first + count) * a.draft_stride;
-  double sum = 0.0;
+  const bool partly = refused && !greedy && t.sum > 0.0;      // a row was rejected: the token comes from what that leaves
+  if (!partly && (group || wave)) return;
+  const void* const src = row_of<RT, PROBS>(a, row);
+  const float* const q = a.draft + (int64_t)(row + 1) * a.draft_stride;
+  double* const rest = a.rest + (int64_t)b * a.pieces;
+  double whole = 0.0;
+  if (partly) {
+    const int piece = group * kChainWaves + wave;
+    if (piece < a.pieces) {
+      const Rest<RT> held = load_rest<RT, N>(a, src, q, piece, lane);
+      double sum = 0.0;
 #pragma unroll
-  for (int s = 0; s < kPieceSteps; ++s) {
-    const int i = (int)min((int64_t)piece * kVerifyPiece + s * kWave * 8 + lane * 8, (int64_t)a.vocab);
-    float x[8], y[8];
-    load_eight<RT, PROBS>(src, i, a.vocab, x);
-    load_eight<TRI_REAL_FP32, true>(q, i, a.vocab, y);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double w = PROBS ? (double)x[e] : weight_of(x[e], t.most, c);
-      sum += fmax(w / t.sum - (double)y[e], 0.0);
+      for (int s = 0; s < kPieceSteps; ++s) {
+        double w[8];
+        rest_of<RT, PROBS>(powers, held, s, t.most, 1.0 / t.sum, c, w);
+        sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      }
+      sum = sum_of_wave(sum);
+      if (lane == 0) rest[piece] = sum;
     }
+    if (!last_to_arrive(a, b, groups) || wave) return;
+    for (int i = lane; i < a.pieces; i += kWave) whole += rest[i];
+    whole = sum_of_wave(whole);
   }
-  sum = sum_of_wave(sum);
-  if (lane == 0) a.rest[(int64_t)b * a.pieces + piece] = sum;
-}
-
-template <int RT, bool PROBS>
-__global__ __launch_bounds__(kWave) void verify_draw_kernel(VerifyLaunch a) {
-  const int b = blockIdx.x, lane = threadIdx.x;
-  int first;
-  const int n = rows_of_sequence(a, b, first);
-  if (n == 0) return write_path(a, b, lane, 0, 0, -1);
-  bool greedy;
-  const double c = sharpness_of(a, b, greedy);
-  const VerifyState st = a.state[b];
-  const int row = first + st.count - 1;
-  const RowTotal t{st.sum, st.most, st.where};
-  const float u = a.uniforms[2 * (int64_t)row + 1];
   int token = t.where;
-  if (!greedy) {
-    double whole = 0.0;
-    const double* const rest = a.rest + (int64_t)b * a.pieces;
-    if (st.rest) {
-      for (int i = lane; i < a.pieces; i += kWave) whole += rest[i];
-      whole = sum_of_wave(whole);
-    }
-    if (whole > 0.0) {
-      const void* const src = row_of<RT, PROBS>(a, row);
-      const float* const q = a.draft + (int64_t)(row + 1) * a.draft_stride;
-      token = draw(a, whole, u, lane, [&](int i) { return rest[i]; },
-                   [&](int i, double (&w)[8]) {
-                     float x[8], y[8];
-                     load_eight<RT, PROBS>(src, min(i, a.vocab), a.vocab, x);
-                     load_eight<TRI_REAL_FP32, true>(q, min(i, a.vocab), a.vocab, y);
-#pragma unroll
-                     for (int e = 0; e < 8; ++e)
-                       w[e] = fmax((PROBS ? (double)x[e] : weight_of(x[e], t.most, c)) / t.sum - (double)y[e], 0.0);
-                   });
-    } else {
-      token = draw_from_row<RT, PROBS>(a, row, t, c, u, lane);
-    }
+  if (!greedy && n > 0) {
+    const float u = a.uniforms[2 * (int64_t)row + 1];
+    const bool left = whole > 0.0;       // (or rounding left nothing)
+    const VerifyPart* const part = a.part + (int64_t)row * a.pieces;
+    const double per_sum = left ? 1.0 / t.sum : 1.0;
+    token = draw(a, left ? whole : t.sum, u, lane, [&](int piece) { return left ? rest[piece] : against<PROBS>(powers, part[piece], t.most, c); },
+                 [&](int piece) { return load_rest<RT, N>(a, src, left ? q : nullptr, piece, lane); },
+                 [&](const Rest<RT>& held, int s, double (&w)[8]) { rest_of<RT, PROBS>(powers, held, s, t.most, per_sum, c, w); });
   }
-  write_path(a, b, lane, lane, st.count, token);
+  write_path(a, b, lane, lane, count, token);
 }
 
 // Rows [first new token + rows[j]] to [first new token + j], j = 1 .. count - 1, of one side of one layer.  Lists ascend, so rows[j] >= j:
@@ -501,15 +679,14 @@ __global__ __launch_bounds__(kVerifyThreads) void accept_rows_kernel(AcceptLaunc
 
 template <int RT, bool PROBS>
 hipError_t verify_of(const VerifyLaunch& a, hipStream_t s) {
-  if (a.num_rows > 0)
-    hipLaunchKernelGGL((verify_sums_kernel<RT, PROBS>), dim3((unsigned)ceil_div64((int64_t)a.num_rows * a.pieces, kVerifyWaves)),
-                       dim3(kVerifyThreads), 0, s, a);
+  const int64_t units = std::max<int64_t>((int64_t)a.num_rows * a.pieces, 1);
+  hipLaunchKernelGGL((verify_sums_kernel<RT, PROBS>), dim3((unsigned)ceil_div64(units, kVerifyWaves)), dim3(kVerifyThreads), 0, s, a);
   if (!a.draft) {
-    hipLaunchKernelGGL((verify_walk_kernel<RT, PROBS>), dim3(a.B), dim3(kWalkThreads), 0, s, a);
+    const int groups = ceil_div(a.max_rows, kVerifyWaves);
+    hipLaunchKernelGGL((verify_walk_kernel<RT, PROBS>), dim3((unsigned)(a.B * groups)), dim3(kVerifyThreads), 0, s, a, groups);
   } else {
-    const int groups = ceil_div(a.pieces, kVerifyWaves);
-    hipLaunchKernelGGL((verify_chain_kernel<RT, PROBS>), dim3((unsigned)(a.B * groups)), dim3(kVerifyThreads), 0, s, a, groups);
-    hipLaunchKernelGGL((verify_draw_kernel<RT, PROBS>), dim3(a.B), dim3(kWave), 0, s, a);
+    const int groups = ceil_div(a.pieces, kChainWaves);
+    hipLaunchKernelGGL((verify_chain_kernel<RT, PROBS>), dim3((unsigned)(a.B * groups)), dim3(kChainThreads), 0, s, a, groups);
   }
   return hipGetLastError();
 }

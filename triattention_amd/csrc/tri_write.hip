@@ -19,10 +19,11 @@ namespace {
 
 constexpr int kWriteThreads = 256;
 constexpr int kWriteWaves = kWriteThreads / kWave;
-constexpr int kStepsAtOnce = 4;            // steps of a wave asked for together
+constexpr int kStepsAtOnce = 2;            // steps of a wave asked for together
 typedef __attribute__((address_space(1))) char* GlobalOut;
 typedef __attribute__((address_space(1))) u32x2* GlobalOutU2;
 typedef __attribute__((address_space(1))) uint32_t* GlobalOutU1;
+typedef __attribute__((address_space(1))) u32x4* GlobalOutU4;
 typedef __attribute__((address_space(1))) float* GlobalOutF32;
 enum CacheKind { kPlainRows = 0, kTensorScale = 1, kRowScales = 2 };
 
@@ -87,162 +88,257 @@ __device__ __forceinline__ uint32_t pack_codes(const float* x, float inv) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
 }
 
-// A wave's step is 64 / (D / 8) heads of one kind (queries, keys or values) of a row, eight elements a lane: those whose pairs lie in
-// the lane (4l to 4l + 3 and the same behind the head's middle, or 8l to 8l + 7), so that the rotation needs no other lane, and a lane
-// has the same four angles in every head.  A row's steps are shared by waves_per_row waves, which find the angles once each.
-template <int D, int QT, int KIND>
-__global__ __launch_bounds__(kWriteThreads) void write_paged_kernel(WriteLaunch a) {
+// A wave's step is 64 / (D / 8) heads of one kind (queries, keys or values) of a row, eight elements a lane: four pairs of the rotation (4l to
+// 4l + 3 and the same behind the head's middle, or 8l to 8l + 7), so that it needs no other lane, and a lane has the same four
+// angles in every head.  A row's steps are shared by waves_per_row waves, which find the angles once each.  Norm and rotation
+// are a product by (w1 cos, w2 sin, w2 cos, w1 sin), the same in every head, and one by the head's 1 / sqrt(mean).
+template <int D, int QT, int KIND, bool HALF>
+__global__ __launch_bounds__(kWriteThreads, 6) void write_paged_kernel(WriteLaunch a) {
   constexpr int LPH = D / 8, HPW = kWave / LPH;
-  const int lane = threadIdx.x % kWave, l = lane % LPH, sub = lane / LPH;
+  // elements of a head that are this lane's: first to first + 3 and first + apart to first + apart + 3
+  constexpr int apart = HALF ? D / 2 : 4;
+  const int lane = threadIdx.x % kWave, l = lane % LPH, sub = lane / LPH, first = HALF ? 4 * l : 8 * l;
   const int unit = blockIdx.x * kWriteWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int row = unit / a.waves_per_row, part = unit % a.waves_per_row;
+  const int row = unit / a.waves_per_row, part = unit % a.waves_per_row, W = a.waves_per_row;
   if (row >= a.num_rows) return;
-  int b = row;
-  if (a.row_starts) {
-    b = __builtin_amdgcn_readfirstlane(sequence_of_row(a.row_starts, a.B, row, lane));
-    if (b < 0) return;
-  }
-  const int q_steps = ceil_div(a.Hq, HPW), kv_steps = ceil_div(a.Hkv, HPW), steps = q_steps + 2 * kv_steps;
-  // elements of a head that are this lane's: first to first + 3 and second to second + 3
-  const bool half = a.rope_style == TRI_ROPE_HALF;
-  const int first = half ? 4 * l : 8 * l, second = half ? D / 2 + 4 * l : 8 * l + 4;
+  const int q_steps = ceil_div(a.Hq, HPW), kv_steps = ceil_div(a.Hkv, HPW);
+  // this wave's first step of each kind; the steps of a row are dealt out one behind the other
+  const int q_from = part, k_from = (part - q_steps % W + W) % W, v_from = (part - (q_steps + kv_steps) % W + W) % W;
 
-  float cs[4], sn[4];
-  if (part < q_steps + kv_steps) {
+  // kStepsAtOnce steps from `from` on
+  struct Source {
+    GlobalBytes row;
+    int64_t step;          // bytes from a step to the next
+    uint32_t lane;         // of this lane
+    int heads;
+  };
+  auto source = [&](const void* x, int64_t stride_row, int64_t stride_head, int heads) {
+    return Source{(GlobalBytes)(uintptr_t)x + row * stride_row * 2, HPW * stride_head * 2, (uint32_t)(sub * (int)stride_head + first) * 2, heads};
+  };
+  auto load = [&](const Source& x, int from, u32x2 (&raw)[kStepsAtOnce][2]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int f = 4 * l + e;
+    for (int u = 0; u < kStepsAtOnce; ++u) {
+      const int s = from + u * W;
+      raw[u][0] = raw[u][1] = u32x2{0, 0};
+      if (s * HPW + sub < x.heads) {
+        const GlobalBytes at = x.row + s * x.step;
+        if (a.stream_rows) {
+          raw[u][0] = __builtin_nontemporal_load((GlobalU2)(at + x.lane));
+          raw[u][1] = __builtin_nontemporal_load((GlobalU2)(at + (x.lane + apart * 2)));
+        } else {
+          raw[u][0] = *(GlobalU2)(at + x.lane);
+          raw[u][1] = *(GlobalU2)(at + (x.lane + apart * 2));
+        }
+      }
+    }
+  };
+  const Source q = source(a.q, a.q_stride_row, a.q_stride_head, a.Hq), k = source(a.k, a.k_stride_row, a.k_stride_head, a.Hkv),
+               v = source(a.v, a.v_stride_row, a.v_stride_head, a.Hkv);
+  u32x2 now[kStepsAtOnce][2], next[kStepsAtOnce][2];
+  load(q, q_from, now);
+
+  auto load_norm = [&](const void* norm, float (&w)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = e < 4 ? first + e : first + apart + e - 4;
+      w[e] = !norm ? 1.f : a.norm_fp32 ? reinterpret_cast<const float*>(norm)[d] : elem_lo<QT>(reinterpret_cast<const uint16_t*>(norm)[d]);
+    }
+  };
+  float qw[8], kw[8], cs[4], sn[4];
+  load_norm(a.q_norm, qw);
+  load_norm(a.k_norm, kw);
+  // the angles of all D / 2 frequencies, each found by one lane (two, of 256 dimensions), then handed to the lanes that use them
+  {
+    constexpr int own = D == 256 ? 2 : 1;
+    float c[own], s[own];
+#pragma unroll
+    for (int i = 0; i < own; ++i) {
+      const int f = (lane * own + i) % (D / 2);
       int axis = a.freq_axes ? a.freq_axes[f] : 0;
       if (axis < 0 || axis >= a.num_axes) axis = 0;
       const int64_t at = axis * a.position_stride + row;
       const double position = a.positions_64 ? (double)reinterpret_cast<const int64_t*>(a.positions)[at]
                                              : (double)reinterpret_cast<const int32_t*>(a.positions)[at];
-      turn(position, a.inv_freq[f], a.rotary_scale, cs[e], sn[e]);
+      turn(position, a.inv_freq[f], a.rotary_scale, c[i], s[i]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      cs[e] = __shfl(c[e % own], (4 * l + e) / own);
+      sn[e] = __shfl(s[e % own], (4 * l + e) / own);
     }
   }
-  int page = -1, off = 0;
-  if (part + (steps - 1 - part) / a.waves_per_row * a.waves_per_row >= q_steps) {
-    const int t = token_of_row(a.row_starts, a.seq_lens, a.Tmax, b, row);
-    if (t >= 0) {
-      page = page_of_token(a.block_table, a.block_table_pitch, a.block_size, a.num_blocks, b, t);
-      off = t % a.block_size;
+  int b = row;
+  if (a.row_starts) {
+    b = __builtin_amdgcn_readfirstlane(sequence_of_row(a.row_starts, a.B, row, lane));
+    if (b < 0) return;
+  }
+
+  float by[4][4];
+  auto make_products = [&](const float (&w)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float w1 = HALF ? w[e] : w[2 * e], w2 = HALF ? w[4 + e] : w[2 * e + 1];
+      by[e][0] = w1 * cs[e];
+      by[e][1] = w2 * sn[e];
+      by[e][2] = w2 * cs[e];
+      by[e][3] = w1 * sn[e];
+    }
+  };
+  // four pairs of a head, normalised and rotated
+  auto turned = [&](const u32x2 (&raw)[2], bool norm, float (&x)[8]) {
+    float y[8] = {elem_lo<QT>(raw[0].x), elem_hi<QT>(raw[0].x), elem_lo<QT>(raw[0].y), elem_hi<QT>(raw[0].y),
+                  elem_lo<QT>(raw[1].x), elem_hi<QT>(raw[1].x), elem_lo<QT>(raw[1].y), elem_hi<QT>(raw[1].y)};
+    float inv = 1.f;
+    if (norm) {
+      float squares = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) squares += y[e] * y[e];
+      inv = rsqrtf(sum_of_head<LPH>(squares) * (1.f / D) + a.eps);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = HALF ? e : 2 * e, j = HALF ? 4 + e : 2 * e + 1;
+      x[i] = (y[i] * by[e][0] - y[j] * by[e][1]) * inv;
+      x[j] = (y[j] * by[e][2] + y[i] * by[e][3]) * inv;
+    }
+  };
+
+  make_products(qw);
+  {
+    const uint32_t out_lane = (sub * (int)a.out_stride_head + first) * 2;
+    const GlobalOut out = (GlobalOut)(uintptr_t)a.out + row * a.out_stride_row * 2;
+    const int64_t out_step = HPW * a.out_stride_head * 2;
+    for (int s0 = q_from; s0 < q_steps; s0 += kStepsAtOnce * W) {
+      const bool more = s0 + kStepsAtOnce * W < q_steps;
+      if (more) load(q, s0 + kStepsAtOnce * W, next);
+#pragma unroll
+      for (int u = 0; u < kStepsAtOnce; ++u) {
+        const int s = s0 + u * W;
+        if (s >= q_steps) break;
+        float x[8];
+        turned(now[u], a.q_norm != nullptr, x);
+        if (s * HPW + sub < a.Hq) {
+          const GlobalOut dst = out + s * out_step;
+          *(GlobalOutU2)(dst + out_lane) = u32x2{pack_half<QT>(x[0], x[1]), pack_half<QT>(x[2], x[3])};
+          *(GlobalOutU2)(dst + (out_lane + apart * 2)) = u32x2{pack_half<QT>(x[4], x[5]), pack_half<QT>(x[6], x[7])};
+        }
+      }
+      if (more) {
+#pragma unroll
+        for (int u = 0; u < kStepsAtOnce; ++u) {
+          now[u][0] = next[u][0];
+          now[u][1] = next[u][1];
+        }
+      }
     }
   }
 
-  float w[8];
-  const void* have = nullptr;
-  for (int s0 = part; s0 < steps; s0 += kStepsAtOnce * a.waves_per_row) {
-    uint2 raw[kStepsAtOnce][2];
+  if (k_from >= kv_steps && v_from >= kv_steps) return;
+  const int t = __builtin_amdgcn_readfirstlane(token_of_row(a.row_starts, a.seq_lens, a.Tmax, b, row));
+  if (t < 0) return;
+  load(k, k_from, now);
+  load(v, v_from, next);
+  const int page = __builtin_amdgcn_readfirstlane(page_of_token(a.block_table, a.block_table_pitch, a.block_size, a.num_blocks, b, t));
+  if (page < 0) return;
+  const int off = t % a.block_size;
+  const int64_t row_at = (page * a.stride_block + off * a.stride_token) * (KIND == kPlainRows ? 2 : 1);
+  const int64_t beside = ((int64_t)page * a.block_size + off) * a.Hkv;
+  const uint32_t cache_lane = (sub * (int)a.stride_head + first) * (KIND == kPlainRows ? 2 : 1);
+  const int64_t cache_step = HPW * a.stride_head * (KIND == kPlainRows ? 2 : 1);
+  // a step of K or V into the cache
+  auto store = [&](int s, const float (&x)[8], GlobalOut rows, GlobalOutF32 scales, float inv) {
+    const GlobalOut dst = rows + s * cache_step;
+    if constexpr (KIND == kPlainRows) {
+      if (s * HPW + sub >= a.Hkv) return;
+      *(GlobalOutU2)(dst + cache_lane) = u32x2{pack_half<QT>(x[0], x[1]), pack_half<QT>(x[2], x[3])};
+      *(GlobalOutU2)(dst + (cache_lane + apart * 2)) = u32x2{pack_half<QT>(x[4], x[5]), pack_half<QT>(x[6], x[7])};
+    } else {
+      float scale = 0.f;
+      if constexpr (KIND == kRowScales) {
+        // of the finite elements: an infinity or NaN is a NaN in its place and leaves the others as they are
+        float most = 0.f;
 #pragma unroll
-    for (int u = 0; u < kStepsAtOnce; ++u) {
-      const int s = s0 + u * a.waves_per_row;
-      const int kind = s < q_steps ? 0 : s < q_steps + kv_steps ? 1 : 2;
-      const int h = (s - (kind == 0 ? 0 : kind == 1 ? q_steps : q_steps + kv_steps)) * HPW + sub;
-      raw[u][0] = raw[u][1] = uint2{0, 0};
-      if (s < steps && h < (kind == 0 ? a.Hq : a.Hkv)) {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
-                              row * (kind == 0 ? a.q_stride_row : kind == 1 ? a.k_stride_row : a.v_stride_row) +
-                              h * (kind == 0 ? a.q_stride_head : kind == 1 ? a.k_stride_head : a.v_stride_head);
-        raw[u][0] = *reinterpret_cast<const uint2*>(src + first);
-        raw[u][1] = *reinterpret_cast<const uint2*>(src + second);
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, is_number(x[e]) ? fabsf(x[e]) : 0.f);
+        scale = fmaxf(max_of_head<LPH>(most) / 448.f, FLT_MIN);
+        inv = 1.f / scale;
+      }
+      if (s * HPW + sub >= a.Hkv) return;
+      *(GlobalOutU1)(dst + cache_lane) = pack_codes(x, inv);
+      *(GlobalOutU1)(dst + (cache_lane + apart)) = pack_codes(x + 4, inv);
+      if constexpr (KIND == kRowScales)
+        if (l == 0) scales[s * HPW + sub] = scale;
+    }
+  };
+  make_products(kw);
+  {
+    const GlobalOut rows = (GlobalOut)(uintptr_t)a.k_layers[a.layer] + row_at;
+    const GlobalOutF32 scales = KIND == kRowScales ? (GlobalOutF32)(uintptr_t)a.k_scale_layers[a.layer] + beside : nullptr;
+    for (int s0 = k_from; s0 < kv_steps; s0 += kStepsAtOnce * W) {
+      if (s0 != k_from) load(k, s0, now);
+#pragma unroll
+      for (int u = 0; u < kStepsAtOnce; ++u) {
+        const int s = s0 + u * W;
+        if (s >= kv_steps) break;
+        float x[8];
+        turned(now[u], a.k_norm != nullptr, x);
+        store(s, x, rows, scales, a.k_inv_scale);
       }
     }
+  }
+  const GlobalOut rows = (GlobalOut)(uintptr_t)a.v_layers[a.layer] + row_at;
+  const GlobalOutF32 scales = KIND == kRowScales ? (GlobalOutF32)(uintptr_t)a.v_scale_layers[a.layer] + beside : nullptr;
+  for (int s0 = v_from; s0 < kv_steps; s0 += kStepsAtOnce * W) {
+    if (s0 != v_from) load(v, s0, next);
 #pragma unroll
     for (int u = 0; u < kStepsAtOnce; ++u) {
-      const int s = s0 + u * a.waves_per_row;
-      if (s >= steps) break;
-      const int kind = s < q_steps ? 0 : s < q_steps + kv_steps ? 1 : 2;
-      const int h = (s - (kind == 0 ? 0 : kind == 1 ? q_steps : q_steps + kv_steps)) * HPW + sub;
-      const bool mine = h < (kind == 0 ? a.Hq : a.Hkv);
-      const uint32_t word[4] = {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y};
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = elem_lo<QT>(word[e]);
-        x[2 * e + 1] = elem_hi<QT>(word[e]);
-      }
-      if (kind != 2) {
-        const void* norm = kind == 0 ? a.q_norm : a.k_norm;
-        if (norm) {
-          if (norm != have) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int d = e < 4 ? first + e : second + e - 4;
-              if (a.norm_fp32) w[e] = reinterpret_cast<const float*>(norm)[d];
-              else w[e] = elem_lo<QT>(reinterpret_cast<const uint16_t*>(norm)[d]);
-            }
-            have = norm;
-          }
-          float squares = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) squares += x[e] * x[e];
-          const float inv = rsqrtf(sum_of_head<LPH>(squares) * (1.f / D) + a.eps);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
-        }
-        if (half) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = x[e], z = x[4 + e];
-            x[e] = y * cs[e] - z * sn[e];
-            x[4 + e] = z * cs[e] + y * sn[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y = x[2 * e], z = x[2 * e + 1];
-            x[2 * e] = y * cs[e] - z * sn[e];
-            x[2 * e + 1] = z * cs[e] + y * sn[e];
-          }
-        }
-      }
-      if (kind == 0) {
-        if (!mine) continue;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + row * a.out_stride_row + h * a.out_stride_head;
-        *reinterpret_cast<uint2*>(dst + first) = uint2{pack_half<QT>(x[0], x[1]), pack_half<QT>(x[2], x[3])};
-        *reinterpret_cast<uint2*>(dst + second) = uint2{pack_half<QT>(x[4], x[5]), pack_half<QT>(x[6], x[7])};
-        continue;
-      }
-      if (page < 0) continue;
-      const GlobalOut base = (GlobalOut)(uintptr_t)(kind == 1 ? a.k_layers : a.v_layers)[a.layer];
-      const int64_t at = (int64_t)page * a.stride_block + off * a.stride_token + h * a.stride_head;
+      const int s = s0 + u * W;
+      if (s >= kv_steps) break;
+      const u32x2 (&raw)[2] = next[u];
       if constexpr (KIND == kPlainRows) {
-        if (!mine) continue;
-        *(GlobalOutU2)(base + (at + first) * 2) = u32x2{pack_half<QT>(x[0], x[1]), pack_half<QT>(x[2], x[3])};
-        *(GlobalOutU2)(base + (at + second) * 2) = u32x2{pack_half<QT>(x[4], x[5]), pack_half<QT>(x[6], x[7])};
+        if (s * HPW + sub >= a.Hkv) continue;
+        const GlobalOut dst = rows + s * cache_step;
+        *(GlobalOutU2)(dst + cache_lane) = raw[0];
+        *(GlobalOutU2)(dst + (cache_lane + apart * 2)) = raw[1];
       } else {
-        float inv = kind == 1 ? a.k_inv_scale : a.v_inv_scale;
-        float scale = 0.f;
-        if constexpr (KIND == kRowScales) {
-          // of the finite elements: an infinity or NaN is a NaN in its place and leaves the others as they are
-          float most = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) most = fmaxf(most, is_number(x[e]) ? fabsf(x[e]) : 0.f);
-          scale = fmaxf(max_of_head<LPH>(most) / 448.f, FLT_MIN);
-          inv = 1.f / scale;
-        }
-        if (!mine) continue;
-        *(GlobalOutU1)(base + at + first) = pack_codes(x, inv);
-        *(GlobalOutU1)(base + at + second) = pack_codes(x + 4, inv);
-        if constexpr (KIND == kRowScales)
-          if (l == 0)
-            *((GlobalOutF32)(uintptr_t)(kind == 1 ? a.k_scale_layers : a.v_scale_layers)[a.layer] + ((int64_t)page * a.block_size + off) * a.Hkv + h) = scale;
+        const float x[8] = {elem_lo<QT>(raw[0].x), elem_hi<QT>(raw[0].x), elem_lo<QT>(raw[0].y), elem_hi<QT>(raw[0].y),
+                            elem_lo<QT>(raw[1].x), elem_hi<QT>(raw[1].x), elem_lo<QT>(raw[1].y), elem_hi<QT>(raw[1].y)};
+        store(s, x, rows, scales, a.v_inv_scale);
       }
     }
   }
 }
 
-// A wave takes rows_per_wave rows one behind the other; their places are found a row a lane.  Lanes are pieces of eight elements
-// of the row's K, then of its V.
-constexpr int kReadAtOnce = 8;             // pieces of a lane asked for together
+// A wave takes rows_per_wave rows; their places are found a row a lane.  Lanes are pieces of 16 bytes of a row's K and V alike (of several
+// rows, where a row has fewer than 64), four rows' of both asked for at a time.
+constexpr int kRowsAtOnce = 2;
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(GlobalBytes at, uint32_t (&x)[WORDS]) {
+  if constexpr (WORDS == 4) {
+    const u32x4 w = *(GlobalU4)at;
+    x[0] = w.x; x[1] = w.y; x[2] = w.z; x[3] = w.w;
+  } else if constexpr (WORDS == 2) {
+    const u32x2 w = *(GlobalU2)at;
+    x[0] = w.x; x[1] = w.y;
+  } else {
+    x[0] = *(const __attribute__((address_space(1))) uint32_t*)at;
+  }
+}
 
 template <int CT, int OT>
 __global__ __launch_bounds__(kWriteThreads) void read_paged_kernel(ReadLaunch a) {
+  constexpr int EPL = OT == TRI_REAL_FP32 ? 4 : 8, ES = elem_size<CT>(), words = EPL * ES / 4;
   const int lane = threadIdx.x % kWave;
   const int64_t r0 = ((int64_t)blockIdx.x * kWriteWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * a.rows_per_wave;
   if (r0 >= a.num_rows) return;
   const int rows = (int)min((int64_t)a.rows_per_wave, a.num_rows - r0);
-  // lane i has row i's place: slot >= 0, -1 for a row without a cached token (zeros), -2 for one that no sequence has
+  const GlobalBytes k = (GlobalBytes)(uintptr_t)a.k_layers[a.layer], v = (GlobalBytes)(uintptr_t)a.v_layers[a.layer];
+  GlobalF32 ks = nullptr, vs = nullptr;
+  if (a.k_scale_layers) {
+    ks = (GlobalF32)(uintptr_t)a.k_scale_layers[a.layer];
+    vs = (GlobalF32)(uintptr_t)a.v_scale_layers[a.layer];
+  }
+  // lane i has row i's place: a page, -1 for a row without a cached token (zeros), -2 for one that no sequence has
   int page = -2, off = 0;
   if (lane < rows) {
     const int row = (int)r0 + lane;
@@ -258,81 +354,83 @@ __global__ __launch_bounds__(kWriteThreads) void read_paged_kernel(ReadLaunch a)
       off = t < 0 ? 0 : t % a.block_size;
     }
   }
-  const int shift = a.D == 64 ? 3 : a.D == 128 ? 4 : 5, pieces = a.Hkv << shift, per_row = ceil_div(2 * pieces, kWave);
-  const int total = rows * per_row;
-  for (int i0 = 0; i0 < total; i0 += kReadAtOnce) {
-    uint4 raw[kReadAtOnce];
-    float scale[kReadAtOnce];
+  const int shift = 31 - __clz(a.D / EPL), pieces = a.Hkv << shift;
+  // lanes of a row: all 64, or the power of two that holds its pieces
+  const int width = pieces >= kWave ? kWave : 1 << (32 - __clz(pieces - 1)), together = kWave / width, own = lane / width;
+  for (int p0 = 0; p0 < pieces; p0 += width) {
+    const int piece = p0 + lane % width, h = piece >> shift;
+    const int64_t head_at = h * a.stride_head + (piece & ((1 << shift) - 1)) * EPL;
+    for (int i0 = 0; i0 < rows; i0 += kRowsAtOnce * together) {
+      uint32_t x[kRowsAtOnce][2][words];
+      float scale[kRowsAtOnce][2];
+      int pg[kRowsAtOnce];
 #pragma unroll
-    for (int u = 0; u < kReadAtOnce; ++u) {
-      const int i = min(i0 + u, total - 1), r = i / per_row, item = (i - r * per_row) * kWave + lane;
-      const bool v = item >= pieces;
-      const int piece = v ? item - pieces : item, h = piece >> shift, d = (piece & ((1 << shift) - 1)) * 8;
-      const int p = __builtin_amdgcn_readlane(page, r), o = __builtin_amdgcn_readlane(off, r);
-      raw[u] = uint4{0, 0, 0, 0};
-      scale[u] = 0.f;
-      if (p >= 0 && item < 2 * pieces) {
-        const int64_t at = (int64_t)p * a.stride_block + o * a.stride_token + h * a.stride_head + d;
-        const GlobalBytes base = (GlobalBytes)(uintptr_t)(v ? a.v_layers : a.k_layers)[a.layer];
-        scale[u] = v ? a.v_scale : a.k_scale;
-        if constexpr (CT == TRI_KV_FP8_E4M3) {
-          const u32x2 x = *(GlobalU2)(base + at);
-          raw[u] = uint4{x.x, x.y, 0, 0};
-          if (a.k_scale_layers)
-            scale[u] *= *((GlobalF32)(uintptr_t)(v ? a.v_scale_layers : a.k_scale_layers)[a.layer] + ((int64_t)p * a.block_size + o) * a.Hkv + h);
-        } else {
-          const u32x4 x = *(GlobalU4)(base + at * 2);
-          raw[u] = uint4{x.x, x.y, x.z, x.w};
-        }
-      }
-    }
+      for (int u = 0; u < kRowsAtOnce; ++u) {
+        const int r = i0 + u * together + own;
+        const int o = __shfl(off, min(r, kWave - 1));
+        pg[u] = __shfl(page, min(r, kWave - 1));
+        if (r >= rows || piece >= pieces) pg[u] = -2;
 #pragma unroll
-    for (int u = 0; u < kReadAtOnce; ++u) {
-      const int i = i0 + u;
-      if (i >= total) break;
-      const int r = i / per_row, item = (i - r * per_row) * kWave + lane;
-      const bool v = item >= pieces;
-      const int piece = v ? item - pieces : item;
-      if (__builtin_amdgcn_readlane(page, r) == -2 || item >= 2 * pieces) continue;
-      float x[8];
-      if constexpr (CT == TRI_KV_FP8_E4M3) {
-        x[0] = fp8_byte<0>(raw[u].x); x[1] = fp8_byte<1>(raw[u].x); x[2] = fp8_byte<2>(raw[u].x); x[3] = fp8_byte<3>(raw[u].x);
-        x[4] = fp8_byte<0>(raw[u].y); x[5] = fp8_byte<1>(raw[u].y); x[6] = fp8_byte<2>(raw[u].y); x[7] = fp8_byte<3>(raw[u].y);
-      } else {
-        const uint32_t word[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = elem_lo<CT>(word[e]);
-          x[2 * e + 1] = elem_hi<CT>(word[e]);
+        for (int i = 0; i < words; ++i) x[u][0][i] = x[u][1][i] = 0;
+        scale[u][0] = scale[u][1] = 0.f;
+        if (pg[u] >= 0) {
+          const int64_t at = (pg[u] * a.stride_block + o * a.stride_token + head_at) * ES;
+          load_words<words>(k + at, x[u][0]);
+          load_words<words>(v + at, x[u][1]);
+          if constexpr (CT == TRI_KV_FP8_E4M3)
+            if (a.k_scale_layers) {
+              const int64_t slot = ((int64_t)pg[u] * a.block_size + o) * a.Hkv + h;
+              scale[u][0] = ks[slot];
+              scale[u][1] = vs[slot];
+            }
         }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] *= scale[u];
-      const int64_t to = ((r0 + r) * pieces + piece) * 8;
-      void* const out = v ? a.v_out : a.k_out;
-      if constexpr (OT == TRI_REAL_FP32) {
-        float4* dst = reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + to);
-        dst[0] = float4{x[0], x[1], x[2], x[3]};
-        dst[1] = float4{x[4], x[5], x[6], x[7]};
-      } else {
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(out) + to) =
-            uint4{pack_half<OT>(x[0], x[1]), pack_half<OT>(x[2], x[3]), pack_half<OT>(x[4], x[5]), pack_half<OT>(x[6], x[7])};
+      for (int u = 0; u < kRowsAtOnce; ++u) {
+        if (pg[u] == -2) continue;
+        const int64_t to = ((r0 + i0 + u * together + own) * pieces + piece) * EPL;
+#pragma unroll
+        for (int side = 0; side < 2; ++side) {
+          float f = side ? a.v_scale : a.k_scale;
+          if constexpr (CT == TRI_KV_FP8_E4M3)
+            if (a.k_scale_layers) f *= scale[u][side];
+          float y[EPL];
+#pragma unroll
+          for (int i = 0; i < words; ++i) {
+            const uint32_t word = x[u][side][i];
+            if constexpr (CT == TRI_KV_FP8_E4M3) {
+              y[4 * i] = fp8_byte<0>(word) * f;
+              y[4 * i + 1] = fp8_byte<1>(word) * f;
+              y[4 * i + 2] = fp8_byte<2>(word) * f;
+              y[4 * i + 3] = fp8_byte<3>(word) * f;
+            } else {
+              y[2 * i] = elem_lo<CT>(word) * f;
+              y[2 * i + 1] = elem_hi<CT>(word) * f;
+            }
+          }
+          const GlobalOut out = (GlobalOut)(uintptr_t)(side ? a.v_out : a.k_out) + to * (OT == TRI_REAL_FP32 ? 4 : 2);
+          if constexpr (OT == TRI_REAL_FP32)
+            __builtin_nontemporal_store(u32x4{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])}, (GlobalOutU4)out);
+          else
+            __builtin_nontemporal_store(u32x4{pack_half<OT>(y[0], y[1]), pack_half<OT>(y[2], y[3]), pack_half<OT>(y[4], y[5]), pack_half<OT>(y[6], y[7])}, (GlobalOutU4)out);
+        }
       }
     }
   }
 }
 
-template <int D, int QT>
+template <int D, int QT, bool HALF>
 void write_of_kind(const WriteLaunch& a, hipStream_t s) {
   const dim3 grid((unsigned)ceil_div64((int64_t)a.num_rows * a.waves_per_row, kWriteWaves));
-  if (a.kv_dtype != TRI_KV_FP8_E4M3) hipLaunchKernelGGL((write_paged_kernel<D, QT, kPlainRows>), grid, dim3(kWriteThreads), 0, s, a);
-  else if (!a.k_scale_layers) hipLaunchKernelGGL((write_paged_kernel<D, QT, kTensorScale>), grid, dim3(kWriteThreads), 0, s, a);
-  else hipLaunchKernelGGL((write_paged_kernel<D, QT, kRowScales>), grid, dim3(kWriteThreads), 0, s, a);
+  if (a.kv_dtype != TRI_KV_FP8_E4M3) hipLaunchKernelGGL((write_paged_kernel<D, QT, kPlainRows, HALF>), grid, dim3(kWriteThreads), 0, s, a);
+  else if (!a.k_scale_layers) hipLaunchKernelGGL((write_paged_kernel<D, QT, kTensorScale, HALF>), grid, dim3(kWriteThreads), 0, s, a);
+  else hipLaunchKernelGGL((write_paged_kernel<D, QT, kRowScales, HALF>), grid, dim3(kWriteThreads), 0, s, a);
 }
 template <int D>
 void write_of_type(const WriteLaunch& a, hipStream_t s) {
-  if (a.q_dtype == TRI_KV_FP16) write_of_kind<D, TRI_KV_FP16>(a, s);
-  else write_of_kind<D, TRI_KV_BF16>(a, s);
+  const bool half = a.rope_style == TRI_ROPE_HALF;
+  if (a.q_dtype == TRI_KV_FP16) half ? write_of_kind<D, TRI_KV_FP16, true>(a, s) : write_of_kind<D, TRI_KV_FP16, false>(a, s);
+  else half ? write_of_kind<D, TRI_KV_BF16, true>(a, s) : write_of_kind<D, TRI_KV_BF16, false>(a, s);
 }
 template <int CT>
 void read_to_type(const ReadLaunch& a, hipStream_t s) {
@@ -346,8 +444,8 @@ void read_to_type(const ReadLaunch& a, hipStream_t s) {
 
 hipError_t launch_write_paged(WriteLaunch a, hipStream_t s) {
   const int heads = kWave / (a.D / 8), steps = ceil_div(a.Hq, heads) + 2 * ceil_div(a.Hkv, heads);
-  // As many waves a row as fill the chip, down to a step each.
-  a.waves_per_row = (int)std::min<int64_t>(steps, std::max<int64_t>(1, 8192 / a.num_rows));
+  a.waves_per_row = (int)std::min<int64_t>(steps, std::max<int64_t>(1, 2048 / a.num_rows));
+  a.stream_rows = (int64_t)a.num_rows * (a.Hq + 2 * a.Hkv) * a.D * 2 > (128ll << 20);
   if (a.D == 64) write_of_type<64>(a, s);
   else if (a.D == 128) write_of_type<128>(a, s);
   else write_of_type<256>(a, s);
@@ -355,7 +453,10 @@ hipError_t launch_write_paged(WriteLaunch a, hipStream_t s) {
 }
 
 hipError_t launch_read_paged(ReadLaunch a, hipStream_t s) {
-  a.rows_per_wave = (int)std::min<int64_t>(8, std::max<int64_t>(1, a.num_rows / 8192));
+  const int pieces = a.Hkv * (a.D / (a.out_dtype == TRI_REAL_FP32 ? 4 : 8));
+  int together = 1;
+  while (together < kWave && 2 * together * pieces <= kWave) together *= 2;
+  a.rows_per_wave = together * (a.num_rows >= 8192 * together ? kRowsAtOnce : 1);
   if (a.kv_dtype == TRI_KV_FP8_E4M3) read_to_type<TRI_KV_FP8_E4M3>(a, s);
   else if (a.kv_dtype == TRI_KV_FP16) read_to_type<TRI_KV_FP16>(a, s);
   else read_to_type<TRI_KV_BF16>(a, s);

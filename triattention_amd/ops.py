@@ -967,18 +967,32 @@ def evict_step(kv: PagedKV, batch: StepBatch, weights: torch.Tensor, ev: EvictCo
     return keep
 
 
-def _check_rows(kv: PagedKV, name: str, t: torch.Tensor, dtype, heads: int | None, rows: int | None):
+_write_params, _read_params = _lib.packer(WriteParams), _lib.packer(ReadParams)
+_verify_params, _accept_params = _lib.packer(VerifyParams), _lib.packer(AcceptParams)
+
+
+def _call(device: torch.device, fn, *args) -> None:
+    """A call of the library on the current stream of a device."""
+    now = torch._C._cuda_getDevice()
+    if device.index == now or device.index is None:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(now))
+    else:
+        with _on_device(device):
+            code = fn(*args, _stream())
+    if code:
+        _lib.check(code)
+
+
+def _check_rows(kv: PagedKV, name: str, t: torch.Tensor, dtype, heads: int, rows: int):
     """Strides of a tensor of rows [rows, heads, head_dim] on the cache's device."""
-    shape, strides = t.shape, t.stride()
-    if (t.device != kv.device or t.dtype != dtype or len(shape) != 3 or shape[2] != kv.head_dim or strides[2] != 1
-            or (heads is not None and shape[1] != heads) or (rows is not None and shape[0] != rows)):
-        raise ValueError(f"{name} must be a {dtype} tensor [{'rows' if rows is None else rows}, {heads or 'heads'}, {kv.head_dim}] on {kv.device} "
-                         "with head_dim contiguous")
+    strides = t.stride()
+    if t.shape != (rows, heads, kv.head_dim) or t.dtype is not dtype or t.device != kv.device or strides[2] != 1:
+        raise ValueError(f"{name} must be a {dtype} tensor [{rows}, {heads}, {kv.head_dim}] on {kv.device} with head_dim contiguous")
     return strides
 
 
 def _check_vector(kv, name: str, t: torch.Tensor, dtype, shape: tuple) -> int:
-    if t.device != kv.device or t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+    if t.shape != shape or t.dtype is not dtype or t.device != kv.device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {kv.device}")
     return t.data_ptr()
 
@@ -1005,45 +1019,46 @@ def write_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, k: torch.Tensor,
 
     ``out`` may be ``q`` itself; otherwise it has no element in common with ``q``, ``k`` and ``v``.  Rows behind ``row_starts[-1]`` are left as they
     were.  A captured call may be replayed with everything on the device rewritten in place."""
-    lib = _lib.load()
     _check_attention_batch(kv, batch)
     if kv.v_ptrs is None:
         raise ValueError("write_paged needs the values of the cache")
-    dtype = q.dtype
-    if dtype not in (torch.bfloat16, torch.float16):
+    dtype, shape = q.dtype, q.shape
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or len(shape) != 3:
         raise ValueError(f"q must be a bf16 or fp16 tensor [rows, heads, {kv.head_dim}]")
-    qs = _check_rows(kv, "q", q, dtype, None, None)
-    rows, heads, dim = q.shape
+    rows, heads, dim = shape
+    qs = _check_rows(kv, "q", q, dtype, heads, rows)
     ks = _check_rows(kv, "k", k, dtype, kv.num_kv_heads, rows)
     vs = _check_rows(kv, "v", v, dtype, kv.num_kv_heads, rows)
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=dtype, device=kv.device)
-    os = _check_rows(kv, "out", out, dtype, heads, rows)
+        out = q.new_empty(shape)
+        os = out.stride()
+    else:
+        os = _check_rows(kv, "out", out, dtype, heads, rows)
     if not 0 <= layer < kv.num_layers:
         raise IndexError(f"layer {layer} of {kv.num_layers}")
-    axes = positions.shape[0] if positions.ndim == 2 else 1
-    if (positions.device != kv.device or positions.dtype not in (torch.int32, torch.int64) or positions.shape[-1:] != (rows,)
-            or positions.ndim > 2 or axes < 1 or (rows > 1 and positions.stride(-1) != 1)):
+    at, axes, apart = positions.shape, 1, 0
+    if len(at) == 2:
+        axes, apart = at[0], positions.stride(0)
+    wide = positions.dtype is torch.int64
+    if (not 1 <= len(at) <= 2 or at[-1] != rows or axes < 1 or not (wide or positions.dtype is torch.int32) or positions.device != kv.device
+            or (rows > 1 and positions.stride(-1) != 1)):
         raise ValueError(f"positions must be an int32 or int64 tensor [{rows}] or [axes, {rows}] on {kv.device}, the rows contiguous")
     if axes > 1 and freq_axes is None:
         raise ValueError("positions on several axes need freq_axes")
-    half = (dim // 2,)
+    half, full = (dim // 2,), (dim,)
     norm = k_norm if q_norm is None else q_norm
-    norm_fp32 = norm is not None and norm.dtype == torch.float32
+    norm_fp32 = norm is not None and norm.dtype is torch.float32
     kind = torch.float32 if norm_fp32 else dtype
-    if row_starts is not None:
-        _check_vector(kv, "row_starts", row_starts, torch.int32, (batch.num_seqs + 1,))
-    # (in the order of the fields: by name they cost some microseconds of a call whose kernel takes a few)
-    p = WriteParams(layer, heads, rows, kv.num_blocks, _DTYPES[dtype], axes, positions.dtype == torch.int64, norm_fp32,
-                    q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], out.data_ptr(), os[0], os[1],
-                    positions.data_ptr(), positions.stride(0) if axes > 1 else 0,
-                    None if freq_axes is None else _check_vector(kv, "freq_axes", freq_axes, torch.int32, half),
-                    _check_vector(kv, "inv_freq", inv_freq, torch.float32, half),
-                    None if q_norm is None else _check_vector(kv, "q_norm", q_norm, kind, (dim,)),
-                    None if k_norm is None else _check_vector(kv, "k_norm", k_norm, kind, (dim,)), _ptr(row_starts), eps, rotary_scale, k_scale,
-                    v_scale)
-    with _on_device(kv.device):
-        _lib.check(lib.tri_write_paged(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _stream()))
+    p = _write_params(layer, heads, rows, kv.num_blocks, _DTYPES[dtype], axes, wide, norm_fp32,
+                      q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], out.data_ptr(), os[0], os[1],
+                      positions.data_ptr(), apart,
+                      0 if freq_axes is None else _check_vector(kv, "freq_axes", freq_axes, torch.int32, half),
+                      _check_vector(kv, "inv_freq", inv_freq, torch.float32, half),
+                      0 if q_norm is None else _check_vector(kv, "q_norm", q_norm, kind, full),
+                      0 if k_norm is None else _check_vector(kv, "k_norm", k_norm, kind, full),
+                      0 if row_starts is None else _check_vector(kv, "row_starts", row_starts, torch.int32, (batch.num_seqs + 1,)),
+                      eps, rotary_scale, k_scale, v_scale)
+    _call(kv.device, _lib.load().tri_write_paged, C.byref(kv.struct), C.byref(batch.struct), p)
     return out
 
 
@@ -1055,7 +1070,6 @@ def read_paged(kv: PagedKV, batch: StepBatch, row_starts: torch.Tensor, num_rows
     Sequence b has the rows ``row_starts[b]`` to ``row_starts[b + 1] - 1`` (int32 [sequences + 1] on the device, ascending): the running
     sum of the lengths reads everything.  ``dtype`` bf16, fp16 or fp32 (None: the cache's; fp8: bf16).  Rows of tokens
     that the cache does not have are zeros; rows behind ``row_starts[-1]`` are left as they were.  ``out``: contiguous tensors for K and V."""
-    lib = _lib.load()
     _check_attention_batch(kv, batch)
     if kv.v_ptrs is None:
         raise ValueError("read_paged needs the values of the cache")
@@ -1071,12 +1085,13 @@ def read_paged(kv: PagedKV, batch: StepBatch, row_starts: torch.Tensor, num_rows
         raise TypeError(f"rows are read as bf16, fp16 or fp32, not {dtype}")
     shape = (num_rows, kv.num_kv_heads, kv.head_dim)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=kv.device), torch.empty(shape, dtype=dtype, device=kv.device)
-    k_out, v_out = out
-    p = ReadParams(layer, num_rows, kv.num_blocks, _REALS[dtype], _check_vector(kv, "row_starts", row_starts, torch.int32, (batch.num_seqs + 1,)),
-                   _check_vector(kv, "out[0]", k_out, dtype, shape), _check_vector(kv, "out[1]", v_out, dtype, shape), k_scale, v_scale)
-    with _on_device(kv.device):
-        _lib.check(lib.tri_read_paged(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _stream()))
+        k_out = torch.empty(shape, dtype=dtype, device=kv.device)
+        v_out = torch.empty_like(k_out)
+    else:
+        k_out, v_out = out
+    p = _read_params(layer, num_rows, kv.num_blocks, _REALS[dtype], _check_vector(kv, "row_starts", row_starts, torch.int32, (batch.num_seqs + 1,)),
+                     _check_vector(kv, "out[0]", k_out, dtype, shape), _check_vector(kv, "out[1]", v_out, dtype, shape), k_scale, v_scale)
+    _call(kv.device, _lib.load().tri_read_paged, C.byref(kv.struct), C.byref(batch.struct), p)
     return k_out, v_out
 
 
@@ -1101,39 +1116,41 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, row_starts: torch.
     lib = _lib.load()
     if not target.is_cuda:
         raise RuntimeError("verify_drafts needs device tensors (there is no CPU fallback)")
-    if target.ndim != 2 or target.dtype not in _REALS or (target.shape[1] > 1 and target.stride(1) != 1):
+    shape, dtype = target.shape, target.dtype
+    if len(shape) != 2 or dtype not in _REALS or (shape[1] > 1 and target.stride(1) != 1):
         raise ValueError("target must be a bf16, fp16 or fp32 tensor [rows, vocab], the vocabulary contiguous")
-    if probs and target.dtype != torch.float32:
+    if probs and dtype is not torch.float32:
         raise ValueError("probabilities must be fp32")
-    rows, vocab = target.shape
-    if row_starts.ndim != 1 or row_starts.shape[0] < 2:
+    rows, vocab = shape
+    seqs = row_starts.numel() - 1
+    if seqs < 1:
         raise ValueError("row_starts must have an entry for every sequence and one behind the last")
-    seqs = row_starts.shape[0] - 1
     if max_rows is None:
         max_rows = min(max(rows, 1), 64)
     elif not 1 <= max_rows <= 64:
         raise ValueError(f"max_rows must be 1 to 64, got {max_rows}")
-    if draft_probs is not None and (draft_probs.shape != target.shape or draft_probs.dtype != torch.float32 or draft_probs.device != target.device
-                                    or (vocab > 1 and draft_probs.stride(1) != 1)):
-        raise ValueError(f"draft_probs must be a fp32 tensor [{rows}, {vocab}] on {target.device}, the vocabulary contiguous")
+    draft, draft_stride = 0, 0
+    if draft_probs is not None:
+        if (draft_probs.shape != shape or draft_probs.dtype is not torch.float32 or draft_probs.device != target.device
+                or (vocab > 1 and draft_probs.stride(1) != 1)):
+            raise ValueError(f"draft_probs must be a fp32 tensor [{rows}, {vocab}] on {target.device}, the vocabulary contiguous")
+        draft, draft_stride = draft_probs.data_ptr(), draft_probs.stride(0)
     # one allocation for the three answers
-    answer = torch.empty(seqs * (max_rows + 2), dtype=torch.int32, device=target.device)
-    at = answer.data_ptr()
-    p = VerifyParams(seqs, rows, max_rows, vocab, _REALS[target.dtype], probs, target.data_ptr(), target.stride(0),
-                     _check_vector(target, "tokens", tokens, torch.int32, (rows,)),
-                     _check_vector(target, "row_starts", row_starts, torch.int32, (seqs + 1,)),
-                     None if parents is None else _check_vector(target, "parents", parents, torch.int32, (rows,)),
-                     _check_vector(target, "uniforms", uniforms, torch.float32, (rows, 2)),
-                     None if temperatures is None else _check_vector(target, "temperatures", temperatures, torch.float32, (seqs,)),
-                     _ptr(draft_probs), 0 if draft_probs is None else draft_probs.stride(0), at, at + 4 * seqs * max_rows,
-                     at + 4 * seqs * (max_rows + 1))
-    with _on_device(target.device):
-        ps = C.byref(p)
-        nbytes = lib.tri_verify_workspace_bytes(ps)
-        buf, ws = _scratch(target, nbytes, "verification")
-        _lib.check(lib.tri_verify_drafts(ps, ws, nbytes, _stream()))
     n = seqs * max_rows
-    return answer[:n].view(seqs, max_rows), answer[n:n + seqs], answer[n + seqs:]
+    answer = torch.empty(n + 2 * seqs, dtype=torch.int32, device=target.device)
+    at = answer.data_ptr()
+    p = _verify_params(seqs, rows, max_rows, vocab, _REALS[dtype], probs, target.data_ptr(), target.stride(0),
+                       _check_vector(target, "tokens", tokens, torch.int32, (rows,)),
+                       _check_vector(target, "row_starts", row_starts, torch.int32, (seqs + 1,)),
+                       0 if parents is None else _check_vector(target, "parents", parents, torch.int32, (rows,)),
+                       _check_vector(target, "uniforms", uniforms, torch.float32, (rows, 2)),
+                       0 if temperatures is None else _check_vector(target, "temperatures", temperatures, torch.float32, (seqs,)),
+                       draft, draft_stride, at, at + 4 * n, at + 4 * (n + seqs))
+    nbytes = lib.tri_verify_workspace_bytes(p)
+    buf, ws = _scratch(target, nbytes, "verification")
+    _call(target.device, lib.tri_verify_drafts, p, ws, nbytes)
+    accepted, counts, following = torch.split_with_sizes(answer, (n, seqs, seqs))
+    return accepted.view(seqs, max_rows), counts, following
 
 
 def accept_drafts(kv: PagedKV, batch: StepBatch, row_starts: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor, *,
@@ -1142,17 +1159,16 @@ def accept_drafts(kv: PagedKV, batch: StepBatch, row_starts: torch.Tensor, rows:
     fp8 row's scales and the accumulated ``weights``.  ``batch.seq_lens`` counts all drafted rows (the last tokens, by
     ``row_starts``), ``rows`` and ``counts`` are ``verify_drafts``'.  Returns the new lengths, int32 [sequences]: the batch's less the rows that
     were not accepted.  Block bounds of the blocks concerned are to be updated behind it."""
-    lib = _lib.load()
     _check_attention_batch(kv, batch)
     if kv.v_ptrs is None:
         raise ValueError("accept_drafts needs the values of the cache")
     n = batch.num_seqs
     if rows.ndim != 2 or not 1 <= rows.shape[1] <= 64:
         raise ValueError(f"rows must be an int32 tensor [{n}, 1 to 64]")
+    width = rows.shape[1]
     lens = torch.empty(n, dtype=torch.int32, device=kv.device)
-    p = AcceptParams(kv.num_blocks, rows.shape[1], _check_vector(kv, "row_starts", row_starts, torch.int32, (n + 1,)),
-                     _check_vector(kv, "rows", rows, torch.int32, (n, rows.shape[1])), _check_vector(kv, "counts", counts, torch.int32, (n,)),
-                     None if weights is None else _weights_address(kv, weights), 0 if weights is None else weights.stride(0), lens.data_ptr())
-    with _on_device(kv.device):
-        _lib.check(lib.tri_accept_drafts(C.byref(kv.struct), C.byref(batch.struct), C.byref(p), _stream()))
+    p = _accept_params(kv.num_blocks, width, _check_vector(kv, "row_starts", row_starts, torch.int32, (n + 1,)),
+                       _check_vector(kv, "rows", rows, torch.int32, (n, width)), _check_vector(kv, "counts", counts, torch.int32, (n,)),
+                       0 if weights is None else _weights_address(kv, weights), 0 if weights is None else weights.stride(0), lens.data_ptr())
+    _call(kv.device, _lib.load().tri_accept_drafts, C.byref(kv.struct), C.byref(batch.struct), p)
     return lens
