@@ -63,6 +63,7 @@ FP8 = dict(kv_dtype=2, k_scale_layers=8)
     ({}, {}, dict(num_blocks=0), INVALID, b"num_blocks"),
     ({}, {}, dict(num_rows=-1), INVALID, b"num_rows"),
     ({}, {}, dict(num_rows=4), INVALID, b"row_starts"),
+    ({}, {}, dict(num_rows=1 << 26, row_starts=8), UNSUPPORTED, b"in one call"),
     ({}, {}, dict(q=None), INVALID, b"q is NULL"),
     ({}, {}, dict(k=None), INVALID, b"k is NULL"),
     ({}, {}, dict(v=None), INVALID, b"v is NULL"),
@@ -101,6 +102,7 @@ def test_writing_refuses(layout, batch, params, code, word):
     ({}, {}, dict(row_starts=None), INVALID, b"row_starts"),
     ({}, {}, dict(out_dtype=3), INVALID, b"out_dtype"),
     ({}, {}, dict(num_rows=-1), INVALID, b"num_rows"),
+    ({}, {}, dict(num_rows=1 << 26), UNSUPPORTED, b"in one call"),
     ({}, {}, dict(k_out=None), INVALID, b"k_out"),
     ({}, {}, dict(v_out=8), INVALID, b"aligned"),
     ({}, {}, dict(k_scale=math.inf), INVALID, b"finite"),
@@ -125,6 +127,7 @@ def test_reading_refuses(layout, batch, params, code, word):
     (dict(target_stride=999), INVALID, b"stride"),
     (dict(draft_probs=8, draft_stride=999), INVALID, b"stride"),
     (dict(num_rows=1 << 20, vocab=1 << 25, target_stride=1 << 25), UNSUPPORTED, b"in one call"),
+    (dict(num_rows=1 << 20, vocab=1 << 17, target_stride=1 << 17), UNSUPPORTED, b"in one call"),
 ])
 def test_verification_refuses(params, code, word):
     lib = _lib.load()
@@ -168,6 +171,7 @@ def test_verification_needs_its_workspace():
     ({}, {}, dict(rows=None), INVALID, b"rows"),
     ({}, {}, dict(counts=None), INVALID, b"counts"),
     ({}, dict(seq_lens=24), dict(new_lens=24), INVALID, b"new_lens"),
+    (dict(num_layers=4096), dict(num_seqs=2048), {}, UNSUPPORTED, b"in one call"),
     ({}, {}, dict(weights=16, weights_stride_layer=40 * 16 * 4 - 1), INVALID, b"less than a layer"),
 ])
 def test_acceptance_refuses(layout, batch, params, code, word):

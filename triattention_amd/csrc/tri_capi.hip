@@ -1285,6 +1285,8 @@ int check_heads(const char* name, const void* p, int64_t stride_row, int64_t str
   return TRI_OK;
 }
 
+constexpr int64_t kMostWaves = (1ll << 26) - 64;      // of a launch, which has less than 2^32 threads
+
 struct VerifyPlan {
   tri::VerifyLaunch a{};
   int64_t part, arrived, picked, rest, total;
@@ -1307,8 +1309,9 @@ int plan_verify(const tri_verify_params* p, VerifyPlan& d) {
     return fail(TRI_ERR_INVALID_ARGUMENT, "a row's stride is less than vocab %d", p->vocab);
   tri::VerifyLaunch& a = d.a;
   a.pieces = (int)tri::ceil_div64(p->vocab, tri::kVerifyPiece);
-  const int64_t most = std::max<int64_t>(p->num_rows, p->num_seqs);
-  if (most * a.pieces > INT_MAX || (int64_t)p->num_seqs * p->max_rows > INT_MAX)
+  // (a wave for each piece of a row, and of what a rejection leaves of a sequence's: a launch has less than 2^32 threads)
+  const int64_t most = std::max<int64_t>(p->num_rows, (int64_t)p->num_seqs * 2);
+  if (most * a.pieces > kMostWaves || (int64_t)p->num_seqs * p->max_rows > kMostWaves)
     return fail(TRI_ERR_UNSUPPORTED, "%d rows of %d logits in one call", p->num_rows, p->vocab);
   a.B = p->num_seqs; a.num_rows = p->num_rows; a.max_rows = p->max_rows; a.vocab = p->vocab;
   a.target_dtype = p->target_dtype; a.probs = p->target_probs ? 1 : 0;
@@ -1337,6 +1340,7 @@ int tri_write_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_w
   if (kv->kv_dtype != TRI_KV_FP8_E4M3 && p->dtype != kv->kv_dtype)
     return fail(TRI_ERR_UNSUPPORTED, "rows of type %d into a cache of type %d", p->dtype, kv->kv_dtype);
   if (p->num_rows < 0 || p->num_rows > INT_MAX / p->num_q_heads) return fail(TRI_ERR_INVALID_ARGUMENT, "num_rows %d", p->num_rows);
+  if (p->num_rows > kMostWaves) return fail(TRI_ERR_UNSUPPORTED, "num_rows %d in one call", p->num_rows);
   if (!p->row_starts && p->num_rows != batch->num_seqs)
     return fail(TRI_ERR_INVALID_ARGUMENT, "without row_starts there is one row per sequence (%d rows, %d sequences)", p->num_rows, batch->num_seqs);
   const int D = kv->head_dim, n = p->num_rows;
@@ -1385,6 +1389,7 @@ int tri_read_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_re
   if (!p->row_starts) return fail(TRI_ERR_INVALID_ARGUMENT, "row_starts is NULL");
   if (p->out_dtype < TRI_REAL_BF16 || p->out_dtype > TRI_REAL_FP32) return fail(TRI_ERR_INVALID_ARGUMENT, "out_dtype %d", p->out_dtype);
   if (p->num_rows < 0) return fail(TRI_ERR_INVALID_ARGUMENT, "num_rows %d", p->num_rows);
+  if (p->num_rows > kMostWaves) return fail(TRI_ERR_UNSUPPORTED, "num_rows %d in one call", p->num_rows);
   if (!is_finite(p->k_scale) || !is_finite(p->v_scale)) return fail(TRI_ERR_INVALID_ARGUMENT, "k_scale and v_scale must be finite");
   if (p->num_rows > 0 && (!p->k_out || !p->v_out)) return fail(TRI_ERR_INVALID_ARGUMENT, "k_out / v_out is NULL");
   if (!is_aligned(p->k_out, 16) || !is_aligned(p->v_out, 16)) return fail(TRI_ERR_INVALID_ARGUMENT, "k_out and v_out must be 16-byte aligned");
@@ -1437,7 +1442,7 @@ int tri_accept_drafts(const tri_kv_layout* kv, const tri_batch* batch, const tri
   if (p->new_lens == batch->seq_lens) return fail(TRI_ERR_INVALID_ARGUMENT, "new_lens is the batch's seq_lens, which the call reads");
   if (p->weights && kv->num_layers > 1 && p->weights_stride_layer < (int64_t)p->num_blocks * kv->block_size * kv->num_kv_heads)
     return fail(TRI_ERR_INVALID_ARGUMENT, "weights_stride_layer %lld is less than a layer", (long long)p->weights_stride_layer);
-  if ((int64_t)batch->num_seqs * kv->num_layers > INT_MAX / 2)
+  if ((int64_t)batch->num_seqs * kv->num_layers * 8 > kMostWaves)
     return fail(TRI_ERR_UNSUPPORTED, "%d sequences and %d layers in one call", batch->num_seqs, kv->num_layers);
   tri::AcceptLaunch a{};
   a.B = batch->num_seqs; a.L = kv->num_layers; a.Hkv = kv->num_kv_heads; a.D = kv->head_dim; a.elem_bytes = elem_bytes(kv->kv_dtype);

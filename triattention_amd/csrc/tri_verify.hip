@@ -88,26 +88,28 @@ __device__ const double kPowerTable[kPowers] = {
     1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
     1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
-__device__ __forceinline__ void make_powers(double* table) {
+// A thread's word of the table is asked for before all else and put into LDS where it has come (the counter of a wave's loads goes in
+// their order: a load behind those of a piece would be waited for with them).
+__device__ __forceinline__ double own_power() { return kPowerTable[threadIdx.x % kPowers]; }
+__device__ __forceinline__ void keep_power(double* table, double own) {
   if (threadIdx.x < kPowers) {
-    u32x2 words = __builtin_bit_cast(u32x2, kPowerTable[threadIdx.x]);
+    u32x2 words = __builtin_bit_cast(u32x2, own);
     words.y -= threadIdx.x << 15;
     table[threadIdx.x] = __builtin_bit_cast(double, words);
   }
 }
 
-// w of eight logits against the largest one, c = log2 e / T: exactly nothing where it is below 2^-1000 of that, -inf or NaN.
+// What weighs no more than this beside the largest (-inf, NaN, and numbers that far below it) has nothing.
+constexpr double kNothing = 0x1p-900;
+// w of logits against the largest one, c = log2 e / T; of what has nothing 2^-1000 at least.
 __device__ __forceinline__ void weights_of(const Powers& powers, const float (&x)[8], double most, double c, double (&w)[8]) {
-  double y[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = y[e] = ((double)x[e] - most) * c;
+  for (int e = 0; e < 8; ++e) w[e] = ((double)x[e] - most) * c;
   powers(w);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = y[e] > kLeastPower ? w[e] : 0.0;
 }
 __device__ __forceinline__ double weight_of(const Powers& powers, float x, double most, double c) {
-  const double y = ((double)x - most) * c, w = powers(y);
-  return y > kLeastPower ? w : 0.0;
+  const double w = powers(((double)x - most) * c);
+  return w > kNothing ? w : 0.0;
 }
 
 typedef __attribute__((address_space(1))) char* GlobalRows;
@@ -244,10 +246,12 @@ __device__ __forceinline__ int rows_of_sequence(const VerifyLaunch& a, int b, in
   return min(end - first, a.max_rows);
 }
 // log2 e / T; 0 where the sequence takes the largest (T not above 0).
+__device__ __forceinline__ double sharpness(float temperature, bool& greedy) {
+  greedy = !(temperature > 0.f);
+  return greedy ? 0.0 : 1.44269504088896340736 / (double)temperature;
+}
 __device__ __forceinline__ double sharpness_of(const VerifyLaunch& a, int b, bool& greedy) {
-  const float t = a.temperatures ? a.temperatures[b] : 1.f;
-  greedy = !(t > 0.f);
-  return greedy ? 0.0 : 1.44269504088896340736 / (double)t;
+  return sharpness(a.temperatures ? a.temperatures[b] : 1.f, greedy);
 }
 
 template <int RT, bool PROBS>
@@ -264,15 +268,27 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunc
   const int64_t unit = (int64_t)blockIdx.x * kVerifyWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int row = (int)(unit / a.pieces), piece = (int)(unit % a.pieces);
   constexpr int N = PROBS ? kProbs : kRawLogits;
+  // what is needed to know the row's temperature comes before the piece: of up to 64 sequences all of it at once
+  const double power = own_power();
+  const int mine = min(lane, a.B - 1);
+  const int32_t start = a.row_starts[mine], end = a.row_starts[mine + 1];
+  const float temperature = a.temperatures ? a.temperatures[mine] : 1.f;
   Piece<RT> held;
   if (row < a.num_rows) held = load_piece<RT, N>(a, row_of<RT, PROBS>(a, row), piece, lane);
-  make_powers(table);
+  keep_power(table, power);
   __syncthreads();
   if (row >= a.num_rows) return;
-  const int b = __builtin_amdgcn_readfirstlane(sequence_of_row(a.row_starts, a.B, row, lane));
-  if (b < 0 || row - a.row_starts[b] >= a.max_rows) return;
   bool greedy;
-  const double c = sharpness_of(a, b, greedy);
+  double c;
+  if (a.B <= kWave) {
+    const uint64_t own = __ballot(lane < a.B && start <= row && row < end && row - start < a.max_rows);
+    if (!own) return;
+    c = sharpness(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(temperature), __ffsll((unsigned long long)own) - 1)), greedy);
+  } else {
+    const int b = __builtin_amdgcn_readfirstlane(sequence_of_row(a.row_starts, a.B, row, lane));
+    if (b < 0 || row - a.row_starts[b] >= a.max_rows) return;
+    c = sharpness_of(a, b, greedy);
+  }
   float most = -INFINITY;
 #pragma unroll
   for (int s = 0; s < kPieceSteps; ++s) {
@@ -344,13 +360,14 @@ __device__ __forceinline__ double against(const Powers& powers, const VerifyPart
   else return p.sum == 0.0 ? 0.0 : p.sum * weight_of(powers, p.most, most, c);
 }
 
+__device__ __forceinline__ VerifyPart first_part(const VerifyLaunch& a, int row, int lane) {
+  return lane < a.pieces ? a.part[(int64_t)row * a.pieces + lane] : VerifyPart{0.0, -INFINITY, INT32_MAX};
+}
+// (a row of up to 2^17 numbers: one piece a lane, `mine`)
 template <bool PROBS>
-__device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, const Powers& powers, int row, double c, int lane) {
+__device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, const Powers& powers, int row, const VerifyPart& mine, double c, int lane) {
   const VerifyPart* part = a.part + (int64_t)row * a.pieces;
   RowTotal t{0.0, -INFINITY, INT32_MAX};
-  // (a row of up to 2^17 numbers: one piece a lane, read once)
-  VerifyPart mine{0.0, -INFINITY, INT32_MAX};
-  if (lane < a.pieces) mine = part[lane];
   t.most = mine.most;
   t.where = mine.where;
   for (int i = lane + kWave; i < a.pieces; i += kWave)
@@ -379,7 +396,7 @@ __device__ __forceinline__ int draw(const VerifyLaunch& a, double whole, float u
   for (int i0 = 0; i0 < a.pieces && piece < 0; i0 += kWave) {
     const double v = i0 + lane < a.pieces ? piece_sum(i0 + lane) : 0.0;
     const double upto = before + running_sum(v);
-    const uint64_t some = __ballot(v > 0.0), over = __ballot(v > 0.0 && upto > mark);
+    const uint64_t some = __ballot(v > kNothing), over = __ballot(v > kNothing && upto > mark);
     if (over) {
       const int at = __ffsll((unsigned long long)over) - 1;
       piece = i0 + at;
@@ -409,7 +426,7 @@ __device__ __forceinline__ int draw(const VerifyLaunch& a, double whole, float u
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       running += w[e];
-      if (w[e] > 0.0) {
+      if (w[e] > kNothing) {
         if (mine < 0 && running > mark) mine = i + e;
         final = i + e;
       }
@@ -450,19 +467,21 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunc
   __shared__ double table[kPowers];
   const int b = blockIdx.x / max_groups, group = blockIdx.x % max_groups;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const double power = own_power();
+  bool greedy;
+  const double c = sharpness_of(a, b, greedy);
   int first;
   const int n = rows_of_sequence(a, b, first), groups = max(1, ceil_div(n, kVerifyWaves));
   if (group >= groups) return;
-  make_powers(table);
-  __syncthreads();
-  const Powers powers(table);
   const int i = group * kVerifyWaves + wave;
   int32_t* const picked = a.picked + (int64_t)b * a.max_rows;
+  const VerifyPart mine = i < n ? first_part(a, first + i, lane) : VerifyPart{};
+  const float u = i < n ? a.uniforms[2 * (int64_t)(first + i) + 1] : 0.f;
+  keep_power(table, power);
+  __syncthreads();
+  const Powers powers(table);
   if (i < n) {
-    bool greedy;
-    const double c = sharpness_of(a, b, greedy);
-    const float u = a.uniforms[2 * (int64_t)(first + i) + 1];
-    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, c, lane);
+    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, mine, c, lane);
     int token = t.where;
     if (!greedy) {
       const void* const src = row_of<RT, PROBS>(a, first + i);
@@ -537,14 +556,17 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
   __shared__ double table[kPowers];
   const int b = blockIdx.x / groups, group = blockIdx.x % groups;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const double power = own_power();
   int first;
   const int n = rows_of_sequence(a, b, first);
   bool greedy;
   const double c = sharpness_of(a, b, greedy);
-  make_powers(table);
+  VerifyPart mine = wave < n ? first_part(a, first + wave, lane) : VerifyPart{};
+  keep_power(table, power);
   __syncthreads();
   const Powers powers(table);
   for (int i = wave; i < n; i += kChainWaves) {
+    if (i != wave) mine = first_part(a, first + i, lane);
     // what the decision on the next row needs is asked for before the sums are joined
     int token = -1;
     float x = -INFINITY, q = 0.f, u = 0.f;
@@ -557,7 +579,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
         q = counted<kProbs>(a.draft[next * a.draft_stride + token]);
       }
     }
-    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, c, lane);
+    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, mine, c, lane);
     bool ok = false;
     if (greedy) {
       ok = t.where >= 0 && token == t.where;
@@ -601,7 +623,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
   int token = t.where;
   if (!greedy && n > 0) {
     const float u = a.uniforms[2 * (int64_t)row + 1];
-    const bool left = whole > 0.0;       // (or rounding left nothing)
+    const bool left = whole > kNothing;  // (or rounding left nothing)
     const VerifyPart* const part = a.part + (int64_t)row * a.pieces;
     const double per_sum = left ? 1.0 / t.sum : 1.0;
     token = draw(a, left ? whole : t.sum, u, lane, [&](int piece) { return left ? rest[piece] : against<PROBS>(powers, part[piece], t.most, c); },
@@ -646,7 +668,7 @@ __global__ __launch_bounds__(kVerifyThreads) void accept_rows_kernel(AcceptLaunc
   __syncthreads();
   const GlobalRows cache = (GlobalRows)(uintptr_t)(side ? a.v_layers : a.k_layers)[l];
   const int lanes = a.D * a.elem_bytes / 16, pieces = a.Hkv * lanes;
-  for (int p = threadIdx.x; p < pieces; p += kVerifyThreads) {
+  for (int p = threadIdx.x; p < pieces; p += blockDim.x) {
     const int h = p / lanes;
     const int64_t at = (int64_t)h * a.stride_head * a.elem_bytes + (p - h * lanes) * 16;
     for (int j0 = 0; j0 < m; j0 += kAcceptAtOnce) {
@@ -662,7 +684,7 @@ __global__ __launch_bounds__(kVerifyThreads) void accept_rows_kernel(AcceptLaunc
   // numbers beside the rows: an fp8 row's scale, a token's weight
   float* const scales = a.v_scale_layers ? (side ? a.v_scale_layers : a.k_scale_layers)[l] : nullptr;
   float* const weights = a.weights && side ? a.weights + l * a.weights_stride_layer : nullptr;
-  for (int p = threadIdx.x; p < 2 * a.Hkv; p += kVerifyThreads) {
+  for (int p = threadIdx.x; p < 2 * a.Hkv; p += blockDim.x) {
     const int h = p % a.Hkv;
     float* const x = p < a.Hkv ? scales : weights;
     if (!x) continue;
@@ -701,7 +723,9 @@ hipError_t launch_verify_drafts(const VerifyLaunch& a, hipStream_t s) {
 }
 
 hipError_t launch_accept_rows(const AcceptLaunch& a, hipStream_t s) {
-  hipLaunchKernelGGL(accept_rows_kernel, dim3((unsigned)(a.B * a.L * 2)), dim3(kVerifyThreads), 0, s, a);
+  // (a thread for every 16 bytes of a row)
+  const int threads = std::min<int>(kVerifyThreads, (int)align_up(a.Hkv * a.D * a.elem_bytes / 16, kWave));
+  hipLaunchKernelGGL(accept_rows_kernel, dim3((unsigned)(a.B * a.L * 2)), dim3(threads), 0, s, a);
   return hipGetLastError();
 }
 

@@ -104,10 +104,6 @@ class PagedKV:
         self.num_blocks, self.block_size, self.num_kv_heads, self.head_dim = (int(x) for x in k0.shape)
         self.rope_style = rope_style
         self._keep = (list(k_views), list(v_views) if v_views is not None else None, k_scales, v_scales)
-        self.k_ptrs = torch.tensor([t.data_ptr() for t in k_views], dtype=torch.int64, device=self.device)
-        self.v_ptrs = (torch.tensor([t.data_ptr() for t in v_views], dtype=torch.int64, device=self.device)
-                       if v_views is not None else None)
-        self.ks_ptrs = self.vs_ptrs = None
         if _DTYPES[self.dtype] == KV_FP8_E4M3:
             if k_scales is None:
                 # A cache with one scale per tensor (vLLM's fp8 KV cache): the codes are scored as
@@ -118,9 +114,16 @@ class PagedKV:
                 unit = _unit_scales(self.device, self.num_blocks * self.block_size * self.num_kv_heads)
                 k_scales = [unit] * self.num_layers
                 self._unit = unit           # ours, so kept alive here whatever becomes of _keep
-            self.ks_ptrs = torch.tensor([t.data_ptr() for t in k_scales], dtype=torch.int64, device=self.device)
-            if v_scales is not None:
-                self.vs_ptrs = torch.tensor([t.data_ptr() for t in v_scales], dtype=torch.int64, device=self.device)
+        else:
+            k_scales = v_scales = None
+        # one copy to the device for the pointers of all of them
+        sides = [s for s in (k_views, v_views, k_scales, v_scales) if s is not None]
+        tables = iter(torch.tensor([t.data_ptr() for s in sides for t in s], dtype=torch.int64, device=self.device)
+                      .split([len(s) for s in sides]))
+        self.k_ptrs = next(tables)
+        self.v_ptrs = next(tables) if v_views is not None else None
+        self.ks_ptrs = next(tables) if k_scales is not None else None
+        self.vs_ptrs = next(tables) if v_scales is not None else None
         self.struct = KvLayout(
             num_layers=self.num_layers, num_kv_heads=self.num_kv_heads, head_dim=self.head_dim,
             block_size=self.block_size, kv_dtype=_DTYPES[self.dtype],
