@@ -352,7 +352,7 @@ hipError_t launch_move_weights(const EvictLaunch& a, hipStream_t s);
 struct WriteLaunch {
   int B, Hq, Hkv, D, block_size, kv_dtype, q_dtype, rope_style, layer, Tmax, num_blocks, num_rows;
   int num_axes, positions_64, norm_fp32;
-  int waves_per_row, stream_rows;                          // set by the launcher
+  int waves_per_row;                                       // set by the launcher
   int64_t stride_block, stride_token, stride_head;         // elements
   void* const* k_layers;
   void* const* v_layers;
