@@ -508,8 +508,8 @@ int tri_read_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_re
  * where that is 0).  A draw takes the least token whose running sum exceeds uniforms[row][1] of the whole.  A temperature that is not above 0:
  * the largest logit, the first among equals, in place of every draw, and a draft is accepted iff it is that.  So next and the accepted
  * tokens have the distribution of the target, whatever drafted them.
- *  Weights and sums are 64-bit.  NaN logits count as -inf, probabilities that are no positive finite number as 0; a row without any
- * weight draws -1.  Tokens outside [0, vocab) are never accepted.  Rows beyond max_rows of a sequence are not looked at.
+ *  Weights and sums are 64-bit (what weighs less than 2^-900 of the largest weighs nothing).  NaN logits count as -inf, +inf as the
+ * largest finite number, probabilities that are no positive finite number as 0; a row without any weight draws -1.  Tokens outside [0, vocab) are never accepted.  Rows beyond max_rows of a sequence are not looked at.
  * rows: int32 [num_seqs][max_rows], the accepted rows ascending, row 0 first, -1 behind them; counts: how many; next: the token
  * behind them.  A sequence without rows: 0 and -1. */
 typedef struct tri_verify_params {

@@ -258,6 +258,26 @@ def test_write_finds_the_sequence_of_a_row(seqs):
     _check_written(s, out, before)
 
 
+def test_rows_before_the_first_sequence():
+    """row_starts need not begin at 0: rows before it belong to no sequence, in every call."""
+    s = Step([20, 33], rows=[4, 6], norm=FP32, seed=23, pad_rows=5)
+    s.starts = [3, 7, 13]
+    kv, batch = s.device()
+    before = torch.full((s.num_rows, s.hq, s.d), 7.0, dtype=BF16, device=DEV)
+    out = s.write(kv, batch, out=before.clone())
+    _check_written(s, out, before)
+    got = tuple(torch.full((s.num_rows, s.h, s.d), 9.0, dtype=BF16, device=DEV) for _ in range(2))
+    ops.read_paged(kv, batch, s.dstarts, s.num_rows, out=got)
+    mine = torch.zeros(s.num_rows, dtype=torch.bool)
+    mine[3:13] = True
+    assert torch.equal(_bits(got[1].cpu()[mine]), _bits(s.v[mine])) and bool((got[1].cpu()[~mine] == 9).all()) and bool((got[0].cpu()[~mine] == 9).all())
+    for draft in (False, True):
+        d = Drafts([4, 6], 3000, draft=draft, seed=24, pad=5)
+        d.starts, d.target, d.uniforms, d.tokens = [3, 7, 13], d.target.roll(3, 0), d.uniforms.roll(3, 0), d.tokens.roll(3, 0)
+        d.draft = None if d.draft is None else d.draft.roll(3, 0)
+        d.check(d.run(max_rows=8), 8)
+
+
 def test_write_more_rows_than_tokens_and_pages_outside():
     s = Step([5, 40, 0], rows=[9, 20, 2], seed=10)
     kv, batch = s.device(lens=[5, 40, 1])
@@ -346,6 +366,27 @@ def test_write_many_rows(rows):
         want = odec.rotated(n, pick[None], inv, None, True)
         both = (n[..., :d // 2].abs() + n[..., d // 2:].abs()).repeat(1, 1, 2)
         _near(got, want, (d / 2 + 20) * 2.0 ** -24 * both, BF16, "sample")
+
+
+def test_without_a_block_table():
+    """A dense cache: a sequence is one block of it.  Written, read, and its accepted rows moved."""
+    s = Step([40, 33, 12], rows=[40, 5, 12], block=64, layers=2, norm=FP32, seed=22)
+    s.tables = [[0], [1], [2]]
+    kv, _ = s.device()
+    batch = ops.StepBatch(torch.device(DEV), s.lens)
+    out = s.write(kv, batch, layer=1)
+    _check_written(s, out, layer=1)
+    k, v = ops.read_paged(kv, batch, s.dstarts, s.num_rows, layer=1)
+    assert torch.equal(_bits(v.cpu()), _bits(s.v))
+    for l in range(2):
+        for side, cache in ((0, s.dk), (1, s.dv)):
+            s.cache[side][l] = cache[l].cpu()
+    paths = [[0, 3, 39, -1], [1, 2, 4, -1], [0, 1, 2, 11]]
+    counts = [3, 3, 4]
+    lens = ops.accept_drafts(kv, batch, s.dstarts, torch.tensor(paths, dtype=torch.int32, device=DEV), torch.tensor(counts, dtype=torch.int32, device=DEV))
+    _check_accepted(s, paths, counts, lens.cpu(), None, 4)
+    with pytest.raises(ValueError):
+        s.write(kv, ops.StepBatch(torch.device(DEV), [65, 33, 12]))
 
 
 def test_write_refuses_tensors():
@@ -627,6 +668,22 @@ def test_verify_masks_and_odd_numbers(kind):
     x[30:33, 4096:] = math.inf                         # greedy, the first of many
     x[33] = torch.finfo(torch.float32).min             # all alike
     d.check(d.run())
+
+
+def test_verify_infinities_among_the_largest_numbers():
+    """+inf counts as the largest finite number, in one piece of a row and across pieces, greedy and drawn."""
+    most = torch.finfo(torch.float32).max
+    d = Drafts([1] * 8, 9000, temperatures=[0.0, 0.0, 0.0, 0.0, 1.0, 1.0, 1.0, 1.0], seed=21)
+    for b in (0, 4):
+        d.target[b, [17, 30]] = torch.tensor([most, math.inf])
+        d.target[b + 1, [17, 5000]] = torch.tensor([most, math.inf])
+        d.target[b + 2, [17, 5000]] = torch.tensor([math.inf, most])
+        d.target[b + 3, [4500, 4501, 8999]] = torch.tensor([math.nan, math.inf, math.inf])
+    for u in (0.0, 0.49, 0.51, 0.99):
+        d.uniforms[:] = u
+        got = d.run()
+        d.check(got)
+        assert got[2].cpu().tolist() == [17, 17, 17, 4501] + ([17, 17, 17, 4501] if u < 0.5 else [30, 5000, 5000, 8999])
 
 
 def test_verify_uniforms_at_their_ends():

@@ -9,10 +9,13 @@
 // near a random number once in 2^25 draws.
 //
 //  verify_sums_kernel  : every row's pieces of 2048 logits, a wave each: largest, where, and the sum of w against that
-//  verify_walk_kernel  : (no draft probabilities) a workgroup per sequence: a wave draws a row's token, then the walk
-//  verify_chain_kernel : (draft probabilities) which rows are accepted, and sums of max(p - q, 0) by pieces
-//  verify_draw_kernel  : the token behind them
+//  verify_walk_kernel  : (no draft probabilities) a wave draws a row's token, a sequence's last workgroup walks
+//  verify_chain_kernel : (draft probabilities) which rows are accepted, sums of max(p - q, 0) by pieces; the last workgroup draws
 //  accept_rows_kernel  : rows of the accepted path to consecutive slots, every layer
+//
+// Two launches a call.  A third, for what the last workgroup of a sequence does, took 4 us more of the host and 3 of the GPU; one launch for
+// all of it would need counters cleared before it.  One chain of six rows of 32768 logits 4.2 + 7.0 us, 60 greedy rows of 131072
+// 4.7 + 4.5: launches and dependent reads; the host behind them takes 15.
 #include <algorithm>
 #include <cfloat>
 
@@ -32,10 +35,11 @@ constexpr int kChainThreads = 512;
 constexpr int kChainWaves = kChainThreads / kWave;
 
 // 2^y, y <= 0, never less than 2^-1000 (which NaN gives too): y = n + j / 32 + f, rounded by an addition; 2^f on [-1/64, 1/64] by its Chebyshev
-// interpolation of degree 4 (off by 2^-43.5 of it), 2^(j/32) out of LDS, n into the exponent.  Sixteen instructions for a logit, with
-// the series alone (degree 9) it would be twenty.  The table is 32 numbers because those lie in 64 different banks: lanes read the
-// same word or different banks.  The coefficients are kept from being constants that the compiler copies into vector registers before
-// every step: they are the products' scalar operand.
+// interpolation of degree 4 (off by 2^-43.5 of it), 2^(j/32) out of LDS, n into the exponent: twelve vector instructions and an LDS read.
+// 262 rows of 131072 logits, the sums' kernel as it then was: a Taylor series of degree 11 on [-1/2, 1/2] 43 us, the interpolation of
+// degree 9 with scalar coefficients (fourteen instructions) 32, this one 27.  The table is 32 numbers because those lie in 64 different banks: lanes read
+// the same word or different banks.  The coefficients are kept from being constants that the compiler copies into vector registers
+// before every step: they are the products' scalar operand.
 constexpr double kLeastPower = -1000.0;
 constexpr int kPowers = 32;
 struct Powers {
@@ -259,7 +263,10 @@ __device__ __forceinline__ const void* row_of(const VerifyLaunch& a, int row) {
   return reinterpret_cast<const char*>(a.target) + row * a.target_stride * (RT == TRI_REAL_FP32 ? 4 : 2);
 }
 
-// A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.
+// A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.  Bound by vector instructions
+// (20 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 23.4 us, of which those take 20;
+// 161 rows of 100003 fp32 ones, 64 MB, in 16.3, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
+// the caches, two halves of 16 bytes side by side for fp32 and a shorter form for rows whose numbers lie near each other gained nothing.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunch a) {
   __shared__ double table[kPowers];
@@ -297,6 +304,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunc
     for (int e = 0; e < 8; ++e) most = fmaxf(most, n.x[e]);
   }
   most = most_of_wave(most);
+  const float top = PROBS ? most : fminf(most, FLT_MAX);      // (infinities are the largest finite number)
   double sum = 0.0;
   int where = 0;
   if (greedy) {
@@ -306,34 +314,34 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunc
       const Numbers8 n = numbers_of<RT, N>(held.step[s]);
 #pragma unroll
       for (int e = 7; e >= 0; --e)
-        if (n.x[e] == most) where = s * kWave * 8 + lane * 8 + e;
+        if (n.x[e] >= top) where = s * kWave * 8 + lane * 8 + e;
     }
     where = most > -INFINITY ? least_of_wave(where) : 0;
   } else if (PROBS || most == INFINITY) {
-    // (what counts as nothing weighs nothing, and beside infinities all else does)
+    // (beside infinities all else weighs nothing)
 #pragma unroll
     for (int s = 0; s < kPieceSteps; ++s) {
       const Numbers8 n = numbers_of<RT, N>(held.step[s]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum += PROBS ? (double)n.x[e] : n.x[e] == INFINITY ? 1.0 : 0.0;
+      for (int e = 0; e < 8; ++e) sum += PROBS ? (double)n.x[e] : n.x[e] >= top ? 1.0 : 0.0;
     }
     sum = sum_of_wave(sum);
   } else if (most > -INFINITY) {
     // (what weighs less than 2^-1000 counts as that here: the largest weighs 1)
     const Powers powers(table);
-    const double top = most;
+    const double largest = most;
 #pragma unroll
     for (int s = 0; s < kPieceSteps; ++s) {
       const Numbers8 n = numbers_of<RT, N>(held.step[s]);
       double w[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = ((double)n.x[e] - top) * c;
+      for (int e = 0; e < 8; ++e) w[e] = ((double)n.x[e] - largest) * c;
       powers(w);
       sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     }
     sum = sum_of_wave(sum);
   }
-  if (lane == 0) a.part[unit] = VerifyPart{sum, PROBS ? most : fminf(most, FLT_MAX), piece * kVerifyPiece + where};
+  if (lane == 0) a.part[unit] = VerifyPart{sum, top, piece * kVerifyPiece + where};
 }
 
 template <bool PROBS>
@@ -448,6 +456,7 @@ __device__ __forceinline__ void write_path(const VerifyLaunch& a, int b, int lan
 }
 
 // Whether this workgroup is the last of `groups` of sequence b to come here: what the others wrote before is then seen by its first wave.
+// (One thread's release after the barrier stands for the workgroup's writes: every wave's own fence made the kernel of 48 chains take 61 us.)
 __device__ __forceinline__ bool last_to_arrive(const VerifyLaunch& a, int b, int groups) {
   __shared__ int count;
   __syncthreads();
@@ -461,6 +470,8 @@ __device__ __forceinline__ bool last_to_arrive(const VerifyLaunch& a, int b, int
   return true;
 }
 
+// A wave a row, four to a workgroup: the rows of a sequence are drawn at once, not only those of the path, which is known one row after the
+// other.  8 trees of up to 32 rows of 100003 logits 7.8 us (one workgroup of sixteen waves a sequence 26), dependent reads and one piece's weights.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunch a, int max_groups) {
   constexpr int N = PROBS ? kProbs : kLogits;
@@ -547,7 +558,9 @@ __device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& he
 }
 
 // Every workgroup of a sequence finds for itself which rows are accepted (a wave a row); where one is not, each takes some pieces of what
-// that leaves, and the last one draws from it.
+// that leaves, and the last one draws from it.  48 chains of up to eight rows of 131072 logits 18.3 us: 4 until the rows are decided, 8 for the
+// 38 MB of logits and draft probabilities of the rejected ones (4.7 TB/s), 1.5 until the last has come, 5 for its draw.  Workgroups of four
+// and of sixteen waves 19.0 and 19.8.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLaunch a, int groups) {
   constexpr int N = PROBS ? kProbs : kLogits;
@@ -633,8 +646,9 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
   write_path(a, b, lane, lane, count, token);
 }
 
-// Rows [first new token + rows[j]] to [first new token + j], j = 1 .. count - 1, of one side of one layer.  Lists ascend, so rows[j] >= j:
-// a thread has one place of every row, and what it writes lies before all that it still reads.
+// Rows [first new token + rows[j]] to [first new token + j], j < count, of one side of one layer.  Lists ascend, so rows[j] >= j: a thread has one
+// place of every row, and what it writes lies before all that it still reads.  32 sequences, 36 layers, 96 rows of 8 x 128 fp8 with scales
+// and weights in 8.4 us, one sequence in 4.0: four dependent reads (starts, list, table, row); 15 MB moved would take 3.
 constexpr int kAcceptAtOnce = 8;
 __global__ __launch_bounds__(kVerifyThreads) void accept_rows_kernel(AcceptLaunch a) {
   __shared__ int64_t from_row[64], to_row[64];           // elements of the cache
