@@ -26,6 +26,7 @@ typedef __attribute__((address_space(1))) uint32_t* GlobalOutU1;
 typedef __attribute__((address_space(1))) u32x4* GlobalOutU4;
 typedef __attribute__((address_space(1))) float* GlobalOutF32;
 enum CacheKind { kPlainRows = 0, kTensorScale = 1, kRowScales = 2 };
+enum PastCaches { kCached = 0, kReadPast = 1, kAllPast = 2 };       // what goes past the caches: reads of q, k and v, stores of q too
 
 // cos and sin of position * inv_freq.  The product and its reduction by pi / 2 are 64-bit: the remainder of an angle of 2^31
 // is off by 2^-54 a step, where an angle in 32 bits would be off by whole turns.  On [-pi/4, pi/4] the Taylor series up to r^9
@@ -93,11 +94,11 @@ __device__ __forceinline__ uint32_t pack_codes(const float* x, float inv) {
 // angles in every head.  A row's steps are shared by waves_per_row waves, which find the angles once each.  Norm and rotation
 // are a product by (w1 cos, w2 sin, w2 cos, w1 sin), the same in every head, and one by the head's 1 / sqrt(mean).
 //
-// Bound by reading and writing the rows: 16384 rows of 32 + 2 x 8 heads of 128, 403 MB, in 77 us (5.2 TB/s, a copy's rate); 11392 rows of
-// 28 + 2 x 4 heads into fp8, 199 MB, in 38.  One row 4.8 us, 64 rows of 64 + 2 x 8 heads with scales 5.5: a launch and its dependent reads.
-// What got there from 98 and 53: angles found a lane each in place of four times over (D 128), products of norm and rotation
-// made once a row, two steps at once and six waves a SIMD (four steps at once and five 103, eight waves with spills 99).
-template <int D, int QT, int KIND, bool HALF, bool ONCE>
+// Bound by reading and writing the rows: 16384 rows of 32 + 2 x 8 heads of 128, 403 MB, in 80 us (5.0 TB/s, a copy's 5.2 to 5.4); 11392
+// rows of 28 + 2 x 4 heads into fp8, 199 MB, in 38.  One row 4.8 us, 64 rows of 64 + 2 x 8 heads with scales 5.5: a launch and its
+// dependent reads.  The second took 53 while angles were found four times over and products of norm and rotation made in every head;
+// four steps at once with five waves a SIMD, and eight waves, which spill, were a tenth slower than two steps and six.
+template <int D, int QT, int KIND, bool HALF, int PAST>
 __global__ __launch_bounds__(kWriteThreads, 6) void write_paged_kernel(WriteLaunch a) {
   constexpr int LPH = D / 8, HPW = kWave / LPH;
   // elements of a head that are this lane's: first to first + 3 and first + apart to first + apart + 3
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(kWriteThreads, 6) void write_paged_kernel(WriteLaun
       raw[u][0] = raw[u][1] = u32x2{0, 0};
       if (s * HPW + sub < x.heads) {
         const GlobalBytes at = x.row + s * x.step;
-        if constexpr (ONCE) {
+        if constexpr (PAST != kCached) {
           raw[u][0] = __builtin_nontemporal_load((GlobalU2)(at + x.lane));
           raw[u][1] = __builtin_nontemporal_load((GlobalU2)(at + (x.lane + apart * 2)));
         } else {
@@ -224,8 +225,14 @@ __global__ __launch_bounds__(kWriteThreads, 6) void write_paged_kernel(WriteLaun
         turned(now[u], a.q_norm != nullptr, x);
         if (s * HPW + sub < a.Hq) {
           const GlobalOut dst = out + s * out_step;
-          *(GlobalOutU2)(dst + out_lane) = u32x2{pack_half<QT>(x[0], x[1]), pack_half<QT>(x[2], x[3])};
-          *(GlobalOutU2)(dst + (out_lane + apart * 2)) = u32x2{pack_half<QT>(x[4], x[5]), pack_half<QT>(x[6], x[7])};
+          const u32x2 low = {pack_half<QT>(x[0], x[1]), pack_half<QT>(x[2], x[3])}, high = {pack_half<QT>(x[4], x[5]), pack_half<QT>(x[6], x[7])};
+          if constexpr (PAST == kAllPast) {
+            __builtin_nontemporal_store(low, (GlobalOutU2)(dst + out_lane));
+            __builtin_nontemporal_store(high, (GlobalOutU2)(dst + (out_lane + apart * 2)));
+          } else {
+            *(GlobalOutU2)(dst + out_lane) = low;
+            *(GlobalOutU2)(dst + (out_lane + apart * 2)) = high;
+          }
         }
       }
       if (more) {
@@ -426,22 +433,28 @@ __global__ __launch_bounds__(kWriteThreads) void read_paged_kernel(ReadLaunch a)
   }
 }
 
-template <int D, int QT, bool HALF, bool ONCE>
+template <int D, int QT, bool HALF, int PAST>
 void write_of_kind(const WriteLaunch& a, hipStream_t s) {
   const dim3 grid((unsigned)ceil_div64((int64_t)a.num_rows * a.waves_per_row, kWriteWaves));
-  if (a.kv_dtype != TRI_KV_FP8_E4M3) hipLaunchKernelGGL((write_paged_kernel<D, QT, kPlainRows, HALF, ONCE>), grid, dim3(kWriteThreads), 0, s, a);
-  else if (!a.k_scale_layers) hipLaunchKernelGGL((write_paged_kernel<D, QT, kTensorScale, HALF, ONCE>), grid, dim3(kWriteThreads), 0, s, a);
-  else hipLaunchKernelGGL((write_paged_kernel<D, QT, kRowScales, HALF, ONCE>), grid, dim3(kWriteThreads), 0, s, a);
+  if (a.kv_dtype != TRI_KV_FP8_E4M3) hipLaunchKernelGGL((write_paged_kernel<D, QT, kPlainRows, HALF, PAST>), grid, dim3(kWriteThreads), 0, s, a);
+  else if (!a.k_scale_layers) hipLaunchKernelGGL((write_paged_kernel<D, QT, kTensorScale, HALF, PAST>), grid, dim3(kWriteThreads), 0, s, a);
+  else hipLaunchKernelGGL((write_paged_kernel<D, QT, kRowScales, HALF, PAST>), grid, dim3(kWriteThreads), 0, s, a);
+}
+template <int D, int QT, bool HALF>
+void write_past(const WriteLaunch& a, PastCaches past, hipStream_t s) {
+  if (past == kAllPast) write_of_kind<D, QT, HALF, kAllPast>(a, s);
+  else if (past == kReadPast) write_of_kind<D, QT, HALF, kReadPast>(a, s);
+  else write_of_kind<D, QT, HALF, kCached>(a, s);
 }
 template <int D, int QT>
-void write_of_style(const WriteLaunch& a, bool once, hipStream_t s) {
-  if (a.rope_style == TRI_ROPE_HALF) once ? write_of_kind<D, QT, true, true>(a, s) : write_of_kind<D, QT, true, false>(a, s);
-  else once ? write_of_kind<D, QT, false, true>(a, s) : write_of_kind<D, QT, false, false>(a, s);
+void write_of_style(const WriteLaunch& a, PastCaches past, hipStream_t s) {
+  if (a.rope_style == TRI_ROPE_HALF) write_past<D, QT, true>(a, past, s);
+  else write_past<D, QT, false>(a, past, s);
 }
 template <int D>
-void write_of_type(const WriteLaunch& a, bool once, hipStream_t s) {
-  if (a.q_dtype == TRI_KV_FP16) write_of_style<D, TRI_KV_FP16>(a, once, s);
-  else write_of_style<D, TRI_KV_BF16>(a, once, s);
+void write_of_type(const WriteLaunch& a, PastCaches past, hipStream_t s) {
+  if (a.q_dtype == TRI_KV_FP16) write_of_style<D, TRI_KV_FP16>(a, past, s);
+  else write_of_style<D, TRI_KV_BF16>(a, past, s);
 }
 template <int CT>
 void read_to_type(const ReadLaunch& a, hipStream_t s) {
@@ -459,12 +472,15 @@ hipError_t launch_write_paged(WriteLaunch a, hipStream_t s) {
   // heads of 128, calls aiming at 8192, 4096 and 2048 waves: 256 rows 6.1, 6.1, 6.2 us, 512 rows 8.9, 9.2, 7.2, 1024 rows 16.1, 11.4, 10.8,
   // 2048 rows 18.5, 13.8, 13.9.
   a.waves_per_row = (int)std::min<int64_t>(steps, std::max<int64_t>(1, 2048 / a.num_rows));
-  // Rows that the last cache (256 MB) cannot have held from the product that made them are read past the caches, which then
-  // keep what is written: 16384 of those rows (201 MB) 77 us against 90.  Of 4096 rows, which can come out of that cache, 24 against 20.
-  const bool once = (int64_t)a.num_rows * (a.Hq + 2 * a.Hkv) * a.D * 2 > (128ll << 20);
-  if (a.D == 64) write_of_type<64>(a, once, s);
-  else if (a.D == 128) write_of_type<128>(a, once, s);
-  else write_of_type<256>(a, once, s);
+  // Many rows are read past the caches, which keep what is written; of even more rows the queries go past them too, and what is
+  // cached stays.  Calls on three sets of rows in turn, outputs kept for one call, plain, reads past, both past, us: 42 MB of rows 20.1,
+  // 22.8, 21.6; 50 MB 24.7, 23.9, 24.6; 84 MB 41.4, 34.3, 36.8; 100 MB 49.3, 44.2, 44.4; 105 MB 43.8, 37.7, 41.0; 168 MB 75.1, 73.0, 68.9;
+  // 201 MB 90.2, 89.9, 79.9.
+  const int64_t bytes = (int64_t)a.num_rows * (a.Hq + 2 * a.Hkv) * a.D * 2;
+  const PastCaches past = bytes > (128ll << 20) ? kAllPast : bytes > (64ll << 20) ? kReadPast : kCached;
+  if (a.D == 64) write_of_type<64>(a, past, s);
+  else if (a.D == 128) write_of_type<128>(a, past, s);
+  else write_of_type<256>(a, past, s);
   return hipGetLastError();
 }
 
