@@ -137,6 +137,19 @@ def test_verification_refuses(params, code, word):
     assert word in lib.tri_last_error()
 
 
+@pytest.mark.parametrize("params", [
+    dict(num_seqs=1 << 24, max_rows=1),                                     # 2^24 sequences of four waves would fit, of eight not
+    dict(num_seqs=(1 << 23) + 1, max_rows=1, draft_probs=8, draft_stride=1000),
+    dict(num_seqs=1 << 21, max_rows=64),
+])
+def test_verification_refuses_launches_beyond_the_largest(params):
+    """Whole workgroups count: a sequence of one row or piece takes one."""
+    lib = _lib.load()
+    p = _verify(**params)
+    assert lib.tri_verify_drafts(C.byref(p), 256, 1 << 40, None) == UNSUPPORTED
+    assert b"in one call" in lib.tri_last_error()
+
+
 @pytest.mark.parametrize("params,word", [
     (dict(rows=None), b"rows"), (dict(counts=None), b"counts"), (dict(next=None), b"next"), (dict(row_starts=None), b"row_starts"),
     (dict(target=None), b"target"), (dict(tokens=None), b"tokens"), (dict(uniforms=None), b"uniforms"),

@@ -1309,10 +1309,10 @@ int plan_verify(const tri_verify_params* p, VerifyPlan& d) {
     return fail(TRI_ERR_INVALID_ARGUMENT, "a row's stride is less than vocab %d", p->vocab);
   tri::VerifyLaunch& a = d.a;
   a.pieces = (int)tri::ceil_div64(p->vocab, tri::kVerifyPiece);
-  // (a wave for each piece of a row, and of what a rejection leaves of a sequence's: a launch has less than 2^32 threads)
-  const int64_t most = std::max<int64_t>(p->num_rows, (int64_t)p->num_seqs * 2);
-  if (most * a.pieces > kMostWaves || (int64_t)p->num_seqs * p->max_rows > kMostWaves)
-    return fail(TRI_ERR_UNSUPPORTED, "%d rows of %d logits in one call", p->num_rows, p->vocab);
+  // (a wave for each piece of a row, and of a sequence for each row or each piece of what a rejection leaves, in workgroups of up to eight)
+  const int64_t beside = tri::align_up(p->draft_probs ? a.pieces : p->max_rows, 8);
+  if ((int64_t)p->num_rows * a.pieces > kMostWaves || p->num_seqs * beside > kMostWaves)
+    return fail(TRI_ERR_UNSUPPORTED, "%d sequences, %d rows of %d logits in one call", p->num_seqs, p->num_rows, p->vocab);
   a.B = p->num_seqs; a.num_rows = p->num_rows; a.max_rows = p->max_rows; a.vocab = p->vocab;
   a.target_dtype = p->target_dtype; a.probs = p->target_probs ? 1 : 0;
   a.target = p->target; a.target_stride = p->target_stride; a.tokens = p->tokens; a.row_starts = p->row_starts; a.parents = p->parents;
