@@ -264,8 +264,8 @@ __device__ __forceinline__ const void* row_of(const VerifyLaunch& a, int row) {
 }
 
 // A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.  Bound by vector instructions
-// (20 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 23.4 us, of which those take 20;
-// 161 rows of 100003 fp32 ones, 64 MB, in 16.3, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
+// (19 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 22.9 us, of which those take 17 at
+// 2.4 GHz; 161 rows of 100003 fp32 ones, 64 MB, in 16.3, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
 // the caches, two halves of 16 bytes side by side for fp32 and a shorter form for rows whose numbers lie near each other gained nothing.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunch a) {
