@@ -368,6 +368,78 @@ def test_write_many_rows(rows):
         _near(got, want, (d / 2 + 20) * 2.0 ** -24 * both, BF16, "sample")
 
 
+@pytest.mark.parametrize("rows", [8000, 15000])
+@pytest.mark.parametrize("dtype,row_scales", [(BF16, False), (FP16, False), (FP8, True), (FP8, False)])
+@pytest.mark.parametrize("half,norm", [(True, True), (False, False)])
+def test_write_of_many_rows_is_that_of_few(rows, dtype, row_scales, half, norm):
+    """74 and 138 MB of rows, read and stored past the caches: the bits of three calls of a third, with the queries in place and beside."""
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    hq, h, d, block, n = 28, 4, 128, 16, rows // 3
+    lens = [n, n, rows - 2 * n]
+    query = FP16 if dtype is FP16 else BF16
+    tables, at = [], 0
+    for x in lens:
+        tables.append(list(range(at, at + -(-x // block))))
+        at += -(-x // block)
+    starts = [0, n, 2 * n, rows]
+    qkv = torch.randn(rows, hq + 2 * h, d, generator=g, device=DEV).to(query)
+    w = (1 + 0.2 * torch.randn(d, generator=g, device=DEV)).to(query) if norm else None
+    pos = torch.arange(rows, device=DEV) + 1000
+    inv = rope.default_inv_freq(d, 1e6).to(DEV)
+    style = "half" if half else "interleaved"
+
+    def cache():
+        k, v = (torch.zeros(at, block, h, d, dtype=torch.uint8 if dtype is FP8 else dtype, device=DEV) for _ in range(2))
+        if dtype is FP8:
+            k, v = k.view(FP8), v.view(FP8)
+        scales = [torch.zeros(at * block * h, device=DEV) for _ in range(2)] if row_scales else None
+        return k, v, scales, ops.PagedKV([k], [v], style, [scales[0]] if scales else None, [scales[1]] if scales else None)
+
+    def write(kv, of, a, b, out=None):
+        batch = ops.StepBatch(torch.device(DEV), [lens[i] for i in of], block_tables=[tables[i] for i in of])
+        dstarts = torch.tensor([starts[i] - a for i in of] + [b - a], dtype=torch.int32, device=DEV)
+        x = rest[a:b]
+        return ops.write_paged(kv, batch, x[:, :hq], x[:, hq:hq + h], x[:, hq + h:], pos[a:b], inv, row_starts=dstarts, q_norm=w, k_norm=w, out=out)
+
+    rest = qkv
+    k1, v1, s1, kv1 = cache()
+    parts = torch.cat([write(kv1, [i], starts[i], starts[i + 1]) for i in range(3)])
+    for in_place in (False, True):
+        rest = qkv.clone()
+        k2, v2, s2, kv2 = cache()
+        whole = write(kv2, [0, 1, 2], 0, rows, rest[:, :hq] if in_place else None)
+        for a, b in [(parts, whole), (k1, k2), (v1, v2)] + (list(zip(s1, s2)) if s1 else []):
+            assert torch.equal(_bits(a), _bits(b))
+
+
+def test_a_step_on_another_stream_than_the_default_one():
+    """Behind work of that stream which its inputs come from, without a wait of the host."""
+    s = Step([50, 21], rows=[9, 4], dtype=FP8, row_scales=True, norm=BF16, seed=33)
+    kv, batch = s.device()
+    want = s.write(kv, batch).clone()
+    rk, rv = ops.read_paged(kv, batch, s.dstarts, s.num_rows)
+    accepted = torch.tensor([[0, 3, 8], [0, 2, -1]], dtype=torch.int32, device=DEV)
+    counts = torch.tensor([3, 2], dtype=torch.int32, device=DEV)
+    lens = ops.accept_drafts(kv, batch, s.dstarts, accepted, counts)
+    after = [x.clone() for x in (s.dk[0], s.dv[0])]
+    kv, batch = s.device()
+    q = s.dq.clone()
+    s.dq.zero_()
+    accepted_too = torch.zeros_like(accepted)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        s.dq.copy_(q)
+        accepted_too.copy_(accepted)
+        out = s.write(kv, batch)
+        k2, v2 = ops.read_paged(kv, batch, s.dstarts, s.num_rows)
+        lens2 = ops.accept_drafts(kv, batch, s.dstarts, accepted_too, counts)
+    torch.cuda.synchronize()
+    for a, b in ((want, out), (rk, k2), (rv, v2), (lens, lens2), (after[0], s.dk[0]), (after[1], s.dv[0])):
+        assert torch.equal(_bits(a), _bits(b))
+
+
 def test_without_a_block_table():
     """A dense cache: a sequence is one block of it.  Written, read, and its accepted rows moved."""
     s = Step([40, 33, 12], rows=[40, 5, 12], block=64, layers=2, norm=FP32, seed=22)
