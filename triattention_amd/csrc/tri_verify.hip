@@ -15,7 +15,7 @@
 //
 // Two launches a call.  A third, for what the last workgroup of a sequence does, took 4 us more of the host and 3 of the GPU; one launch for
 // all of it would need counters cleared before it.  One chain of six rows of 32768 logits 4.2 + 7.0 us, 60 greedy rows of 131072
-// 4.7 + 4.5: launches and dependent reads; the host behind them takes 15.
+// 4.7 + 4.5: launches and dependent reads; the host behind them takes 14.
 #include <algorithm>
 #include <cfloat>
 

@@ -1138,21 +1138,24 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, row_starts: torch.
                 or (vocab > 1 and draft_probs.stride(1) != 1)):
             raise ValueError(f"draft_probs must be a fp32 tensor [{rows}, {vocab}] on {target.device}, the vocabulary contiguous")
         draft, draft_stride = draft_probs.data_ptr(), draft_probs.stride(0)
-    # one allocation for the three answers
+    given = (seqs, rows, max_rows, vocab, _REALS[dtype], probs, target.data_ptr(), target.stride(0),
+             _check_vector(target, "tokens", tokens, torch.int32, (rows,)),
+             _check_vector(target, "row_starts", row_starts, torch.int32, (seqs + 1,)),
+             0 if parents is None else _check_vector(target, "parents", parents, torch.int32, (rows,)),
+             _check_vector(target, "uniforms", uniforms, torch.float32, (rows, 2)),
+             0 if temperatures is None else _check_vector(target, "temperatures", temperatures, torch.float32, (seqs,)),
+             draft, draft_stride)
+    nbytes = lib.tri_verify_workspace_bytes(_verify_params(*given, 0, 0, 0))
+    if nbytes == 0:
+        raise ValueError("invalid verification: " + lib.tri_last_error().decode("utf-8", "replace"))
+    # one allocation for the three answers and, behind them, the scratch (16 bytes for 2048 logits; two allocations take 1.2 us more)
     n = seqs * max_rows
-    answer = torch.empty(n + 2 * seqs, dtype=torch.int32, device=target.device)
-    at = answer.data_ptr()
-    p = _verify_params(seqs, rows, max_rows, vocab, _REALS[dtype], probs, target.data_ptr(), target.stride(0),
-                       _check_vector(target, "tokens", tokens, torch.int32, (rows,)),
-                       _check_vector(target, "row_starts", row_starts, torch.int32, (seqs + 1,)),
-                       0 if parents is None else _check_vector(target, "parents", parents, torch.int32, (rows,)),
-                       _check_vector(target, "uniforms", uniforms, torch.float32, (rows, 2)),
-                       0 if temperatures is None else _check_vector(target, "temperatures", temperatures, torch.float32, (seqs,)),
-                       draft, draft_stride, at, at + 4 * n, at + 4 * (n + seqs))
-    nbytes = lib.tri_verify_workspace_bytes(p)
-    buf, ws = _scratch(target, nbytes, "verification")
-    _call(target.device, lib.tri_verify_drafts, p, ws, nbytes)
-    accepted, counts, following = torch.split_with_sizes(answer, (n, seqs, seqs))
+    buf = row_starts.new_empty(n + 2 * seqs + nbytes // 4 + 64)
+    at = buf.data_ptr()
+    ws = at + 4 * (n + 2 * seqs)
+    ws += -ws % 256
+    _call(target.device, lib.tri_verify_drafts, _verify_params(*given, at, at + 4 * n, at + 4 * (n + seqs)), ws, nbytes)
+    accepted, counts, following, _ = torch.split_with_sizes(buf, (n, seqs, seqs, nbytes // 4 + 64))
     return accepted.view(seqs, max_rows), counts, following
 
 
