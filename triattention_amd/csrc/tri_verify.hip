@@ -266,14 +266,16 @@ __device__ __forceinline__ const void* row_of(const VerifyLaunch& a, int row) {
 // A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.  Bound by vector instructions
 // (19 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 22.9 us, of which those take 17 at
 // 2.4 GHz; 161 rows of 100003 fp32 ones, 64 MB, in 16.3, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
-// the caches, two halves of 16 bytes side by side for fp32 and a shorter form for rows whose numbers lie near each other gained nothing.
+// the caches, two halves of 16 bytes side by side for fp32 and a shorter form for rows whose numbers lie near each other gained nothing; weights
+// against the first step's largest number, while the other steps' loads are on their way, 1 us of the second and lost half of one in the first.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunch a) {
   __shared__ double table[kPowers];
   const int lane = threadIdx.x % kWave;
   for (int64_t i = (int64_t)blockIdx.x * kVerifyThreads + threadIdx.x; i < a.B; i += (int64_t)gridDim.x * kVerifyThreads) a.arrived[i] = 0;
-  const int64_t unit = (int64_t)blockIdx.x * kVerifyWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int row = (int)(unit / a.pieces), piece = (int)(unit % a.pieces);
+  // (scalar numbers, and less than 2^26: a launch's threads are less than 2^32)
+  const int unit = (int)blockIdx.x * kVerifyWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int row = __builtin_amdgcn_readfirstlane(unit / a.pieces), piece = unit - row * a.pieces;
   constexpr int N = PROBS ? kProbs : kRawLogits;
   // what is needed to know the row's temperature comes before the piece: of up to 64 sequences all of it at once
   const double power = own_power();
@@ -394,8 +396,8 @@ __device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, const Po
 }
 
 // The least place whose running sum exceeds u of the whole; piece_sum(i) is piece i's sum, weights(load(i), s, w) a lane's eight weights in
-// its step s.  A wave's work: the pieces' sums tell the piece, whose weights are found anew.  Where rounding leaves nothing above the
-// mark, and for u >= 1, the last place of any weight; -1 if there is none.
+// its step s (of the first 64 pieces lane i asks for piece i's sum).  A wave's work: the pieces' sums tell the piece, whose weights are found
+// anew.  Where rounding leaves nothing above the mark, and for u >= 1, the last place of any weight; -1 if there is none.
 template <class PieceSum, class Load, class Weights>
 __device__ __forceinline__ int draw(const VerifyLaunch& a, double whole, float u, int lane, PieceSum piece_sum, Load load, Weights weights) {
   const double mark = (u > 0.f ? (double)u : 0.0) * whole;
@@ -497,7 +499,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunc
     if (!greedy) {
       const void* const src = row_of<RT, PROBS>(a, first + i);
       const VerifyPart* const part = a.part + (int64_t)(first + i) * a.pieces;
-      token = draw(a, t.sum, u, lane, [&](int piece) { return against<PROBS>(powers, part[piece], t.most, c); },
+      token = draw(a, t.sum, u, lane, [&](int piece) { return against<PROBS>(powers, piece < kWave ? mine : part[piece], t.most, c); },
                    [&](int piece) { return load_piece<RT, N>(a, src, piece, lane); },
                    [&](const Piece<RT>& held, int s, double (&w)[8]) { weights_or_probs<PROBS>(powers, numbers_of<RT, N>(held.step[s]), t.most, c, w); });
     }
@@ -614,7 +616,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
   const void* const src = row_of<RT, PROBS>(a, row);
   const float* const q = a.draft + (int64_t)(row + 1) * a.draft_stride;
   double* const rest = a.rest + (int64_t)b * a.pieces;
-  double whole = 0.0;
+  double whole = 0.0, own = 0.0;
   if (partly) {
     const int piece = group * kChainWaves + wave;
     if (piece < a.pieces) {
@@ -630,7 +632,9 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
       if (lane == 0) rest[piece] = sum;
     }
     if (!last_to_arrive(a, b, groups) || wave) return;
-    for (int i = lane; i < a.pieces; i += kWave) whole += rest[i];
+    own = lane < a.pieces ? rest[lane] : 0.0;
+    whole = own;
+    for (int i = lane + kWave; i < a.pieces; i += kWave) whole += rest[i];
     whole = sum_of_wave(whole);
   }
   int token = t.where;
@@ -639,7 +643,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
     const bool left = whole > kNothing;  // (or rounding left nothing)
     const VerifyPart* const part = a.part + (int64_t)row * a.pieces;
     const double per_sum = left ? 1.0 / t.sum : 1.0;
-    token = draw(a, left ? whole : t.sum, u, lane, [&](int piece) { return left ? rest[piece] : against<PROBS>(powers, part[piece], t.most, c); },
+    token = draw(a, left ? whole : t.sum, u, lane, [&](int piece) { return left ? (piece < kWave ? own : rest[piece]) : against<PROBS>(powers, part[piece], t.most, c); },
                  [&](int piece) { return load_rest<RT, N>(a, src, left ? q : nullptr, piece, lane); },
                  [&](const Rest<RT>& held, int s, double (&w)[8]) { rest_of<RT, PROBS>(powers, held, s, t.most, per_sum, c, w); });
   }
