@@ -264,8 +264,8 @@ __device__ __forceinline__ const void* row_of(const VerifyLaunch& a, int row) {
 }
 
 // A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.  Bound by vector instructions
-// (19 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 22.9 us, of which those take 17 at
-// 2.4 GHz; 161 rows of 100003 fp32 ones, 64 MB, in 16.3, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
+// (18 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 22.6 us, 80 % of whose cycles those
+// take; 161 rows of 100003 fp32 ones, 64 MB, in 16.7 and 66 %, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
 // the caches, two halves of 16 bytes side by side for fp32 and a shorter form for rows whose numbers lie near each other gained nothing; weights
 // against the first step's largest number, while the other steps' loads are on their way, 1 us of the second and lost half of one in the first.
 template <int RT, bool PROBS>
@@ -560,9 +560,9 @@ __device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& he
 }
 
 // Every workgroup of a sequence finds for itself which rows are accepted (a wave a row); where one is not, each takes some pieces of what
-// that leaves, and the last one draws from it.  48 chains of up to eight rows of 131072 logits 18.3 us: 4 until the rows are decided, 8 for the
-// 38 MB of logits and draft probabilities of the rejected ones (4.7 TB/s), 1.5 until the last has come, 5 for its draw.  Workgroups of four
-// and of sixteen waves 19.0 and 19.8.
+// that leaves, and the last one draws from it.  48 chains of up to eight rows of 131072 logits 17.5 us: 4 until the rows are decided, 8 for the
+// 38 MB of logits and draft probabilities of the rejected ones (4.7 TB/s), 1.5 until the last has come, 4 for its draw.  Workgroups of four
+// and of sixteen waves were 1 us slower.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLaunch a, int groups) {
   constexpr int N = PROBS ? kProbs : kLogits;
