@@ -5,8 +5,8 @@
 // the last accepted row the next token is drawn from p, or where a row was rejected from max(p - q, 0) over its sum.  Without
 // them (chain or tree): every row's token is drawn from p (T = 0: the first largest), and the walk goes on to the child that holds it.
 // A draw is the least x whose running sum exceeds u times the whole.  Which token that is must not depend on the order of a sum:
-// exponentials and sums are 64-bit, off by some 2^-43 of the whole, and of 2^17 boundaries between tokens one lies that
-// near a random number once in 2^25 draws.
+// exponentials and sums are 64-bit, off by some 2^-44 of the whole, and of 2^17 boundaries between tokens one lies that
+// near a random number once in 2^26 draws.
 //
 //  verify_sums_kernel  : every row's pieces of 2048 logits, a wave each: largest, where, and the sum of w against that
 //  verify_walk_kernel  : (no draft probabilities) a wave draws a row's token, a sequence's last workgroup walks
@@ -14,8 +14,8 @@
 //  accept_rows_kernel  : rows of the accepted path to consecutive slots, every layer
 //
 // Two launches a call.  A third, for what the last workgroup of a sequence does, took 4 us more of the host and 3 of the GPU; one launch for
-// all of it would need counters cleared before it.  One chain of six rows of 32768 logits 4.2 + 7.0 us, 60 greedy rows of 131072
-// 4.7 + 4.5: launches and dependent reads; the host behind them takes 14.
+// all of it would need counters cleared before it.  One chain of six rows of 32768 logits 4.1 + 7.4 us, 60 greedy rows of 131072
+// 5.7 + 4.6: launches and dependent reads; the host behind them takes 14.
 #include <algorithm>
 #include <cfloat>
 
@@ -34,56 +34,71 @@ constexpr int kVerifyWaves = kVerifyThreads / kWave;
 constexpr int kChainThreads = 512;
 constexpr int kChainWaves = kChainThreads / kWave;
 
-// 2^y, y <= 0, never less than 2^-1000 (which NaN gives too): y = n + j / 32 + f, rounded by an addition; 2^f on [-1/64, 1/64] by its Chebyshev
-// interpolation of degree 4 (off by 2^-43.5 of it), 2^(j/32) out of LDS, n into the exponent: twelve vector instructions and an LDS read.
-// 262 rows of 131072 logits, the sums' kernel as it then was: a Taylor series of degree 11 on [-1/2, 1/2] 43 us, the interpolation of
-// degree 9 with scalar coefficients (fourteen instructions) 32, this one 27.  The table is 32 numbers because those lie in 64 different banks: lanes read
-// the same word or different banks.  The coefficients are kept from being constants that the compiler copies into vector registers
-// before every step: they are the products' scalar operand.
+// 2^(c d) of numbers d <= 0 times c >= 2^-200, never less than about 2^-1000 (which NaN gives too): c d = n + j / 256 + f, rounded by an addition; 2^f on
+// [-1/512, 1/512] by 1 and f times the Chebyshev interpolation of degree 2 (off by 2^-44.7 of it), 2^(j/256) out of LDS, n into the exponent:
+// ten vector instructions and an LDS read.  262 rows of 131072 logits, the sums' kernel as it then was: a Taylor series of degree 11 on
+// [-1/2, 1/2] 43 us, the interpolation of degree 9 with scalar coefficients 32, degree 4 and a table of 32 numbers 27; that table's whole
+// call at its best 39.5, this one's 37.  Lanes meet in the banks of 256 numbers and not in those of 32, but a place among 256 is the low
+// byte of the units and needs no mask, and a product is saved.  The coefficients are kept from being constants that the compiler copies
+// into vector registers before every step: they are the products' scalar operand.
 constexpr double kLeastPower = -1000.0;
-constexpr int kPowers = 32;
+constexpr int kTable = 256;
+static_assert(kVerifyThreads >= kTable && kChainThreads >= kTable, "a thread makes a number of the table");
 struct Powers {
-  const double* table;      // 2^(j/32) with j << 15 taken off its high word: what y's units of 1/32, shifted as far, add to it is n alone
-  double c[4];
-  __device__ __forceinline__ explicit Powers(const double* in_lds) : table(in_lds) {
-    const double exact[4] = {0.6931471805351095, 0.24022650695623157, 0.055504515573860415, 0.009618176115571158};
+  const double* table;      // 2^(j/256) with j << 12 taken off its high word: what the units of 1/256, shifted as far, add to it is n alone
+  double per, least;
+  double c[3];
+  __device__ __forceinline__ Powers(const double* in_lds, double per_number)
+      : table(in_lds), per(per_number), least(kLeastPower * __builtin_amdgcn_rcp(per_number)) {
+    const double exact[3] = {0.6931471805599453, 0.24022653447679007, 0.05550411247958329};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 3; ++i) {
       c[i] = exact[i];
       asm("" : "+s"(c[i]));
     }
   }
-  // eight of them: the table's words are all asked for before the first is used
-  __device__ __forceinline__ void operator()(double (&y)[8]) const {
+  // Factors of eight of them, one in [2^-1/512, 2^1/512]: the table's words are all asked for before the first is used.
+  __device__ __forceinline__ void factors(double (&d)[8], double (&power)[8]) const {
+    constexpr double kUnits = 26388279066624.0;      // 1.5 * 2^44: a sum's low bits are units of 1/256
     uint32_t units[8];
-    double power[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      y[e] = fmax(y[e], kLeastPower);
-      const double shifted = y[e] + 211106232532992.0;      // 1.5 * 2^47: the sum's low bits are the units
+      d[e] = fmax(d[e], least);
+      const double shifted = __builtin_fma(d[e], per, kUnits);
       units[e] = (uint32_t)__builtin_bit_cast(uint64_t, shifted);
-      power[e] = table[units[e] % kPowers];
-      y[e] -= shifted - 211106232532992.0;
+      power[e] = table[units[e] % kTable];
+      d[e] = __builtin_fma(d[e], per, kUnits - shifted);
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      double p = __builtin_fma(c[3], y[e], c[2]);
-      p = __builtin_fma(p, y[e], c[1]);
-      p = __builtin_fma(p, y[e], c[0]);
-      p = __builtin_fma(p, y[e], 1.0);
+      const double p = __builtin_fma(__builtin_fma(c[2], d[e], c[1]), d[e], c[0]);
+      d[e] = __builtin_fma(p, d[e], 1.0);
       u32x2 words = __builtin_bit_cast(u32x2, power[e]);
-      words.y += units[e] << 15;
-      y[e] = p * __builtin_bit_cast(double, words);
+      words.y += units[e] << 12;
+      power[e] = __builtin_bit_cast(double, words);
     }
   }
-  __device__ __forceinline__ double operator()(double y) const {
-    double eight[8] = {y, 0, 0, 0, 0, 0, 0, 0};
+  __device__ __forceinline__ void operator()(double (&d)[8]) const {
+    double power[8];
+    factors(d, power);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e] *= power[e];
+  }
+  // added to two sums
+  __device__ __forceinline__ void add(double (&d)[8], double (&sums)[2]) const {
+    double power[8];
+    factors(d, power);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[e % 2] = __builtin_fma(d[e], power[e], sums[e % 2]);
+  }
+  __device__ __forceinline__ double operator()(double d) const {
+    double eight[8] = {d, 0, 0, 0, 0, 0, 0, 0};
     (*this)(eight);
     return eight[0];
   }
 };
-// 2^(j/32), as the table holds them.
-__device__ const double kPowerTable[kPowers] = {
+// 2^(j/32) and 2^(j/256), whose products the table holds.
+__device__ const double kCoarse[32] = {
     1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
     1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
     1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
@@ -92,27 +107,27 @@ __device__ const double kPowerTable[kPowers] = {
     1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
     1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
     1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
+__device__ const double kFine[8] = {1.0, 1.0027112750502025, 1.0054299011128027, 1.0081558981184175,
+                                   1.0108892860517005, 1.0136300849514894, 1.016378314910953, 1.019133996077738};
 // A thread's word of the table is asked for before all else and put into LDS where it has come (the counter of a wave's loads goes in
 // their order: a load behind those of a piece would be waited for with them).
-__device__ __forceinline__ double own_power() { return kPowerTable[threadIdx.x % kPowers]; }
+__device__ __forceinline__ double own_power() { return kCoarse[threadIdx.x / 8 % 32] * kFine[threadIdx.x % 8]; }
 __device__ __forceinline__ void keep_power(double* table, double own) {
-  if (threadIdx.x < kPowers) {
-    u32x2 words = __builtin_bit_cast(u32x2, own);
-    words.y -= threadIdx.x << 15;
-    table[threadIdx.x] = __builtin_bit_cast(double, words);
-  }
+  u32x2 words = __builtin_bit_cast(u32x2, own);
+  words.y -= threadIdx.x % kTable << 12;
+  if (threadIdx.x < kTable) table[threadIdx.x] = __builtin_bit_cast(double, words);
 }
 
 // What weighs no more than this beside the largest (-inf, NaN, and numbers that far below it) has nothing.
 constexpr double kNothing = 0x1p-900;
-// w of logits against the largest one, c = log2 e / T; of what has nothing 2^-1000 at least.
-__device__ __forceinline__ void weights_of(const Powers& powers, const float (&x)[8], double most, double c, double (&w)[8]) {
+// w of logits against the largest one; of what has nothing 2^-1000 at least.
+__device__ __forceinline__ void weights_of(const Powers& powers, const float (&x)[8], double most, double (&w)[8]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = ((double)x[e] - most) * c;
+  for (int e = 0; e < 8; ++e) w[e] = (double)x[e] - most;
   powers(w);
 }
-__device__ __forceinline__ double weight_of(const Powers& powers, float x, double most, double c) {
-  const double w = powers(((double)x - most) * c);
+__device__ __forceinline__ double weight_of(const Powers& powers, float x, double most) {
+  const double w = powers((double)x - most);
   return w > kNothing ? w : 0.0;
 }
 
@@ -249,10 +264,10 @@ __device__ __forceinline__ int rows_of_sequence(const VerifyLaunch& a, int b, in
   if (first < 0 || end <= first) return 0;
   return min(end - first, a.max_rows);
 }
-// log2 e / T; 0 where the sequence takes the largest (T not above 0).
+// log2 e / T (of an infinite T so little that all finite logits weigh the same); 0 where the sequence takes the largest (T not above 0).
 __device__ __forceinline__ double sharpness(float temperature, bool& greedy) {
   greedy = !(temperature > 0.f);
-  return greedy ? 0.0 : 1.44269504088896340736 / (double)temperature;
+  return greedy ? 0.0 : fmax(1.44269504088896340736 / (double)temperature, 0x1p-200);
 }
 __device__ __forceinline__ double sharpness_of(const VerifyLaunch& a, int b, bool& greedy) {
   return sharpness(a.temperatures ? a.temperatures[b] : 1.f, greedy);
@@ -264,13 +279,13 @@ __device__ __forceinline__ const void* row_of(const VerifyLaunch& a, int row) {
 }
 
 // A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.  Bound by vector instructions
-// (18 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 22.6 us, 80 % of whose cycles those
-// take; 161 rows of 100003 fp32 ones, 64 MB, in 16.7 and 66 %, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
+// (16 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 20.6 us, 79 % of whose cycles those
+// take; 161 rows of 100003 fp32 ones, 64 MB, in 15.8 and 58 %, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
 // the caches, two halves of 16 bytes side by side for fp32 and a shorter form for rows whose numbers lie near each other gained nothing; weights
 // against the first step's largest number, while the other steps' loads are on their way, 1 us of the second and lost half of one in the first.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunch a) {
-  __shared__ double table[kPowers];
+  __shared__ double table[kTable];
   const int lane = threadIdx.x % kWave;
   for (int64_t i = (int64_t)blockIdx.x * kVerifyThreads + threadIdx.x; i < a.B; i += (int64_t)gridDim.x * kVerifyThreads) a.arrived[i] = 0;
   // (scalar numbers, and less than 2^26: a launch's threads are less than 2^32)
@@ -330,29 +345,30 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunc
     sum = sum_of_wave(sum);
   } else if (most > -INFINITY) {
     // (what weighs less than 2^-1000 counts as that here: the largest weighs 1)
-    const Powers powers(table);
+    const Powers powers(table, c);
     const double largest = most;
+    double sums[2] = {0.0, 0.0};
 #pragma unroll
     for (int s = 0; s < kPieceSteps; ++s) {
       const Numbers8 n = numbers_of<RT, N>(held.step[s]);
-      double w[8];
+      double d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = ((double)n.x[e] - largest) * c;
-      powers(w);
-      sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      for (int e = 0; e < 8; ++e) d[e] = (double)n.x[e] - largest;
+      powers.add(d, sums);
     }
+    sum = sums[0] + sums[1];
     sum = sum_of_wave(sum);
   }
   if (lane == 0) a.part[unit] = VerifyPart{sum, top, piece * kVerifyPiece + where};
 }
 
 template <bool PROBS>
-__device__ __forceinline__ void weights_or_probs(const Powers& powers, const Numbers8& n, float most, double c, double (&w)[8]) {
+__device__ __forceinline__ void weights_or_probs(const Powers& powers, const Numbers8& n, float most, double (&w)[8]) {
   if constexpr (PROBS) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = n.x[e];
   } else {
-    weights_of(powers, n.x, most, c, w);
+    weights_of(powers, n.x, most, w);
   }
 }
 
@@ -365,9 +381,9 @@ struct RowTotal {
 
 // The sum of a piece's weights against the row's largest number.
 template <bool PROBS>
-__device__ __forceinline__ double against(const Powers& powers, const VerifyPart& p, float most, double c) {
+__device__ __forceinline__ double against(const Powers& powers, const VerifyPart& p, float most) {
   if constexpr (PROBS) return p.sum;
-  else return p.sum == 0.0 ? 0.0 : p.sum * weight_of(powers, p.most, most, c);
+  else return p.sum == 0.0 ? 0.0 : p.sum * weight_of(powers, p.most, most);
 }
 
 __device__ __forceinline__ VerifyPart first_part(const VerifyLaunch& a, int row, int lane) {
@@ -375,7 +391,7 @@ __device__ __forceinline__ VerifyPart first_part(const VerifyLaunch& a, int row,
 }
 // (a row of up to 2^17 numbers: one piece a lane, `mine`)
 template <bool PROBS>
-__device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, const Powers& powers, int row, const VerifyPart& mine, double c, int lane) {
+__device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, const Powers& powers, int row, const VerifyPart& mine, int lane) {
   const VerifyPart* part = a.part + (int64_t)row * a.pieces;
   RowTotal t{0.0, -INFINITY, INT32_MAX};
   t.most = mine.most;
@@ -389,8 +405,8 @@ __device__ __forceinline__ RowTotal total_of_row(const VerifyLaunch& a, const Po
   t.where = least_of_wave(t.most == most ? t.where : INT32_MAX);
   t.most = most;
   if (t.most == -INFINITY) t.where = -1;
-  t.sum = against<PROBS>(powers, mine, t.most, c);
-  for (int i = lane + kWave; i < a.pieces; i += kWave) t.sum += against<PROBS>(powers, part[i], t.most, c);
+  t.sum = against<PROBS>(powers, mine, t.most);
+  for (int i = lane + kWave; i < a.pieces; i += kWave) t.sum += against<PROBS>(powers, part[i], t.most);
   t.sum = sum_of_wave(t.sum);
   return t;
 }
@@ -477,7 +493,7 @@ __device__ __forceinline__ bool last_to_arrive(const VerifyLaunch& a, int b, int
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunch a, int max_groups) {
   constexpr int N = PROBS ? kProbs : kLogits;
-  __shared__ double table[kPowers];
+  __shared__ double table[kTable];
   const int b = blockIdx.x / max_groups, group = blockIdx.x % max_groups;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const double power = own_power();
@@ -492,16 +508,16 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunc
   const float u = i < n ? a.uniforms[2 * (int64_t)(first + i) + 1] : 0.f;
   keep_power(table, power);
   __syncthreads();
-  const Powers powers(table);
+  const Powers powers(table, c);
   if (i < n) {
-    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, mine, c, lane);
+    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, mine, lane);
     int token = t.where;
     if (!greedy) {
       const void* const src = row_of<RT, PROBS>(a, first + i);
       const VerifyPart* const part = a.part + (int64_t)(first + i) * a.pieces;
-      token = draw(a, t.sum, u, lane, [&](int piece) { return against<PROBS>(powers, piece < kWave ? mine : part[piece], t.most, c); },
+      token = draw(a, t.sum, u, lane, [&](int piece) { return against<PROBS>(powers, piece < kWave ? mine : part[piece], t.most); },
                    [&](int piece) { return load_piece<RT, N>(a, src, piece, lane); },
-                   [&](const Piece<RT>& held, int s, double (&w)[8]) { weights_or_probs<PROBS>(powers, numbers_of<RT, N>(held.step[s]), t.most, c, w); });
+                   [&](const Piece<RT>& held, int s, double (&w)[8]) { weights_or_probs<PROBS>(powers, numbers_of<RT, N>(held.step[s]), t.most, w); });
     }
     if (lane == 0) picked[i] = token;
   }
@@ -552,15 +568,15 @@ __device__ __forceinline__ Rest<RT> load_rest(const VerifyLaunch& a, const void*
   return x;
 }
 template <int RT, bool PROBS>
-__device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& held, int s, float most, double per_sum, double c, double (&w)[8]) {
+__device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& held, int s, float most, double per_sum, double (&w)[8]) {
   const Numbers8 q = numbers_of<TRI_REAL_FP32, kProbs>(held.draft.step[s]);
-  weights_or_probs<PROBS>(powers, numbers_of<RT, PROBS ? kProbs : kLogits>(held.row.step[s]), most, c, w);
+  weights_or_probs<PROBS>(powers, numbers_of<RT, PROBS ? kProbs : kLogits>(held.row.step[s]), most, w);
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(w[e], per_sum, -(double)q.x[e]), 0.0);
 }
 
 // Every workgroup of a sequence finds for itself which rows are accepted (a wave a row); where one is not, each takes some pieces of what
-// that leaves, and the last one draws from it.  48 chains of up to eight rows of 131072 logits 17.5 us: 4 until the rows are decided, 8 for the
+// that leaves, and the last one draws from it.  48 chains of up to eight rows of 131072 logits 17.2 us: 4 until the rows are decided, 8 for the
 // 38 MB of logits and draft probabilities of the rejected ones (4.7 TB/s), 1.5 until the last has come, 4 for its draw.  Workgroups of four
 // and of sixteen waves were 1 us slower.
 template <int RT, bool PROBS>
@@ -568,7 +584,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
   constexpr int N = PROBS ? kProbs : kLogits;
   __shared__ RowTotal totals[64];
   __shared__ int fits[64];
-  __shared__ double table[kPowers];
+  __shared__ double table[kTable];
   const int b = blockIdx.x / groups, group = blockIdx.x % groups;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const double power = own_power();
@@ -579,7 +595,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
   VerifyPart mine = wave < n ? first_part(a, first + wave, lane) : VerifyPart{};
   keep_power(table, power);
   __syncthreads();
-  const Powers powers(table);
+  const Powers powers(table, c);
   for (int i = wave; i < n; i += kChainWaves) {
     if (i != wave) mine = first_part(a, first + i, lane);
     // what the decision on the next row needs is asked for before the sums are joined
@@ -594,12 +610,12 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
         q = counted<kProbs>(a.draft[next * a.draft_stride + token]);
       }
     }
-    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, mine, c, lane);
+    const RowTotal t = total_of_row<PROBS>(a, powers, first + i, mine, lane);
     bool ok = false;
     if (greedy) {
       ok = t.where >= 0 && token == t.where;
     } else if (token >= 0 && token < a.vocab) {
-      const double w = PROBS ? (double)x : weight_of(powers, x, t.most, c);
+      const double w = PROBS ? (double)x : weight_of(powers, x, t.most);
       ok = (u > 0.f ? (double)u : 0.0) * (double)q * t.sum < w;
     }
     if (lane == 0) {
@@ -625,7 +641,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
 #pragma unroll
       for (int s = 0; s < kPieceSteps; ++s) {
         double w[8];
-        rest_of<RT, PROBS>(powers, held, s, t.most, 1.0 / t.sum, c, w);
+        rest_of<RT, PROBS>(powers, held, s, t.most, 1.0 / t.sum, w);
         sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       }
       sum = sum_of_wave(sum);
@@ -643,9 +659,9 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
     const bool left = whole > kNothing;  // (or rounding left nothing)
     const VerifyPart* const part = a.part + (int64_t)row * a.pieces;
     const double per_sum = left ? 1.0 / t.sum : 1.0;
-    token = draw(a, left ? whole : t.sum, u, lane, [&](int piece) { return left ? (piece < kWave ? own : rest[piece]) : against<PROBS>(powers, part[piece], t.most, c); },
+    token = draw(a, left ? whole : t.sum, u, lane, [&](int piece) { return left ? (piece < kWave ? own : rest[piece]) : against<PROBS>(powers, part[piece], t.most); },
                  [&](int piece) { return load_rest<RT, N>(a, src, left ? q : nullptr, piece, lane); },
-                 [&](const Rest<RT>& held, int s, double (&w)[8]) { rest_of<RT, PROBS>(powers, held, s, t.most, per_sum, c, w); });
+                 [&](const Rest<RT>& held, int s, double (&w)[8]) { rest_of<RT, PROBS>(powers, held, s, t.most, per_sum, w); });
   }
   write_path(a, b, lane, lane, count, token);
 }
