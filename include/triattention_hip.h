@@ -458,7 +458,7 @@ typedef enum tri_real { TRI_REAL_BF16 = 0, TRI_REAL_FP16 = 1, TRI_REAL_FP32 = 2 
  * layer of the cache.  fp8 caches: with v_scale_layers a row's scale is max(largest finite |element| / 448, 2^-126) and is
  * written with it; without, codes stand for code * k_scale (v_scale), numbers beyond 448 of those are the largest code; infinities and NaN become NaN
  * either way.  Angles are 64-bit, norms and rotations 32-bit (what that cannot hold is infinite; the squares of a norm are that from
- * 2^64 on), and every output is rounded once, to nearest.
+ * 2^64 on), scales and the numbers over them too, and every output is rounded once, to nearest, from its 32 bits.
  * A row whose sequence has fewer tokens than rows, or whose block lies outside [0, num_blocks), is not cached, its query is written all the same.
  * Two rows of a call may not have the same slot. */
 typedef struct tri_write_params {

@@ -1,0 +1,71 @@
+"""Writing and reading the paged cache, verification of drafts and the move of accepted rows on an MI355X: the calls at the edge of what
+the entry points allow, against the definitions in 64 bits (oracle/decoding.py) or, where the header states each step of the
+arithmetic, against those steps bit for bit.  Cases and tolerances are those of test_gpu_decoding.py.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import decoding as odec
+from test_gpu_decoding import BF16, DEV, FP8, FP16, FP32, Step, _bits
+from triattention_amd import ops
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------- codes
+def _codes(x: torch.Tensor, unit) -> torch.Tensor:
+    """e4m3 codes as the header states them: the 32-bit quotient, rounded to nearest, beyond 448 the largest."""
+    return (x.float() / unit).clamp(-448, 448).to(FP8).view(torch.uint8)
+
+
+def _still(s: Step):
+    """Positions of zero: keys go into the cache as they come."""
+    s.positions = torch.zeros_like(s.positions)
+    return s
+
+
+def _slots(s: Step, cache):
+    where = odec.places(s.lens, s.starts, s.num_rows, s.tables, s.block, s.pool)
+    return torch.stack([cache.cpu().view(s.pool, s.block, s.h, -1)[page, off] for _, page, off in where])
+
+
+@pytest.mark.parametrize("query", [BF16, FP16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_codes_of_rows_are_those_of_their_quotients(query, dim):
+    """Rows whose largest number is an odd multiple of a power of two and that hold 3/64 of it, 21 of their scales: a tie of two codes, but
+    for the rounding of the scale.  Behind them rows of ordinary numbers, 2^19 in all."""
+    rows = 2 ** 18 // (8 * dim)
+    s = _still(Step([rows + 9], rows=[rows], q_heads=8, kv_heads=8, dim=dim, dtype=FP8, query=query, row_scales=True, seed=dim))
+    for i in range(128):
+        s.qkv[i // 8, 8 + i % 8, 5], s.qkv[i // 8, 16 + i % 8, 9] = 64.0 + i / 2, -64.0 - i / 2
+        s.qkv[i // 8, 8 + i % 8, 6], s.qkv[i // 8, 16 + i % 8, 60] = 3 * (64 + i / 2) / 64, 3 * (64 + i / 2) / 64
+    kv, batch = s.device()
+    s.write(kv, batch)
+    for cache, scales, x in ((s.dk[0], s.dks[0], s.k), (s.dv[0], s.dvs[0], s.v)):
+        unit = (x.float().abs().amax(-1) / 448).clamp(min=2.0 ** -126)
+        assert torch.equal(_bits(_slots(s, scales).squeeze(-1)), _bits(unit))
+        got, want = _slots(s, cache.view(torch.uint8)), _codes(x, unit.unsqueeze(-1))
+        assert torch.equal(got, want), int((got != want).sum())
+
+
+@pytest.mark.parametrize("unit", [130 / 19, 156 / 21, 148 / 31 * 2.0 ** -7, 0.02, 1.9 * 2.0 ** -120, 3e38, 2.0 ** -100, 1.3 * 2.0 ** 90])
+def test_codes_of_a_tensors_scale_are_those_of_the_quotients(unit):
+    """One scale for all: all bf16 numbers whose codes are not 0 or the largest, and some that are."""
+    unit = float(torch.tensor(unit, dtype=FP32))
+    s = _still(Step([2100], rows=[2048], q_heads=2, kv_heads=2, dim=64, dtype=FP8, seed=3))
+    numbers = torch.arange(0, 0x7f80, dtype=torch.int32).to(torch.int16).view(BF16)
+    ratio = numbers.double() / unit
+    numbers = numbers[(ratio > 2.0 ** -13) & (ratio < 2000)]
+    assert numbers.numel() > 1000
+    both = torch.cat([numbers, -numbers])
+    x = both.repeat(-(-2048 * 2 * 64 // both.numel()))[:2048 * 2 * 64].view(2048, 2, 64)
+    s.qkv[:, 2:4], s.qkv[:, 4:6] = x, x.flip(-1)
+    kv, batch = s.device()
+    s.write(kv, batch, k_scale=unit, v_scale=unit)
+    for cache, rows in ((s.dk[0], s.k), (s.dv[0], s.v)):
+        got, want = _slots(s, cache.view(torch.uint8)), _codes(rows, unit)
+        # (a rotation by nothing makes + 0 of - 0 + 0)
+        zero = want & 0x7f == 0
+        assert torch.equal(got[~zero], want[~zero]) and bool((got[zero] & 0x7f == 0).all()), int((got != want)[~zero].sum())

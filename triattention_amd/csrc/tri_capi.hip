@@ -1378,7 +1378,7 @@ int tri_write_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_w
   a.v_stride_row = p->v_stride_row; a.v_stride_head = p->v_stride_head; a.out_stride_row = p->out_stride_row; a.out_stride_head = p->out_stride_head;
   a.positions = p->positions; a.position_stride = p->position_stride; a.freq_axes = p->freq_axes; a.inv_freq = p->inv_freq;
   a.q_norm = p->q_norm; a.k_norm = p->k_norm; a.eps = p->eps; a.rotary_scale = p->rotary_scale;
-  a.k_inv_scale = 1.f / p->k_scale; a.v_inv_scale = 1.f / p->v_scale;
+  a.k_scale = p->k_scale; a.v_scale = p->v_scale;
   return launch_status(tri::launch_write_paged(a, (hipStream_t)stream), "write_paged");
 }
 

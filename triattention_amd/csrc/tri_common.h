@@ -371,7 +371,7 @@ struct WriteLaunch {
   const int32_t* freq_axes;                                // [D / 2], or NULL: axis 0
   const float* inv_freq;
   const void* q_norm; const void* k_norm;                  // [D], or NULL
-  float eps, rotary_scale, k_inv_scale, v_inv_scale;
+  float eps, rotary_scale, k_scale, v_scale;
 };
 hipError_t launch_write_paged(WriteLaunch a, hipStream_t s);
 struct ReadLaunch {
