@@ -4,13 +4,15 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import re
+import subprocess
 
 import pytest
 import torch
 
 from oracle import decoding as odec
 from test_attention import _batch, _layout
-from triattention_amd import _lib, ops, rope
+from triattention_amd import _lib, build, ops, rope
 
 INVALID, UNSUPPORTED = _lib.TRI_ERR_INVALID_ARGUMENT, _lib.TRI_ERR_UNSUPPORTED
 
@@ -307,3 +309,36 @@ def test_oracle_moves_end_where_a_list_is_no_path():
     assert odec.accepted_moves([0, 2, 6], 3, 6) == [(0, 0), (2, 1)]
     assert odec.accepted_moves([-1, 2], 2, 6) == []
     assert odec.accepted_moves([0, 1, 2], 9, 2) == [(0, 0), (1, 1)]
+
+
+# ------------------------------------------------------------------------------------- waits
+def test_stores_of_every_wave_have_arrived_before_its_workgroup_is_counted(tmp_path):
+    """The last workgroup of a sequence reads what every wave of the others stored.  A barrier does not wait for stores on their way, and the
+    counting thread's write-back waits for its own wave's alone: in the compiled kernels each wave waits for its stores right before
+    the barrier behind which the write-back stands."""
+    try:
+        compiler = build.hipcc()
+    except RuntimeError as exc:
+        pytest.skip(str(exc))
+    out = tmp_path / "verify.s"
+    subprocess.run([compiler, *build.HIPCC_FLAGS, f"-I{build.INCLUDE}", f"-I{build.CSRC}", "--cuda-device-only", "-S", str(build.CSRC / "tri_verify.hip"),
+                    "-o", str(out)], check=True, capture_output=True)
+    kernels, lines = {}, None
+    for line in out.read_text().splitlines():
+        if m := re.match(r"(_Z\w*verify_(?:walk|chain)_kernel\w*):", line):
+            lines = kernels.setdefault(m[1], [])
+        elif ".end_amdhsa_kernel" in line or line.startswith("\t.section"):
+            lines = None
+        elif lines is not None and (words := line.split(";")[0].split()):
+            lines.append(words)
+    assert len(kernels) == 8
+    for name, lines in kernels.items():
+        counts = [i for i, words in enumerate(lines) if words[0] == "buffer_wbl2"]
+        assert counts, name
+        for at in counts:
+            barrier = max(i for i in range(at) if lines[i][0] == "s_barrier")
+            # back from the barrier, with no way in from elsewhere and no store between
+            for words in reversed(lines[:barrier]):
+                assert not words[0].endswith(":") and "store" not in words[0] and "atomic" not in words[0], (name, words)
+                if words[0] == "s_waitcnt" and "vmcnt(0)" in words[1:]:
+                    break

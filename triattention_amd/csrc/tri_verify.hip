@@ -474,9 +474,11 @@ __device__ __forceinline__ void write_path(const VerifyLaunch& a, int b, int lan
 }
 
 // Whether this workgroup is the last of `groups` of sequence b to come here: what the others wrote before is then seen by its first wave.
-// (One thread's release after the barrier stands for the workgroup's writes: every wave's own fence made the kernel of 48 chains take 61 us.)
+// Every wave waits until its own stores have left it, which the barrier does not; then one thread's write-back, which waits for its own wave's
+// alone, finds the workgroup's in the cache that it writes back.  (A release of every wave made the kernel of 48 chains take 61 us.)
 __device__ __forceinline__ bool last_to_arrive(const VerifyLaunch& a, int b, int groups) {
   __shared__ int count;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
