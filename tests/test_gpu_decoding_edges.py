@@ -4,11 +4,13 @@ arithmetic, against those steps bit for bit.  Cases and tolerances are those of 
 """
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
 from oracle import decoding as odec
-from test_gpu_decoding import BF16, DEV, FP8, FP16, FP32, Step, _bits
+from test_gpu_decoding import BF16, DEV, FP8, FP16, FP32, Drafts, Step, _bits
 from triattention_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -69,3 +71,28 @@ def test_codes_of_a_tensors_scale_are_those_of_the_quotients(unit):
         # (a rotation by nothing makes + 0 of - 0 + 0)
         zero = want & 0x7f == 0
         assert torch.equal(got[~zero], want[~zero]) and bool((got[zero] & 0x7f == 0).all()), int((got != want)[~zero].sum())
+
+
+# --------------------------------------------------------------------------------- verification
+@pytest.mark.parametrize("least", [-895, -899, -901, -906, -910, -950])
+@pytest.mark.parametrize("kind", ["tree", "draft"])
+def test_verify_pieces_of_weights_that_are_nothing_together_are_something(least, kind):
+    """Tokens of 2^least of the largest, 2048 and more of them one behind the other: beyond 2^-900 each is one that a random number of 0 or 1 names, below
+    it they are nothing, whatever they are together."""
+    vocab, a, b = 3 * 2048 + 100, 4096 - 7, 2048 + 5
+    for low in (range(0, 2048), range(4096, vocab)):
+        for u in (0.0, 0.5, 1.0):
+            d = Drafts([2], vocab, tree=kind == "tree", draft=kind == "draft", seed=1)
+            d.target[0] = -math.inf
+            d.target[0, low.start:low.stop] = least * math.log(2)
+            d.target[0, a], d.target[0, b] = 0.0, -1.0
+            d.uniforms[0, 1] = u
+            if kind == "draft":        # the draft is sure of a, which is rejected
+                d.draft[1] = 0.0
+                d.draft[1, a], d.tokens[1], d.uniforms[1, 0] = 1.0, a, 0.999
+            there = ([b] if kind == "draft" else [b, a]) + (list(low) if least > -900 else [])
+            want = min(there) if u == 0 else max(there) if u == 1 else b if kind == "draft" else a
+            if kind == "tree":
+                d.tokens[1] = -1       # (no child holds the drawn token)
+            rows, counts, following = d.run(max_rows=2)
+            assert (rows.tolist(), counts.tolist(), following.tolist()) == ([[0, -1]], [1], [want]), (low, u)

@@ -2,7 +2,7 @@
 //
 //   w(x) = exp((l(x) - max l) / T),  E = sum w,  p = w / E             (probabilities as they come: w = p)
 // Chain with draft probabilities q: row i + 1, drawn from q[i + 1] behind row i, is accepted iff u q(x) E < w(x) of row i; behind
-// the last accepted row the next token is drawn from p, or where a row was rejected from max(p - q, 0) over its sum.  Without
+// the last accepted row the next token is drawn from p, or where a row was rejected from max(w - q E, 0) over its sum.  Without
 // them (chain or tree): every row's token is drawn from p (T = 0: the first largest), and the walk goes on to the child that holds it.
 // A draw is the least x whose running sum exceeds u times the whole.  Which token that is must not depend on the order of a sum:
 // exponentials and sums are 64-bit, off by some 2^-44 of the whole, and of 2^17 boundaries between tokens one lies that
@@ -10,7 +10,7 @@
 //
 //  verify_sums_kernel  : every row's pieces of 2048 logits, a wave each: largest, where, and the sum of w against that
 //  verify_walk_kernel  : (no draft probabilities) a wave draws a row's token, a sequence's last workgroup walks
-//  verify_chain_kernel : (draft probabilities) which rows are accepted, sums of max(p - q, 0) by pieces; the last workgroup draws
+//  verify_chain_kernel : (draft probabilities) which rows are accepted, sums of max(w - q E, 0) by pieces; the last workgroup draws
 //  accept_rows_kernel  : rows of the accepted path to consecutive slots, every layer
 //
 // Two launches a call.  A third, for what the last workgroup of a sequence does, took 4 us more of the host and 3 of the GPU; one launch for
@@ -548,8 +548,9 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunc
   write_path(a, b, lane, path, count, n > 0 ? __builtin_amdgcn_readlane(want, here) : -1);
 }
 
-// A piece of a row and of the draft probabilities of the row behind it, and what a rejection leaves of its tokens: max(w / E - q, 0).  Where the
-// token comes from the row itself, q is no pointer, and per_sum 1.
+// A piece of a row and of the draft probabilities of the row behind it, and what a rejection leaves of its tokens: max(w - q E, 0), each of them cut
+// where it is nothing (the sums of a piece and of the whole are then something only where a token is).  Where the token comes from the row
+// itself, q is no pointer.
 template <int RT>
 struct Rest {
   Piece<RT> row;
@@ -570,11 +571,14 @@ __device__ __forceinline__ Rest<RT> load_rest(const VerifyLaunch& a, const void*
   return x;
 }
 template <int RT, bool PROBS>
-__device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& held, int s, float most, double per_sum, double (&w)[8]) {
+__device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& held, int s, float most, double sum, double (&w)[8]) {
   const Numbers8 q = numbers_of<TRI_REAL_FP32, kProbs>(held.draft.step[s]);
   weights_or_probs<PROBS>(powers, numbers_of<RT, PROBS ? kProbs : kLogits>(held.row.step[s]), most, w);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = fmax(__builtin_fma(w[e], per_sum, -(double)q.x[e]), 0.0);
+  for (int e = 0; e < 8; ++e) {
+    const double rest = __builtin_fma(-(double)q.x[e], sum, w[e]);
+    w[e] = rest > kNothing ? rest : 0.0;
+  }
 }
 
 // Every workgroup of a sequence finds for itself which rows are accepted (a wave a row); where one is not, each takes some pieces of what
@@ -643,7 +647,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
 #pragma unroll
       for (int s = 0; s < kPieceSteps; ++s) {
         double w[8];
-        rest_of<RT, PROBS>(powers, held, s, t.most, 1.0 / t.sum, w);
+        rest_of<RT, PROBS>(powers, held, s, t.most, t.sum, w);
         sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
       }
       sum = sum_of_wave(sum);
@@ -660,10 +664,9 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
     const float u = a.uniforms[2 * (int64_t)row + 1];
     const bool left = whole > kNothing;  // (or rounding left nothing)
     const VerifyPart* const part = a.part + (int64_t)row * a.pieces;
-    const double per_sum = left ? 1.0 / t.sum : 1.0;
     token = draw(a, left ? whole : t.sum, u, lane, [&](int piece) { return left ? (piece < kWave ? own : rest[piece]) : against<PROBS>(powers, part[piece], t.most); },
                  [&](int piece) { return load_rest<RT, N>(a, src, left ? q : nullptr, piece, lane); },
-                 [&](const Rest<RT>& held, int s, double (&w)[8]) { rest_of<RT, PROBS>(powers, held, s, t.most, per_sum, w); });
+                 [&](const Rest<RT>& held, int s, double (&w)[8]) { rest_of<RT, PROBS>(powers, held, s, t.most, t.sum, w); });
   }
   write_path(a, b, lane, lane, count, token);
 }
