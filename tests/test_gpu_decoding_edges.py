@@ -96,3 +96,30 @@ def test_verify_pieces_of_weights_that_are_nothing_together_are_something(least,
                 d.tokens[1] = -1       # (no child holds the drawn token)
             rows, counts, following = d.run(max_rows=2)
             assert (rows.tolist(), counts.tolist(), following.tolist()) == ([[0, -1]], [1], [want]), (low, u)
+
+
+@pytest.mark.parametrize("temperature", [math.inf, 1e38, 1e36, 1e31, 1e30, 1e28, 1e27, 1.0])
+@pytest.mark.parametrize("kind", ["tree", "draft"])
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+def test_verify_infinities_beside_numbers_that_weigh_something(temperature, kind, dtype):
+    """An infinity is the largest finite number: at a temperature high enough the others of its piece and of other pieces weigh as much, or what
+    their distance leaves them."""
+    d = Drafts([3, 2, 4, 2], 4500, dtype=dtype, tree=kind == "tree", draft=kind == "draft", temperatures=[temperature] * 4, seed=17)
+    for r, places in enumerate([[3000], [7, 8, 4400], [0], [2047, 2048], [], [4499], [100], list(range(0, 4500, 9)), [1, 3001], [5], [9]]):
+        if dtype is FP32:              # numbers next to the largest, 2^104 of one another
+            d.target[r, 20:24] = torch.tensor([0x7f7fffff, 0x7f7ffffe, 0x7f7ffff0, 0x7f7f0000], dtype=torch.int32).view(FP32)
+            d.target[r, 3000:3004] = d.target[r, 20:24].clone()
+        d.target[r, 50:60], d.target[r, 60:62] = -math.inf, math.nan
+        d.target[r, places] = math.inf
+    if kind == "draft":
+        g = torch.Generator().manual_seed(18)
+        d.draft = torch.softmax(0.5 * torch.randn(d.draft.shape, generator=g), -1)
+        for r in range(d.draft.shape[0]):
+            d.tokens[r] = odec.draw(d.draft[r].double(), float(torch.rand(1, generator=g)))
+    else:
+        for b, m in enumerate(d.rows):
+            for r in range(d.starts[b] + 1, d.starts[b] + m):
+                up = d.starts[b] + d.parents[r]
+                d.tokens[r] = odec.draw(odec.distribution(d.target[up], temperature, False), float(d.uniforms[up, 1]))
+    lengths = d.check(d.run(max_rows=4), 4)
+    assert kind == "draft" or max(lengths) > 1

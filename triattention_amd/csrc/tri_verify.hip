@@ -118,6 +118,8 @@ __device__ __forceinline__ void keep_power(double* table, double own) {
   if (threadIdx.x < kTable) table[threadIdx.x] = __builtin_bit_cast(double, words);
 }
 
+// A sharpness from which on infinities, which count as the largest finite number, leave nothing to any other: the next one of 32 bits is 2^104 less.
+constexpr double kAlone = 0x1p-94;
 // What weighs no more than this beside the largest (-inf, NaN, and numbers that far below it) has nothing.
 constexpr double kNothing = 0x1p-900;
 // w of logits against the largest one; of what has nothing 2^-1000 at least.
@@ -334,7 +336,7 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunc
         if (n.x[e] >= top) where = s * kWave * 8 + lane * 8 + e;
     }
     where = most > -INFINITY ? least_of_wave(where) : 0;
-  } else if (PROBS || most == INFINITY) {
+  } else if (PROBS || (most == INFINITY && c >= kAlone)) {
     // (beside infinities all else weighs nothing)
 #pragma unroll
     for (int s = 0; s < kPieceSteps; ++s) {
@@ -342,6 +344,14 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunc
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum += PROBS ? (double)n.x[e] : n.x[e] >= top ? 1.0 : 0.0;
     }
+    sum = sum_of_wave(sum);
+  } else if (most == INFINITY) {
+    // (a temperature of 1e28 or more; one number at a time, so that the loop below keeps its registers)
+    const Powers powers(table, c);
+    const int end = min(kVerifyPiece, a.vocab - piece * kVerifyPiece);
+#pragma unroll 1
+    for (int i = lane; i < end; i += kWave)
+      sum += powers((double)load_one<RT, kLogits>(row_of<RT, PROBS>(a, row), (int64_t)piece * kVerifyPiece + i) - (double)top);
     sum = sum_of_wave(sum);
   } else if (most > -INFINITY) {
     // (what weighs less than 2^-1000 counts as that here: the largest weighs 1)
