@@ -73,6 +73,40 @@ def test_codes_of_a_tensors_scale_are_those_of_the_quotients(unit):
         assert torch.equal(got[~zero], want[~zero]) and bool((got[zero] & 0x7f == 0).all()), int((got != want)[~zero].sum())
 
 
+# -------------------------------------------------------------------------------------- norm
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("norm", [BF16, FP32])
+@pytest.mark.parametrize("dtype,row_scales", [(BF16, False), (FP8, True), (FP8, False)])
+def test_rows_whose_squares_are_infinite_are_nothing(half, norm, dtype, row_scales):
+    """Squares beyond 32 bits are infinite, and numbers over their root 0, the largest bf16 numbers too (times a norm's 1.9 they pass 32 bits); an
+    infinity over it is none, and its pair with it.  A row whose squares 32 bits hold stays what it is."""
+    s = Step([20], rows=[6], dtype=dtype, row_scales=row_scales, half=half, norm=norm, seed=31)
+    s.norms = [torch.full_like(w, 1.875) for w in s.norms]
+    most = float(torch.finfo(BF16).max)
+    s.qkv[0, :10, 7] = most                       # a pair's first, then its second, then both, then all
+    s.qkv[1, :10, 64 + 7] = -most
+    s.qkv[2, :10, 0::2] = most
+    s.qkv[3, :10] = most
+    s.qkv[4, :10, 9] = math.inf
+    s.qkv[5, :10] = s.qkv[5, :10] * 2.0 ** 50
+    kv, batch = s.device()
+    out = s.write(kv, batch).cpu().double()
+    where = odec.places(s.lens, s.starts, s.num_rows, s.tables, s.block, s.pool)
+    (wq, off_q), _ = s.expected()
+    k = torch.stack([s.dk[0].cpu()[page, off].float().double() for _, page, off in where])
+    pair = [9, 9 + 64] if half else [8, 9]
+    for got in (out, k):
+        assert bool((got[:4] == 0).all())
+        assert bool(torch.isnan(got[4][:, pair]).all())
+        rest = torch.ones(128, dtype=torch.bool)
+        rest[pair] = False
+        assert bool((got[4][:, rest] == 0).all()) and bool((got[5] != 0).any())
+    assert bool(((out[5] - wq[5]).abs() <= off_q[5] * (1 + 2 ** -8) + 2.0 ** -8 * wq[5].abs() + 2.0 ** -133).all())
+    if row_scales:
+        scales = _slots(s, s.dks[0]).squeeze(-1)
+        assert bool((scales[:5] == 2.0 ** -126).all()) and bool((scales[5] > 2.0 ** -126).all())
+
+
 # --------------------------------------------------------------------------------- verification
 @pytest.mark.parametrize("least", [-895, -899, -901, -906, -910, -950])
 @pytest.mark.parametrize("kind", ["tree", "draft"])

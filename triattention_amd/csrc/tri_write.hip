@@ -103,7 +103,7 @@ __device__ __forceinline__ uint32_t pack_codes(const float* x, const Unit& u) {
 // A wave's step is 64 / (D / 8) heads of one kind (queries, keys or values) of a row, eight elements a lane: four pairs of the rotation (4l to
 // 4l + 3 and the same behind the head's middle, or 8l to 8l + 7), so that it needs no other lane, and a lane has the same four
 // angles in every head.  A row's steps are shared by waves_per_row waves, which find the angles once each.  Norm and rotation
-// are a product by (w1 cos, w2 sin, w2 cos, w1 sin), the same in every head, and one by the head's 1 / sqrt(mean).
+// are a product by the head's 1 / sqrt(mean) and one by (w1 cos, w2 sin, w2 cos, w1 sin), the same in every head.
 //
 // Bound by reading and writing the rows: 16384 rows of 32 + 2 x 8 heads of 128, 403 MB, in 80 us (5.0 TB/s, a copy's 5.2 to 5.4); 11392
 // rows of 28 + 2 x 4 heads into fp8, 199 MB, in 38.  One row 4.8 us, 64 rows of 64 + 2 x 8 heads with scales 5.5: a launch and its
@@ -215,8 +215,10 @@ __global__ __launch_bounds__(kWriteThreads, 6) void write_paged_kernel(WriteLaun
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int i = HALF ? e : 2 * e, j = HALF ? 4 + e : 2 * e + 1;
-      x[i] = (y[i] * by[e][0] - y[j] * by[e][1]) * inv;
-      x[j] = (y[j] * by[e][2] + y[i] * by[e][3]) * inv;
+      // (the norm first: a product beyond 32 bits times nothing is no number)
+      const float y1 = y[i] * inv, y2 = y[j] * inv;
+      x[i] = y1 * by[e][0] - y2 * by[e][1];
+      x[j] = y2 * by[e][2] + y1 * by[e][3];
     }
   };
 
