@@ -457,7 +457,7 @@ typedef enum tri_real { TRI_REAL_BF16 = 0, TRI_REAL_FP16 = 1, TRI_REAL_FP32 = 2 
  * f][row] * inv_freq[f], times rotary_scale.  The queries go to out, keys and the values as they are into the slots of their tokens in one
  * layer of the cache.  fp8 caches: with v_scale_layers a row's scale is max(largest finite |element| / 448, 2^-126) and is
  * written with it; without, codes stand for code * k_scale (v_scale), numbers beyond 448 of those are the largest code; infinities and NaN become NaN
- * either way.  Angles are 64-bit, norms and rotations 32-bit (what that cannot hold is infinite; the squares of a norm are that from
+ * either way.  Angles are 64-bit products, their cosines and sines times rotary_scale rounded to 32 bits; norms and rotations are 32-bit (what that cannot hold is infinite; the squares of a norm are that from
  * 2^64 on), scales and the numbers over them too, and every output is rounded once, to nearest, from its 32 bits.
  * A row whose sequence has fewer tokens than rows, or whose block lies outside [0, num_blocks), is not cached, its query is written all the same.
  * Two rows of a call may not have the same slot. */

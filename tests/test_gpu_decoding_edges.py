@@ -73,6 +73,35 @@ def test_codes_of_a_tensors_scale_are_those_of_the_quotients(unit):
         assert torch.equal(got[~zero], want[~zero]) and bool((got[zero] & 0x7f == 0).all()), int((got != want)[~zero].sum())
 
 
+# ------------------------------------------------------------------------------------ angles
+@pytest.mark.parametrize("far", [1 << 12, 1 << 20, (1 << 31) - 1, 1 << 44])
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("dim,scale", [(64, 1.0), (128, 1.3), (256, 1.0)])
+def test_unit_pairs_are_turned_into_cosines_and_sines_rounded_once(far, half, dim, scale):
+    """Pairs (1, 0) and (0, 1): 2^20 and more cosines and sines of the 64-bit angle, in 32 bits and then in fp16.  The kernel's are off by 2^-40 of a
+    number of ordinary size before that: 2^20 numbers lie that near the middle between two of 32 bits, where that is one of fp16 too, 2^-9 times."""
+    rows, f = 4096 * 128 // dim, dim // 2
+    s = Step([rows], rows=[rows], q_heads=2, kv_heads=2, dim=dim, dtype=FP16, half=half, far=far, seed=dim)
+    s.qkv[:, :4] = 0.0
+    first = torch.zeros(dim, dtype=torch.bool)
+    first[:f] = True
+    if not half:
+        first = torch.arange(dim) % 2 == 0
+    s.qkv[:, 0::2, first] = 1.0
+    s.qkv[:, 1:4:2, ~first] = 1.0
+    kv, batch = s.device()
+    out = s.write(kv, batch, rotary_scale=scale).cpu()
+    keys = _slots(s, s.dk[0])
+    angle = s.positions[0].double()[:, None] * s.inv_freq.double()
+    c, n = (torch.tensor(scale, dtype=FP32).double() * x for x in (torch.cos(angle), torch.sin(angle)))
+    c, n = c.float().to(FP16), n.float().to(FP16)
+    for got in (out, keys):
+        for head, (one, two) in enumerate(((c, n), (-n, c))):
+            # (by value: the sign of a zero is that of a sum)
+            assert torch.equal(got[:, head, first], one), int((got[:, head, first] != one).sum())
+            assert torch.equal(got[:, head, ~first], two), int((got[:, head, ~first] != two).sum())
+
+
 # -------------------------------------------------------------------------------------- norm
 @pytest.mark.parametrize("half", [True, False])
 @pytest.mark.parametrize("norm", [BF16, FP32])

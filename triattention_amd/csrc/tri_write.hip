@@ -28,21 +28,32 @@ typedef __attribute__((address_space(1))) float* GlobalOutF32;
 enum CacheKind { kPlainRows = 0, kTensorScale = 1, kRowScales = 2 };
 enum PastCaches { kCached = 0, kReadPast = 1, kAllPast = 2 };       // what goes past the caches: reads of q, k and v, stores of q too
 
-// cos and sin of position * inv_freq.  The product and its reduction by pi / 2 are 64-bit: the remainder of an angle of 2^31
-// is off by 2^-54 a step, where an angle in 32 bits would be off by whole turns.  On [-pi/4, pi/4] the Taylor series up to r^9
-// and r^10 in 32 bits (the next terms are below 2e-9).
+// cos and sin of position * inv_freq, times scale, rounded once.  The angle is the 64-bit product: exact for positions below 2^29, at 2^31 off by up to
+// 2^-23, at 2^40 by 2^-14.  What is left of it beside a multiple of pi / 2 is off by 2^-53, and on [-pi/4, pi/4] the Taylor series up to r^13 and
+// r^14 by 2^-45.  (In 32 bits the series were off by a step: one rotated number in 30000 was its neighbour in fp16.)
 __device__ __forceinline__ void turn(double position, float inv_freq, float scale, float& c_out, float& s_out) {
   const double x = position * (double)inv_freq;
   const double n = __builtin_rint(x * 0.636619772367581343075535);
-  double rest = __builtin_fma(-n, 1.57079632679489655799898, x);
-  rest = __builtin_fma(-n, 6.12323399573676603586882e-17, rest);
+  double r = __builtin_fma(-n, 1.57079632679489655799898, x);
+  r = __builtin_fma(-n, 6.12323399573676603586882e-17, r);
   const int quadrant = (int)(n - 4.0 * __builtin_floor(n * 0.25));
-  const float r = (float)rest, z = r * r;
-  const float s = r + r * z * (-1.f / 6 + z * (1.f / 120 + z * (-1.f / 5040 + z * (1.f / 362880))));
-  const float c = 1.f + z * (-0.5f + z * (1.f / 24 + z * (-1.f / 720 + z * (1.f / 40320 + z * (-1.f / 3628800)))));
-  const float cq = quadrant & 1 ? s : c, sq = quadrant & 1 ? c : s;
-  c_out = (quadrant == 1 || quadrant == 2 ? -cq : cq) * scale;
-  s_out = (quadrant >= 2 ? -sq : sq) * scale;
+  const double z = r * r;
+  double s = 1.0 / 6227020800, c = -1.0 / 87178291200;
+  s = __builtin_fma(s, z, -1.0 / 39916800);
+  c = __builtin_fma(c, z, 1.0 / 479001600);
+  s = __builtin_fma(s, z, 1.0 / 362880);
+  c = __builtin_fma(c, z, -1.0 / 3628800);
+  s = __builtin_fma(s, z, -1.0 / 5040);
+  c = __builtin_fma(c, z, 1.0 / 40320);
+  s = __builtin_fma(s, z, 1.0 / 120);
+  c = __builtin_fma(c, z, -1.0 / 720);
+  s = __builtin_fma(s, z, -1.0 / 6);
+  c = __builtin_fma(c, z, 1.0 / 24);
+  s = __builtin_fma(s * z, r, r);
+  c = __builtin_fma(__builtin_fma(c, z, -0.5), z, 1.0);
+  const double cq = quadrant & 1 ? s : c, sq = quadrant & 1 ? c : s;
+  c_out = (float)((quadrant == 1 || quadrant == 2 ? -cq : cq) * scale);
+  s_out = (float)((quadrant >= 2 ? -sq : sq) * scale);
 }
 
 // Over the lanes of a head (8, 16 or 32 of them), the result in each.
