@@ -457,8 +457,9 @@ typedef enum tri_real { TRI_REAL_BF16 = 0, TRI_REAL_FP16 = 1, TRI_REAL_FP32 = 2 
  * f][row] * inv_freq[f], times rotary_scale.  The queries go to out, keys and the values as they are into the slots of their tokens in one
  * layer of the cache.  fp8 caches: with v_scale_layers a row's scale is max(largest finite |element| / 448, 2^-126) and is
  * written with it; without, codes stand for code * k_scale (v_scale), numbers beyond 448 of those are the largest code; infinities and NaN become NaN
- * either way.  Angles are 64-bit products, their cosines and sines times rotary_scale rounded to 32 bits; norms and rotations are 32-bit (what that cannot hold is infinite; the squares of a norm are that from
- * 2^64 on), scales and the numbers over them too, and every output is rounded once, to nearest, from its 32 bits.
+ * either way.  Angles are 64-bit products, their cosines and sines times rotary_scale are rounded to 32 bits, norms and rotations are 32-bit (what
+ * that cannot hold is infinite; the squares of a norm are that from 2^64 on), scales and the numbers over them too, and every
+ * output is rounded once, to nearest, from its 32 bits.
  * A row whose sequence has fewer tokens than rows, or whose block lies outside [0, num_blocks), is not cached, its query is written all the same.
  * Two rows of a call may not have the same slot. */
 typedef struct tri_write_params {
@@ -477,7 +478,7 @@ typedef struct tri_write_params {
   void* out;                    /* may be q itself (same strides); any other element of it may not be one of q's, k's or v's */
   int64_t out_stride_row, out_stride_head;
   const void* positions;        /* element (axis, row) at axis*position_stride + row */
-  int64_t position_stride;
+  int64_t position_stride;      /* of several axes num_rows or more, or 0: all axes have the same numbers */
   const int32_t* freq_axes;     /* [head_dim/2]: the axis of each frequency (any number that is none counts as 0), or NULL: axis 0 */
   const float* inv_freq;        /* [head_dim/2] */
   const void* q_norm;           /* [head_dim], or NULL */

@@ -311,6 +311,14 @@ def test_oracle_moves_end_where_a_list_is_no_path():
     assert odec.accepted_moves([0, 1, 2], 9, 2) == [(0, 0), (1, 1)]
 
 
+@pytest.mark.parametrize("stride,word", [(0, b"eps"), (3, b"eps"), (1, b"axes"), (2, b"axes"), (-1, b"axes"), (-3, b"axes")])
+def test_axes_of_positions_are_apart_or_the_same(stride, word):
+    """(what is refused behind them says that they are not)"""
+    params = _write(num_axes=3, position_stride=stride, eps=-1.0)
+    assert _lib.load().tri_write_paged(C.byref(_layout()), C.byref(_batch()), C.byref(params), None) == INVALID
+    assert word in _lib.load().tri_last_error()
+
+
 # ------------------------------------------------------------------------------------- waits
 def test_stores_of_every_wave_have_arrived_before_its_workgroup_is_counted(tmp_path):
     """The last workgroup of a sequence reads what every wave of the others stored.  A barrier does not wait for stores on their way, and the

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import decoding as odec
-from test_gpu_decoding import BF16, DEV, FP8, FP16, FP32, Drafts, Step, _bits
+from test_gpu_decoding import BF16, DEV, FP8, FP16, FP32, Drafts, Step, _bits, _check_written
 from triattention_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -100,6 +100,28 @@ def test_unit_pairs_are_turned_into_cosines_and_sines_rounded_once(far, half, di
             # (by value: the sign of a zero is that of a sum)
             assert torch.equal(got[:, head, first], one), int((got[:, head, first] != one).sum())
             assert torch.equal(got[:, head, ~first], two), int((got[:, head, ~first] != two).sum())
+
+
+@pytest.mark.parametrize("rows", [1, 9])
+@pytest.mark.parametrize("wide", [True, False])
+def test_one_axis_of_positions_for_all(rows, wide):
+    """Plain text on three axes: one axis expanded, a slice of a longer one, is what three copies of it are."""
+    s = Step([40, 7], rows=[rows, rows if rows < 7 else 7], axes=3, norm=BF16, seed=41, wide=wide, far=100000)
+    s.positions = s.positions[:1].expand(3, -1).contiguous()
+    kv, batch = s.device()
+    want = s.write(kv, batch)
+    _check_written(s, want)
+    k, v = s.dk[0].clone(), s.dv[0].clone()
+    line = torch.cat([s.dpos[0], s.dpos[0] + 1])
+    s.dpos = line[:s.num_rows].expand(3, -1)
+    assert rows == 1 or s.dpos.stride(0) == 0
+    s.dk[0].view(torch.int16).zero_(), s.dv[0].view(torch.int16).zero_()
+    got = s.write(kv, batch)
+    where = odec.places(s.lens, s.starts, s.num_rows, s.tables, s.block, s.pool)
+    assert torch.equal(_bits(got), _bits(want))
+    for new, old in ((s.dk[0], k), (s.dv[0], v)):
+        for _, page, off in where:
+            assert torch.equal(_bits(new[page, off]), _bits(old[page, off]))
 
 
 # -------------------------------------------------------------------------------------- norm

@@ -1350,7 +1350,8 @@ int tri_write_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_w
   if (!rc) rc = check_heads("out", p->out, p->out_stride_row, p->out_stride_head, n, p->num_q_heads, D, true);
   if (rc) return rc;
   if (!p->inv_freq || (n > 0 && !p->positions)) return fail(TRI_ERR_INVALID_ARGUMENT, "inv_freq / positions is NULL");
-  if (p->num_axes < 1 || (p->num_axes > 1 && p->position_stride < n))
+  // (0: all axes are the same numbers, those of plain text)
+  if (p->num_axes < 1 || (p->num_axes > 1 && p->position_stride != 0 && p->position_stride < n))
     return fail(TRI_ERR_INVALID_ARGUMENT, "%d axes of positions, %lld apart", p->num_axes, (long long)p->position_stride);
   if (!(p->eps >= 0.f) || !is_finite(p->eps) || !is_finite(p->rotary_scale))
     return fail(TRI_ERR_INVALID_ARGUMENT, "eps must be finite and not negative, rotary_scale finite");

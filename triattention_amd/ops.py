@@ -1013,7 +1013,7 @@ def write_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, k: torch.Tensor,
     sequence: the last tokens of ``batch.seq_lens``, one per sequence without ``row_starts``.
 
     ``positions`` int32 or int64 [rows], or [axes, rows] with ``freq_axes`` (int32 [D / 2]: the axis each frequency goes by;
-    ``rope.section_axes`` makes it) for images and video.  ``inv_freq`` fp32 [D / 2], the pairs by the cache's ``rope_style``.
+    ``rope.section_axes`` makes it) for images and video; plain text on several axes may be one axis expanded.  ``inv_freq`` fp32 [D / 2], the pairs by the cache's ``rope_style``.
     ``q_norm`` and ``k_norm`` [D], both of q's type or both fp32: y = x / sqrt(mean(x^2) + eps) * norm.  ``rotary_scale`` multiplies what is rotated.
 
     An fp8 cache with a scale per row gets each row's: its largest finite magnitude / 448, at least 2^-126.  One without takes codes for code * ``k_scale``
