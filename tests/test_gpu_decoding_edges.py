@@ -208,3 +208,36 @@ def test_verify_infinities_beside_numbers_that_weigh_something(temperature, kind
                 d.tokens[r] = odec.draw(odec.distribution(d.target[up], temperature, False), float(d.uniforms[up, 1]))
     lengths = d.check(d.run(max_rows=4), 4)
     assert kind == "draft" or max(lengths) > 1
+
+
+@pytest.mark.parametrize("seqs", [64, 65, 130, 4097, 5000])
+@pytest.mark.parametrize("kind", ["tree", "chain", "draft"])
+def test_verify_finds_the_sequence_of_a_row(seqs, kind):
+    """Uneven and empty sequences with temperatures of their own, greedy ones among them, rows behind the last one and rows beyond
+    max_rows: on both sides of 64 sequences, where a row's sequence is found another way, and of 64 x 64."""
+    g = torch.Generator().manual_seed(seqs)
+    many = seqs > 1000
+    rows = torch.randint(0, 3 if many else 6, (seqs,), generator=g).tolist()
+    rows[0], rows[1], rows[-1] = 7, 0, 2
+    temperatures = [(0.0, 0.4, 1.0, 2.5)[int(torch.randint(0, 4, (1,), generator=g))] for _ in rows]
+    d = Drafts(rows, 37, tree=kind == "tree", draft=kind == "draft", temperatures=temperatures, seed=seqs, pad=5)
+    for width in ((4,) if many else (3, 4, 7)):
+        lengths = d.check(d.run(max_rows=width), width)
+        assert max(lengths) > 1 and min(lengths) == 0
+
+
+@pytest.mark.parametrize("kind", ["tree", "draft"])
+def test_verify_many_sequences_of_several_pieces(kind):
+    g = torch.Generator().manual_seed(9)
+    rows = torch.randint(0, 4, (70,), generator=g).tolist()
+    temperatures = [(0.0, 0.3, 1.0, math.inf)[i % 4] for i in range(70)]
+    d = Drafts(rows, 4100, tree=kind == "tree", draft=kind == "draft", temperatures=temperatures, seed=10, pad=1)
+    d.check(d.run(max_rows=2), 2)
+
+
+def test_verify_probabilities_of_many_sequences():
+    g = torch.Generator().manual_seed(11)
+    rows = torch.randint(0, 5, (200,), generator=g).tolist()
+    for draft in (False, True):
+        d = Drafts(rows, 50, tree=not draft, draft=draft, probs=True, seed=12, pad=2)
+        d.check(d.run(max_rows=3), 3)
