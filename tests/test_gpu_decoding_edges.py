@@ -241,3 +241,17 @@ def test_verify_probabilities_of_many_sequences():
     for draft in (False, True):
         d = Drafts(rows, 50, tree=not draft, draft=draft, probs=True, seed=12, pad=2)
         d.check(d.run(max_rows=3), 3)
+
+
+@pytest.mark.parametrize("dtype,bits", [(FP32, 0x7f800001), (FP32, -0x800001 + 2), (BF16, 0x7f81), (BF16, -127), (FP16, 0x7c01), (FP16, -1023)])
+@pytest.mark.parametrize("kind", ["tree", "draft"])
+@pytest.mark.parametrize("greedy", [False, True])
+def test_verify_signalling_nan_count_as_nothing(dtype, bits, kind, greedy):
+    """NaN of either sign whose highest bit of the mantissa is not set, in every piece, and one row of nothing else."""
+    d = Drafts([4, 3, 6], 4500, dtype=dtype, tree=kind == "tree", draft=kind == "draft", temperatures=[0.0 if greedy else 0.8] * 3, seed=51)
+    raw = d.target.view({4: torch.int32, 2: torch.int16}[d.target.element_size()])
+    raw[:, 0::7] = bits
+    raw[:, 2047:2050] = bits
+    raw[5] = bits
+    assert bool(torch.isnan(d.target[5]).all())
+    d.check(d.run(max_rows=6), 6)

@@ -320,7 +320,17 @@ __global__ __launch_bounds__(kVerifyThreads) void verify_sums_kernel(VerifyLaunc
   for (int s = 0; s < kPieceSteps; ++s) {
     const Numbers8 n = numbers_of<RT, N>(held.step[s]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = fmaxf(most, n.x[e]);
+    for (int e = 0; e < 8; ++e) most = __builtin_elementwise_maximum(most, n.x[e]);
+  }
+  // NaN, which that hands on, count as -inf (fmaxf is no way past them: behind a signalling one it has lost what was before)
+  if (!PROBS && __ballot(most != most)) {
+    most = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < kPieceSteps; ++s) {
+      const Numbers8 n = numbers_of<RT, N>(held.step[s]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = n.x[e] > most ? n.x[e] : most;
+    }
   }
   most = most_of_wave(most);
   const float top = PROBS ? most : fminf(most, FLT_MAX);      // (infinities are the largest finite number)
