@@ -458,8 +458,9 @@ typedef enum tri_real { TRI_REAL_BF16 = 0, TRI_REAL_FP16 = 1, TRI_REAL_FP32 = 2 
  * layer of the cache.  fp8 caches: with v_scale_layers a row's scale is max(largest finite |element| / 448, 2^-126) and is
  * written with it; without, codes stand for code * k_scale (v_scale), numbers beyond 448 of those are the largest code; infinities and NaN become NaN
  * either way.  Angles are 64-bit products, their cosines and sines times rotary_scale are rounded to 32 bits, norms and rotations are 32-bit (what
- * that cannot hold is infinite; the squares of a norm are that from 2^64 on), scales and the numbers over them too, and every
- * output is rounded once, to nearest, from its 32 bits.
+ * that cannot hold is infinite; the squares of a norm are that from 2^64 on, so that numbers over their root are 0, and are 0 below
+ * 2^-75, where only an eps above 0 keeps a row finite), scales and the numbers over them too, and every output is rounded once, to
+ * nearest, from its 32 bits.
  * A row whose sequence has fewer tokens than rows, or whose block lies outside [0, num_blocks), is not cached, its query is written all the same.
  * Two rows of a call may not have the same slot. */
 typedef struct tri_write_params {
@@ -509,8 +510,10 @@ int tri_read_paged(const tri_kv_layout* kv, const tri_batch* batch, const tri_re
  * where that is 0).  A draw takes the least token whose running sum exceeds uniforms[row][1] of the whole.  A temperature that is not above 0:
  * the largest logit, the first among equals, in place of every draw, and a draft is accepted iff it is that.  So next and the accepted
  * tokens have the distribution of the target, whatever drafted them.
- *  Weights and sums are 64-bit (what weighs less than 2^-900 of the largest weighs nothing).  NaN logits count as -inf, +inf as the
- * largest finite number, probabilities that are no positive finite number as 0; a row without any weight draws -1.  Tokens outside [0, vocab) are never accepted.  Rows beyond max_rows of a sequence are not looked at.
+ *  Weights and sums are 64-bit numbers, a weight right to 2^-44 of itself: a random number that near the border between two tokens, or between a
+ * draft taken and rejected, may fall on either side.  What weighs less than 2^-900 of the largest weighs nothing.  NaN logits count as -inf, +inf as the
+ * largest finite number, probabilities that are no positive finite number as 0; a row without any weight draws -1.  Tokens outside
+ * [0, vocab) are never accepted.  Rows beyond max_rows of a sequence are not looked at.
  * rows: int32 [num_seqs][max_rows], the accepted rows ascending, row 0 first, -1 behind them; counts: how many; next: the token
  * behind them.  A sequence without rows: 0 and -1. */
 typedef struct tri_verify_params {

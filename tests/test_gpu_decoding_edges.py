@@ -255,3 +255,46 @@ def test_verify_signalling_nan_count_as_nothing(dtype, bits, kind, greedy):
     raw[5] = bits
     assert bool(torch.isnan(d.target[5]).all())
     d.check(d.run(max_rows=6), 6)
+
+
+# --------------------------------------------------------------------------- one step after another
+@pytest.mark.parametrize("dtype,row_scales", [(BF16, False), (FP8, True)])
+def test_the_next_steps_lengths_stay_on_the_device(dtype, row_scales):
+    """A batch made for the longest lengths, its lengths rewritten from what acceptance returns: what batches made anew for every step give, in
+    the cache and read back from it."""
+    g = torch.Generator().manual_seed(61)
+    now, longest, steps = [30, 5, 17], [64, 64, 64], 4
+    tables = torch.randperm(3 * 4 + 2, generator=g)[:12].view(3, 4).tolist()
+    inv = torch.tensor([1e4 ** (-i / 64) for i in range(64)], dtype=FP32, device=DEV)
+    caches = []
+    for _ in range(2):
+        k, v = (torch.zeros(14, 16, 2, 128, dtype=dtype, device=DEV) for _ in range(2))
+        scales = [torch.ones(14 * 16 * 2, device=DEV) for _ in range(2)] if row_scales else [None, None]
+        caches.append((k, v, scales, ops.PagedKV([k], [v], "half", *([x] if x is not None else None for x in scales))))
+    kept = ops.StepBatch(torch.device(DEV), longest, block_tables=tables)
+    lens = torch.tensor(now, dtype=torch.int32, device=DEV)
+    for step in range(steps):
+        rows = torch.randint(1, 6, (3,), generator=g).tolist()
+        starts = torch.tensor([0, rows[0], rows[0] + rows[1], sum(rows)], dtype=torch.int32, device=DEV)
+        torch.add(lens, torch.tensor(rows, dtype=torch.int32, device=DEV), out=kept.seq_lens)
+        anew = ops.StepBatch(torch.device(DEV), [t + n for t, n in zip(now, rows)], block_tables=tables)
+        qkv = torch.randn(sum(rows), 8, 128, generator=g).to(BF16).to(DEV)
+        pos = torch.arange(sum(rows), device=DEV)
+        counts = [1 + int(torch.randint(0, n, (1,), generator=g)) for n in rows]
+        path = torch.full((3, 6), -1, dtype=torch.int32)
+        for b, (n, c) in enumerate(zip(rows, counts)):
+            path[b, :c] = torch.tensor([0] + sorted((torch.randperm(n - 1, generator=g)[:c - 1] + 1).tolist()))
+        outs, new = [], []
+        for (_, _, _, kv), batch in zip(caches, (kept, anew)):
+            outs.append(ops.write_paged(kv, batch, qkv[:, :4], qkv[:, 4:6], qkv[:, 6:], pos, inv, row_starts=starts))
+            new.append(ops.accept_drafts(kv, batch, starts, path.to(DEV), torch.tensor(counts, dtype=torch.int32, device=DEV)))
+        assert torch.equal(_bits(outs[0]), _bits(outs[1])) and torch.equal(new[0], new[1])
+        lens, now = new[0], [t + c for t, c in zip(now, counts)]
+        assert lens.tolist() == now
+    for a, b in zip(caches[0][:2], caches[1][:2]):
+        assert torch.equal(_bits(a), _bits(b))
+    kept.seq_lens.copy_(lens)
+    starts = torch.tensor([0, now[0], now[0] + now[1], sum(now)], dtype=torch.int32, device=DEV)
+    anew = ops.StepBatch(torch.device(DEV), now, block_tables=tables)
+    for x, y in zip(ops.read_paged(caches[0][3], kept, starts, sum(now)), ops.read_paged(caches[1][3], anew, starts, sum(now))):
+        assert torch.equal(_bits(x), _bits(y))

@@ -14,8 +14,8 @@
 //  accept_rows_kernel  : rows of the accepted path to consecutive slots, every layer
 //
 // Two launches a call.  A third, for what the last workgroup of a sequence does, took 4 us more of the host and 3 of the GPU; one launch for
-// all of it would need counters cleared before it.  One chain of six rows of 32768 logits 4.1 + 7.4 us, 60 greedy rows of 131072
-// 5.7 + 4.6: launches and dependent reads; the host behind them takes 14.
+// all of it would need counters cleared before it.  One chain of six rows of 32768 logits 4.4 + 7.0 us, 60 greedy rows of 131072
+// 5.8 + 4.4: launches and dependent reads; the host behind them takes 14.
 #include <algorithm>
 #include <cfloat>
 
@@ -281,8 +281,8 @@ __device__ __forceinline__ const void* row_of(const VerifyLaunch& a, int row) {
 }
 
 // A wave's 2048 numbers of a row.  Sampled rows want the sum, greedy ones the place of the largest.  Bound by vector instructions
-// (16 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 20.6 us, 79 % of whose cycles those
-// take; 161 rows of 100003 fp32 ones, 64 MB, in 15.8 and 58 %, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
+// (16 a logit, most of them 64-bit) where rows fill the chip: 262 rows of 131072 bf16 logits, 69 MB, in 21.1 us, 83 % of whose cycles those
+// take; 161 rows of 100003 fp32 ones, 64 MB, in 16.4 and 55 %, one round of waves that wait for their loads and then compute.  Pieces of fewer numbers, loads past
 // the caches, two halves of 16 bytes side by side for fp32 and a shorter form for rows whose numbers lie near each other gained nothing; weights
 // against the first step's largest number, while the other steps' loads are on their way, 1 us of the second and lost half of one in the first.
 template <int RT, bool PROBS>
@@ -511,7 +511,7 @@ __device__ __forceinline__ bool last_to_arrive(const VerifyLaunch& a, int b, int
 }
 
 // A wave a row, four to a workgroup: the rows of a sequence are drawn at once, not only those of the path, which is known one row after the
-// other.  8 trees of up to 32 rows of 100003 logits 7.8 us (one workgroup of sixteen waves a sequence 26), dependent reads and one piece's weights.
+// other.  8 trees of up to 32 rows of 100003 logits 7.5 us (one workgroup of sixteen waves a sequence 26), dependent reads and one piece's weights.
 template <int RT, bool PROBS>
 __global__ __launch_bounds__(kVerifyThreads) void verify_walk_kernel(VerifyLaunch a, int max_groups) {
   constexpr int N = PROBS ? kProbs : kLogits;
@@ -602,7 +602,7 @@ __device__ __forceinline__ void rest_of(const Powers& powers, const Rest<RT>& he
 }
 
 // Every workgroup of a sequence finds for itself which rows are accepted (a wave a row); where one is not, each takes some pieces of what
-// that leaves, and the last one draws from it.  48 chains of up to eight rows of 131072 logits 17.2 us: 4 until the rows are decided, 8 for the
+// that leaves, and the last one draws from it.  48 chains of up to eight rows of 131072 logits 16.9 us: 4 until the rows are decided, 8 for the
 // 38 MB of logits and draft probabilities of the rejected ones (4.7 TB/s), 1.5 until the last has come, 4 for its draw.  Workgroups of four
 // and of sixteen waves were 1 us slower.
 template <int RT, bool PROBS>
@@ -693,7 +693,7 @@ __global__ __launch_bounds__(kChainThreads, 4) void verify_chain_kernel(VerifyLa
 
 // Rows [first new token + rows[j]] to [first new token + j], j < count, of one side of one layer.  Lists ascend, so rows[j] >= j: a thread has one
 // place of every row, and what it writes lies before all that it still reads.  32 sequences, 36 layers, 96 rows of 8 x 128 fp8 with scales
-// and weights in 8.4 us, one sequence in 4.0: four dependent reads (starts, list, table, row); 15 MB moved would take 3.
+// and weights in 8.3 us, one sequence in 3.7: four dependent reads (starts, list, table, row); 15 MB moved would take 3.
 constexpr int kAcceptAtOnce = 8;
 __global__ __launch_bounds__(kVerifyThreads) void accept_rows_kernel(AcceptLaunch a) {
   __shared__ int64_t from_row[64], to_row[64];           // elements of the cache

@@ -116,10 +116,11 @@ __device__ __forceinline__ uint32_t pack_codes(const float* x, const Unit& u) {
 // angles in every head.  A row's steps are shared by waves_per_row waves, which find the angles once each.  Norm and rotation
 // are a product by the head's 1 / sqrt(mean) and one by (w1 cos, w2 sin, w2 cos, w1 sin), the same in every head.
 //
-// Bound by reading and writing the rows: 16384 rows of 32 + 2 x 8 heads of 128, 403 MB, in 80 us (5.0 TB/s, a copy's 5.2 to 5.4); 11392
-// rows of 28 + 2 x 4 heads into fp8, 199 MB, in 38.  One row 4.8 us, 64 rows of 64 + 2 x 8 heads with scales 5.5: a launch and its
-// dependent reads.  The second took 53 while angles were found four times over and products of norm and rotation made in every head;
-// four steps at once with five waves a SIMD, and eight waves, which spill, were a tenth slower than two steps and six.
+// Bound by reading and writing the rows: 16384 rows of 32 + 2 x 8 heads of 128, 403 MB, in 80 us (5.0 TB/s, a copy's 5.2 to 5.4); without a norm,
+// whose sums over lanes are not all hidden, in 69; interleaved, whose loads and stores of 8 bytes take turns in a line, in 103.  The same
+// into fp8 with scales 370 MB in 81; 11392 rows of 28 + 2 x 4 heads into fp8, 199 MB, in 37.  One row 5.4 us, 64 rows of 64 + 2 x 8 heads with
+// scales 7.2: a launch and its dependent reads.  11392 rows took 53 while angles were found four times over and products of norm and
+// rotation made in every head; four steps at once with five waves a SIMD, and eight waves, which spill, were a tenth slower than two steps and six.
 template <int D, int QT, int KIND, bool HALF, int PAST>
 __global__ __launch_bounds__(kWriteThreads, 6) void write_paged_kernel(WriteLaunch a) {
   constexpr int LPH = D / 8, HPW = kWave / LPH;
@@ -496,9 +497,10 @@ hipError_t launch_write_paged(WriteLaunch a, hipStream_t s) {
   // 2048 rows 18.5, 13.8, 13.9.
   a.waves_per_row = (int)std::min<int64_t>(steps, std::max<int64_t>(1, 2048 / a.num_rows));
   // Many rows are read past the caches, which keep what is written; of even more rows the queries go past them too, and what is
-  // cached stays.  Calls on three sets of rows in turn, outputs kept for one call, plain, reads past, both past, us: 42 MB of rows 20.1,
-  // 22.8, 21.6; 50 MB 24.7, 23.9, 24.6; 84 MB 41.4, 34.3, 36.8; 100 MB 49.3, 44.2, 44.4; 105 MB 43.8, 37.7, 41.0; 168 MB 75.1, 73.0, 68.9;
-  // 201 MB 90.2, 89.9, 79.9.
+  // cached stays.  Between a copy that writes q, k and v and an addition that reads the queries, the three together on three sets of rows in turn,
+  // plain, reads past, both past, us: 42 MB of rows 47.6, 45.4, 46.3; 57 MB 59.4, 58.8, 58.6; 67 MB 71.5, 67.6, 68.0; 84 MB 88.3, 85.5, 84.1; 101 MB 103.5,
+  // 100.8, 96.4; 135 MB 146, 130, 128; 201 MB 209, 199, 187; 403 MB 402, 406, 384.  Calls alone, inputs cold and outputs kept for one call: 42 MB 18.0, 21.3,
+  // 21.2; 57 MB 28.2, 25.3, 26.0; 67 MB 33.7, 29.3, 30.5; 84 MB 45.0, 39.2, 41.3; 101 MB 49.0, 45.3, 43.8; 135 MB 62.8, 61.7, 56.8; 201 MB 89.0, 88.6, 79.0.
   const int64_t bytes = (int64_t)a.num_rows * (a.Hq + 2 * a.Hkv) * a.D * 2;
   const PastCaches past = bytes > (128ll << 20) ? kAllPast : bytes > (64ll << 20) ? kReadPast : kCached;
   if (a.D == 64) write_of_type<64>(a, past, s);

@@ -1018,7 +1018,7 @@ def write_paged(kv: PagedKV, batch: StepBatch, q: torch.Tensor, k: torch.Tensor,
 
     An fp8 cache with a scale per row gets each row's: its largest finite magnitude / 448, at least 2^-126.  One without takes codes for code * ``k_scale``
     (``v_scale``), as ``attend_paged`` reads them with these; larger numbers are the largest code.  Infinities and NaN become NaN
-    in either.  Everything is computed in 32 bits (angles in 64) and rounded once.
+    in either.  Everything is computed in 32 bits (angles, cosines and sines in 64, rounded to 32) and rounded once.
 
     ``out`` may be ``q`` itself; otherwise it has no element in common with ``q``, ``k`` and ``v``.  Rows behind ``row_starts[-1]`` are left as they
     were.  A captured call may be replayed with everything on the device rewritten in place."""
@@ -1111,7 +1111,8 @@ def verify_drafts(target: torch.Tensor, tokens: torch.Tensor, row_starts: torch.
     Without ``draft_probs`` a token is drawn from every row's p, and the walk goes from the first row on to the child that holds it (the
     first of several), as long as there is one.  With them (fp32 [rows, vocab]: what each row's token was drawn from; chains only) a row is accepted
     iff uniforms[row, 0] * draft(token) < p(token), and after a rejection the next token comes from max(p - draft, 0).  Either way accepted and next
-    tokens have the target's distribution.  A draw: the least token whose running sum exceeds uniforms[row, 1] of the whole, in 64 bits.
+    tokens have the target's distribution.  A draw: the least token whose running sum exceeds uniforms[row, 1] of the whole, in 64-bit
+    sums of weights that are right to 2^-44 each.
     A temperature of 0 takes the largest logit (the first of equals) instead.
 
     Returns (rows int32 [sequences, max_rows]: accepted rows ascending, the first row first, -1 behind them; counts int32 [sequences];
