@@ -73,6 +73,18 @@ def test_codes_of_a_tensors_scale_are_those_of_the_quotients(unit):
         assert torch.equal(got[~zero], want[~zero]) and bool((got[zero] & 0x7f == 0).all()), int((got != want)[~zero].sum())
 
 
+@pytest.mark.parametrize("row_scales", [True, False])
+def test_values_of_nothing_keep_their_sign_as_codes(row_scales):
+    s = _still(Step([20], rows=[8], q_heads=2, kv_heads=2, dim=64, dtype=FP8, row_scales=row_scales, seed=4))
+    s.qkv[:, 4:, 0::3], s.qkv[:, 4:, 1::3] = -0.0, 0.0
+    s.qkv[0, 4:] = -0.0
+    s.qkv[1, 4:, 2::3] = -2.0 ** -30
+    kv, batch = s.device()
+    s.write(kv, batch, **({} if row_scales else dict(v_scale=0.3)))
+    unit = (s.v.float().abs().amax(-1, keepdim=True) / 448).clamp(min=2.0 ** -126) if row_scales else torch.tensor(0.3)
+    assert torch.equal(_slots(s, s.dv[0].view(torch.uint8)), _codes(s.v, unit))
+
+
 # ------------------------------------------------------------------------------------ angles
 @pytest.mark.parametrize("far", [1 << 12, 1 << 20, (1 << 31) - 1, 1 << 44])
 @pytest.mark.parametrize("half", [True, False])

@@ -97,14 +97,14 @@ struct Unit {
 // Four e4m3 codes of the 32-bit quotients x / scale: rounded to nearest, beyond 448 the largest; infinities and NaN are NaN.  A product by the
 // reciprocal is off by up to 1.5 steps, and one remainder corrects it but for quotients within 2^-22 of a step of the middle between two
 // numbers.  Where one of those is a tie of codes (17, 19 .. 31 times a power of two) and the scale's mantissa hence within 8 of a multiple of 2^20, all
-// corrected products are the quotients: the codes are those of a division, which takes more (11392 rows into
-// fp8 38.0 us, this 37.1, the product alone 36.8, but 1 code in 2000 its neighbour).
+// corrected products are the quotients: the codes are those of a division, which takes more (11392 rows into fp8 38.0 us, this 37.1, the product
+// alone 36.8, but 1 code in 2000 its neighbour).
 __device__ __forceinline__ uint32_t pack_codes(const float* x, const Unit& u) {
   float y[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float a = x[e] * u.up, q = fminf(fmaxf(a * u.inv, -512.f), 512.f);
-    const float v = __builtin_fmaf(__builtin_fmaf(-q, u.unit, a), u.inv, q);
+    const float over = __builtin_fmaf(q, u.unit, -a), v = __builtin_fmaf(-over, u.inv, q);      // (of - 0 that is - 0)
     y[e] = is_number(x[e]) ? fminf(fmaxf(v, -448.f), 448.f) : __builtin_nanf("");
   }
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
