@@ -79,6 +79,8 @@ __device__ __forceinline__ float max_of_head(float v) {
 template <int T>
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   if constexpr (T == TRI_KV_FP16) {
+    // (numbers of 32 bits: the rounding is not drawn into the product before it)
+    asm("" : "+v"(a), "+v"(b));
     f16x2 v = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, v);
   } else {
